@@ -1,0 +1,238 @@
+"""The attention kernels against the formula in 64 bits, with bounds that count each rounding (attention_util.reference)."""
+import math
+
+import pytest
+import torch
+
+from attention_util import check, reference
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def make(b, s, h, hk, d, dtype, seed=0, amp=1.0):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    q, k, v, do = (torch.randn(b, s, n, d, generator=g, device=DEV).mul(amp).to(dtype) for n in (h, hk, hk, h))
+    return q.requires_grad_(), k.requires_grad_(), v.requires_grad_(), do
+
+
+def run(q, k, v, do, **kw):
+    from tips_b200.ops.attention import attention
+    y = attention(q, k, v, **kw)
+    dq, dk, dv = torch.autograd.grad(y, (q, k, v), do)
+    return {"out": y.detach(), "dq": dq, "dk": dk, "dv": dv}
+
+
+def status():
+    from tips_b200.ops import base
+    return base.K().tipsk_attention_status()
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b,s,h,hk,d", [
+    (1, 1, 1, 1, 64), (2, 2, 2, 1, 8), (1, 17, 3, 1, 40), (1, 127, 2, 2, 64), (1, 128, 1, 1, 128), (2, 129, 4, 2, 96),
+    (1, 255, 2, 2, 32), (1, 257, 2, 1, 128), (2, 300, 6, 3, 72), (1, 513, 2, 2, 64), (1, 640, 8, 1, 120), (3, 384, 2, 2, 16),
+    (1, 1500, 2, 1, 64), (1, 1031, 2, 2, 128)])
+def test_sizes(b, s, h, hk, d, causal):
+    dtype = torch.bfloat16 if (s + d) % 3 else torch.float16
+    q, k, v, do = make(b, s, h, hk, d, dtype, seed=s)
+    check(run(q, k, v, do, causal=causal), *reference(q, k, v, do, causal))
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths", [[0, 1, 333, 128], [200, 0, 0, 129], [127, 256, 257, 2], [-5, 1000, 64, 300]])
+def test_padded_batches(lengths, causal, dtype):
+    """Lengths of nothing, of one, at and around the tiles' borders and out of range; NaN and infinities in the padding."""
+    q, k, v, do = make(4, 333, 4, 2, 64, dtype, seed=sum(lengths))
+    n = torch.tensor(lengths, device=DEV, dtype=torch.int32 if causal else torch.int64)
+    want, bound = reference(q, k, v, do, causal, n)
+    with torch.no_grad():
+        for i, m in enumerate(lengths):
+            m = max(0, min(333, m))
+            for t, x in ((q, math.nan), (k, math.inf), (v, math.nan), (do, -math.inf)):
+                t[i, m:] = x
+    got = run(q, k, v, do, causal=causal, lengths=n)
+    check(got, want, bound)
+    for i, m in enumerate(lengths):
+        for x in got.values():
+            assert not x[i, max(0, min(333, m)):].any()  # exactly zero
+
+
+def test_scale_and_large_scores():
+    """Scores of some hundred: the running maximum carries the row."""
+    q, k, v, do = make(2, 400, 2, 2, 64, torch.bfloat16, seed=3, amp=2.0)
+    check(run(q, k, v, do, scale=0.5, causal=True), *reference(q, k, v, do, True, scale=0.5))
+
+
+def test_rising_scores_rescale_the_output():
+    """Every key tile raises the maximum of every row."""
+    q, k, v, do = make(1, 700, 2, 1, 64, torch.bfloat16, seed=4)
+    with torch.no_grad():
+        q[..., 0] = 4.0
+        k[..., 0] = torch.linspace(-40, 40, 700, device=DEV)[None, :, None].to(k.dtype)
+    check(run(q, k, v, do), *reference(q, k, v, do))
+
+
+def test_strides_orders_and_alignment():
+    """[b, h, s, d] order, slices of wider tensors, rows that start on 4 bytes, a broadcast key head and a broadcast gradient."""
+    b, s, h, d = 2, 200, 4, 64
+    q, k, v, do = make(b, s, h, h, d, torch.bfloat16, seed=5)
+    want, bound = reference(q, k, v, do)
+
+    def leaf(t):
+        return t.detach().requires_grad_()
+
+    def other(t, kind):
+        if kind == "heads first":
+            return t.detach().transpose(1, 2).contiguous().transpose(1, 2)
+        if kind == "batch last":
+            return t.detach().permute(1, 2, 0, 3).contiguous().permute(2, 0, 1, 3)
+        if kind == "wide":
+            return torch.cat([t.detach(), t.detach()], 3)[..., :d]
+        if kind == "odd start":
+            return torch.cat([t.detach()[..., :2], t.detach()], 3)[..., 2:]
+        return t.detach().transpose(1, 3).contiguous().transpose(1, 3)  # last axis not contiguous
+
+    for kind in ("heads first", "batch last", "wide", "odd start", "columns"):
+        check(run(*(leaf(other(t, kind)) for t in (q, k, v)), other(do, kind)), want, bound)
+    one = k.detach()[:, :, :1]
+    want, bound = reference(q, one.expand(b, s, h, d), v, do)
+    got = run(leaf(q), leaf(one.expand(b, s, h, d)), leaf(v), do)
+    check(got, want, bound)
+    ones = torch.ones((), device=DEV, dtype=q.dtype).expand(b, s, h, d)
+    check(run(leaf(q), leaf(k), leaf(v), ones), *reference(q, k, v, ones))
+
+
+@pytest.mark.parametrize("h,hk,lengths", [(4, 4, None), (6, 2, [70, 190])])
+def test_packed(h, hk, lengths):
+    from tips_b200.ops.attention import packed_attention
+    b, s, d = 2, 190, 32
+    q, k, v, do = make(b, s, h, hk, d, torch.bfloat16, seed=6)
+    n = None if lengths is None else torch.tensor(lengths, device=DEV)
+    want, bound = reference(q, k, v, do, False, n)
+    qkv = torch.cat([t.detach().reshape(b, s, -1) for t in (q, k, v)], 2).requires_grad_()
+    y = packed_attention(qkv, h, kv_heads=hk, lengths=n)
+    (g,) = torch.autograd.grad(y, qkv, do.reshape(b, s, -1))
+    g = g.view(b, s, h + 2 * hk, d)
+    check({"out": y.detach().view(b, s, h, d), "dq": g[:, :, :h], "dk": g[:, :, h:h + hk], "dv": g[:, :, h + hk:]}, want, bound)
+
+
+def test_gradient_against_differences():
+    """<dO, O(x + e w)> in 64 bits, by central differences, against the gradients' product with w."""
+    q, k, v, do = make(1, 150, 4, 2, 40, torch.bfloat16, seed=8)
+    got = run(q, k, v, do, causal=True)
+    _, bound = reference(q, k, v, do, True)
+    g = torch.Generator(device=DEV)
+    g.manual_seed(9)
+    e = 1e-4
+    for name, t in (("dq", q), ("dk", k), ("dv", v)):
+        w = torch.randn(t.shape, generator=g, device=DEV, dtype=torch.float64)
+        vals = []
+        for sign in (1, -1):
+            args = [x.detach().double() + (sign * e * w if x is t else 0) for x in (q, k, v)]
+            out, _ = reference(*args, do.double(), True, store=torch.bfloat16)
+            vals.append(float((out["out"] * do.double()).sum()))
+        slope = (vals[0] - vals[1]) / (2 * e)
+        # e^2 times the third derivative is far below the bound's 2^-8
+        assert abs(slope - float((got[name].double() * w).sum())) <= float((bound[name] * w.abs()).sum())
+
+
+def test_the_same_bits_twice_on_other_streams_and_in_graphs():
+    q, k, v, do = make(2, 500, 4, 2, 64, torch.bfloat16, seed=10)
+    n = torch.tensor([500, 131], device=DEV)
+    first = run(q, k, v, do, lengths=n)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run(q, k, v, do, lengths=n)
+    torch.cuda.current_stream().wait_stream(side)
+    for name in first:
+        assert torch.equal(first[name], other[name]), name
+    # two graphs with their own outputs; replayed on other inputs, then in turn
+    from tips_b200.ops.attention import _attention_bwd, _attention_fwd
+    bufs = [t.detach().clone() for t in (q, k, v, do)]
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out, lse, a, b, c = _attention_fwd(*bufs[:3], n, 0.125, False)
+            grads = [torch.empty_like(t) for t in (a, b, c)]
+            _attention_bwd(bufs[3], a, b, c, out, lse, n, 0.125, False, *grads)
+        graphs.append((g, dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))))
+    for t, x in zip(bufs, make(2, 500, 4, 2, 64, torch.bfloat16, seed=11)):
+        t.copy_(x)
+    n.copy_(torch.tensor([60, 499], device=DEV))
+    want = run(*(t.clone().requires_grad_() for t in bufs[:3]), bufs[3], lengths=n)
+    for g, got in graphs + graphs[:1]:
+        g.replay()
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+    assert status() == 0
+
+
+def test_infinities_in_valid_places_are_not_hidden():
+    q, k, v, do = make(1, 200, 1, 1, 64, torch.bfloat16, seed=12)
+    with torch.no_grad():
+        v[0, 7, 0, 3] = math.inf
+    got = run(q, k, v, do)
+    assert not got["out"][..., 3].isfinite().any() and got["out"][..., 4].isfinite().all()
+    assert not got["dq"].isfinite().all()
+
+
+def test_refusals_on_a_gpu():
+    from tips_b200.ops.attention import attention, packed_attention
+    q, k, v, _ = make(1, 16, 2, 2, 64, torch.bfloat16)
+    with pytest.raises(TypeError):
+        attention(q.float(), k.float(), v.float())
+    big = torch.zeros(1, 16, 2, 136, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        attention(big, big, big)
+    with pytest.raises(ValueError):
+        attention(big[..., :12], big[..., :12], big[..., :12])
+    with pytest.raises(ValueError):
+        attention(q, k, v, lengths=torch.tensor([16]))  # on the CPU
+    with pytest.raises(TypeError):
+        attention(q, k.cpu(), v)
+    with pytest.raises(ValueError):
+        packed_attention(torch.zeros(1, 16, 384, device=DEV, dtype=torch.bfloat16), 5, kv_heads=1, scale=1.0)
+    # gradients of gradients are refused, not wrong
+    y = attention(q, k, v)
+    (g,) = torch.autograd.grad(y.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_empty_inputs():
+    from tips_b200.ops.attention import attention
+    for b, s in ((0, 5), (3, 0)):
+        x = torch.zeros(b, s, 2, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+        y = attention(x, x, x)
+        assert y.shape == x.shape
+        y.sum().backward()
+        assert x.grad.shape == x.shape
+
+
+def test_encoder_on_a_padded_batch():
+    """What stands in the padding does not matter, and a full batch matches the unpadded path."""
+    from tips_b200.models.bert import synthetic_mlm_batch, tiny_bert
+    torch.manual_seed(0)
+    model = tiny_bert()
+    ids, pos, labels = (t.to(DEV) for t in synthetic_mlm_batch(3, 64, 1024, seed=1))
+    n = torch.tensor([64, 20, 33], device=DEV)
+    pos = pos % n[:, None]
+    other = torch.where(torch.arange(64, device=DEV)[None] < n[:, None], ids, (ids + 7) % 1024)
+    grads = []
+    for x in (ids, other):
+        model.zero_grad()
+        loss = model.loss(x, pos, labels, lengths=n)
+        loss.backward()
+        grads.append([loss.detach()] + [p.grad.clone() for p in model.layers.parameters()])
+    # dropped positions still pass the row-wise layers, whose weight gradients they reach with factors of exactly zero
+    for a, b in zip(*grads):
+        assert torch.allclose(a.float(), b.float(), rtol=2 ** -6, atol=2 ** -8 * float(a.float().abs().max()))
+    full = torch.full((3,), 64, device=DEV)
+    a, b = model.encode(ids), model.encode(ids, full)
+    assert (a.float() - b.float()).norm() <= 2 ** -5 * a.float().norm()

@@ -1,0 +1,942 @@
+// Self-attention on the 5th-generation tensor cores, forward and backward, for bf16 and fp16.
+//
+//   valid(i, j) = i < len, j < len and, if causal, j <= i        len: the sequence's length in a padded batch
+//   S = scale Q K^T,  L_i = log sum_j exp S_ij,  P = exp(S - L) where valid and 0 elsewhere,  O = P V
+//   dV = P^T dO,  dP = dO V^T,  D_i = dO_i . O_i,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Nothing of size s x s reaches memory: the forward pass keeps a running maximum and sum per row and leaves L, the backward
+// pass computes P again from S and L.  Exponentials are taken to base 2 (scale and log2 e in one factor), L is kept in
+// units of log2.  Rows that the mask leaves empty (i >= len) get O = 0, L = +inf, and gradients of 0.
+//
+// All products run as tcgen05.mma on 128 x 128 tiles with fp32 accumulators in TMEM.  A tile of probabilities goes back to
+// TMEM in 16 bits and is the A operand of the next product from there; tiles of Q, K, V and dO come by TMA in the
+// 128-byte-swizzled layout, which serves as a K-major operand (contraction over d) and as an MN-major one (contraction over
+// tokens) alike.  Head sizes up to 128 run on tiles of 64 or 128 columns; TMA fills what lies beyond d with zeros.
+//
+// The last tile of a sequence may hold positions beyond its length.  Whatever stands there must not count, and 0 * NaN
+// is NaN, so rows of a streamed tile that lie beyond the length are cleared in shared memory before they are contracted over.
+//
+// Every mbarrier wait is bounded; on a timeout the kernel sets an error word, frees its TMEM and returns.
+//
+// The reference contains no attention; this serves the BERT-shaped encoder.
+#include <cuda.h>
+
+#include <atomic>
+#include <cmath>
+
+#include "kernels/common.cuh"
+#include "kernels/tcgen05.cuh"
+#include "kernels/tips_kernels.h"
+
+namespace tipsk {
+namespace {
+
+constexpr int kTile        = 128;  // rows of a tile of queries or keys
+constexpr int kBoxBytes    = kTile * 128;  // 128 rows of 64 16-bit values
+constexpr int kAttnThreads = 320;  // eight softmax warps, one TMA warp, one MMA warp
+constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ int32_t g_attn_error;  // one per device
+
+struct Strides {
+  int64_t b, s, h;  // elements
+};
+
+__host__ __device__ __forceinline__ int TilesOf(int n, int tile) { return n / tile + (n % tile != 0); }
+
+struct AttnParams {
+  const void* lengths;  // [b] int32 or int64, or null
+  int len64;
+  int b, s, sp;         // sp: s rounded up to whole tiles, the row pitch of lse and delta
+  int h, hk, d;
+  int causal;
+  float scale, c;       // c = scale * log2(e)
+  float* lse;           // [b, h, sp]
+  float* delta;         // [b, h, sp]
+  void *o, *dq, *dk, *dv;
+  const void* dout;
+  Strides so, sdo, sdq, sdk, sdv;
+};
+
+struct AttnMaps {
+  CUtensorMap q, k, v, dout;
+};
+
+__device__ __forceinline__ int SeqLen(const AttnParams& p, int b) {
+  if (p.lengths == nullptr) return p.s;
+  const int64_t n = p.len64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
+  return static_cast<int>(n < 0 ? 0 : n > p.s ? p.s : n);
+}
+
+// 64 columns x 128 rows of one head: x along d, then position, head, batch.
+__device__ __forceinline__ void TmaLoadHead(void* dst, const CUtensorMap* map, int x, int s, int h, int b, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(SmemAddr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(s), "r"(h), "r"(b), "r"(SmemAddr(bar))
+      : "memory");
+}
+template <int HD>
+__device__ __forceinline__ void TmaLoadTile(uint8_t* dst, const CUtensorMap* map, int s, int h, int b, uint64_t* bar) {
+#pragma unroll
+  for (int x = 0; x < HD / 64; ++x) TmaLoadHead(dst + x * kBoxBytes, map, x * 64, s, h, b, bar);
+}
+// `bytes` (a multiple of 16) from 16-byte-aligned global memory.
+__device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(SmemAddr(dst)),
+               "l"(src), "r"(bytes), "r"(SmemAddr(bar))
+               : "memory");
+}
+
+// D += A B with A (128 x 16) in TMEM: lane = row, two 16-bit values per column.
+__device__ __forceinline__ void UmmaTmemA(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum)
+      : "memory");
+}
+__device__ __forceinline__ void TmemStore16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void TmemStore32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void TmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t Pack2(float lo, float hi) {
+  uint32_t r;
+  if (kBf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    r = *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    r = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return r;
+}
+template <bool kBf16>
+__device__ __forceinline__ float2 Unpack2(uint32_t r) {
+  if (kBf16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r));
+  return __half22float2(*reinterpret_cast<const __half2*>(&r));
+}
+
+// Instruction descriptor of a 128 x n product with fp32 accumulators; b_mn: B is MN-major.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t InstrDesc(int n, bool b_mn) {
+  return (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+
+// [128 x d] x [128 x d]^T: both operands K-major in shared memory, boxes of 64 columns.
+template <bool kBf16>
+__device__ __forceinline__ void IssueScores(uint32_t tmem_d, uint32_t a_addr, uint32_t b_addr, int ksteps) {
+  const uint64_t a = SmemDescSw128(a_addr), b = SmemDescSw128(b_addr);
+  const uint32_t idesc = InstrDesc<kBf16>(kTile, false);
+#pragma unroll 4
+  for (int k = 0; k < ksteps; ++k) {
+    const uint32_t off = (k >> 2) * (kBoxBytes >> 4) + (k & 3) * 2;
+    UmmaBf16(tmem_d, a + off, b + off, idesc, k > 0);
+  }
+}
+// [128 x 128] (16-bit, TMEM) x [128 x n]: B MN-major in shared memory.  The 128 columns of A lie in two runs of 32 TMEM
+// columns, `gap` columns apart.
+template <bool kBf16>
+__device__ __forceinline__ void IssueFromTmem(uint32_t tmem_d, uint32_t tmem_a, uint32_t gap, uint32_t b_addr, int n, bool accum) {
+  const uint64_t b     = SmemDescMnSw128(b_addr, kBoxBytes);
+  const uint32_t idesc = InstrDesc<kBf16>(n, true);
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    UmmaTmemA(tmem_d, tmem_a + (k >> 2) * gap + (k & 3) * 8, b + 128 * k, idesc, accum || k > 0);
+}
+
+// Clears rows [first, 128) of a tile of `boxes` boxes (a whole warp; the swizzle stays within a row's 128 bytes) and
+// orders the writes before the MMAs that follow.
+__device__ __forceinline__ void ClearRows(uint8_t* tile, int boxes, int first) {
+  const int lane = threadIdx.x & 31;
+  for (int x = 0; x < boxes; ++x)
+    for (int i = first * 8 + lane; i < kTile * 8; i += 32)
+      *reinterpret_cast<uint4*>(tile + x * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void StoreCols32(uint16_t* row, int col0, int d, const uint32_t (&acc)[32], float factor) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    if (col0 + g * 8 >= d) break;  // d is a multiple of 8
+    uint4 v;
+    v.x = Pack2<kBf16>(__uint_as_float(acc[g * 8 + 0]) * factor, __uint_as_float(acc[g * 8 + 1]) * factor);
+    v.y = Pack2<kBf16>(__uint_as_float(acc[g * 8 + 2]) * factor, __uint_as_float(acc[g * 8 + 3]) * factor);
+    v.z = Pack2<kBf16>(__uint_as_float(acc[g * 8 + 4]) * factor, __uint_as_float(acc[g * 8 + 5]) * factor);
+    v.w = Pack2<kBf16>(__uint_as_float(acc[g * 8 + 6]) * factor, __uint_as_float(acc[g * 8 + 7]) * factor);
+    *reinterpret_cast<uint4*>(row + col0 + g * 8) = v;
+  }
+}
+__device__ __forceinline__ void StoreZeroRow(uint16_t* row, int c0, int c1) {
+  for (int c = c0; c < c1; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+}
+
+__device__ __forceinline__ float Exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint8_t* AlignedSmem(uint8_t* raw) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+}
+
+// ---------------------------------------------------------------- forward
+// A CTA takes 256 queries of one head as two tiles, a softmax warpgroup for each, and streams the keys and values: while one
+// warpgroup computes probabilities, the tensor cores run the products of the other.  A thread owns a row, so maximum and sum
+// need no exchange.
+template <int HD>
+struct FwdCfg {
+  static constexpr int kTileBytes = (HD / 64) * kBoxBytes;
+  static constexpr int kStages    = HD == 64 ? 6 : 4;  // tiles of K and V in turn
+  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 1024 + 256;
+};
+
+template <int HD, bool kBf16>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
+  using Cfg = FwdCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem_q   = AlignedSmem(smem_raw);
+  uint8_t* ring     = smem_q + 2 * Cfg::kTileBytes;
+  uint64_t* full    = reinterpret_cast<uint64_t*>(ring + Cfg::kStages * Cfg::kTileBytes);
+  uint64_t* empty   = full + Cfg::kStages;
+  uint64_t* q_full  = empty + Cfg::kStages;  // [1]
+  uint64_t* s_full  = q_full + 1;            // [2] scores of a tile are in TMEM
+  uint64_t* p_full  = s_full + 2;            // [2] its probabilities are
+  uint64_t* o_full  = p_full + 2;            // [2] the last product of a tile has completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // causal: the tiles with the most keys first; otherwise neighbours share a head's keys
+  const int blocks_q = TilesOf(p.s, 2 * kTile);
+  const int heads    = p.b * p.h;
+  const int qb = p.causal ? blocks_q - 1 - static_cast<int>(blockIdx.x) / heads : static_cast<int>(blockIdx.x) % blocks_q;
+  const int bh = p.causal ? static_cast<int>(blockIdx.x) % heads : static_cast<int>(blockIdx.x) / blocks_q;
+  const int b = bh / p.h, h = bh % p.h, hk = h / (p.h / p.hk);
+  const int q0  = qb * 2 * kTile;
+  const int len = SeqLen(p, b);
+  const int tiles = TilesOf(len, kTile);
+  int count[2];  // key tiles of either query tile
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int first = q0 + i * kTile;
+    count[i] = first >= len ? 0 : p.causal ? min(tiles, first / kTile + 1) : tiles;
+  }
+  const int total = max(count[0], count[1]);
+
+  if (total > 0) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < Cfg::kStages; ++s) {
+        MbarInit(&full[s], 1);
+        MbarInit(&empty[s], 1);
+      }
+      MbarInit(q_full, 1);
+      for (int i = 0; i < 2; ++i) {
+        MbarInit(&s_full[i], 1);
+        MbarInit(&p_full[i], 4);
+        MbarInit(&o_full[i], 1);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAddr(tmem_slot)), "r"(512u)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    TcFenceBefore();
+  }
+  __syncthreads();
+  uint32_t tmem = 0;
+  if (total > 0) {
+    TcFenceAfter();
+    tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  }
+  // columns: scores of either tile (their probabilities in the same place), then either output
+  const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + HD};
+
+  if (warp == kTmaWarp) {
+    if (total > 0 && ElectOne()) {
+      MbarExpectTx(q_full, 2 * Cfg::kTileBytes);
+      TmaLoadTile<HD>(smem_q, &maps.q, q0, h, b, q_full);
+      TmaLoadTile<HD>(smem_q + Cfg::kTileBytes, &maps.q, q0 + kTile, h, b, q_full);
+      for (int e = 0; e < 2 * total; ++e) {
+        const int st = e % Cfg::kStages;
+        if (!MbarWait(&empty[st], ((e / Cfg::kStages) & 1) ^ 1)) {
+          atomicExch(&g_attn_error, 1);
+          break;
+        }
+        MbarExpectTx(&full[st], Cfg::kTileBytes);
+        TmaLoadTile<HD>(ring + st * Cfg::kTileBytes, e & 1 ? &maps.v : &maps.k, (e >> 1) * kTile, hk, b, &full[st]);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (total > 0) {
+      const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity) {
+        if (ok && !MbarWaitWarp(bar, parity)) {
+          if (lane == 0) atomicExch(&g_attn_error, 2);
+          ok = false;
+        }
+        TcFenceAfter();
+        return ok;
+      };
+      auto entry = [&](int e) { return wait(&full[e % Cfg::kStages], (e / Cfg::kStages) & 1); };
+      auto tile  = [&](int e) { return ring + (e % Cfg::kStages) * Cfg::kTileBytes; };
+      if (wait(q_full, 0) && entry(0)) {
+        if (ElectOne()) {
+          for (int i = 0; i < 2; ++i)
+            if (count[i] > 0) {
+              IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(0)), ksteps);
+              UmmaCommit(&s_full[i]);
+            }
+          UmmaCommit(&empty[0]);
+        }
+        for (int j = 0; j < total && ok; ++j) {
+          const int ev = 2 * j + 1, ek = 2 * j + 2;
+          if (!entry(ev)) break;
+          if (j == tiles - 1 && len < p.s && len % kTile != 0) ClearRows(tile(ev), HD / 64, len % kTile);
+          if (j + 1 < total && !entry(ek)) break;
+          for (int i = 0; i < 2; ++i) {
+            if (j >= count[i]) continue;
+            if (!wait(&p_full[i], j & 1)) break;
+            if (ElectOne()) {
+              // the probabilities lie where the next scores go: products complete in the order of their issue
+              IssueFromTmem<kBf16>(t_o[i], t_s[i], 32, SmemAddr(tile(ev)), n_out, j > 0);
+              if (j + 1 < count[i]) {
+                IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(ek)), ksteps);
+                UmmaCommit(&s_full[i]);
+              } else {
+                UmmaCommit(&o_full[i]);
+              }
+            }
+          }
+          if (ok && ElectOne()) {
+            UmmaCommit(&empty[ev % Cfg::kStages]);
+            if (j + 1 < total) UmmaCommit(&empty[ek % Cfg::kStages]);
+          }
+        }
+      }
+    }
+  } else {
+    const int i = warp >> 2;             // query tile
+    const int quarter = warp & 3;        // TMEM lanes that this warp may access
+    const int row = q0 + i * kTile + quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and the sum
+    bool ok = true;
+    for (int j = 0; j < count[i]; ++j) {
+      if (!MbarWaitWarp(&s_full[i], j & 1)) {
+        if (lane == 0) atomicExch(&g_attn_error, 3);
+        ok = false;
+        break;
+      }
+      TcFenceAfter();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) TmemLoad32Async(t_s[i] + lanes + g * 32, s[g]);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) TmemLoadWait(s[g]);
+      const int kv0 = j * kTile;
+      if (kv0 + kTile > len || (p.causal && kv0 + kTile - 1 > q0 + i * kTile)) {
+        const int limit = (p.causal ? min(len, row + 1) : len) - kv0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (g * 32 + k >= limit) s[g][k] = 0xff800000u;  // -inf
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(s[g][k]));
+      if (top == -INFINITY) top = 0.f;
+      if (j == 0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, top > m)) {
+        const float up = fmaxf(top, m);
+        const float f  = Exp2((m - up) * p.c);
+        m = up;
+        l *= f;
+#pragma unroll 1
+        for (int g = 0; g < HD / 32; ++g) {
+          uint32_t o[32];
+          TmemLoad32(t_o[i] + lanes + g * 32, o);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          TmemStore32(t_o[i] + lanes + g * 32, o);
+        }
+      }
+      const float mc = m * p.c;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float x = Exp2(fmaf(__uint_as_float(s[g][2 * k]), p.c, -mc));
+          const float y = Exp2(fmaf(__uint_as_float(s[g][2 * k + 1]), p.c, -mc));
+          sum[0] += x;
+          sum[1] += y;
+          w[k] = Pack2<kBf16>(x, y);
+        }
+        TmemStore16(t_s[i] + lanes + g * 16, w);
+      }
+      l += sum[0] + sum[1];
+      TmemStoreWait();
+      TcFenceBefore();
+      __syncwarp();
+      if (lane == 0) MbarArrive(&p_full[i]);
+    }
+    if (count[i] > 0 && ok && !MbarWaitWarp(&o_full[i], 0)) {
+      if (lane == 0) atomicExch(&g_attn_error, 4);
+      ok = false;
+    }
+    TcFenceAfter();
+    if (ok) {
+      const bool live = row < len;
+      uint16_t* dst = static_cast<uint16_t*>(p.o) + b * p.so.b + row * p.so.s + h * p.so.h;
+      if (count[i] > 0) {
+        const float inv = 1.f / l;
+#pragma unroll 1
+        for (int g = 0; g < HD / 32; ++g) {
+          uint32_t o[32];
+          TmemLoad32(t_o[i] + lanes + g * 32, o);
+          if (live) StoreCols32<kBf16>(dst, g * 32, p.d, o, inv);
+        }
+      }
+      if (!live && row < p.s) StoreZeroRow(dst, 0, p.d);
+      if (row < p.sp) p.lse[static_cast<int64_t>(bh) * p.sp + row] = live ? fmaf(m, p.c, log2f(l)) : INFINITY;
+    }
+  }
+  TcFenceBefore();
+  __syncthreads();
+  if (warp == kMmaWarp && total > 0) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------- backward
+// D_i = dO_i . O_i, eight lanes per row; the heads of a position are neighbours, so contiguous tensors are read in order.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ AttnParams p) {
+  const int64_t rows = static_cast<int64_t>(p.b) * p.sp * p.h;
+  const int part = threadIdx.x & 7;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 32; r0 < rows; r0 += static_cast<int64_t>(gridDim.x) * 32) {
+    const int64_t r = r0 + (threadIdx.x >> 3);
+    const int h     = static_cast<int>(r % p.h);
+    const int i     = static_cast<int>(r / p.h % p.sp);
+    const int64_t b = r / p.h / p.sp;
+    float sum = 0.f;
+    if (r < rows && i < SeqLen(p, static_cast<int>(b))) {
+      const uint16_t* o  = static_cast<const uint16_t*>(p.o) + b * p.so.b + i * p.so.s + h * p.so.h;
+      const uint16_t* g  = static_cast<const uint16_t*>(p.dout) + b * p.sdo.b + i * p.sdo.s + h * p.sdo.h;
+      for (int c = part * 8; c < p.d; c += 64) {
+        const uint4 x = *reinterpret_cast<const uint4*>(o + c), y = *reinterpret_cast<const uint4*>(g + c);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 u = Unpack2<kBf16>(xs[k]), v = Unpack2<kBf16>(ys[k]);
+          sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 4; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    if (part == 0 && r < rows) p.delta[(b * p.h + h) * p.sp + i] = sum;
+  }
+}
+
+// One tile of 128 keys (kKeys) or queries (!kKeys) stays, the tiles of the other side stream past it:
+//             stays (X1, X2)   streams (Y1, Y2)   S = X1 Y1^T, dP = X2 Y2^T       accumulated
+//   kKeys     K, V             Q, dO              rows are keys: P^T and dS^T     dV += P^T dO,  dK += dS^T Q
+//   !kKeys    Q, dO            K, V               rows are queries                dQ += dS K
+// Both passes compute S and dP, seven products instead of five, and in exchange every sum has one owner: no atomics, no
+// fp32 copy of dQ in memory, and results that do not depend on the order of the blocks.
+// The softmax warps take S of a tile, then its dP; while they work on one, the tensor cores run the products that the
+// other has released and the next tile's.
+template <int HD>
+struct BwdCfg {
+  static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;
+  static constexpr int kStages     = HD == 64 ? 4 : 2;
+  static constexpr int kStageBytes = 2 * kTileBytes;           // Y1, Y2
+  static constexpr int kRowBytes   = 2 * kTile * 4;            // L and D of a streamed tile of queries
+  static constexpr int kSmemBytes  = 2 * kTileBytes + kStages * (kStageBytes + kRowBytes) + 1024 + 256;
+};
+
+template <int HD, bool kBf16, bool kKeys>
+__device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnParams& p, int tile, int b, int head, uint8_t* smem) {
+  using Cfg = BwdCfg<HD>;
+  uint8_t* x1     = smem;
+  uint8_t* x2     = x1 + Cfg::kTileBytes;
+  uint8_t* ring   = x2 + Cfg::kTileBytes;
+  float* ld       = reinterpret_cast<float*>(ring + Cfg::kStages * Cfg::kStageBytes);
+  uint64_t* full  = reinterpret_cast<uint64_t*>(ld + Cfg::kStages * 2 * kTile);
+  uint64_t* empty = full + Cfg::kStages;
+  uint64_t* x_full   = empty + Cfg::kStages;
+  uint64_t* s_full   = x_full + 1;    // S of a tile is in TMEM
+  uint64_t* s_done   = s_full + 1;    // keys: P has taken its place; queries: S has been read
+  uint64_t* dp_full  = s_done + 1;    // dP is in TMEM
+  uint64_t* ds_full  = dp_full + 1;   // dS has taken its place
+  uint64_t* acc_full = ds_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.h / p.hk;
+  const int x0    = tile * kTile;
+  const int len   = SeqLen(p, b);
+  const int tiles = TilesOf(len, kTile);
+  // streamed tiles: [first, last) of each of `heads` heads, starting at head `head0`
+  const int first = kKeys && p.causal ? tile : 0;
+  const int last  = !kKeys && p.causal ? min(tiles, tile + 1) : tiles;
+  const int per   = last - first;
+  const int total = x0 >= len ? 0 : per * (kKeys ? group : 1);
+  const int xhead = head, yhead = kKeys ? head * group : head / group;
+
+  if (total > 0) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < Cfg::kStages; ++s) {
+        MbarInit(&full[s], 1);
+        MbarInit(&empty[s], 1);
+      }
+      MbarInit(x_full, 1);
+      MbarInit(s_full, 1);
+      MbarInit(s_done, 8);
+      MbarInit(dp_full, 1);
+      MbarInit(ds_full, 8);
+      MbarInit(acc_full, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAddr(tmem_slot)), "r"(512u)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    TcFenceBefore();
+  }
+  __syncthreads();
+  uint32_t tmem = 0;
+  if (total > 0) {
+    TcFenceAfter();
+    tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  }
+  const uint32_t t_s = tmem, t_dp = tmem + 128, t_acc1 = tmem + 256, t_acc2 = tmem + 256 + HD;
+  // a half's 16-bit values start where its 64 fp32 columns do
+  constexpr uint32_t kGap = 64;
+
+  if (warp == kTmaWarp) {
+    if (total > 0 && ElectOne()) {
+      MbarExpectTx(x_full, 2 * Cfg::kTileBytes);
+      TmaLoadTile<HD>(x1, kKeys ? &maps.k : &maps.q, x0, xhead, b, x_full);
+      TmaLoadTile<HD>(x2, kKeys ? &maps.v : &maps.dout, x0, xhead, b, x_full);
+      for (int it = 0; it < total; ++it) {
+        const int st = it % Cfg::kStages;
+        if (!MbarWait(&empty[st], ((it / Cfg::kStages) & 1) ^ 1)) {
+          atomicExch(&g_attn_error, 5);
+          break;
+        }
+        const int y0 = (first + it % per) * kTile, yh = yhead + it / per;
+        MbarExpectTx(&full[st], Cfg::kStageBytes + (kKeys ? Cfg::kRowBytes : 0));
+        uint8_t* dst = ring + st * Cfg::kStageBytes;
+        TmaLoadTile<HD>(dst, kKeys ? &maps.q : &maps.k, y0, yh, b, &full[st]);
+        TmaLoadTile<HD>(dst + Cfg::kTileBytes, kKeys ? &maps.dout : &maps.v, y0, yh, b, &full[st]);
+        if (kKeys) {
+          const int64_t at = (static_cast<int64_t>(b) * p.h + yh) * p.sp + y0;
+          BulkLoad(ld + st * 2 * kTile, p.lse + at, kTile * 4, &full[st]);
+          BulkLoad(ld + st * 2 * kTile + kTile, p.delta + at, kTile * 4, &full[st]);
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (total > 0) {
+      const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
+      const bool ragged = len < p.s && len % kTile != 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity) {
+        if (ok && !MbarWaitWarp(bar, parity)) {
+          if (lane == 0) atomicExch(&g_attn_error, 6);
+          ok = false;
+        }
+        TcFenceAfter();
+        return ok;
+      };
+      auto y1 = [&](int it) { return ring + (it % Cfg::kStages) * Cfg::kStageBytes; };
+      auto arrived = [&](int it) {
+        if (!wait(&full[it % Cfg::kStages], (it / Cfg::kStages) & 1)) return false;
+        if (ragged && first + it % per == tiles - 1) ClearRows(y1(it), 2 * (HD / 64), len % kTile);
+        return true;
+      };
+      auto issue_s = [&](int it) {
+        if (ElectOne()) {
+          IssueScores<kBf16>(t_s, SmemAddr(x1), SmemAddr(y1(it)), ksteps);
+          UmmaCommit(s_full);
+        }
+      };
+      auto issue_dp = [&](int it) {
+        if (ElectOne()) {
+          IssueScores<kBf16>(t_dp, SmemAddr(x2), SmemAddr(y1(it) + Cfg::kTileBytes), ksteps);
+          UmmaCommit(dp_full);
+        }
+      };
+      if (wait(x_full, 0) && arrived(0)) {
+        issue_s(0);
+        issue_dp(0);
+        for (int it = 0; it < total && ok; ++it) {
+          if (!wait(s_done, it & 1)) break;
+          if (kKeys && ElectOne())
+            IssueFromTmem<kBf16>(t_acc2, t_s, kGap, SmemAddr(y1(it) + Cfg::kTileBytes), n_out, it > 0);
+          if (it + 1 < total) {
+            if (!arrived(it + 1)) break;
+            issue_s(it + 1);
+          }
+          if (!wait(ds_full, it & 1)) break;
+          if (ElectOne()) {
+            IssueFromTmem<kBf16>(t_acc1, t_dp, kGap, SmemAddr(y1(it)), n_out, it > 0);
+            UmmaCommit(&empty[it % Cfg::kStages]);
+          }
+          if (it + 1 < total) issue_dp(it + 1);
+        }
+        if (ok && ElectOne()) UmmaCommit(acc_full);
+      }
+    }
+  } else {
+    const int quarter = warp & 3, half = warp >> 2;  // TMEM lanes; columns [64 half, 64 half + 64)
+    const int row = x0 + quarter * 32 + lane;
+    const uint32_t at = (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
+    float row_l = 0.f, row_d = 0.f;
+    if (!kKeys && total > 0) {  // row < sp
+      const int64_t i = (static_cast<int64_t>(b) * p.h + head) * p.sp + row;
+      row_l = p.lse[i];
+      row_d = p.delta[i];
+    }
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int parity) {
+      if (ok && !MbarWaitWarp(bar, parity)) {
+        if (lane == 0) atomicExch(&g_attn_error, 7);
+        ok = false;
+      }
+      TcFenceAfter();
+      return ok;
+    };
+    for (int it = 0; it < total; ++it) {
+      const int st = it % Cfg::kStages;
+      const int y0 = (first + it % per) * kTile;
+      if (kKeys && !wait(&full[st], (it / Cfg::kStages) & 1)) break;  // L and D
+      if (!wait(s_full, it & 1)) break;
+      uint32_t s[2][32];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) TmemLoad32Async(t_s + at + g * 32, s[g]);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) TmemLoadWait(s[g]);
+      if (!kKeys) {
+        TcFenceBefore();
+        __syncwarp();
+        if (lane == 0) MbarArrive(s_done);
+      }
+      const float* ls = ld + st * 2 * kTile + half * 64;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          float4 l4;
+          if (kKeys) l4 = *reinterpret_cast<const float4*>(ls + g * 32 + k);
+          else l4 = make_float4(row_l, row_l, row_l, row_l);
+          s[g][k]     = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k]), p.c, -l4.x)));
+          s[g][k + 1] = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k + 1]), p.c, -l4.y)));
+          s[g][k + 2] = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k + 2]), p.c, -l4.z)));
+          s[g][k + 3] = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k + 3]), p.c, -l4.w)));
+        }
+      if (kKeys) {
+        if (p.causal && y0 == x0) {  // a key counts for the queries from its own position on
+          const int from = row - y0 - half * 64;
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (g * 32 + k < from) s[g][k] = 0u;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            w[k] = Pack2<kBf16>(__uint_as_float(s[g][2 * k]), __uint_as_float(s[g][2 * k + 1]));
+          TmemStore16(t_s + at + g * 16, w);
+        }
+        TmemStoreWait();
+        TcFenceBefore();
+        __syncwarp();
+        if (lane == 0) MbarArrive(s_done);
+      } else if (y0 + kTile > len || (p.causal && y0 == x0)) {
+        const int limit = (p.causal ? min(len, row + 1) : len) - y0 - half * 64;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (g * 32 + k >= limit) s[g][k] = 0u;
+      }
+      if (!wait(dp_full, it & 1)) break;
+      uint32_t t[2][32];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) TmemLoad32Async(t_dp + at + g * 32, t[g]);
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        TmemLoadWait(t[g]);
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          float4 d4;
+          if (kKeys) d4 = *reinterpret_cast<const float4*>(ls + kTile + g * 32 + k);
+          else d4 = make_float4(row_d, row_d, row_d, row_d);
+          const float a0 = __uint_as_float(s[g][k]) * (__uint_as_float(t[g][k]) - d4.x);
+          const float a1 = __uint_as_float(s[g][k + 1]) * (__uint_as_float(t[g][k + 1]) - d4.y);
+          const float a2 = __uint_as_float(s[g][k + 2]) * (__uint_as_float(t[g][k + 2]) - d4.z);
+          const float a3 = __uint_as_float(s[g][k + 3]) * (__uint_as_float(t[g][k + 3]) - d4.w);
+          w[k / 2]     = Pack2<kBf16>(a0, a1);
+          w[k / 2 + 1] = Pack2<kBf16>(a2, a3);
+        }
+        TmemStore16(t_dp + at + g * 16, w);
+      }
+      TmemStoreWait();
+      TcFenceBefore();
+      __syncwarp();
+      if (lane == 0) MbarArrive(ds_full);
+    }
+    if (total > 0) wait(acc_full, 0);
+    if (ok) {
+      const bool live = row < len;
+      const int c0 = half * (HD / 2);
+      const uint32_t acc_at = (static_cast<uint32_t>(quarter * 32) << 16) + c0;
+#pragma unroll
+      for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
+        const Strides& st = out ? p.sdv : kKeys ? p.sdk : p.sdq;
+        uint16_t* dst = static_cast<uint16_t*>(out ? p.dv : kKeys ? p.dk : p.dq) + b * st.b + row * st.s + head * st.h;
+        if (total > 0) {
+#pragma unroll 1
+          for (int g = 0; g < HD / 64; ++g) {
+            uint32_t o[32];
+            TmemLoad32((out ? t_acc2 : t_acc1) + acc_at + g * 32, o);
+            if (live) StoreCols32<kBf16>(dst, c0 + g * 32, p.d, o, out ? 1.f : p.scale);
+          }
+        }
+        if (!live && row < p.s) StoreZeroRow(dst, c0, min(p.d, c0 + HD / 2));
+      }
+    }
+  }
+  TcFenceBefore();
+  __syncthreads();
+  if (warp == kMmaWarp && total > 0) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// Both passes in one launch, so that neither leaves a tail of idle SMs: first the blocks of the keys, whose tiles stream past
+// every query head of their group.  Causal: the tiles with the longest streams first.
+template <int HD, bool kBf16>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem   = AlignedSmem(smem_raw);
+  const int tiles = p.sp / kTile;
+  int i = blockIdx.x;
+  if (i < tiles * p.b * p.hk) {
+    const int heads = p.b * p.hk;
+    const int tile  = p.causal ? i / heads : i % tiles, bh = p.causal ? i % heads : i / tiles;
+    AttnBwdTile<HD, kBf16, true>(maps, p, tile, bh / p.hk, bh % p.hk, smem);
+  } else {
+    i -= tiles * p.b * p.hk;
+    const int heads = p.b * p.h;
+    const int tile  = p.causal ? tiles - 1 - i / heads : i % tiles, bh = p.causal ? i % heads : i / tiles;
+    AttnBwdTile<HD, kBf16, false>(maps, p, tile, bh / p.h, bh % p.h, smem);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+
+// One head-split tensor [b, s, heads, d] with any strides that are multiples of 16 bytes; boxes of 64 columns x 128 positions.
+int HeadMap(CUtensorMap* out, const void* base, int dtype, int b, int s, int heads, int d, const Strides& st) {
+  EncodeFn enc = GetEncodeFn();
+  if (!enc) return SetError(-7, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[4]    = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(s), static_cast<cuuint64_t>(heads),
+                           static_cast<cuuint64_t>(b)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(st.s) * 2, static_cast<cuuint64_t>(st.h) * 2,
+                           static_cast<cuuint64_t>(st.b) * 2};
+  cuuint32_t box[4]     = {64, kTile, 1, 1};
+  cuuint32_t estr[4]    = {1, 1, 1, 1};
+  CUresult r = enc(out, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return SetError(-7, "attention: cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return 0;
+}
+
+bool Aligned(const void* base, const Strides& st) {
+  return reinterpret_cast<uintptr_t>(base) % 16 == 0 && st.b % 8 == 0 && st.s % 8 == 0 && st.h % 8 == 0;
+}
+// What a tensor map can express on top: every stride a positive number of bytes below 2^40.
+bool Mappable(const Strides& st) {
+  for (int64_t v : {st.b, st.s, st.h})
+    if (v <= 0 || v >= (int64_t{1} << 39)) return false;
+  return true;
+}
+
+// Raises a kernel's limit of dynamic shared memory once per device.
+template <typename Kernel>
+int AllowSmem(Kernel* kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  TIPSK_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? uint64_t{1} << dev : 0;
+  if (bit && (done->load(std::memory_order_acquire) & bit)) return 0;
+  TIPSK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done->fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+
+int CheckSizes(int b, int s, int h, int hk, int d, int dtype, float scale) {
+  TIPSK_REQUIRE(dtype == kBF16 || dtype == kF16, "attention: bf16 or fp16");
+  TIPSK_REQUIRE(b > 0 && s > 0 && h > 0 && hk > 0 && h % hk == 0, "attention: empty shape, or heads that kv_heads does not divide");
+  TIPSK_REQUIRE(d > 0 && d <= 128 && d % 8 == 0, "attention: the head size must be a multiple of 8 up to 128");
+  TIPSK_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), "attention: scale must be positive and finite");
+  TIPSK_REQUIRE(s <= (1 << 30) && static_cast<int64_t>(b) * (h + hk) * TilesOf(s, kTile) < (int64_t{1} << 31),
+                "attention: too many tiles for one launch");
+  return 0;
+}
+
+Strides Take(const int64_t* host, int i) { return Strides{host[3 * i], host[3 * i + 1], host[3 * i + 2]}; }
+
+AttnParams MakeParams(const void* lengths, int len64, int b, int s, int h, int hk, int d, float scale, int causal) {
+  AttnParams p{};
+  p.lengths = lengths;
+  p.len64   = len64;
+  p.b = b; p.s = s; p.h = h; p.hk = hk; p.d = d;
+  p.sp      = TilesOf(s, kTile) * kTile;
+  p.causal  = causal ? 1 : 0;
+  p.scale   = scale;
+  p.c       = scale * kLog2e;
+  return p;
+}
+
+template <int HD, bool kBf16>
+int LaunchFwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  int rc = AllowSmem(AttnFwdKernel<HD, kBf16>, FwdCfg<HD>::kSmemBytes, &done);
+  if (rc) return rc;
+  const int grid = TilesOf(p.s, 2 * kTile) * p.b * p.h;
+  AttnFwdKernel<HD, kBf16><<<grid, kAttnThreads, FwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  TIPSK_LAUNCH_CHECK();
+  return 0;
+}
+
+template <int HD, bool kBf16>
+int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  int rc = AllowSmem(AttnBwdKernel<HD, kBf16>, BwdCfg<HD>::kSmemBytes, &done);
+  if (rc) return rc;
+  const int64_t rows = static_cast<int64_t>(p.b) * p.sp * p.h;
+  const int64_t cap  = static_cast<int64_t>(NumSMs()) * 16;
+  AttnDeltaKernel<kBf16><<<static_cast<int>(rows / 32 < cap ? rows / 32 : cap), 256, 0, s>>>(p);  // sp: whole tiles
+  TIPSK_LAUNCH_CHECK();
+  const int grid = (p.sp / kTile) * p.b * (p.h + p.hk);
+  AttnBwdKernel<HD, kBf16><<<grid, kAttnThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  TIPSK_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace
+}  // namespace tipsk
+
+using namespace tipsk;
+
+extern "C" {
+
+/* O = softmax(scale Q K^T + mask) V and L.  host_strides: q, k, v, out. */
+int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const void* lengths, int len64,
+                        int b, int s, int h, int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal,
+                        void* stream) {
+  int rc = CheckSizes(b, s, h, hk, d, dtype, scale);
+  if (rc) return rc;
+  const Strides sq = Take(host_strides, 0), sk = Take(host_strides, 1), sv = Take(host_strides, 2);
+  AttnParams p = MakeParams(lengths, len64, b, s, h, hk, d, scale, causal);
+  p.so  = Take(host_strides, 3);
+  p.o   = out;
+  p.lse = lse;
+  TIPSK_REQUIRE(Aligned(q, sq) && Aligned(k, sk) && Aligned(v, sv) && Aligned(out, p.so),
+                "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");
+  TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv), "attention: strides of q, k and v must be positive");
+  AttnMaps maps;
+  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq))) return rc;
+  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk))) return rc;
+  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv))) return rc;
+  maps.dout = maps.q;  // not read
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == kBF16) return d <= 64 ? LaunchFwd<64, true>(maps, p, st) : LaunchFwd<128, true>(maps, p, st);
+  return d <= 64 ? LaunchFwd<64, false>(maps, p, st) : LaunchFwd<128, false>(maps, p, st);
+}
+
+/* Gradients from dO, the inputs, O and L of the forward pass.  host_strides: q, k, v, out, dout, dq, dk, dv. */
+int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                        float* delta, void* dq, void* dk, void* dv, const void* lengths, int len64, int b, int s, int h,
+                        int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal, void* stream) {
+  int rc = CheckSizes(b, s, h, hk, d, dtype, scale);
+  if (rc) return rc;
+  const Strides sq = Take(host_strides, 0), sk = Take(host_strides, 1), sv = Take(host_strides, 2);
+  AttnParams p = MakeParams(lengths, len64, b, s, h, hk, d, scale, causal);
+  p.so    = Take(host_strides, 3);
+  p.sdo   = Take(host_strides, 4);
+  p.sdq   = Take(host_strides, 5);
+  p.sdk   = Take(host_strides, 6);
+  p.sdv   = Take(host_strides, 7);
+  p.o     = const_cast<void*>(out);
+  p.dout  = dout;
+  p.lse   = const_cast<float*>(lse);
+  p.delta = delta;
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  TIPSK_REQUIRE(Aligned(q, sq) && Aligned(k, sk) && Aligned(v, sv) && Aligned(out, p.so) && Aligned(dout, p.sdo) &&
+                    Aligned(dq, p.sdq) && Aligned(dk, p.sdk) && Aligned(dv, p.sdv),
+                "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");
+  TIPSK_REQUIRE(reinterpret_cast<uintptr_t>(lse) % 16 == 0 && reinterpret_cast<uintptr_t>(delta) % 16 == 0,
+                "attention: lse and delta must be 16-byte aligned");
+  TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.sdo), "attention: strides must be positive");
+  AttnMaps maps;
+  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq))) return rc;
+  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk))) return rc;
+  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv))) return rc;
+  if ((rc = HeadMap(&maps.dout, dout, dtype, b, s, h, d, p.sdo))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == kBF16) return d <= 64 ? LaunchBwd<64, true>(maps, p, st) : LaunchBwd<128, true>(maps, p, st);
+  return d <= 64 ? LaunchBwd<64, false>(maps, p, st) : LaunchBwd<128, false>(maps, p, st);
+}
+
+/* Reads and clears the attention error word of the current device (0: ok). Synchronises. */
+int tipsk_attention_status(void) {
+  int32_t v = 0;
+  const int32_t zero = 0;
+  if (cudaMemcpyFromSymbol(&v, g_attn_error, sizeof(v)) != cudaSuccess) return -7;
+  if (v && cudaMemcpyToSymbol(g_attn_error, &zero, sizeof(zero)) != cudaSuccess) return -7;
+  return v;
+}
+
+}  // extern "C"

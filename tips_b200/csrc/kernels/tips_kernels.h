@@ -224,6 +224,18 @@ int tipsk_gemm_bf16_tt(const void* a, const void* b, void* c, int m, int n, int 
                        void* stream);
 int tipsk_gemm_status(void);
 
+/* ---- self-attention (attention.cu): q [b, s, h, d], k and v [b, s, hk, d], bf16 or fp16, d a multiple of 8 up to 128.
+ * host_strides: (batch, position, head) in elements for every tensor in the order of the arguments that have a head axis,
+ * multiples of 8; the last axis is contiguous.  lengths: [b] int32 (len64 = 0) or int64, or null: positions from a
+ * sequence's length on neither count nor receive anything but zeros.  lse, delta: fp32 [b, h, s rounded up to 128]. ---- */
+int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const void* lengths, int len64,
+                        int b, int s, int h, int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal,
+                        void* stream);
+int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                        float* delta, void* dq, void* dk, void* dv, const void* lengths, int len64, int b, int s, int h,
+                        int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal, void* stream);
+int tipsk_attention_status(void);
+
 /* ---- 3x3 / stride 2 / pad 1 max pooling on NHWC (pool.cu); idx holds the argmax position 0..8 per output ---- */
 /* Global average pooling on NHWC (x [n, hw, c] -> y [n, c]) and its backward (pool.cu). */
 int tipsk_global_avgpool_fwd(const void* x, void* y, int n, int hw, int c, int dtype, void* stream);

@@ -4,7 +4,8 @@ FFN 4096, vocab 30522, sequence 512 by default).
 The reference does not contain the model (it trains TensorFlow models through its collective mode);
 this is the second data-parallel benchmark workload.  Linear layers run on the tcgen05 GEMM with bias and
 GELU fused into the epilogue, layer norms and the softmax cross-entropy are the fused kernels of this
-package (the input embedding as well), the attention core is the library scaled-dot-product attention.
+package (the input embedding as well), the attention core is the library scaled-dot-product attention, or this package's own
+for padded batches.
 """
 from __future__ import annotations
 
@@ -33,11 +34,11 @@ class BertLayer(nn.Module):
         self.fc2 = Linear(ffn, hidden)
         self.ln2 = LayerNorm(hidden, eps=1e-12)
 
-    def forward(self, x):
+    def forward(self, x, lengths=None):
         # the residual adds are fused into the layer norms; in backward the gradient of each block input is summed
         # inside the GEMM that produces its second term (the "passthrough" linears)
         qkv, x = self.qkv(x, passthrough=True)
-        att = packed_attention(qkv, self.heads)
+        att = packed_attention(qkv, self.heads, lengths=lengths)
         x = self.ln1(self.proj(att), residual=x)
         h, x = self.fc1(x, passthrough=True)
         return self.ln2(self.fc2(h), residual=x)
@@ -63,7 +64,7 @@ class BertMLM(nn.Module):
             if isinstance(m, Linear):
                 nn.init.normal_(m.weight, std=0.02)
 
-    def encode(self, ids):
+    def encode(self, ids, lengths=None):
         if _TORCH_EMBED:  # TIPS_BERT_TORCH_EMBED=1: torch's embedding kernels, kept for A/B measurements
             pos = torch.arange(ids.shape[1], device=ids.device)
             x = self.tok(ids) + self.pos(pos)[None] + self.typ.weight[0]
@@ -71,12 +72,13 @@ class BertMLM(nn.Module):
             x = embed_sum(ids, self.tok.weight, self.pos.weight, self.typ.weight[0])
         x = self.ln_emb(x)
         for layer in self.layers:
-            x = layer(x)
+            x = layer(x, lengths)
         return x
 
-    def loss(self, ids, masked_positions, masked_labels):
-        """ids [B, S]; masked_positions [B, P] indices into S; masked_labels [B, P] (-100 = unused slot)."""
-        x = self.encode(ids)
+    def loss(self, ids, masked_positions, masked_labels, lengths=None):
+        """ids [B, S]; masked_positions [B, P] indices into S; masked_labels [B, P] (-100 = unused slot); lengths [B]: of a
+        padded batch, positions from a sequence's length on are not attended to (their ids must still be valid)."""
+        x = self.encode(ids, lengths)
         b, p = masked_positions.shape
         picked = torch.gather(x, 1, masked_positions[..., None].expand(b, p, x.shape[-1])).reshape(b * p, -1)
         hcur = self.head_ln(self.head_dense(picked))

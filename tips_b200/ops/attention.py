@@ -1,16 +1,21 @@
-"""Self-attention on a packed QKV projection without layout glue.
+"""Self-attention without layout glue.
+
+``attention(q, k, v)`` is this package's own attention (csrc/kernels/attention.cu): causal or padded batches, shared key and
+value heads, forward and a backward pass that recomputes the probabilities.
 
 ``packed_attention(qkv, heads)`` takes the output of the fused QKV linear layer, ``[batch, seq, 3 * hidden]``, and
-returns ``[batch, seq, hidden]``.  The attention itself is the library's fused scaled-dot-product attention (the
+returns ``[batch, seq, hidden]``.  With ``kv_heads``, ``lengths`` or ``scale`` it runs ``attention`` on views of the packed
+tensor.  Without them the attention itself is the library's fused scaled-dot-product attention (the
 reference has no attention at all; its models are TensorFlow's), but everything around it is done here so that
 no tensor is re-laid by generic strided copies: q, k and v are strided views of the packed tensor, the output and
-the incoming gradient change layout with one vectorised pass of ``tipsk_copy4d`` each, and the three gradients
+the incoming gradient change layout with one vectorised pass of ``tipsk_copy4d`` each.  Either way the three gradients
 are written straight into one packed ``[batch, seq, 3, heads, d]`` buffer (instead of three zero-filled tensors that
 autograd then sums).
 """
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 import torch.nn.functional as F
@@ -71,8 +76,199 @@ class _PackedAttentionFn(torch.autograd.Function):
         return dqkv.view(b, s, 3 * heads * d), None, None
 
 
-def packed_attention(qkv: torch.Tensor, heads: int, causal: bool = False) -> torch.Tensor:
-    """Multi-head self-attention on ``qkv = [batch, seq, 3 * hidden]`` (q, k, v concatenated on the last axis)."""
+def _check_lengths(lengths, b: int, device) -> None:
+    if lengths is None:
+        return
+    if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError("lengths must be an int32 or int64 tensor")
+    if tuple(lengths.shape) != (b,):
+        raise ValueError(f"lengths must have one entry per sequence: shape ({b},), got {tuple(lengths.shape)}")
+    if lengths.device != device:
+        raise ValueError(f"lengths are on {lengths.device}, the inputs on {device}")
+
+
+def _check_attention(q, k, v, lengths, scale) -> float:
+    """Checks the arguments of `attention` and returns the scale to use."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [batch, seq, heads, head_size], got {tuple(t.shape)}")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise TypeError(f"q, k and v must share dtype and device: {name} is {t.dtype} on {t.device}, q {q.dtype} on {q.device}")
+    b, s, h, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
+        raise ValueError(f"k and v must be [{b}, {s}, kv_heads, {d}] like q, got {tuple(k.shape)} and {tuple(v.shape)}")
+    hk = k.shape[2]
+    if h == 0 or hk == 0 or h % hk != 0:
+        raise ValueError(f"{h} heads cannot share {hk} key and value heads evenly")
+    if d == 0:
+        raise ValueError("the head size must be positive")
+    _check_lengths(lengths, b, q.device)
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    scale = float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if q.is_cuda:
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"attention on a GPU takes bfloat16 or float16, got {q.dtype}")
+        if d % 8 != 0 or d > 128:
+            raise ValueError(f"attention on a GPU takes head sizes that are multiples of 8 up to 128, got {d}")
+    return scale
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy where the kernels cannot read it in place: they need a contiguous last axis, positive strides of whole
+    16 bytes and a 16-byte-aligned start."""
+    st = t.stride()
+    if t.data_ptr() % 16 == 0 and st[3] == 1 and all(x > 0 and x % 8 == 0 for x in st[:3]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(*tensors):
+    return base.i64_array([x for t in tensors for x in t.stride()[:3]])
+
+
+def _attention_fwd(q, k, v, lengths, scale, causal):
+    """(out, lse, and q, k, v as the kernel read them) for CUDA tensors."""
+    b, s, h, d = q.shape
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    out = torch.empty(b, s, h, d, dtype=q.dtype, device=q.device)
+    lse = torch.empty(b, h, -(-s // 128) * 128, dtype=torch.float32, device=q.device)
+    if out.numel() == 0:
+        return out, lse, q, k, v
+    with torch.cuda.device(q.device):
+        base.check(base.K().tipsk_attention_fwd(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), base.ptr(lengths),
+            int(lengths is not None and lengths.dtype == torch.int64), b, s, h, k.shape[2], d, base.code(q),
+            _strides(q, k, v, out), scale, int(causal), base.stream()), "attention_fwd")
+    return out, lse, q, k, v
+
+
+def _attention_bwd(dout, q, k, v, out, lse, lengths, scale, causal, dq, dk, dv):
+    """Writes the gradients into dq, dk, dv (views whose last axis is contiguous)."""
+    b, s, h, d = q.shape
+    if out.numel() == 0:
+        return
+    dout = _rows16(dout)
+    delta = torch.empty_like(lse)
+    with torch.cuda.device(q.device):
+        base.check(base.K().tipsk_attention_bwd(
+            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), delta.data_ptr(),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), base.ptr(lengths),
+            int(lengths is not None and lengths.dtype == torch.int64), b, s, h, k.shape[2], d, base.code(q),
+            _strides(q, k, v, out, dout, dq, dk, dv), scale, int(causal), base.stream()), "attention_bwd")
+    base.count_launches(1)
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, scale, causal):
+        out, lse, q, k, v = _attention_fwd(q, k, v, lengths, scale, causal)
+        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        ctx.scale, ctx.causal = scale, causal
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        _attention_bwd(dout, q, k, v, out, lse, lengths, ctx.scale, ctx.causal, dq, dk, dv)
+        return dq, dk, dv, None, None, None
+
+
+def _split_heads(t: torch.Tensor, h: int, hk: int):
+    """q, k, v views [b, s, heads, d] of a packed [b, s, (h + 2 hk) * d] tensor."""
+    b, s, width = t.shape
+    x = t.view(b, s, h + 2 * hk, width // (h + 2 * hk))
+    return x[:, :, :h], x[:, :, h:h + hk], x[:, :, h + hk:]
+
+
+class _PackedOwnAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, h, hk, lengths, scale, causal):
+        qkv = qkv.contiguous()
+        q, k, v = _split_heads(qkv, h, hk)
+        out, lse, _, _, _ = _attention_fwd(q, k, v, lengths, scale, causal)
+        ctx.save_for_backward(qkv, out, lse, lengths)
+        ctx.meta = (h, hk, scale, causal)
+        return out.view(*qkv.shape[:2], -1)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        qkv, out, lse, lengths = ctx.saved_tensors
+        h, hk, scale, causal = ctx.meta
+        q, k, v = (_rows16(t) for t in _split_heads(qkv, h, hk))
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _attention_bwd(dy.reshape(out.shape), q, k, v, out, lse, lengths, scale, causal, *_split_heads(dqkv, h, hk))
+        return dqkv, None, None, None, None, None
+
+
+def _plain_attention(q, k, v, lengths, scale, causal):
+    """The formula, for CPU tensors."""
+    b, s, h, d = q.shape
+    group = h // k.shape[2]
+    qf, kf, vf = (t.float().transpose(1, 2) for t in (q, k, v))
+    kf, vf = kf.repeat_interleave(group, 1), vf.repeat_interleave(group, 1)
+    pos = torch.arange(s, device=q.device)
+    rows = torch.ones(b, s, dtype=torch.bool, device=q.device)
+    if lengths is not None:
+        rows = pos[None] < lengths[:, None]
+        # what stands beyond a length must not count, whatever it is
+        qf, kf, vf = (torch.where(rows[:, None, :, None], t, 0.0) for t in (qf, kf, vf))
+    valid = rows[:, None, None, :]
+    if causal:
+        valid = valid & (pos[None, :] <= pos[:, None])
+    logits = (qf @ kf.transpose(-1, -2)) * scale
+    # a row without any valid key: zeros, by way of a softmax over all keys whose result is dropped
+    logits = logits.masked_fill(~valid & rows[:, None, :, None], -math.inf)
+    out = torch.where(rows[:, None, :, None], torch.softmax(logits, -1) @ vf, 0.0)
+    return out.transpose(1, 2).to(q.dtype)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = False, lengths: torch.Tensor | None = None,
+              scale: float | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v for ``q [batch, seq, heads, d]`` and ``k, v [batch, seq, kv_heads, d]``; returns
+    ``[batch, seq, heads, d]``.
+
+    `kv_heads` divides `heads`: query head i reads key and value head ``i // (heads // kv_heads)``.  `causal`: a position sees
+    itself and what is before it.  `lengths` (int32 or int64 ``[batch]``, on the inputs' device): the positions of a sequence
+    from its length on are padding.  They are not read as keys or values, their rows of the output are zero, and so are their
+    gradients, whatever stands in them; a length outside 0..seq counts as the nearer of the two.  `scale` (positive) defaults
+    to ``1 / sqrt(d)``.
+
+    On a GPU: bfloat16 or float16, d a multiple of 8 up to 128, any strides (inputs whose last axis is not contiguous, or
+    whose rows do not start on 16 bytes, are copied).  The softmax is held in fp32; the probabilities, and their
+    gradient in the backward pass, are rounded to the inputs' type as operands of the products.  Gradients do not depend on
+    the order of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
+    do not see it, as 0 * inf does in the formula.  `lengths` may not change between forward and backward."""
+    scale = _check_attention(q, k, v, lengths, scale)
+    if not q.is_cuda:
+        return _plain_attention(q, k, v, lengths, scale, causal)
+    if lengths is not None:
+        lengths = lengths.contiguous()
+    return _AttentionFn.apply(q, k, v, lengths, scale, bool(causal))
+
+
+def packed_attention(qkv: torch.Tensor, heads: int, causal: bool = False, kv_heads: int | None = None,
+                     lengths: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Multi-head self-attention on ``qkv = [batch, seq, 3 * hidden]`` (q, k, v concatenated on the last axis).
+
+    With any of `kv_heads`, `lengths`, `scale` it is `attention` (see there) on the heads of the packed tensor, whose last axis
+    holds ``heads`` heads of q and then `kv_heads` (default: `heads`) heads of k and of v."""
+    if kv_heads is not None or lengths is not None or scale is not None:
+        hk = heads if kv_heads is None else kv_heads
+        if qkv.dim() != 3 or heads <= 0 or hk <= 0 or qkv.shape[2] == 0 or qkv.shape[2] % (heads + 2 * hk) != 0:
+            raise ValueError(f"qkv must be [batch, seq, ({heads} + 2 * {hk}) * head_size], got {tuple(qkv.shape)}")
+        q, k, v = _split_heads(qkv.contiguous(), heads, hk)
+        scale = _check_attention(q.detach(), k.detach(), v.detach(), lengths, scale)
+        if not qkv.is_cuda:
+            return _plain_attention(q, k, v, lengths, scale, causal).reshape(*qkv.shape[:2], -1)
+        if lengths is not None:
+            lengths = lengths.contiguous()
+        return _PackedOwnAttentionFn.apply(qkv, heads, hk, lengths, scale, bool(causal))
     b, s, three_h = qkv.shape
     d = three_h // 3 // heads
     if _fast_ok(qkv, d) and qkv.is_contiguous():
