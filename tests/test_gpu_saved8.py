@@ -1,0 +1,185 @@
+"""The 8-bit kernels against the CPU form, bit by bit, and the linear layer's gradients against 64 bits."""
+import math
+
+import pytest
+import torch
+
+from test_saved8_cpu import blocks_to_try
+from tips_b200.ops.linear import gemm_status, gemm_tn, linear, linear_passthrough
+from tips_b200.ops.saved8 import act_bwd8, pack8
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def same(x):
+    """pack8 on the GPU gives the CPU's bytes, and unpack its values in every type."""
+    a, b = pack8(x), pack8(x.cpu())
+    assert a.shape == b.shape and torch.equal(a.q.cpu(), b.q) and torch.equal(a.e.cpu(), b.e)
+    for dtype in DTYPES:
+        u, v = a.unpack(dtype).cpu(), b.unpack(dtype)
+        assert u.dtype == v.dtype and torch.equal(u.nan_to_num(nan=-7.0), v.nan_to_num(nan=-7.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1,), (15,), (16,), (17,), (31,), (33,), (47,), (37, 101), (256, 512), (3, 7, 1000), (0,), ()])
+def test_pack(shape, dtype):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(len(shape))
+    same((torch.randn(shape, generator=g, device=DEV) * 5).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_special_values(dtype):
+    same(blocks_to_try().to(dtype).to(DEV))
+    ties = (torch.arange(-4096, 4096, device=DEV) * 0.25).to(dtype)  # many halves of a step
+    same(ties)
+
+
+def test_strides_and_alignment():
+    x = torch.randn(64, 130, device=DEV).to(torch.bfloat16)
+    for y in (x.t(), x[:, 1:], x[::2, 3:77], x.view(-1)[1:], x[:1].expand(5, 130)):
+        same(y)
+
+
+def test_long_tensor():
+    """More values than the grid takes in one round."""
+    x = torch.randn(148 * 8 * 256 * 16 + 77, device=DEV).to(torch.bfloat16)
+    same(x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 8), (7, 24), (33, 264), (1000, 512), (4097, 40), (3, 4104), (5, 13)])
+def test_activation_backward(rows, cols, dtype):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(rows)
+    dy = torch.randn(rows, cols, generator=g, device=DEV).to(dtype)
+    p = pack8((torch.randn(rows, cols, generator=g, device=DEV) * 2).to(dtype))
+    z = p.unpack(torch.float32).double()
+    want = dy.double() * (0.5 * (1 + torch.erf(z / math.sqrt(2))) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi))
+    u = torch.finfo(dtype).eps / 2
+    # the derivative is computed in 32 bits, to 4e-6 at worst (erf by a rational approximation within 1.5e-7, approximate exp
+    # and reciprocal at 2^-22 of factors up to 3); fp16's least half step is 2^-25
+    slack = 4e-6 * dy.double().abs()
+    for bias_dtype in DTYPES + [None]:
+        dz, db = act_bwd8(dy, p.q, p.e, bias_dtype)
+        assert dz.dtype == dtype and ((dz.double() - want).abs() <= u * want.abs() + slack + 2.0 ** -25).all()
+        if bias_dtype is None:
+            assert db is None
+            continue
+        # sums of the unrounded values in 32 bits: 2^-24 per addition, at most rows of them in a row
+        off = (slack + rows * 2.0 ** -24 * want.abs()).sum(0) + torch.finfo(bias_dtype).eps / 2 * want.sum(0).abs() + 2.0 ** -25
+        assert db.dtype == bias_dtype and ((db.double() - want.sum(0)).abs() <= off).all()
+        assert torch.equal(db, act_bwd8(dy, p.q, p.e, bias_dtype)[1])
+    same_dy, db = act_bwd8(dy, None, None, torch.float32)
+    assert same_dy.data_ptr() == dy.data_ptr()
+    off = rows * 2.0 ** -24 * dy.double().abs().sum(0) + 2.0 ** -24 * dy.double().sum(0).abs()
+    assert ((db.double() - dy.double().sum(0)).abs() <= off).all()
+
+
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 64), (100, 128, 512), (257, 520, 1096), (777, 72, 200), (2048, 1024, 4096),
+                                      (4096, 512, 64), (64, 40, 13)])
+def test_linear(rows, k, n, act):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(rows + k)
+    bf = torch.bfloat16
+    x, dy = (torch.randn(rows, c, generator=g, device=DEV).to(bf) for c in (k, n))
+    w = (torch.randn(n, k, generator=g, device=DEV) / math.sqrt(k)).to(bf)
+    b = torch.randn(n, generator=g, device=DEV).to(bf)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = linear(*leaves, act, save8=True)
+    assert torch.equal(y, linear(*leaves, act))
+    got = torch.autograd.grad(y, leaves, dy)
+    assert gemm_status() == 0
+    u, slack = 2.0 ** -8, 2.0 ** -14
+    dz = dy.double()
+    if act:
+        z = pack8(gemm_tn(x, w, b, act, want_pre=True)[1]).unpack().double()  # the value that the layer stores
+        dz = dz * (0.5 * (1 + torch.erf(z / math.sqrt(2))) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi))
+        e = u * dz.abs() + 4e-6 * dy.double().abs()  # dz is rounded to bf16 as an operand
+    else:
+        e = torch.zeros_like(dz)
+    x8, wd = pack8(x).unpack().double(), w.double()
+    # products accumulate in 32 bits: slack times the sums of absolute values covers 2^-24 for each of up to 2^10 partial sums
+    want = [dz @ wd, dz.t() @ x8, dz.sum(0)]
+    mag = [dz.abs() @ wd.abs(), dz.abs().t() @ x8.abs(), dz.abs().sum(0)]
+    off = [e @ wd.abs(), e.t() @ x8.abs(), 4e-6 * dy.double().abs().sum(0)]
+    for a, t, m, o in zip(got, want, mag, off):
+        assert a.dtype == bf and ((a.double() - t).abs() <= o + slack * m + u * t.abs()).all()
+
+
+def test_passthrough_and_dtypes():
+    """The residual gradient is added into the input's; fp32 and fp16 layers take the same arguments."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    x, w, dy, da = (torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16) for s in ((300, 128), (256, 128), (300, 256), (300, 128)))
+    x.requires_grad_()
+    w.requires_grad_()
+    y, alias = linear_passthrough(x, w, None, "gelu", save8=True)
+    got = torch.autograd.grad((y, alias), (x, w), (dy, da.clone()))
+    plain = torch.autograd.grad(linear(x, w, None, "gelu", save8=True), (x, w), dy)
+    # dx is rounded to bf16 once in either; the sum once more
+    assert ((got[0].double() - plain[0].double() - da.double()).abs()
+            <= 2.0 ** -8 * (plain[0].double().abs() + got[0].double().abs()) + 2.0 ** -12).all()
+    assert torch.equal(got[1], plain[1])
+    for dtype in (torch.float32, torch.float16):
+        a, b = x.detach().to(dtype).requires_grad_(), w.detach().to(dtype).requires_grad_()
+        y = linear(a, b, None, "gelu", save8=True)
+        got = torch.autograd.grad(y, (a, b), dy.to(dtype))
+        for t, v in zip(got, plain):
+            assert t.dtype == dtype and (t.double() - v.double()).norm() <= 2.0 ** -5 * v.double().norm()
+
+
+def test_graph_and_stream():
+    x = torch.randn(513, 96, device=DEV).to(torch.bfloat16)
+    want = pack8(x).unpack()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = pack8(x).unpack()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, want)
+    buf = torch.zeros_like(x)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = pack8(buf).unpack()
+    buf.copy_(x)
+    g.replay()
+    assert torch.equal(y, want)
+
+
+def test_encoder_keeps_less_and_trains_alike():
+    """A padded batch through the small encoder with its linear layers at 8 bits: the loss is the same, the gradients are near
+    those of the 16-bit form, and less is kept for the backward pass."""
+    from tips_b200.models.bert import synthetic_mlm_batch, tiny_bert
+    torch.manual_seed(0)
+    a = tiny_bert()
+    b = tiny_bert(save8=True)
+    b.load_state_dict(a.state_dict())
+    ids, pos, labels = (t.to(DEV) for t in synthetic_mlm_batch(8, 64, 1024, seed=3))
+    n = torch.tensor([64, 20, 33, 64, 1, 50, 7, 64], device=DEV)
+    pos = pos % n[:, None]
+    kept, losses = [], []
+    for m in (a, b):
+        own = {p.data_ptr() for p in m.parameters()}
+        seen = {}
+
+        def keep(t):
+            if t.data_ptr() not in own:
+                seen[t.data_ptr()] = t.untyped_storage().nbytes()
+            return t
+
+        with torch.autograd.graph.saved_tensors_hooks(keep, lambda t: t):
+            loss = m.loss(ids, pos, labels, lengths=n)
+        kept.append(sum(seen.values()))
+        loss.backward()
+        losses.append(loss.detach())
+    # the same logits; the loss kernel adds the 80 rows' terms, none negative, in any order: 2^-24 of the sum per addition
+    assert torch.allclose(*losses, rtol=80 * 2.0 ** -24, atol=0)
+    assert kept[1] < 0.8 * kept[0]
+    for (name, p), q in zip(a.named_parameters(), b.parameters()):
+        if p.grad is not None and float(p.grad.float().norm()) > 0 and "qkv.bias" not in name:
+            # a stored value is off by 0.8 % of its block's root mean square; through two layers that stays within 10 %
+            assert (p.grad.float() - q.grad.float()).norm() <= 0.1 * p.grad.float().norm(), name

@@ -1,0 +1,267 @@
+// Activations kept for the backward pass in 8 bits.
+//
+// A tensor is taken as one run of values in blocks of 32.  The values of a block share a power-of-two step 2^e and are stored as
+// whole multiples of it:
+//   e = the least integer with rint(amax 2^-e) <= 127, clamped to [-126, 121];   q = clamp(rint(x 2^-e), -127, 127)
+// where amax is the largest finite |x| of the block.  A value that is not finite is stored as q = -128 and stands for NaN.
+// Scaling by a power of two rounds nothing, so the only rounding is rint, off by at most half a step, amax / 127 at
+// most: for a normally distributed block 0.8 % of its root mean square.  And a stored value has at most 7 significant
+// bits, so bf16 holds it exactly: reading it back into the tensor cores' type costs no further rounding.
+// A block takes 32 + 1 bytes.
+//
+// The reference keeps no activations (it trains TensorFlow models); these serve the linear layers of the encoder.
+#include "kernels/common.cuh"
+#include "kernels/tips_kernels.h"
+
+namespace tipsk {
+namespace {
+
+constexpr int kBlock8 = 32;  // values that share a step
+
+// e of a block from the bits of its amax: amax = 1.M 2^(E - 127) needs E - 133, one more if 1.M 64 rounds to 128
+// (1.M >= 127.5 / 64, M >= 0x7f0000).  Zero and subnormal values end in the lower clamp.
+__device__ __forceinline__ int StepExponent(uint32_t amax_bits) {
+  const int e = static_cast<int>((amax_bits + 0x10000u) >> 23) - 133;
+  return e < -126 ? -126 : e > 121 ? 121 : e;
+}
+__device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+__device__ __forceinline__ uint32_t FiniteBits(float x) {
+  const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
+  return a < 0x7f800000u ? a : 0u;
+}
+// One value as its byte; inv = 2^-e.
+__device__ __forceinline__ uint32_t Quantise(float x, float inv) {
+  const int q = __float2int_rn(fminf(fmaxf(x * inv, -127.f), 127.f));
+  return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u ? static_cast<uint32_t>(q) & 0xffu : 0x80u;
+}
+__device__ __forceinline__ float Dequantise(int q, float step) { return q == -128 ? __uint_as_float(0x7fc00000u) : q * step; }
+
+// Sixteen values per thread, so two lanes share a block.
+template <typename T>
+__global__ void __launch_bounds__(256) Pack8Kernel(const T* __restrict__ x, int8_t* __restrict__ q, int8_t* __restrict__ e, int64_t n) {
+  constexpr int N = 16 / sizeof(T), kLoads = 16 / N;
+  const int64_t groups = (n + 31) / 32 * 2;  // both lanes of a block take part, whatever the tail holds
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  const int64_t rounds = (groups + stride - 1) / stride;
+  for (int64_t k = 0; k < rounds; ++k) {  // every lane makes the same number of rounds: the shuffle needs them all
+    const int64_t g  = k * stride + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t at = g * 16;
+    float v[16];
+    if (at + 16 <= n) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const Vec16<T> w = LoadVec(x + at + u * N);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[u * N + j] = ToFloat<T>(w.v[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = at + j < n ? ToFloat<T>(x[at + j]) : 0.f;
+    }
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = max(amax, FiniteBits(v[j]));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    const int ex    = StepExponent(amax);
+    const float inv = PowerOfTwo(-ex);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = Quantise(v[4 * j], inv) | Quantise(v[4 * j + 1], inv) << 8 | Quantise(v[4 * j + 2], inv) << 16 |
+             Quantise(v[4 * j + 3], inv) << 24;
+    if (at + 16 <= n) {
+      *reinterpret_cast<uint4*>(q + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (at + j < n) q[at + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
+    }
+    if ((threadIdx.x & 1) == 0 && at < n) e[at / kBlock8] = static_cast<int8_t>(ex);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) Unpack8Kernel(const int8_t* __restrict__ q, const int8_t* __restrict__ e, T* __restrict__ y, int64_t n) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g * 16 < n; g += stride) {
+    const int64_t at = g * 16;
+    const float step = PowerOfTwo(e[at / kBlock8]);
+    if (at + 16 <= n) {
+      const uint4 w = *reinterpret_cast<const uint4*>(q + at);
+      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int u = 0; u < 16 / N; ++u) {
+        Vec16<T> o;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int i = u * N + j;
+          o.v[j] = FromFloat<T>(Dequantise(static_cast<int8_t>(ws[i / 4] >> (8 * (i % 4))), step));
+        }
+        StoreVec(y + at + u * N, o);
+      }
+    } else {
+      for (int j = 0; at + j < n; ++j) y[at + j] = FromFloat<T>(Dequantise(q[at + j], step));
+    }
+  }
+}
+
+// dz = dy gelu'(z) with z in 8 bits, and sums of dz per column, in fp32 before dz is rounded; without kGelu only the sums, of
+// dy.  Block (32, 8): a thread takes a vector of columns (which lies within a block of the 8-bit form, because both start at
+// multiples of 8 values), every block a share of the rows; the shares' sums go to partial [gridDim.y][cols] and are added in
+// their order by ColumnSumKernel, so a result does not depend on the order of the blocks.
+template <typename T, bool kGelu>
+__global__ void __launch_bounds__(256)
+ActBwd8Kernel(const T* __restrict__ dy, const int8_t* __restrict__ q, const int8_t* __restrict__ e, T* __restrict__ dz,
+               float* __restrict__ partial, int64_t rows, int cols) {
+  constexpr int N = 8;
+  __shared__ float red[8][32][N + 1];
+  const int vc = blockIdx.x * 32 + threadIdx.x;
+  float acc[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) acc[k] = 0.f;
+  if (vc < cols / N) {
+    for (int64_t r = static_cast<int64_t>(blockIdx.y) * 8 + threadIdx.y; r < rows; r += static_cast<int64_t>(gridDim.y) * 8) {
+      const int64_t off = r * cols + static_cast<int64_t>(vc) * N;
+      alignas(16) T g[N], o[N];
+#pragma unroll
+      for (int k = 0; k < N; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(&g[k]) = *reinterpret_cast<const uint4*>(dy + off + k);
+      if (!kGelu) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += ToFloat<T>(g[k]);
+        continue;
+      }
+      const float step = PowerOfTwo(e[off / kBlock8]);
+      const uint2 w    = *reinterpret_cast<const uint2*>(q + off);
+#pragma unroll
+      for (int k = 0; k < N; k += 2) {
+        const uint32_t word = k < 4 ? w.x : w.y;
+        const F2 z = MakeF2(Dequantise(static_cast<int8_t>(word >> (8 * (k & 3))), step),
+                            Dequantise(static_cast<int8_t>(word >> (8 * (k & 3) + 8)), step));
+        const float2 v = SplitF2(Mul2(MakeF2(ToFloat<T>(g[k]), ToFloat<T>(g[k + 1])), GeluGrad2(z)));
+        acc[k] += v.x;
+        acc[k + 1] += v.y;
+        o[k]     = FromFloat<T>(v.x);
+        o[k + 1] = FromFloat<T>(v.y);
+      }
+#pragma unroll
+      for (int k = 0; k < N; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(dz + off + k) = *reinterpret_cast<uint4*>(&o[k]);
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int k = 0; k < N; ++k) red[threadIdx.y][threadIdx.x][k] = acc[k];
+  __syncthreads();
+  const int t = threadIdx.y * 32 + threadIdx.x, c = blockIdx.x * 256 + t;
+  if (c < cols) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += red[j][t / N][t % N];
+    partial[static_cast<int64_t>(blockIdx.y) * cols + c] = s;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) ColumnSumKernel(const float* __restrict__ partial, T* __restrict__ out, int parts, int cols) {
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  __shared__ float red[8][33];
+  float s = 0.f;
+  if (c < cols)
+    for (int p = threadIdx.y; p < parts; p += 8) s += partial[static_cast<int64_t>(p) * cols + c];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < cols) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) s += red[j][threadIdx.x];
+    out[c] = FromFloat<T>(s);
+  }
+}
+
+int Blocks(int64_t threads, int per_sm) {
+  const int64_t want = (threads + 255) / 256, most = static_cast<int64_t>(NumSMs()) * per_sm;
+  return static_cast<int>(want < most ? want : most);
+}
+bool Aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+}  // namespace tipsk
+
+using namespace tipsk;
+
+extern "C" {
+
+/* q[n], e[ceil(n / 32)] = the 8-bit form of x[n] (fp32, bf16 or fp16). */
+int tipsk_pack8(const void* x, void* q, void* e, int64_t n, int dtype, void* stream) {
+  TIPSK_REQUIRE(n > 0 && (dtype == kF32 || dtype == kBF16 || dtype == kF16), "pack8: fp32, bf16 or fp16 and at least one value");
+  TIPSK_REQUIRE(Aligned16(x) && Aligned16(q), "pack8: the values must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int grid = Blocks((n + 31) / 32 * 2, 8);
+  int8_t *qq = static_cast<int8_t*>(q), *ee = static_cast<int8_t*>(e);
+  if (dtype == kF32) Pack8Kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(x), qq, ee, n);
+  else if (dtype == kBF16) Pack8Kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), qq, ee, n);
+  else Pack8Kernel<__half><<<grid, 256, 0, s>>>(static_cast<const __half*>(x), qq, ee, n);
+  TIPSK_LAUNCH_CHECK();
+  return 0;
+}
+
+/* y[n] = the values that q, e stand for; exact in fp32 and bf16, rounded to fp16 where that has fewer bits (below 2^-14). */
+int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, void* stream) {
+  TIPSK_REQUIRE(n > 0 && (dtype == kF32 || dtype == kBF16 || dtype == kF16), "unpack8: fp32, bf16 or fp16 and at least one value");
+  TIPSK_REQUIRE(Aligned16(y) && Aligned16(q), "unpack8: the values must be 16-byte aligned");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int grid = Blocks((n + 15) / 16, 8);
+  const int8_t *qq = static_cast<const int8_t*>(q), *ee = static_cast<const int8_t*>(e);
+  if (dtype == kF32) Unpack8Kernel<float><<<grid, 256, 0, s>>>(qq, ee, static_cast<float*>(y), n);
+  else if (dtype == kBF16) Unpack8Kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(qq, ee, static_cast<__nv_bfloat16*>(y), n);
+  else Unpack8Kernel<__half><<<grid, 256, 0, s>>>(qq, ee, static_cast<__half*>(y), n);
+  TIPSK_LAUNCH_CHECK();
+  return 0;
+}
+
+/* Shares of the rows of tipsk_act_bwd8, for its workspace. */
+int tipsk_act_bwd8_parts(int64_t rows, int cols) {
+  const int64_t tiles = (cols + 255) / 256, fill = (static_cast<int64_t>(NumSMs()) * 8 + tiles - 1) / tiles;
+  const int64_t most  = (rows + 7) / 8;
+  return static_cast<int>(fill < most ? fill : most);
+}
+
+/* dz = dy * gelu'(z) for z [rows, cols] in 8 bits (q, e); without q, e and dz there is no activation.  dbias (optional with z,
+ * of dtype bias_dtype) receives the column sums of dz, or of dy.  partial: fp32 workspace of tipsk_act_bwd8_parts * cols.
+ * cols a multiple of 8. */
+int tipsk_act_bwd8(const void* dy, const void* q, const void* e, void* dz, void* dbias, int bias_dtype, float* partial,
+                   int64_t rows, int cols, int dtype, void* stream) {
+  TIPSK_REQUIRE(rows > 0 && cols > 0 && cols % 8 == 0, "act_bwd8: the number of columns must be a multiple of 8");
+  TIPSK_REQUIRE((dtype == kF32 || dtype == kBF16 || dtype == kF16) &&
+                    (dbias == nullptr || bias_dtype == kF32 || bias_dtype == kBF16 || bias_dtype == kF16),
+                "act_bwd8: fp32, bf16 or fp16");
+  TIPSK_REQUIRE((q == nullptr) == (e == nullptr) && (q == nullptr) == (dz == nullptr), "act_bwd8: q, e and dz go together");
+  TIPSK_REQUIRE(Aligned16(dy) && Aligned16(dz) && reinterpret_cast<uintptr_t>(q) % 8 == 0, "act_bwd8: alignment");
+  TIPSK_REQUIRE(dbias == nullptr ? q != nullptr : partial != nullptr, "act_bwd8: nothing to do, or no workspace for the sums");
+  cudaStream_t s  = static_cast<cudaStream_t>(stream);
+  const int parts = tipsk_act_bwd8_parts(rows, cols);
+  const dim3 grid((cols + 255) / 256, parts), block(32, 8);
+  const int8_t *qq = static_cast<const int8_t*>(q), *ee = static_cast<const int8_t*>(e);
+  float* part = dbias ? partial : nullptr;
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    if (q) ActBwd8Kernel<T, true><<<grid, block, 0, s>>>(static_cast<const T*>(dy), qq, ee, static_cast<T*>(dz), part, rows, cols);
+    else ActBwd8Kernel<T, false><<<grid, block, 0, s>>>(static_cast<const T*>(dy), qq, ee, static_cast<T*>(dz), part, rows, cols);
+  };
+  if (dtype == kF32) run(float{});
+  else if (dtype == kBF16) run(__nv_bfloat16{});
+  else run(__half{});
+  TIPSK_LAUNCH_CHECK();
+  if (dbias) {
+    auto sum = [&](auto t) {
+      using T = decltype(t);
+      ColumnSumKernel<T><<<(cols + 31) / 32, block, 0, s>>>(partial, static_cast<T*>(dbias), parts, cols);
+    };
+    if (bias_dtype == kF32) sum(float{});
+    else if (bias_dtype == kBF16) sum(__nv_bfloat16{});
+    else sum(__half{});
+    TIPSK_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+}  // extern "C"

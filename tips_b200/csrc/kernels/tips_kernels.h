@@ -236,6 +236,13 @@ int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const vo
                         int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal, void* stream);
 int tipsk_attention_status(void);
 
+/* ---- activations in 8 bits (saved8.cu): q int8 per value, e int8 per block of 32, the step of a block is 2^e ---- */
+int tipsk_pack8(const void* x, void* q, void* e, int64_t n, int dtype, void* stream);
+int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, void* stream);
+int tipsk_act_bwd8_parts(int64_t rows, int cols);
+int tipsk_act_bwd8(const void* dy, const void* q, const void* e, void* dz, void* dbias, int bias_dtype, float* partial,
+                   int64_t rows, int cols, int dtype, void* stream);
+
 /* ---- 3x3 / stride 2 / pad 1 max pooling on NHWC (pool.cu); idx holds the argmax position 0..8 per output ---- */
 /* Global average pooling on NHWC (x [n, hw, c] -> y [n, c]) and its backward (pool.cu). */
 int tipsk_global_avgpool_fwd(const void* x, void* y, int n, int hw, int c, int dtype, void* stream);

@@ -24,14 +24,16 @@ _TORCH_EMBED = os.environ.get("TIPS_BERT_TORCH_EMBED", "0") == "1"
 
 
 class BertLayer(nn.Module):
-    def __init__(self, hidden, heads, ffn):
+    """`save8`: the linear layers keep their activations for the backward pass in 8 bits (ops/saved8.py)."""
+
+    def __init__(self, hidden, heads, ffn, save8=False):
         super().__init__()
         self.heads = heads
-        self.qkv = Linear(hidden, 3 * hidden)
-        self.proj = Linear(hidden, hidden)
+        self.qkv = Linear(hidden, 3 * hidden, save8=save8)
+        self.proj = Linear(hidden, hidden, save8=save8)
         self.ln1 = LayerNorm(hidden, eps=1e-12)
-        self.fc1 = Linear(hidden, ffn, act="gelu")
-        self.fc2 = Linear(ffn, hidden)
+        self.fc1 = Linear(hidden, ffn, act="gelu", save8=save8)
+        self.fc2 = Linear(ffn, hidden, save8=save8)
         self.ln2 = LayerNorm(hidden, eps=1e-12)
 
     def forward(self, x, lengths=None):
@@ -45,7 +47,8 @@ class BertLayer(nn.Module):
 
 
 class BertMLM(nn.Module):
-    def __init__(self, vocab=30522, hidden=1024, layers=24, heads=16, ffn=4096, max_seq=512, type_vocab=2):
+    def __init__(self, vocab=30522, hidden=1024, layers=24, heads=16, ffn=4096, max_seq=512, type_vocab=2,
+                 save8=False):
         super().__init__()
         self.vocab = vocab
         # rows padded to a multiple of 64 so the tied decoder GEMM writes 16-byte vectors (unused classes)
@@ -54,7 +57,7 @@ class BertMLM(nn.Module):
         self.pos = nn.Embedding(max_seq, hidden)
         self.typ = nn.Embedding(type_vocab, hidden)
         self.ln_emb = LayerNorm(hidden, eps=1e-12)
-        self.layers = nn.ModuleList([BertLayer(hidden, heads, ffn) for _ in range(layers)])
+        self.layers = nn.ModuleList([BertLayer(hidden, heads, ffn, save8) for _ in range(layers)])
         self.head_dense = Linear(hidden, hidden, act="gelu")
         self.head_ln = LayerNorm(hidden, eps=1e-12)
         self.decoder_bias = nn.Parameter(torch.zeros(self.vocab_padded))
@@ -92,8 +95,8 @@ def bert_large(dtype=torch.bfloat16, device="cuda", **kw):
     return BertMLM(**kw).to(device=device, dtype=dtype)
 
 
-def tiny_bert(dtype=torch.bfloat16, device="cuda"):
-    return BertMLM(vocab=1024, hidden=128, layers=2, heads=4, ffn=512, max_seq=64).to(device=device, dtype=dtype)
+def tiny_bert(dtype=torch.bfloat16, device="cuda", **kw):
+    return BertMLM(vocab=1024, hidden=128, layers=2, heads=4, ffn=512, max_seq=64, **kw).to(device=device, dtype=dtype)
 
 
 def synthetic_mlm_batch(batch, seq, vocab, seed, mask_frac=0.15):

@@ -22,7 +22,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import base
+from . import base, saved8
 
 _ACT = {None: 0, "none": 0, "relu": 1, "gelu": 2}
 
@@ -141,6 +141,75 @@ class _LinearFn(torch.autograd.Function):
         return _linear_backward(ctx, dy, None)
 
 
+class _Linear8Fn(torch.autograd.Function):
+    """linear(x) that keeps x and, with GELU, the value before the activation in 8 bits (ops/saved8.py)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, act):
+        x2 = x.reshape(-1, x.shape[-1])
+        if not x2.is_contiguous():
+            x2 = x2.contiguous()
+        gelu = _ACT[act] == 2
+        xq = xe = pq = pe = None
+        if gelu:
+            y, pre = gemm_tn(x2, weight, bias, act, want_pre=True)
+            if any(ctx.needs_input_grad[:3]):
+                pq, pe = saved8._pack(pre)
+        else:
+            y = gemm_tn(x2, weight, bias, act)
+        if ctx.needs_input_grad[1]:
+            xq, xe = saved8._pack(x2)
+        ctx.save_for_backward(weight, xq, xe, pq, pe)
+        ctx.x_dtype, ctx.bias_dtype = x.dtype, None if bias is None else bias.dtype
+        ctx.in_shape = x.shape
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return _linear8_backward(ctx, dy, None)
+
+
+def _linear8_backward(ctx, dy, d_alias):
+    weight, xq, xe, pq, pe = ctx.saved_tensors  # pq, pe: None without an activation
+    n, k = weight.shape
+    dz = dy.reshape(-1, n)
+    if not dz.is_contiguous():
+        dz = dz.contiguous()
+    want_bias = ctx.bias_dtype if ctx.needs_input_grad[2] else None
+    dz, db = saved8.act_bwd8(dz, pq, pe, want_bias)
+    dx = dw = None
+    if ctx.needs_input_grad[0]:
+        dx = _input_grad(dz, weight, d_alias).view(ctx.in_shape)
+    if ctx.needs_input_grad[1]:
+        dw = _weight_grad(dz, saved8._unpack(xq, xe, (dz.shape[0], k), ctx.x_dtype), weight.dtype).to(weight.dtype)
+    return dx, dw, db, None
+
+
+class _Linear8PassFn(torch.autograd.Function):
+    """_LinearPassFn with the activations in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, act):
+        y = _Linear8Fn.forward(ctx, x, weight, bias, act)
+        return y, x.detach()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, d_alias):
+        return _linear8_backward(ctx, dy, d_alias)
+
+
+def _input_grad(dz: torch.Tensor, weight: torch.Tensor, d_alias: torch.Tensor | None) -> torch.Tensor:
+    """dz @ weight as [rows, k]; with `d_alias` (the gradient of another consumer of the input) added into it by the GEMM."""
+    into = None
+    if d_alias is not None:
+        into = d_alias.reshape(-1, weight.shape[1])
+        if not (into.is_contiguous() and into.dtype == torch.bfloat16 and into.data_ptr() % 16 == 0):
+            into = into.contiguous()
+    return gemm_nn(dz, weight, into=into)
+
+
 def _linear_backward(ctx, dy, d_alias):
     """Gradients of the fused linear layer; `d_alias` (optional) is the gradient of another consumer of x, into
     which dx is accumulated inside the GEMM."""
@@ -176,12 +245,7 @@ def _linear_backward(ctx, dy, d_alias):
             dbias = dz.float().sum(0).to(bias.dtype)
     dx = dw = None
     if ctx.needs_input_grad[0]:
-        into = None
-        if d_alias is not None:
-            into = d_alias.reshape(-1, x2.shape[1])
-            if not (into.is_contiguous() and into.dtype == torch.bfloat16 and into.data_ptr() % 16 == 0):
-                into = into.contiguous()
-        dx = gemm_nn(dz, weight, into=into).view(ctx.in_shape)
+        dx = _input_grad(dz, weight, d_alias).view(ctx.in_shape)
     if ctx.needs_input_grad[1]:
         dw = _weight_grad(dz, x2, weight.dtype).to(weight.dtype)
     return dx, dw, dbias, None
@@ -202,27 +266,44 @@ class _LinearPassFn(torch.autograd.Function):
         return _linear_backward(ctx, dy, d_alias)
 
 
-def linear(x, weight, bias=None, act=None):
-    """act(x @ weight.T + bias) with the epilogue fused into the GEMM."""
+def _check_save8(x, act):
+    if _ACT[act] == 1:
+        raise ValueError("save8 keeps the value before a GELU; a ReLU needs one bit per value, which it does not take")
+    saved8._check(x.dtype, "save8")
+
+
+def linear(x, weight, bias=None, act=None, save8=False):
+    """act(x @ weight.T + bias) with the epilogue fused into the GEMM.
+
+    `save8` (act None or "gelu"): what the backward pass needs of the activations is kept in 8 bits (see ops/saved8.py).  The
+    output is the same; the weight's gradient is computed from the stored x, and with GELU all gradients from the stored
+    pre-activation, which is rounded to x's type before it is stored.  Gradients of gradients are refused."""
+    if save8:
+        _check_save8(x, act)
+        return _Linear8Fn.apply(x, weight, bias, act)
     return _LinearFn.apply(x, weight, bias, act)
 
 
-def linear_passthrough(x, weight, bias=None, act=None):
+def linear_passthrough(x, weight, bias=None, act=None, save8=False):
     """(linear(x), alias of x): use the alias for the residual branch; see _LinearPassFn."""
+    if save8:
+        _check_save8(x, act)
     if x.is_cuda and x.dtype == torch.bfloat16:
-        return _LinearPassFn.apply(x, weight, bias, act)
-    return linear(x, weight, bias, act), x
+        return (_Linear8PassFn if save8 else _LinearPassFn).apply(x, weight, bias, act)
+    return linear(x, weight, bias, act, save8), x
 
 
 class Linear(nn.Module):
-    def __init__(self, in_features, out_features, bias=True, act=None):
+    """`save8`: keep the activations for the backward pass in 8 bits (see `linear`)."""
+
+    def __init__(self, in_features, out_features, bias=True, act=None, save8=False):
         super().__init__()
-        self.in_features, self.out_features, self.act = in_features, out_features, act
+        self.in_features, self.out_features, self.act, self.save8 = in_features, out_features, act, save8
         self.weight = nn.Parameter(torch.empty(out_features, in_features))
         self.bias = nn.Parameter(torch.zeros(out_features)) if bias else None
         nn.init.kaiming_uniform_(self.weight, a=math.sqrt(5))
 
     def forward(self, x, passthrough=False):
         if passthrough:
-            return linear_passthrough(x, self.weight, self.bias, self.act)
-        return linear(x, self.weight, self.bias, self.act)
+            return linear_passthrough(x, self.weight, self.bias, self.act, self.save8)
+        return linear(x, self.weight, self.bias, self.act, self.save8)
