@@ -33,8 +33,9 @@ namespace {
 
 constexpr int kTile        = 128;  // rows of a tile of queries or keys
 constexpr int kBoxBytes    = kTile * 128;  // 128 rows of 64 16-bit values
-constexpr int kAttnThreads = 320;  // eight softmax warps, one TMA warp, one MMA warp
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
+constexpr int kFwdThreads = 384;  // eight softmax warps, one TMA warp, one MMA warp, two idle ones (whole warpgroups)
+constexpr int kBwdWarps   = 16;   // softmax warps of the backward pass
+constexpr int kBwdThreads = (kBwdWarps + 2) * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int32_t g_attn_error;  // one per device
@@ -53,7 +54,7 @@ struct AttnParams {
   int causal;
   float scale, c;       // c = scale * log2(e)
   float* lse;           // [b, h, sp]
-  float* delta;         // [b, h, sp]
+  float* delta;         // [2][b, h, sp]
   void *o, *dq, *dk, *dv;
   const void* dout;
   Strides so, sdo, sdq, sdk, sdv;
@@ -96,6 +97,15 @@ __device__ __forceinline__ void UmmaTmemA(uint32_t tmem_d, uint32_t tmem_a, uint
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum)
       : "memory");
+}
+__device__ __forceinline__ void TmemLoad16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void TmemStore16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -153,15 +163,15 @@ __device__ __forceinline__ void IssueScores(uint32_t tmem_d, uint32_t a_addr, ui
     UmmaBf16(tmem_d, a + off, b + off, idesc, k > 0);
   }
 }
-// [128 x 128] (16-bit, TMEM) x [128 x n]: B MN-major in shared memory.  The 128 columns of A lie in two runs of 32 TMEM
-// columns, `gap` columns apart.
-template <bool kBf16>
-__device__ __forceinline__ void IssueFromTmem(uint32_t tmem_d, uint32_t tmem_a, uint32_t gap, uint32_t b_addr, int n, bool accum) {
+// [128 x 128] (16-bit, TMEM) x [128 x n]: B MN-major in shared memory.  The columns of A lie in runs of kRun, two per TMEM
+// column, kRun columns apart (each where the fp32 values that it was made of had been).
+template <bool kBf16, int kRun>
+__device__ __forceinline__ void IssueFromTmem(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_addr, int n, bool accum) {
   const uint64_t b     = SmemDescMnSw128(b_addr, kBoxBytes);
   const uint32_t idesc = InstrDesc<kBf16>(n, true);
 #pragma unroll
   for (int k = 0; k < 8; ++k)
-    UmmaTmemA(tmem_d, tmem_a + (k >> 2) * gap + (k & 3) * 8, b + 128 * k, idesc, accum || k > 0);
+    UmmaTmemA(tmem_d, tmem_a + k * 16 / kRun * kRun + k * 16 % kRun / 2, b + 128 * k, idesc, accum || k > 0);
 }
 
 // Clears rows [first, 128) of a tile of `boxes` boxes (a whole warp; the swizzle stays within a row's 128 bytes) and
@@ -175,10 +185,10 @@ __device__ __forceinline__ void ClearRows(uint8_t* tile, int boxes, int first) {
   __syncwarp();
 }
 
-template <bool kBf16>
-__device__ __forceinline__ void StoreCols32(uint16_t* row, int col0, int d, const uint32_t (&acc)[32], float factor) {
+template <bool kBf16, int kCols>
+__device__ __forceinline__ void StoreCols(uint16_t* row, int col0, int d, const uint32_t (&acc)[kCols], float factor) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
+  for (int g = 0; g < kCols / 8; ++g) {
     if (col0 + g * 8 >= d) break;  // d is a multiple of 8
     uint4 v;
     v.x = Pack2<kBf16>(__uint_as_float(acc[g * 8 + 0]) * factor, __uint_as_float(acc[g * 8 + 1]) * factor);
@@ -197,6 +207,17 @@ __device__ __forceinline__ float Exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ F2 Add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 Pair(uint32_t a, uint32_t b) { return MakeF2(__uint_as_float(a), __uint_as_float(b)); }
+template <bool kBf16>
+__device__ __forceinline__ uint32_t Pack2(F2 a) {
+  const float2 x = SplitF2(a);
+  return Pack2<kBf16>(x.x, x.y);
+}
 
 __device__ __forceinline__ uint8_t* AlignedSmem(uint8_t* raw) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -214,9 +235,10 @@ struct FwdCfg {
 };
 
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kFwdThreads, 1)
 AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   using Cfg = FwdCfg<HD>;
+  constexpr int kTmaWarp = 8, kMmaWarp = 9;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem_q   = AlignedSmem(smem_raw);
   uint8_t* ring     = smem_q + 2 * Cfg::kTileBytes;
@@ -276,71 +298,76 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   // columns: scores of either tile (their probabilities in the same place), then either output
   const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + HD};
 
-  if (warp == kTmaWarp) {
-    if (total > 0 && ElectOne()) {
-      MbarExpectTx(q_full, 2 * Cfg::kTileBytes);
-      TmaLoadTile<HD>(smem_q, &maps.q, q0, h, b, q_full);
-      TmaLoadTile<HD>(smem_q + Cfg::kTileBytes, &maps.q, q0 + kTile, h, b, q_full);
-      for (int e = 0; e < 2 * total; ++e) {
-        const int st = e % Cfg::kStages;
-        if (!MbarWait(&empty[st], ((e / Cfg::kStages) & 1) ^ 1)) {
-          atomicExch(&g_attn_error, 1);
-          break;
+  // 168 registers per thread at launch; a softmax thread holds a row of 128 scores: 2 x 208 + 88 = 3 x 168
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kTmaWarp) {
+      if (total > 0 && ElectOne()) {
+        MbarExpectTx(q_full, 2 * Cfg::kTileBytes);
+        TmaLoadTile<HD>(smem_q, &maps.q, q0, h, b, q_full);
+        TmaLoadTile<HD>(smem_q + Cfg::kTileBytes, &maps.q, q0 + kTile, h, b, q_full);
+        for (int e = 0; e < 2 * total; ++e) {
+          const int st = e % Cfg::kStages;
+          if (!MbarWait(&empty[st], ((e / Cfg::kStages) & 1) ^ 1)) {
+            atomicExch(&g_attn_error, 1);
+            break;
+          }
+          MbarExpectTx(&full[st], Cfg::kTileBytes);
+          TmaLoadTile<HD>(ring + st * Cfg::kTileBytes, e & 1 ? &maps.v : &maps.k, (e >> 1) * kTile, hk, b, &full[st]);
         }
-        MbarExpectTx(&full[st], Cfg::kTileBytes);
-        TmaLoadTile<HD>(ring + st * Cfg::kTileBytes, e & 1 ? &maps.v : &maps.k, (e >> 1) * kTile, hk, b, &full[st]);
       }
-    }
-  } else if (warp == kMmaWarp) {
-    if (total > 0) {
-      const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int parity) {
-        if (ok && !MbarWaitWarp(bar, parity)) {
-          if (lane == 0) atomicExch(&g_attn_error, 2);
-          ok = false;
-        }
-        TcFenceAfter();
-        return ok;
-      };
-      auto entry = [&](int e) { return wait(&full[e % Cfg::kStages], (e / Cfg::kStages) & 1); };
-      auto tile  = [&](int e) { return ring + (e % Cfg::kStages) * Cfg::kTileBytes; };
-      if (wait(q_full, 0) && entry(0)) {
-        if (ElectOne()) {
-          for (int i = 0; i < 2; ++i)
-            if (count[i] > 0) {
-              IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(0)), ksteps);
-              UmmaCommit(&s_full[i]);
-            }
-          UmmaCommit(&empty[0]);
-        }
-        for (int j = 0; j < total && ok; ++j) {
-          const int ev = 2 * j + 1, ek = 2 * j + 2;
-          if (!entry(ev)) break;
-          if (j == tiles - 1 && len < p.s && len % kTile != 0) ClearRows(tile(ev), HD / 64, len % kTile);
-          if (j + 1 < total && !entry(ek)) break;
-          for (int i = 0; i < 2; ++i) {
-            if (j >= count[i]) continue;
-            if (!wait(&p_full[i], j & 1)) break;
-            if (ElectOne()) {
-              // the probabilities lie where the next scores go: products complete in the order of their issue
-              IssueFromTmem<kBf16>(t_o[i], t_s[i], 32, SmemAddr(tile(ev)), n_out, j > 0);
-              if (j + 1 < count[i]) {
-                IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(ek)), ksteps);
+    } else if (warp == kMmaWarp) {
+      if (total > 0) {
+        const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int parity) {
+          if (ok && !MbarWaitWarp(bar, parity)) {
+            if (lane == 0) atomicExch(&g_attn_error, 2);
+            ok = false;
+          }
+          TcFenceAfter();
+          return ok;
+        };
+        auto entry = [&](int e) { return wait(&full[e % Cfg::kStages], (e / Cfg::kStages) & 1); };
+        auto tile  = [&](int e) { return ring + (e % Cfg::kStages) * Cfg::kTileBytes; };
+        if (wait(q_full, 0) && entry(0)) {
+          if (ElectOne()) {
+            for (int i = 0; i < 2; ++i)
+              if (count[i] > 0) {
+                IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(0)), ksteps);
                 UmmaCommit(&s_full[i]);
-              } else {
-                UmmaCommit(&o_full[i]);
+              }
+            UmmaCommit(&empty[0]);
+          }
+          for (int j = 0; j < total && ok; ++j) {
+            const int ev = 2 * j + 1, ek = 2 * j + 2;
+            if (!entry(ev)) break;
+            if (j == tiles - 1 && len < p.s && len % kTile != 0) ClearRows(tile(ev), HD / 64, len % kTile);
+            if (j + 1 < total && !entry(ek)) break;
+            for (int i = 0; i < 2; ++i) {
+              if (j >= count[i]) continue;
+              if (!wait(&p_full[i], j & 1)) break;
+              if (ElectOne()) {
+                // the probabilities lie where the next scores go: products complete in the order of their issue
+                IssueFromTmem<kBf16, 128>(t_o[i], t_s[i], SmemAddr(tile(ev)), n_out, j > 0);
+                if (j + 1 < count[i]) {
+                  IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(ek)), ksteps);
+                  UmmaCommit(&s_full[i]);
+                } else {
+                  UmmaCommit(&o_full[i]);
+                }
               }
             }
-          }
-          if (ok && ElectOne()) {
-            UmmaCommit(&empty[ev % Cfg::kStages]);
-            if (j + 1 < total) UmmaCommit(&empty[ek % Cfg::kStages]);
+            if (ok && ElectOne()) {
+              UmmaCommit(&empty[ev % Cfg::kStages]);
+              if (j + 1 < total) UmmaCommit(&empty[ek % Cfg::kStages]);
+            }
           }
         }
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int i = warp >> 2;             // query tile
     const int quarter = warp & 3;        // TMEM lanes that this warp may access
     const int row = q0 + i * kTile + quarter * 32 + lane;
@@ -368,44 +395,49 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
           for (int k = 0; k < 32; ++k)
             if (g * 32 + k >= limit) s[g][k] = 0xff800000u;  // -inf
       }
-      float top = -INFINITY;
+      float part[8];
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int k = 0; k < 8; ++k) part[k] = __uint_as_float(s[k >> 1][(k & 1) * 16]);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(s[g][k]));
+      for (int k = 1; k < 16; ++k)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) part[u] = fmaxf(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]));
+      float top = fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])),
+                        fmaxf(fmaxf(part[4], part[5]), fmaxf(part[6], part[7])));
       if (top == -INFINITY) top = 0.f;
+      // The exponents' reference may lag behind the maximum by up to 2^8: probabilities of up to 256 lose nothing in 16 bits,
+      // and the output in TMEM is rescaled a few times per row instead of with every new maximum.
       if (j == 0) {
         m = top;
-      } else if (__any_sync(0xffffffffu, top > m)) {
+      } else if (__any_sync(0xffffffffu, (top - m) * p.c > 8.f)) {
         const float up = fmaxf(top, m);
         const float f  = Exp2((m - up) * p.c);
         m = up;
         l *= f;
 #pragma unroll 1
-        for (int g = 0; g < HD / 32; ++g) {
-          uint32_t o[32];
-          TmemLoad32(t_o[i] + lanes + g * 32, o);
+        for (int g = 0; g < HD / 16; ++g) {
+          uint32_t o[16];
+          TmemLoad16(t_o[i] + lanes + g * 16, o);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-          TmemStore32(t_o[i] + lanes + g * 32, o);
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          TmemStore16(t_o[i] + lanes + g * 16, o);
         }
       }
-      const float mc = m * p.c;
-      float sum[2] = {0.f, 0.f};
+      const F2 c2 = Both(p.c), nm = Both(-m * p.c);
+      F2 sum[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float x = Exp2(fmaf(__uint_as_float(s[g][2 * k]), p.c, -mc));
-          const float y = Exp2(fmaf(__uint_as_float(s[g][2 * k + 1]), p.c, -mc));
-          sum[0] += x;
-          sum[1] += y;
-          w[k] = Pack2<kBf16>(x, y);
+          const F2 x = Exp2Fast(Fma2(Pair(s[g][2 * k], s[g][2 * k + 1]), c2, nm));
+          sum[k & 3] = g == 0 && k < 4 ? x : Add2(sum[k & 3], x);
+          w[k] = Pack2<kBf16>(x);
         }
         TmemStore16(t_s[i] + lanes + g * 16, w);
       }
-      l += sum[0] + sum[1];
+      const float2 both = SplitF2(Add2(Add2(sum[0], sum[1]), Add2(sum[2], sum[3])));
+      l += both.x + both.y;
       TmemStoreWait();
       TcFenceBefore();
       __syncwarp();
@@ -425,7 +457,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         for (int g = 0; g < HD / 32; ++g) {
           uint32_t o[32];
           TmemLoad32(t_o[i] + lanes + g * 32, o);
-          if (live) StoreCols32<kBf16>(dst, g * 32, p.d, o, inv);
+          if (live) StoreCols<kBf16, 32>(dst, g * 32, p.d, o, inv);
         }
       }
       if (!live && row < p.s) StoreZeroRow(dst, 0, p.d);
@@ -441,6 +473,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 
 // ---------------------------------------------------------------- backward
 // D_i = dO_i . O_i, eight lanes per row; the heads of a position are neighbours, so contiguous tensors are read in order.
+// Writes [2][b, h, sp]: -L and -D, the addends as the main kernel uses them.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ AttnParams p) {
   const int64_t rows = static_cast<int64_t>(p.b) * p.sp * p.h;
@@ -466,7 +499,11 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
     }
 #pragma unroll
     for (int k = 4; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-    if (part == 0 && r < rows) p.delta[(b * p.h + h) * p.sp + i] = sum;
+    if (part == 0 && r < rows) {
+      const int64_t at = (b * p.h + h) * p.sp + i;
+      p.delta[at]        = -p.lse[at];
+      p.delta[rows + at] = -sum;
+    }
   }
 }
 
@@ -477,7 +514,8 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
 // Both passes compute S and dP, seven products instead of five, and in exchange every sum has one owner: no atomics, no
 // fp32 copy of dQ in memory, and results that do not depend on the order of the blocks.
 // The softmax warps take S of a tile, then its dP; while they work on one, the tensor cores run the products that the
-// other has released and the next tile's.
+// other has released and the next tile's.  Sixteen of them, four per scheduler, each with 32 rows x 32 columns: with eight and
+// 64 columns the chain of loads, exponentials and stores left two thirds of the issue slots empty.
 template <int HD>
 struct BwdCfg {
   static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;
@@ -490,6 +528,7 @@ struct BwdCfg {
 template <int HD, bool kBf16, bool kKeys>
 __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnParams& p, int tile, int b, int head, uint8_t* smem) {
   using Cfg = BwdCfg<HD>;
+  constexpr int kTmaWarp = kBwdWarps, kMmaWarp = kBwdWarps + 1;
   uint8_t* x1     = smem;
   uint8_t* x2     = x1 + Cfg::kTileBytes;
   uint8_t* ring   = x2 + Cfg::kTileBytes;
@@ -514,6 +553,7 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
   const int last  = !kKeys && p.causal ? min(tiles, tile + 1) : tiles;
   const int per   = last - first;
   const int total = x0 >= len ? 0 : per * (kKeys ? group : 1);
+  const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;  // of -L, -D
   const int xhead = head, yhead = kKeys ? head * group : head / group;
 
   if (total > 0) {
@@ -524,9 +564,9 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
       }
       MbarInit(x_full, 1);
       MbarInit(s_full, 1);
-      MbarInit(s_done, 8);
+      MbarInit(s_done, kBwdWarps);
       MbarInit(dp_full, 1);
-      MbarInit(ds_full, 8);
+      MbarInit(ds_full, kBwdWarps);
       MbarInit(acc_full, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -544,8 +584,6 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
     tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   }
   const uint32_t t_s = tmem, t_dp = tmem + 128, t_acc1 = tmem + 256, t_acc2 = tmem + 256 + HD;
-  // a half's 16-bit values start where its 64 fp32 columns do
-  constexpr uint32_t kGap = 64;
 
   if (warp == kTmaWarp) {
     if (total > 0 && ElectOne()) {
@@ -565,8 +603,8 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
         TmaLoadTile<HD>(dst + Cfg::kTileBytes, kKeys ? &maps.dout : &maps.v, y0, yh, b, &full[st]);
         if (kKeys) {
           const int64_t at = (static_cast<int64_t>(b) * p.h + yh) * p.sp + y0;
-          BulkLoad(ld + st * 2 * kTile, p.lse + at, kTile * 4, &full[st]);
-          BulkLoad(ld + st * 2 * kTile + kTile, p.delta + at, kTile * 4, &full[st]);
+          BulkLoad(ld + st * 2 * kTile, p.delta + at, kTile * 4, &full[st]);
+          BulkLoad(ld + st * 2 * kTile + kTile, p.delta + plane + at, kTile * 4, &full[st]);
         }
       }
     }
@@ -607,14 +645,14 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
         for (int it = 0; it < total && ok; ++it) {
           if (!wait(s_done, it & 1)) break;
           if (kKeys && ElectOne())
-            IssueFromTmem<kBf16>(t_acc2, t_s, kGap, SmemAddr(y1(it) + Cfg::kTileBytes), n_out, it > 0);
+            IssueFromTmem<kBf16, 32>(t_acc2, t_s, SmemAddr(y1(it) + Cfg::kTileBytes), n_out, it > 0);
           if (it + 1 < total) {
             if (!arrived(it + 1)) break;
             issue_s(it + 1);
           }
           if (!wait(ds_full, it & 1)) break;
           if (ElectOne()) {
-            IssueFromTmem<kBf16>(t_acc1, t_dp, kGap, SmemAddr(y1(it)), n_out, it > 0);
+            IssueFromTmem<kBf16, 32>(t_acc1, t_dp, SmemAddr(y1(it)), n_out, it > 0);
             UmmaCommit(&empty[it % Cfg::kStages]);
           }
           if (it + 1 < total) issue_dp(it + 1);
@@ -623,15 +661,16 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
       }
     }
   } else {
-    const int quarter = warp & 3, half = warp >> 2;  // TMEM lanes; columns [64 half, 64 half + 64)
+    const int quarter = warp & 3, part = warp >> 2;  // TMEM lanes; columns [32 part, 32 part + 32)
     const int row = x0 + quarter * 32 + lane;
-    const uint32_t at = (static_cast<uint32_t>(quarter * 32) << 16) + half * 64;
-    float row_l = 0.f, row_d = 0.f;
+    const uint32_t at = (static_cast<uint32_t>(quarter * 32) << 16) + part * 32;
+    F2 row_l{}, row_d{};  // -L, -D
     if (!kKeys && total > 0) {  // row < sp
       const int64_t i = (static_cast<int64_t>(b) * p.h + head) * p.sp + row;
-      row_l = p.lse[i];
-      row_d = p.delta[i];
+      row_l = Both(p.delta[i]);
+      row_d = Both(p.delta[plane + i]);
     }
+    const F2 c2 = Both(p.c);
     bool ok = true;
     auto wait = [&](uint64_t* bar, int parity) {
       if (ok && !MbarWaitWarp(bar, parity)) {
@@ -646,80 +685,61 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
       const int y0 = (first + it % per) * kTile;
       if (kKeys && !wait(&full[st], (it / Cfg::kStages) & 1)) break;  // L and D
       if (!wait(s_full, it & 1)) break;
-      uint32_t s[2][32];
-#pragma unroll
-      for (int g = 0; g < 2; ++g) TmemLoad32Async(t_s + at + g * 32, s[g]);
-#pragma unroll
-      for (int g = 0; g < 2; ++g) TmemLoadWait(s[g]);
+      uint32_t s[32];
+      TmemLoad32(t_s + at, s);
       if (!kKeys) {
         TcFenceBefore();
         __syncwarp();
         if (lane == 0) MbarArrive(s_done);
       }
-      const float* ls = ld + st * 2 * kTile + half * 64;
+      const float* ls = ld + st * 2 * kTile + part * 32;
+      F2 pr[16];
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          float4 l4;
-          if (kKeys) l4 = *reinterpret_cast<const float4*>(ls + g * 32 + k);
-          else l4 = make_float4(row_l, row_l, row_l, row_l);
-          s[g][k]     = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k]), p.c, -l4.x)));
-          s[g][k + 1] = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k + 1]), p.c, -l4.y)));
-          s[g][k + 2] = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k + 2]), p.c, -l4.z)));
-          s[g][k + 3] = __float_as_uint(Exp2(fmaf(__uint_as_float(s[g][k + 3]), p.c, -l4.w)));
+      for (int k = 0; k < 16; k += 2) {
+        F2 l0 = row_l, l1 = row_l;
+        if (kKeys) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + 2 * k);
+          l0.v = v.x;
+          l1.v = v.y;
         }
+        pr[k]     = Exp2Fast(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0));
+        pr[k + 1] = Exp2Fast(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1));
+      }
+      if (kKeys ? p.causal && y0 == x0 : y0 + kTile > len || (p.causal && y0 == x0)) {
+        // rows are keys: they count for the queries from their own position on; rows are queries: keys up to a limit
+        const int from  = kKeys ? row - y0 - part * 32 : 0;
+        const int limit = kKeys ? 32 : (p.causal ? min(len, row + 1) : len) - y0 - part * 32;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float2 x = SplitF2(pr[k]);
+          pr[k] = MakeF2(2 * k >= from && 2 * k < limit ? x.x : 0.f, 2 * k + 1 >= from && 2 * k + 1 < limit ? x.y : 0.f);
+        }
+      }
       if (kKeys) {
-        if (p.causal && y0 == x0) {  // a key counts for the queries from its own position on
-          const int from = row - y0 - half * 64;
+        uint32_t w[16];
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (g * 32 + k < from) s[g][k] = 0u;
-        }
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t w[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k)
-            w[k] = Pack2<kBf16>(__uint_as_float(s[g][2 * k]), __uint_as_float(s[g][2 * k + 1]));
-          TmemStore16(t_s + at + g * 16, w);
-        }
+        for (int k = 0; k < 16; ++k) w[k] = Pack2<kBf16>(pr[k]);
+        TmemStore16(t_s + at, w);
         TmemStoreWait();
         TcFenceBefore();
         __syncwarp();
         if (lane == 0) MbarArrive(s_done);
-      } else if (y0 + kTile > len || (p.causal && y0 == x0)) {
-        const int limit = (p.causal ? min(len, row + 1) : len) - y0 - half * 64;
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (g * 32 + k >= limit) s[g][k] = 0u;
       }
       if (!wait(dp_full, it & 1)) break;
-      uint32_t t[2][32];
+      TmemLoad32(t_dp + at, s);
+      uint32_t w[16];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) TmemLoad32Async(t_dp + at + g * 32, t[g]);
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        TmemLoadWait(t[g]);
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          float4 d4;
-          if (kKeys) d4 = *reinterpret_cast<const float4*>(ls + kTile + g * 32 + k);
-          else d4 = make_float4(row_d, row_d, row_d, row_d);
-          const float a0 = __uint_as_float(s[g][k]) * (__uint_as_float(t[g][k]) - d4.x);
-          const float a1 = __uint_as_float(s[g][k + 1]) * (__uint_as_float(t[g][k + 1]) - d4.y);
-          const float a2 = __uint_as_float(s[g][k + 2]) * (__uint_as_float(t[g][k + 2]) - d4.z);
-          const float a3 = __uint_as_float(s[g][k + 3]) * (__uint_as_float(t[g][k + 3]) - d4.w);
-          w[k / 2]     = Pack2<kBf16>(a0, a1);
-          w[k / 2 + 1] = Pack2<kBf16>(a2, a3);
+      for (int k = 0; k < 16; k += 2) {
+        F2 d0 = row_d, d1 = row_d;
+        if (kKeys) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + kTile + 2 * k);
+          d0.v = v.x;
+          d1.v = v.y;
         }
-        TmemStore16(t_dp + at + g * 16, w);
+        w[k]     = Pack2<kBf16>(Mul2(pr[k], Add2(Pair(s[2 * k], s[2 * k + 1]), d0)));
+        w[k + 1] = Pack2<kBf16>(Mul2(pr[k + 1], Add2(Pair(s[2 * k + 2], s[2 * k + 3]), d1)));
       }
+      TmemStore16(t_dp + at, w);
       TmemStoreWait();
       TcFenceBefore();
       __syncwarp();
@@ -728,21 +748,20 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
     if (total > 0) wait(acc_full, 0);
     if (ok) {
       const bool live = row < len;
-      const int c0 = half * (HD / 2);
+      constexpr int kCols = HD / 4;
+      const int c0 = part * kCols;
       const uint32_t acc_at = (static_cast<uint32_t>(quarter * 32) << 16) + c0;
 #pragma unroll
       for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
         const Strides& st = out ? p.sdv : kKeys ? p.sdk : p.sdq;
         uint16_t* dst = static_cast<uint16_t*>(out ? p.dv : kKeys ? p.dk : p.dq) + b * st.b + row * st.s + head * st.h;
         if (total > 0) {
-#pragma unroll 1
-          for (int g = 0; g < HD / 64; ++g) {
-            uint32_t o[32];
-            TmemLoad32((out ? t_acc2 : t_acc1) + acc_at + g * 32, o);
-            if (live) StoreCols32<kBf16>(dst, c0 + g * 32, p.d, o, out ? 1.f : p.scale);
-          }
+          uint32_t o[kCols];
+          if constexpr (kCols == 32) TmemLoad32((out ? t_acc2 : t_acc1) + acc_at, o);
+          else TmemLoad16((out ? t_acc2 : t_acc1) + acc_at, o);
+          if (live) StoreCols<kBf16, kCols>(dst, c0, p.d, o, out ? 1.f : p.scale);
         }
-        if (!live && row < p.s) StoreZeroRow(dst, c0, min(p.d, c0 + HD / 2));
+        if (!live && row < p.s) StoreZeroRow(dst, c0, min(p.d, c0 + kCols));
       }
     }
   }
@@ -756,7 +775,7 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
 // Both passes in one launch, so that neither leaves a tail of idle SMs: first the blocks of the keys, whose tiles stream past
 // every query head of their group.  Causal: the tiles with the longest streams first.
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem   = AlignedSmem(smem_raw);
@@ -845,7 +864,7 @@ int LaunchFwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   int rc = AllowSmem(AttnFwdKernel<HD, kBf16>, FwdCfg<HD>::kSmemBytes, &done);
   if (rc) return rc;
   const int grid = TilesOf(p.s, 2 * kTile) * p.b * p.h;
-  AttnFwdKernel<HD, kBf16><<<grid, kAttnThreads, FwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  AttnFwdKernel<HD, kBf16><<<grid, kFwdThreads, FwdCfg<HD>::kSmemBytes, s>>>(maps, p);
   TIPSK_LAUNCH_CHECK();
   return 0;
 }
@@ -860,7 +879,7 @@ int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   AttnDeltaKernel<kBf16><<<static_cast<int>(rows / 32 < cap ? rows / 32 : cap), 256, 0, s>>>(p);  // sp: whole tiles
   TIPSK_LAUNCH_CHECK();
   const int grid = (p.sp / kTile) * p.b * (p.h + p.hk);
-  AttnBwdKernel<HD, kBf16><<<grid, kAttnThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  AttnBwdKernel<HD, kBf16><<<grid, kBwdThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
   TIPSK_LAUNCH_CHECK();
   return 0;
 }

@@ -151,7 +151,7 @@ def _attention_bwd(dout, q, k, v, out, lse, lengths, scale, causal, dq, dk, dv):
     if out.numel() == 0:
         return
     dout = _rows16(dout)
-    delta = torch.empty_like(lse)
+    delta = torch.empty(2, *lse.shape, dtype=torch.float32, device=lse.device)
     with torch.cuda.device(q.device):
         base.check(base.K().tipsk_attention_bwd(
             dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), delta.data_ptr(),
