@@ -33,9 +33,10 @@ namespace {
 
 constexpr int kTile        = 128;  // rows of a tile of queries or keys
 constexpr int kBoxBytes    = kTile * 128;  // 128 rows of 64 16-bit values
-constexpr int kFwdThreads = 384;  // eight softmax warps, one TMA warp, one MMA warp, two idle ones (whole warpgroups)
-constexpr int kBwdWarps   = 16;   // softmax warps of the backward pass
-constexpr int kBwdThreads = (kBwdWarps + 2) * 32;
+// Softmax warps, and behind them one that issues TMA loads, two that issue MMAs (a wait costs such a warp as much time as an
+// MMA or two, so each gets half of the products) and one that clears rows beyond a sequence's length.
+constexpr int kFwdWarps = 8, kBwdWarps = 16;
+constexpr int kFwdThreads = (kFwdWarps + 4) * 32, kBwdThreads = (kBwdWarps + 4) * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int32_t g_attn_error;  // one per device
@@ -64,6 +65,10 @@ struct AttnMaps {
   CUtensorMap q, k, v, dout;
 };
 
+// A value that all lanes of a warp hold, as the compiler can tell: what is computed from it stays in uniform registers, from
+// which tcgen05.mma takes its operands, and branches on it do not diverge.
+__device__ __forceinline__ uint32_t Uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 __device__ __forceinline__ int SeqLen(const AttnParams& p, int b) {
   if (p.lengths == nullptr) return p.s;
   const int64_t n = p.len64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
@@ -77,10 +82,13 @@ __device__ __forceinline__ void TmaLoadHead(void* dst, const CUtensorMap* map, i
       ::"r"(SmemAddr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(s), "r"(h), "r"(b), "r"(SmemAddr(bar))
       : "memory");
 }
-template <int HD>
+// kRows positions of a head by boxes of kBox rows; a box of 64 columns with all its rows follows the other.
+template <int HD, int kRows, int kBox>
 __device__ __forceinline__ void TmaLoadTile(uint8_t* dst, const CUtensorMap* map, int s, int h, int b, uint64_t* bar) {
 #pragma unroll
-  for (int x = 0; x < HD / 64; ++x) TmaLoadHead(dst + x * kBoxBytes, map, x * 64, s, h, b, bar);
+  for (int x = 0; x < HD / 64; ++x)
+#pragma unroll
+    for (int r = 0; r < kRows; r += kBox) TmaLoadHead(dst + (x * kRows + r) * 128, map, x * 64, s + r, h, b, bar);
 }
 // `bytes` (a multiple of 16) from 16-byte-aligned global memory.
 __device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -152,35 +160,35 @@ __device__ __forceinline__ uint32_t InstrDesc(int n, bool b_mn) {
          (static_cast<uint32_t>(kTile >> 4) << 24);
 }
 
-// [128 x d] x [128 x d]^T: both operands K-major in shared memory, boxes of 64 columns.
-template <bool kBf16>
+// [128 x d] x [kN x d]^T: both operands K-major in shared memory, boxes of 64 columns.
+template <bool kBf16, int kD, int kN>
 __device__ __forceinline__ void IssueScores(uint32_t tmem_d, uint32_t a_addr, uint32_t b_addr, int ksteps) {
   const uint64_t a = SmemDescSw128(a_addr), b = SmemDescSw128(b_addr);
-  const uint32_t idesc = InstrDesc<kBf16>(kTile, false);
-#pragma unroll 4
-  for (int k = 0; k < ksteps; ++k) {
-    const uint32_t off = (k >> 2) * (kBoxBytes >> 4) + (k & 3) * 2;
-    UmmaBf16(tmem_d, a + off, b + off, idesc, k > 0);
+  const uint32_t idesc = InstrDesc<kBf16>(kN, false);
+#pragma unroll
+  for (int k = 0; k < kD / 16; ++k) {
+    if (k < ksteps) UmmaBf16(tmem_d, a + (k >> 2) * (kBoxBytes >> 4) + (k & 3) * 2, b + (k >> 2) * (kN * 128 >> 4) + (k & 3) * 2, idesc, k > 0);
   }
 }
-// [128 x 128] (16-bit, TMEM) x [128 x n]: B MN-major in shared memory.  The columns of A lie in runs of kRun, two per TMEM
+// [128 x kK] (16-bit, TMEM) x [kK x n]: B MN-major in shared memory.  The columns of A lie in runs of kRun, two per TMEM
 // column, kRun columns apart (each where the fp32 values that it was made of had been).
-template <bool kBf16, int kRun>
+template <bool kBf16, int kK, int kRun>
 __device__ __forceinline__ void IssueFromTmem(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_addr, int n, bool accum) {
-  const uint64_t b     = SmemDescMnSw128(b_addr, kBoxBytes);
+  const uint64_t b     = SmemDescMnSw128(b_addr, kK * 128);
   const uint32_t idesc = InstrDesc<kBf16>(n, true);
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
+  for (int k = 0; k < kK / 16; ++k)
     UmmaTmemA(tmem_d, tmem_a + k * 16 / kRun * kRun + k * 16 % kRun / 2, b + 128 * k, idesc, accum || k > 0);
 }
 
-// Clears rows [first, 128) of a tile of `boxes` boxes (a whole warp; the swizzle stays within a row's 128 bytes) and
+// Clears rows [first, kRows) of `boxes` boxes of kRows rows (a whole warp; the swizzle stays within a row's 128 bytes) and
 // orders the writes before the MMAs that follow.
+template <int kRows>
 __device__ __forceinline__ void ClearRows(uint8_t* tile, int boxes, int first) {
   const int lane = threadIdx.x & 31;
   for (int x = 0; x < boxes; ++x)
-    for (int i = first * 8 + lane; i < kTile * 8; i += 32)
-      *reinterpret_cast<uint4*>(tile + x * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
+    for (int i = first * 8 + lane; i < kRows * 8; i += 32)
+      *reinterpret_cast<uint4*>(tile + (x * kRows * 8 + i) * 16) = make_uint4(0, 0, 0, 0);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }
@@ -207,11 +215,35 @@ __device__ __forceinline__ float Exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Maximum that hands on a NaN of either operand.
+__device__ __forceinline__ float MaxNan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ F2 Add2(F2 a, F2 b) {
   F2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
+// 2^x of two values on the FMA pipe, for a share of the exponentials: ex2.approx runs at 16 per SM and clock, and a tile has
+// 16384.  x = n + f with n = rint(x) (by adding 1.5 * 2^23, whose last bits then hold n), |f| <= 0.5; 2^f by the polynomial of
+// degree 4 with the least relative error on that interval (2.6e-6, by the Remez exchange); times 2^n, made of n's bits.
+// Below -127 the result is 0 (2^-127 has a zero exponent field), a NaN stays one.
+__device__ __forceinline__ F2 Exp2Poly(F2 x) {
+  const float2 v = SplitF2(x);
+  x = MakeF2(MaxNan(v.x, -127.f), MaxNan(v.y, -127.f));
+  const F2 t = Add2(x, Both(12582912.f));
+  const F2 f = Fma2(Add2(t, Both(-12582912.f)), Both(-1.f), x);
+  F2 q = Fma2(f, Both(0.009570102207362652f), Both(0.05591785907745361f));
+  q = Fma2(q, f, Both(0.240247443318367f));
+  q = Fma2(q, f, Both(0.6931217908859253f));
+  q = Fma2(q, f, Both(0.9999992847442627f));
+  const float2 n = SplitF2(t);
+  return Mul2(q, MakeF2(__int_as_float((__float_as_int(n.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(n.y) << 23) + 0x3f800000)));
+}
+// Pair k of a run: every other one by the polynomial.
+__device__ __forceinline__ F2 Exp2Mixed(F2 x, int k) { return k & 1 ? Exp2Poly(x) : Exp2Fast(x); }
 __device__ __forceinline__ F2 Pair(uint32_t a, uint32_t b) { return MakeF2(__uint_as_float(a), __uint_as_float(b)); }
 template <bool kBf16>
 __device__ __forceinline__ uint32_t Pack2(F2 a) {
@@ -238,7 +270,7 @@ template <int HD, bool kBf16>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   using Cfg = FwdCfg<HD>;
-  constexpr int kTmaWarp = 8, kMmaWarp = 9;
+  constexpr int kTmaWarp = kFwdWarps, kMmaWarp = kFwdWarps + 1, kClearWarp = kFwdWarps + 3;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem_q   = AlignedSmem(smem_raw);
   uint8_t* ring     = smem_q + 2 * Cfg::kTileBytes;
@@ -248,9 +280,10 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   uint64_t* s_full  = q_full + 1;            // [2] scores of a tile are in TMEM
   uint64_t* p_full  = s_full + 2;            // [2] its probabilities are
   uint64_t* o_full  = p_full + 2;            // [2] the last product of a tile has completed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* raw     = o_full + 2;            // [1] the last tile of V has arrived and has rows to clear before it counts as full
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   // causal: the tiles with the most keys first; otherwise neighbours share a head's keys
   const int blocks_q = TilesOf(p.s, 2 * kTile);
   const int heads    = p.b * p.h;
@@ -258,7 +291,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   const int bh = p.causal ? static_cast<int>(blockIdx.x) % heads : static_cast<int>(blockIdx.x) / blocks_q;
   const int b = bh / p.h, h = bh % p.h, hk = h / (p.h / p.hk);
   const int q0  = qb * 2 * kTile;
-  const int len = SeqLen(p, b);
+  const int len = Uniform(SeqLen(p, b));
   const int tiles = TilesOf(len, kTile);
   int count[2];  // key tiles of either query tile
 #pragma unroll
@@ -267,14 +300,16 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     count[i] = first >= len ? 0 : p.causal ? min(tiles, first / kTile + 1) : tiles;
   }
   const int total = max(count[0], count[1]);
+  const bool ragged = total == tiles && len < p.s && len % kTile != 0;  // the last tile of V has rows to clear
 
   if (total > 0) {
     if (threadIdx.x == 0) {
       for (int s = 0; s < Cfg::kStages; ++s) {
         MbarInit(&full[s], 1);
-        MbarInit(&empty[s], 1);
+        MbarInit(&empty[s], 2);  // both MMA warps
       }
       MbarInit(q_full, 1);
+      MbarInit(raw, 1);
       for (int i = 0; i < 2; ++i) {
         MbarInit(&s_full[i], 1);
         MbarInit(&p_full[i], 4);
@@ -293,7 +328,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   uint32_t tmem = 0;
   if (total > 0) {
     TcFenceAfter();
-    tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
   }
   // columns: scores of either tile (their probabilities in the same place), then either output
   const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + HD};
@@ -304,65 +339,70 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     if (warp == kTmaWarp) {
       if (total > 0 && ElectOne()) {
         MbarExpectTx(q_full, 2 * Cfg::kTileBytes);
-        TmaLoadTile<HD>(smem_q, &maps.q, q0, h, b, q_full);
-        TmaLoadTile<HD>(smem_q + Cfg::kTileBytes, &maps.q, q0 + kTile, h, b, q_full);
+        TmaLoadTile<HD, kTile, kTile>(smem_q, &maps.q, q0, h, b, q_full);
+        TmaLoadTile<HD, kTile, kTile>(smem_q + Cfg::kTileBytes, &maps.q, q0 + kTile, h, b, q_full);
         for (int e = 0; e < 2 * total; ++e) {
           const int st = e % Cfg::kStages;
           if (!MbarWait(&empty[st], ((e / Cfg::kStages) & 1) ^ 1)) {
             atomicExch(&g_attn_error, 1);
             break;
           }
-          MbarExpectTx(&full[st], Cfg::kTileBytes);
-          TmaLoadTile<HD>(ring + st * Cfg::kTileBytes, e & 1 ? &maps.v : &maps.k, (e >> 1) * kTile, hk, b, &full[st]);
+          uint64_t* bar = ragged && e == 2 * total - 1 ? raw : &full[st];
+          MbarExpectTx(bar, Cfg::kTileBytes);
+          TmaLoadTile<HD, kTile, kTile>(ring + st * Cfg::kTileBytes, e & 1 ? &maps.v : &maps.k, (e >> 1) * kTile, hk, b, bar);
         }
       }
-    } else if (warp == kMmaWarp) {
-      if (total > 0) {
-        const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, int parity) {
-          if (ok && !MbarWaitWarp(bar, parity)) {
-            if (lane == 0) atomicExch(&g_attn_error, 2);
-            ok = false;
-          }
-          TcFenceAfter();
-          return ok;
-        };
-        auto entry = [&](int e) { return wait(&full[e % Cfg::kStages], (e / Cfg::kStages) & 1); };
-        auto tile  = [&](int e) { return ring + (e % Cfg::kStages) * Cfg::kTileBytes; };
-        if (wait(q_full, 0) && entry(0)) {
+    } else if (warp == kClearWarp) {
+      if (total > 0 && ragged) {
+        const int e = 2 * total - 1, st = e % Cfg::kStages;
+        if (MbarWaitWarp(raw, 0)) {
+          ClearRows<kTile>(ring + st * Cfg::kTileBytes, HD / 64, len % kTile);
+          if (lane == 0) MbarArrive(&full[st]);
+        } else if (lane == 0) {
+          atomicExch(&g_attn_error, 2);
+        }
+      }
+    } else if (total > 0) {
+      const int i = warp - kMmaWarp;  // query tile
+      const int mine = count[i], ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
+      const uint32_t q_addr = SmemAddr(smem_q + i * Cfg::kTileBytes);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity) {
+        if (ok && !MbarWaitWarp(bar, parity)) {
+          if (lane == 0) atomicExch(&g_attn_error, 3);
+          ok = false;
+        }
+        TcFenceAfter();
+        return ok;
+      };
+      auto entry = [&](int e) { return wait(&full[e % Cfg::kStages], (e / Cfg::kStages) & 1); };
+      auto tile  = [&](int e) { return SmemAddr(ring + (e % Cfg::kStages) * Cfg::kTileBytes); };
+      if (wait(q_full, 0) && entry(0) && ElectOne()) {
+        if (mine > 0) {
+          IssueScores<kBf16, HD, kTile>(t_s[i], q_addr, tile(0), ksteps);
+          UmmaCommit(&s_full[i]);
+        }
+        UmmaCommit(&empty[0]);
+      }
+      for (int j = 0; j < total && ok; ++j) {  // a tile with fewer keys than the other hands on the rest
+        const int ev = 2 * j + 1, ek = 2 * j + 2;
+        if (!entry(ev) || (j + 1 < total && !entry(ek))) break;
+        if (j < mine) {
+          if (!wait(&p_full[i], j & 1)) break;
           if (ElectOne()) {
-            for (int i = 0; i < 2; ++i)
-              if (count[i] > 0) {
-                IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(0)), ksteps);
-                UmmaCommit(&s_full[i]);
-              }
-            UmmaCommit(&empty[0]);
-          }
-          for (int j = 0; j < total && ok; ++j) {
-            const int ev = 2 * j + 1, ek = 2 * j + 2;
-            if (!entry(ev)) break;
-            if (j == tiles - 1 && len < p.s && len % kTile != 0) ClearRows(tile(ev), HD / 64, len % kTile);
-            if (j + 1 < total && !entry(ek)) break;
-            for (int i = 0; i < 2; ++i) {
-              if (j >= count[i]) continue;
-              if (!wait(&p_full[i], j & 1)) break;
-              if (ElectOne()) {
-                // the probabilities lie where the next scores go: products complete in the order of their issue
-                IssueFromTmem<kBf16, 128>(t_o[i], t_s[i], SmemAddr(tile(ev)), n_out, j > 0);
-                if (j + 1 < count[i]) {
-                  IssueScores<kBf16>(t_s[i], SmemAddr(smem_q + i * Cfg::kTileBytes), SmemAddr(tile(ek)), ksteps);
-                  UmmaCommit(&s_full[i]);
-                } else {
-                  UmmaCommit(&o_full[i]);
-                }
-              }
-            }
-            if (ok && ElectOne()) {
-              UmmaCommit(&empty[ev % Cfg::kStages]);
-              if (j + 1 < total) UmmaCommit(&empty[ek % Cfg::kStages]);
+            // the probabilities lie where the next scores go: products complete in the order of their issue
+            IssueFromTmem<kBf16, kTile, kTile>(t_o[i], t_s[i], tile(ev), n_out, j > 0);
+            if (j + 1 < mine) {
+              IssueScores<kBf16, HD, kTile>(t_s[i], q_addr, tile(ek), ksteps);
+              UmmaCommit(&s_full[i]);
+            } else {
+              UmmaCommit(&o_full[i]);
             }
           }
+        }
+        if (ElectOne()) {
+          UmmaCommit(&empty[ev % Cfg::kStages]);
+          if (j + 1 < total) UmmaCommit(&empty[ek % Cfg::kStages]);
         }
       }
     }
@@ -376,7 +416,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     bool ok = true;
     for (int j = 0; j < count[i]; ++j) {
       if (!MbarWaitWarp(&s_full[i], j & 1)) {
-        if (lane == 0) atomicExch(&g_attn_error, 3);
+        if (lane == 0) atomicExch(&g_attn_error, 4);
         ok = false;
         break;
       }
@@ -401,16 +441,18 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 #pragma unroll
       for (int k = 1; k < 16; ++k)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) part[u] = fmaxf(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]));
-      float top = fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])),
-                        fmaxf(fmaxf(part[4], part[5]), fmaxf(part[6], part[7])));
+        for (int u = 0; u < 8; ++u) part[u] = MaxNan(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]));
+      float top = MaxNan(MaxNan(MaxNan(part[0], part[1]), MaxNan(part[2], part[3])),
+                         MaxNan(MaxNan(part[4], part[5]), MaxNan(part[6], part[7])));
+      // a row without any key so far; and inf - inf: the row is NaN, as by the formula
       if (top == -INFINITY) top = 0.f;
+      else if (top == INFINITY) top = __uint_as_float(0x7fc00000u);
       // The exponents' reference may lag behind the maximum by up to 2^8: probabilities of up to 256 lose nothing in 16 bits,
       // and the output in TMEM is rescaled a few times per row instead of with every new maximum.
       if (j == 0) {
         m = top;
-      } else if (__any_sync(0xffffffffu, (top - m) * p.c > 8.f)) {
-        const float up = fmaxf(top, m);
+      } else if (__any_sync(0xffffffffu, !((top - m) * p.c <= 8.f))) {
+        const float up = MaxNan(top, m);
         const float f  = Exp2((m - up) * p.c);
         m = up;
         l *= f;
@@ -430,7 +472,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const F2 x = Exp2Fast(Fma2(Pair(s[g][2 * k], s[g][2 * k + 1]), c2, nm));
+          const F2 x = Exp2Mixed(Fma2(Pair(s[g][2 * k], s[g][2 * k + 1]), c2, nm), k);
           sum[k & 3] = g == 0 && k < 4 ? x : Add2(sum[k & 3], x);
           w[k] = Pack2<kBf16>(x);
         }
@@ -507,52 +549,55 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
   }
 }
 
-// One tile of 128 keys (kKeys) or queries (!kKeys) stays, the tiles of the other side stream past it:
+// One tile of 128 keys (kKeys) or queries (!kKeys) stays, the tiles of the other side (units) stream past it:
 //             stays (X1, X2)   streams (Y1, Y2)   S = X1 Y1^T, dP = X2 Y2^T       accumulated
 //   kKeys     K, V             Q, dO              rows are keys: P^T and dS^T     dV += P^T dO,  dK += dS^T Q
 //   !kKeys    Q, dO            K, V               rows are queries                dQ += dS K
 // Both passes compute S and dP, seven products instead of five, and in exchange every sum has one owner: no atomics, no
 // fp32 copy of dQ in memory, and results that do not depend on the order of the blocks.
-// The softmax warps take S of a tile, then its dP; while they work on one, the tensor cores run the products that the
-// other has released and the next tile's.  Sixteen of them, four per scheduler, each with 32 rows x 32 columns: with eight and
-// 64 columns the chain of loads, exponentials and stores left two thirds of the issue slots empty.
+// The softmax warps take S of a unit, then its dP; while they work on one, the tensor cores run the products that the other has
+// released and the next unit's.  Sixteen of them, four per scheduler, each with 32 rows x 32 columns.
+constexpr int kUnit = 128;
 template <int HD>
 struct BwdCfg {
   static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;
-  static constexpr int kStages     = HD == 64 ? 4 : 2;
   static constexpr int kStageBytes = 2 * kTileBytes;           // Y1, Y2
-  static constexpr int kRowBytes   = 2 * kTile * 4;            // L and D of a streamed tile of queries
+  static constexpr int kStages     = HD == 64 ? 4 : 2;
+  static constexpr int kSBufs      = HD == 64 ? 2 : 1;         // scores in TMEM; with 128 columns of either accumulator there is room for one
+  static constexpr int kRowBytes   = 2 * kUnit * 4;            // -L and -D of a unit of queries
   static constexpr int kSmemBytes  = 2 * kTileBytes + kStages * (kStageBytes + kRowBytes) + 1024 + 256;
 };
 
 template <int HD, bool kBf16, bool kKeys>
 __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnParams& p, int tile, int b, int head, uint8_t* smem) {
   using Cfg = BwdCfg<HD>;
-  constexpr int kTmaWarp = kBwdWarps, kMmaWarp = kBwdWarps + 1;
+  constexpr int kTmaWarp = kBwdWarps, kMmaWarp = kBwdWarps + 1, kClearWarp = kBwdWarps + 3;
   uint8_t* x1     = smem;
   uint8_t* x2     = x1 + Cfg::kTileBytes;
   uint8_t* ring   = x2 + Cfg::kTileBytes;
   float* ld       = reinterpret_cast<float*>(ring + Cfg::kStages * Cfg::kStageBytes);
-  uint64_t* full  = reinterpret_cast<uint64_t*>(ld + Cfg::kStages * 2 * kTile);
+  uint64_t* full  = reinterpret_cast<uint64_t*>(ld + Cfg::kStages * 2 * kUnit);
   uint64_t* empty = full + Cfg::kStages;
   uint64_t* x_full   = empty + Cfg::kStages;
-  uint64_t* s_full   = x_full + 1;    // S of a tile is in TMEM
-  uint64_t* s_done   = s_full + 1;    // keys: P has taken its place; queries: S has been read
-  uint64_t* dp_full  = s_done + 1;    // dP is in TMEM
+  uint64_t* s_full   = x_full + 1;    // [2] S of a unit is in TMEM
+  uint64_t* s_done   = s_full + 2;    // [2] keys: P has taken its place; queries: S has been read
+  uint64_t* dp_full  = s_done + 2;    // dP is in TMEM
   uint64_t* ds_full  = dp_full + 1;   // dS has taken its place
   uint64_t* acc_full = ds_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* cleared  = acc_full + 1;  // [stages] the unit has no rows beyond the length (any more)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cleared + Cfg::kStages);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int group = p.h / p.hk;
   const int x0    = tile * kTile;
-  const int len   = SeqLen(p, b);
-  const int tiles = TilesOf(len, kTile);
-  // streamed tiles: [first, last) of each of `heads` heads, starting at head `head0`
-  const int first = kKeys && p.causal ? tile : 0;
-  const int last  = !kKeys && p.causal ? min(tiles, tile + 1) : tiles;
+  const int len   = Uniform(SeqLen(p, b));
+  const int units = TilesOf(len, kUnit);
+  // streamed units: [first, last) of the one head, or of each head of the group
+  const int first = kKeys && p.causal ? x0 / kUnit : 0;
+  const int last  = !kKeys && p.causal ? min(units, x0 / kUnit + kTile / kUnit) : units;
   const int per   = last - first;
   const int total = x0 >= len ? 0 : per * (kKeys ? group : 1);
+  const bool ragged = last == units && len < p.s && len % kUnit != 0;  // a head's last unit has rows to clear
   const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;  // of -L, -D
   const int xhead = head, yhead = kKeys ? head * group : head / group;
 
@@ -560,14 +605,17 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
     if (threadIdx.x == 0) {
       for (int s = 0; s < Cfg::kStages; ++s) {
         MbarInit(&full[s], 1);
-        MbarInit(&empty[s], 1);
+        MbarInit(&empty[s], 2);  // both MMA warps
+        MbarInit(&cleared[s], 1);
       }
       MbarInit(x_full, 1);
-      MbarInit(s_full, 1);
-      MbarInit(s_done, kBwdWarps);
+      for (int i = 0; i < Cfg::kSBufs; ++i) {
+        MbarInit(&s_full[i], 1);
+        MbarInit(&s_done[i], kBwdWarps);
+      }
       MbarInit(dp_full, 1);
       MbarInit(ds_full, kBwdWarps);
-      MbarInit(acc_full, 1);
+      MbarInit(acc_full, 2);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -581,37 +629,50 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
   uint32_t tmem = 0;
   if (total > 0) {
     TcFenceAfter();
-    tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
   }
+  // columns: S, dP, the accumulators, the other S
   const uint32_t t_s = tmem, t_dp = tmem + 128, t_acc1 = tmem + 256, t_acc2 = tmem + 256 + HD;
+  auto s_buf = [&](int u) { return Cfg::kSBufs == 1 ? 0 : u & 1; };
+  auto s_par = [&](int u) { return Cfg::kSBufs == 1 ? u & 1 : (u >> 1) & 1; };
+  auto s_col = [&](int u) { return t_s + s_buf(u) * 384; };
 
   if (warp == kTmaWarp) {
     if (total > 0 && ElectOne()) {
       MbarExpectTx(x_full, 2 * Cfg::kTileBytes);
-      TmaLoadTile<HD>(x1, kKeys ? &maps.k : &maps.q, x0, xhead, b, x_full);
-      TmaLoadTile<HD>(x2, kKeys ? &maps.v : &maps.dout, x0, xhead, b, x_full);
-      for (int it = 0; it < total; ++it) {
-        const int st = it % Cfg::kStages;
-        if (!MbarWait(&empty[st], ((it / Cfg::kStages) & 1) ^ 1)) {
+      TmaLoadTile<HD, kTile, kUnit>(x1, kKeys ? &maps.k : &maps.q, x0, xhead, b, x_full);
+      TmaLoadTile<HD, kTile, kUnit>(x2, kKeys ? &maps.v : &maps.dout, x0, xhead, b, x_full);
+      for (int u = 0; u < total; ++u) {
+        const int st = u % Cfg::kStages;
+        if (!MbarWait(&empty[st], ((u / Cfg::kStages) & 1) ^ 1)) {
           atomicExch(&g_attn_error, 5);
           break;
         }
-        const int y0 = (first + it % per) * kTile, yh = yhead + it / per;
+        const int y0 = (first + u % per) * kUnit, yh = yhead + u / per;
         MbarExpectTx(&full[st], Cfg::kStageBytes + (kKeys ? Cfg::kRowBytes : 0));
         uint8_t* dst = ring + st * Cfg::kStageBytes;
-        TmaLoadTile<HD>(dst, kKeys ? &maps.q : &maps.k, y0, yh, b, &full[st]);
-        TmaLoadTile<HD>(dst + Cfg::kTileBytes, kKeys ? &maps.dout : &maps.v, y0, yh, b, &full[st]);
+        TmaLoadTile<HD, kUnit, kUnit>(dst, kKeys ? &maps.q : &maps.k, y0, yh, b, &full[st]);
+        TmaLoadTile<HD, kUnit, kUnit>(dst + Cfg::kTileBytes, kKeys ? &maps.dout : &maps.v, y0, yh, b, &full[st]);
         if (kKeys) {
           const int64_t at = (static_cast<int64_t>(b) * p.h + yh) * p.sp + y0;
-          BulkLoad(ld + st * 2 * kTile, p.delta + at, kTile * 4, &full[st]);
-          BulkLoad(ld + st * 2 * kTile + kTile, p.delta + plane + at, kTile * 4, &full[st]);
+          BulkLoad(ld + st * 2 * kUnit, p.delta + at, kUnit * 4, &full[st]);
+          BulkLoad(ld + st * 2 * kUnit + kUnit, p.delta + plane + at, kUnit * 4, &full[st]);
         }
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == kClearWarp) {
+    for (int u = 0; ragged && u < total; ++u) {  // every unit passes here, so that the phases match those of `full`
+      const int st = u % Cfg::kStages;
+      if (!MbarWaitWarp(&full[st], (u / Cfg::kStages) & 1)) {
+        if (lane == 0) atomicExch(&g_attn_error, 6);
+        break;
+      }
+      if (u % per == per - 1) ClearRows<kUnit>(ring + st * Cfg::kStageBytes, 2 * (HD / 64), len % kUnit);
+      if (lane == 0) MbarArrive(&cleared[st]);
+    }
+  } else if (warp >= kMmaWarp) {
     if (total > 0) {
       const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-      const bool ragged = len < p.s && len % kTile != 0;
       bool ok = true;
       auto wait = [&](uint64_t* bar, int parity) {
         if (ok && !MbarWaitWarp(bar, parity)) {
@@ -621,49 +682,49 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
         TcFenceAfter();
         return ok;
       };
-      auto y1 = [&](int it) { return ring + (it % Cfg::kStages) * Cfg::kStageBytes; };
-      auto arrived = [&](int it) {
-        if (!wait(&full[it % Cfg::kStages], (it / Cfg::kStages) & 1)) return false;
-        if (ragged && first + it % per == tiles - 1) ClearRows(y1(it), 2 * (HD / 64), len % kTile);
-        return true;
-      };
-      auto issue_s = [&](int it) {
-        if (ElectOne()) {
-          IssueScores<kBf16>(t_s, SmemAddr(x1), SmemAddr(y1(it)), ksteps);
-          UmmaCommit(s_full);
-        }
-      };
-      auto issue_dp = [&](int it) {
-        if (ElectOne()) {
-          IssueScores<kBf16>(t_dp, SmemAddr(x2), SmemAddr(y1(it) + Cfg::kTileBytes), ksteps);
-          UmmaCommit(dp_full);
-        }
-      };
-      if (wait(x_full, 0) && arrived(0)) {
-        issue_s(0);
-        issue_dp(0);
-        for (int it = 0; it < total && ok; ++it) {
-          if (!wait(s_done, it & 1)) break;
-          if (kKeys && ElectOne())
-            IssueFromTmem<kBf16, 32>(t_acc2, t_s, SmemAddr(y1(it) + Cfg::kTileBytes), n_out, it > 0);
-          if (it + 1 < total) {
-            if (!arrived(it + 1)) break;
-            issue_s(it + 1);
-          }
-          if (!wait(ds_full, it & 1)) break;
+      auto y1 = [&](int u) { return SmemAddr(ring + (u % Cfg::kStages) * Cfg::kStageBytes); };
+      auto y2 = [&](int u) { return y1(u) + Cfg::kTileBytes; };
+      uint64_t* ready = ragged ? cleared : full;
+      auto arrived = [&](int u) { return wait(&ready[u % Cfg::kStages], (u / Cfg::kStages) & 1); };
+      wait(x_full, 0);
+      if (warp == kMmaWarp) {  // S, and P^T dO
+        auto scores = [&](int u) {
+          IssueScores<kBf16, HD, kUnit>(s_col(u), SmemAddr(x1), y1(u), ksteps);
+          UmmaCommit(&s_full[s_buf(u)]);
+        };
+        for (int u = 0; u < min(Cfg::kSBufs, total) && arrived(u); ++u)
+          if (ElectOne()) scores(u);
+        for (int u = 0; u < total && ok; ++u) {
+          const int next = u + Cfg::kSBufs;
+          if ((next < total && !arrived(next)) || !wait(&s_done[s_buf(u)], s_par(u))) break;
           if (ElectOne()) {
-            IssueFromTmem<kBf16, 32>(t_acc1, t_dp, SmemAddr(y1(it)), n_out, it > 0);
-            UmmaCommit(&empty[it % Cfg::kStages]);
+            if (kKeys) IssueFromTmem<kBf16, kUnit, 32>(t_acc2, s_col(u), y2(u), n_out, u > 0);
+            UmmaCommit(&empty[u % Cfg::kStages]);
+            if (next < total) scores(next);  // in the place of P, which the product before it reads
           }
-          if (it + 1 < total) issue_dp(it + 1);
         }
-        if (ok && ElectOne()) UmmaCommit(acc_full);
+      } else {  // dP, and dS^T Q or dS K
+        auto grads = [&](int u) {
+          IssueScores<kBf16, HD, kUnit>(t_dp, SmemAddr(x2), y2(u), ksteps);
+          UmmaCommit(dp_full);
+        };
+        if (arrived(0) && ElectOne()) grads(0);
+        for (int u = 0; u < total && ok; ++u) {
+          if ((u + 1 < total && !arrived(u + 1)) || !wait(ds_full, u & 1)) break;
+          if (ElectOne()) {
+            IssueFromTmem<kBf16, kUnit, 32>(t_acc1, t_dp, y1(u), n_out, u > 0);
+            UmmaCommit(&empty[u % Cfg::kStages]);
+            if (u + 1 < total) grads(u + 1);
+          }
+        }
       }
+      if (ok && ElectOne()) UmmaCommit(acc_full);
     }
   } else {
-    const int quarter = warp & 3, part = warp >> 2;  // TMEM lanes; columns [32 part, 32 part + 32)
+    const int quarter = warp & 3;    // TMEM lanes
+    const int col = (warp >> 2) * 32;  // first column of this warp in a unit
     const int row = x0 + quarter * 32 + lane;
-    const uint32_t at = (static_cast<uint32_t>(quarter * 32) << 16) + part * 32;
+    const uint32_t at = (static_cast<uint32_t>(quarter * 32) << 16) + col;
     F2 row_l{}, row_d{};  // -L, -D
     if (!kKeys && total > 0) {  // row < sp
       const int64_t i = (static_cast<int64_t>(b) * p.h + head) * p.sp + row;
@@ -680,19 +741,21 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
       TcFenceAfter();
       return ok;
     };
-    for (int it = 0; it < total; ++it) {
-      const int st = it % Cfg::kStages;
-      const int y0 = (first + it % per) * kTile;
-      if (kKeys && !wait(&full[st], (it / Cfg::kStages) & 1)) break;  // L and D
-      if (!wait(s_full, it & 1)) break;
+    for (int u = 0; u < total; ++u) {
+      const int st = u % Cfg::kStages;
+      const int y0 = (first + u % per) * kUnit;
+      if (!wait(&s_full[s_buf(u)], s_par(u))) break;
       uint32_t s[32];
-      TmemLoad32(t_s + at, s);
+      TmemLoad32Async(s_col(u) + at, s);
+      const bool here = !kKeys || wait(&full[st], (u / Cfg::kStages) & 1);  // -L and -D
+      TmemLoadWait(s);
+      if (!here) break;
       if (!kKeys) {
         TcFenceBefore();
         __syncwarp();
-        if (lane == 0) MbarArrive(s_done);
+        if (lane == 0) MbarArrive(&s_done[s_buf(u)]);
       }
-      const float* ls = ld + st * 2 * kTile + part * 32;
+      const float* ls = ld + st * 2 * kUnit + col;
       F2 pr[16];
 #pragma unroll
       for (int k = 0; k < 16; k += 2) {
@@ -702,13 +765,13 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
           l0.v = v.x;
           l1.v = v.y;
         }
-        pr[k]     = Exp2Fast(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0));
-        pr[k + 1] = Exp2Fast(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1));
+        pr[k]     = Exp2Mixed(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0), k);
+        pr[k + 1] = Exp2Mixed(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1), k + 1);
       }
-      if (kKeys ? p.causal && y0 == x0 : y0 + kTile > len || (p.causal && y0 == x0)) {
+      if (kKeys ? p.causal && y0 < x0 + kTile : y0 + kUnit > len || (p.causal && y0 >= x0)) {
         // rows are keys: they count for the queries from their own position on; rows are queries: keys up to a limit
-        const int from  = kKeys ? row - y0 - part * 32 : 0;
-        const int limit = kKeys ? 32 : (p.causal ? min(len, row + 1) : len) - y0 - part * 32;
+        const int from  = kKeys ? row - y0 - col : 0;
+        const int limit = kKeys ? 32 : (p.causal ? min(len, row + 1) : len) - y0 - col;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const float2 x = SplitF2(pr[k]);
@@ -719,20 +782,20 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) w[k] = Pack2<kBf16>(pr[k]);
-        TmemStore16(t_s + at, w);
+        TmemStore16(s_col(u) + at, w);
         TmemStoreWait();
         TcFenceBefore();
         __syncwarp();
-        if (lane == 0) MbarArrive(s_done);
+        if (lane == 0) MbarArrive(&s_done[s_buf(u)]);
       }
-      if (!wait(dp_full, it & 1)) break;
+      if (!wait(dp_full, u & 1)) break;
       TmemLoad32(t_dp + at, s);
       uint32_t w[16];
 #pragma unroll
       for (int k = 0; k < 16; k += 2) {
         F2 d0 = row_d, d1 = row_d;
         if (kKeys) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + kTile + 2 * k);
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + kUnit + 2 * k);
           d0.v = v.x;
           d1.v = v.y;
         }
@@ -749,7 +812,7 @@ __device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnPara
     if (ok) {
       const bool live = row < len;
       constexpr int kCols = HD / 4;
-      const int c0 = part * kCols;
+      const int c0 = (warp >> 2) * kCols;
       const uint32_t acc_at = (static_cast<uint32_t>(quarter * 32) << 16) + c0;
 #pragma unroll
       for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
@@ -795,15 +858,16 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 
 // ---------------------------------------------------------------- host side
 
-// One head-split tensor [b, s, heads, d] with any strides that are multiples of 16 bytes; boxes of 64 columns x 128 positions.
-int HeadMap(CUtensorMap* out, const void* base, int dtype, int b, int s, int heads, int d, const Strides& st) {
+// One head-split tensor [b, s, heads, d] with any strides that are multiples of 16 bytes; boxes of 64 columns x
+// box_rows positions.
+int HeadMap(CUtensorMap* out, const void* base, int dtype, int b, int s, int heads, int d, const Strides& st, int box_rows) {
   EncodeFn enc = GetEncodeFn();
   if (!enc) return SetError(-7, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t dims[4]    = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(s), static_cast<cuuint64_t>(heads),
                            static_cast<cuuint64_t>(b)};
   cuuint64_t strides[3] = {static_cast<cuuint64_t>(st.s) * 2, static_cast<cuuint64_t>(st.h) * 2,
                            static_cast<cuuint64_t>(st.b) * 2};
-  cuuint32_t box[4]     = {64, kTile, 1, 1};
+  cuuint32_t box[4]     = {64, static_cast<cuuint32_t>(box_rows), 1, 1};
   cuuint32_t estr[4]    = {1, 1, 1, 1};
   CUresult r = enc(out, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                    const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -906,9 +970,9 @@ int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, 
                 "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");
   TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv), "attention: strides of q, k and v must be positive");
   AttnMaps maps;
-  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq))) return rc;
-  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk))) return rc;
-  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv))) return rc;
+  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, kTile))) return rc;
+  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, kTile))) return rc;
+  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, kTile))) return rc;
   maps.dout = maps.q;  // not read
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == kBF16) return d <= 64 ? LaunchFwd<64, true>(maps, p, st) : LaunchFwd<128, true>(maps, p, st);
@@ -940,10 +1004,10 @@ int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const vo
                 "attention: lse and delta must be 16-byte aligned");
   TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.sdo), "attention: strides must be positive");
   AttnMaps maps;
-  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq))) return rc;
-  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk))) return rc;
-  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv))) return rc;
-  if ((rc = HeadMap(&maps.dout, dout, dtype, b, s, h, d, p.sdo))) return rc;
+  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, kUnit))) return rc;
+  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, kUnit))) return rc;
+  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, kUnit))) return rc;
+  if ((rc = HeadMap(&maps.dout, dout, dtype, b, s, h, d, p.sdo, kUnit))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == kBF16) return d <= 64 ? LaunchBwd<64, true>(maps, p, st) : LaunchBwd<128, true>(maps, p, st);
   return d <= 64 ? LaunchBwd<64, false>(maps, p, st) : LaunchBwd<128, false>(maps, p, st);
