@@ -23,6 +23,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "kernels/common.cuh"
 #include "kernels/tcgen05.cuh"
@@ -35,8 +36,10 @@ constexpr int kTile        = 128;  // rows of a tile of queries or keys
 constexpr int kBoxBytes    = kTile * 128;  // 128 rows of 64 16-bit values
 // Softmax warps, and behind them one that issues TMA loads, two that issue MMAs (a wait costs such a warp as much time as an
 // MMA or two, so each gets half of the products) and one that clears rows beyond a sequence's length.
-constexpr int kFwdWarps = 8, kBwdWarps = 16;
-constexpr int kFwdThreads = (kFwdWarps + 4) * 32, kBwdThreads = (kBwdWarps + 4) * 32;
+constexpr int kSoftWarps = 16;
+constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kClearWarp = kSoftWarps + 3;
+constexpr int kWarps   = kSoftWarps + 4;
+constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int32_t g_attn_error;  // one per device
@@ -242,8 +245,9 @@ __device__ __forceinline__ F2 Exp2Poly(F2 x) {
   const float2 n = SplitF2(t);
   return Mul2(q, MakeF2(__int_as_float((__float_as_int(n.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(n.y) << 23) + 0x3f800000)));
 }
-// Pair k of a run: every other one by the polynomial.
-__device__ __forceinline__ F2 Exp2Mixed(F2 x, int k) { return k & 1 ? Exp2Poly(x) : Exp2Fast(x); }
+// Pair k of a run: one in kEvery by the polynomial.
+template <int kEvery>
+__device__ __forceinline__ F2 Exp2Mixed(F2 x, int k) { return k % kEvery == kEvery - 1 ? Exp2Poly(x) : Exp2Fast(x); }
 __device__ __forceinline__ F2 Pair(uint32_t a, uint32_t b) { return MakeF2(__uint_as_float(a), __uint_as_float(b)); }
 template <bool kBf16>
 __device__ __forceinline__ uint32_t Pack2(F2 a) {
@@ -255,262 +259,370 @@ __device__ __forceinline__ uint8_t* AlignedSmem(uint8_t* raw) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
 }
 
-// ---------------------------------------------------------------- forward
-// A CTA takes 256 queries of one head as two tiles, a softmax warpgroup for each, and streams the keys and values: while one
-// warpgroup computes probabilities, the tensor cores run the products of the other.  A thread owns a row, so maximum and sum
-// need no exchange.
-template <int HD>
-struct FwdCfg {
-  static constexpr int kTileBytes = (HD / 64) * kBoxBytes;
-  static constexpr int kStages    = HD == 64 ? 6 : 4;  // tiles of K and V in turn
-  static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 1024 + 256;
+// ---------------------------------------------------------------- blocks that take one piece of work after another
+// The grid has a block per piece of work, but a block that is done takes the place of one that has not started yet (cluster
+// launch control): its barriers, its TMEM and its pipelines stay up, loads and scores of the next piece run under the
+// last stores of this one, and pieces of different length still spread evenly.  Every warp runs through the same pieces.  The
+// TMA warp asks for the next one while it works on the present one; the answer lies in one of two slots.
+struct Next {
+  uint4* slot;       // [2] answers
+  uint64_t* full;    // [2]
+  uint64_t* empty;   // [2] all warps have read it
 };
-
-template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kFwdThreads, 1)
-AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
-  using Cfg = FwdCfg<HD>;
-  constexpr int kTmaWarp = kFwdWarps, kMmaWarp = kFwdWarps + 1, kClearWarp = kFwdWarps + 3;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem_q   = AlignedSmem(smem_raw);
-  uint8_t* ring     = smem_q + 2 * Cfg::kTileBytes;
-  uint64_t* full    = reinterpret_cast<uint64_t*>(ring + Cfg::kStages * Cfg::kTileBytes);
-  uint64_t* empty   = full + Cfg::kStages;
-  uint64_t* q_full  = empty + Cfg::kStages;  // [1]
-  uint64_t* s_full  = q_full + 1;            // [2] scores of a tile are in TMEM
-  uint64_t* p_full  = s_full + 2;            // [2] its probabilities are
-  uint64_t* o_full  = p_full + 2;            // [2] the last product of a tile has completed
-  uint64_t* raw     = o_full + 2;            // [1] the last tile of V has arrived and has rows to clear before it counts as full
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw + 1);
-
-  const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  // causal: the tiles with the most keys first; otherwise neighbours share a head's keys
-  const int blocks_q = TilesOf(p.s, 2 * kTile);
-  const int heads    = p.b * p.h;
-  const int qb = p.causal ? blocks_q - 1 - static_cast<int>(blockIdx.x) / heads : static_cast<int>(blockIdx.x) % blocks_q;
-  const int bh = p.causal ? static_cast<int>(blockIdx.x) % heads : static_cast<int>(blockIdx.x) / blocks_q;
-  const int b = bh / p.h, h = bh % p.h, hk = h / (p.h / p.hk);
-  const int q0  = qb * 2 * kTile;
-  const int len = Uniform(SeqLen(p, b));
-  const int tiles = TilesOf(len, kTile);
-  int count[2];  // key tiles of either query tile
-#pragma unroll
+__device__ __forceinline__ void InitNext(const Next& n) {
   for (int i = 0; i < 2; ++i) {
-    const int first = q0 + i * kTile;
-    count[i] = first >= len ? 0 : p.causal ? min(tiles, first / kTile + 1) : tiles;
+    MbarInit(&n.full[i], 1);
+    MbarInit(&n.empty[i], kWarps);
   }
-  const int total = max(count[0], count[1]);
-  const bool ragged = total == tiles && len < p.s && len % kTile != 0;  // the last tile of V has rows to clear
+}
+// One thread, at the start of piece number `turn`.
+__device__ __forceinline__ bool AskNext(const Next& n, uint32_t turn) {
+  const int i = turn & 1;
+  if (!MbarWait(&n.empty[i], ((turn >> 1) & 1) ^ 1)) return false;
+  MbarExpectTx(&n.full[i], 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   SmemAddr(&n.slot[i])),
+               "r"(SmemAddr(&n.full[i]))
+               : "memory");
+  return true;
+}
+// A whole warp, at the end of piece number `turn`: the next piece's block index, or -1.
+__device__ __forceinline__ int TakeNext(const Next& n, uint32_t turn) {
+  const int i = turn & 1;
+  if (!MbarWaitWarp(&n.full[i], (turn >> 1) & 1)) {
+    if ((threadIdx.x & 31) == 0) atomicExch(&g_attn_error, 8);
+    return -1;
+  }
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(SmemAddr(&n.slot[i]))
+      : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) MbarArrive(&n.empty[i]);
+  return static_cast<int>(Uniform(got ? x : ~0u));
+}
 
-  if (total > 0) {
-    if (threadIdx.x == 0) {
-      for (int s = 0; s < Cfg::kStages; ++s) {
-        MbarInit(&full[s], 1);
-        MbarInit(&empty[s], 2);  // both MMA warps
-      }
-      MbarInit(q_full, 1);
-      MbarInit(raw, 1);
-      for (int i = 0; i < 2; ++i) {
-        MbarInit(&s_full[i], 1);
-        MbarInit(&p_full[i], 4);
-        MbarInit(&o_full[i], 1);
-      }
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == kMmaWarp) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAddr(tmem_slot)), "r"(512u)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    TcFenceBefore();
-  }
-  __syncthreads();
-  uint32_t tmem = 0;
-  if (total > 0) {
-    TcFenceAfter();
-    tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
-  }
-  // columns: scores of either tile (their probabilities in the same place), then either output
-  const uint32_t t_s[2] = {tmem, tmem + 128}, t_o[2] = {tmem + 256, tmem + 256 + HD};
-
-  // 168 registers per thread at launch; a softmax thread holds a row of 128 scores: 2 x 208 + 88 = 3 x 168
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == kTmaWarp) {
-      if (total > 0 && ElectOne()) {
-        MbarExpectTx(q_full, 2 * Cfg::kTileBytes);
-        TmaLoadTile<HD, kTile, kTile>(smem_q, &maps.q, q0, h, b, q_full);
-        TmaLoadTile<HD, kTile, kTile>(smem_q + Cfg::kTileBytes, &maps.q, q0 + kTile, h, b, q_full);
-        for (int e = 0; e < 2 * total; ++e) {
-          const int st = e % Cfg::kStages;
-          if (!MbarWait(&empty[st], ((e / Cfg::kStages) & 1) ^ 1)) {
-            atomicExch(&g_attn_error, 1);
-            break;
-          }
-          uint64_t* bar = ragged && e == 2 * total - 1 ? raw : &full[st];
-          MbarExpectTx(bar, Cfg::kTileBytes);
-          TmaLoadTile<HD, kTile, kTile>(ring + st * Cfg::kTileBytes, e & 1 ? &maps.v : &maps.k, (e >> 1) * kTile, hk, b, bar);
-        }
-      }
-    } else if (warp == kClearWarp) {
-      if (total > 0 && ragged) {
-        const int e = 2 * total - 1, st = e % Cfg::kStages;
-        if (MbarWaitWarp(raw, 0)) {
-          ClearRows<kTile>(ring + st * Cfg::kTileBytes, HD / 64, len % kTile);
-          if (lane == 0) MbarArrive(&full[st]);
-        } else if (lane == 0) {
-          atomicExch(&g_attn_error, 2);
-        }
-      }
-    } else if (total > 0) {
-      const int i = warp - kMmaWarp;  // query tile
-      const int mine = count[i], ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-      const uint32_t q_addr = SmemAddr(smem_q + i * Cfg::kTileBytes);
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int parity) {
-        if (ok && !MbarWaitWarp(bar, parity)) {
-          if (lane == 0) atomicExch(&g_attn_error, 3);
-          ok = false;
-        }
-        TcFenceAfter();
-        return ok;
-      };
-      auto entry = [&](int e) { return wait(&full[e % Cfg::kStages], (e / Cfg::kStages) & 1); };
-      auto tile  = [&](int e) { return SmemAddr(ring + (e % Cfg::kStages) * Cfg::kTileBytes); };
-      if (wait(q_full, 0) && entry(0) && ElectOne()) {
-        if (mine > 0) {
-          IssueScores<kBf16, HD, kTile>(t_s[i], q_addr, tile(0), ksteps);
-          UmmaCommit(&s_full[i]);
-        }
-        UmmaCommit(&empty[0]);
-      }
-      for (int j = 0; j < total && ok; ++j) {  // a tile with fewer keys than the other hands on the rest
-        const int ev = 2 * j + 1, ek = 2 * j + 2;
-        if (!entry(ev) || (j + 1 < total && !entry(ek))) break;
-        if (j < mine) {
-          if (!wait(&p_full[i], j & 1)) break;
-          if (ElectOne()) {
-            // the probabilities lie where the next scores go: products complete in the order of their issue
-            IssueFromTmem<kBf16, kTile, kTile>(t_o[i], t_s[i], tile(ev), n_out, j > 0);
-            if (j + 1 < mine) {
-              IssueScores<kBf16, HD, kTile>(t_s[i], q_addr, tile(ek), ksteps);
-              UmmaCommit(&s_full[i]);
-            } else {
-              UmmaCommit(&o_full[i]);
-            }
-          }
-        }
-        if (ElectOne()) {
-          UmmaCommit(&empty[ev % Cfg::kStages]);
-          if (j + 1 < total) UmmaCommit(&empty[ek % Cfg::kStages]);
-        }
-      }
-    }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int i = warp >> 2;             // query tile
-    const int quarter = warp & 3;        // TMEM lanes that this warp may access
-    const int row = q0 + i * kTile + quarter * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and the sum
-    bool ok = true;
-    for (int j = 0; j < count[i]; ++j) {
-      if (!MbarWaitWarp(&s_full[i], j & 1)) {
-        if (lane == 0) atomicExch(&g_attn_error, 4);
-        ok = false;
-        break;
-      }
-      TcFenceAfter();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) TmemLoad32Async(t_s[i] + lanes + g * 32, s[g]);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) TmemLoadWait(s[g]);
-      const int kv0 = j * kTile;
-      if (kv0 + kTile > len || (p.causal && kv0 + kTile - 1 > q0 + i * kTile)) {
-        const int limit = (p.causal ? min(len, row + 1) : len) - kv0;
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (g * 32 + k >= limit) s[g][k] = 0xff800000u;  // -inf
-      }
-      float part[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) part[k] = __uint_as_float(s[k >> 1][(k & 1) * 16]);
-#pragma unroll
-      for (int k = 1; k < 16; ++k)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) part[u] = MaxNan(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]));
-      float top = MaxNan(MaxNan(MaxNan(part[0], part[1]), MaxNan(part[2], part[3])),
-                         MaxNan(MaxNan(part[4], part[5]), MaxNan(part[6], part[7])));
-      // a row without any key so far; and inf - inf: the row is NaN, as by the formula
-      if (top == -INFINITY) top = 0.f;
-      else if (top == INFINITY) top = __uint_as_float(0x7fc00000u);
-      // The exponents' reference may lag behind the maximum by up to 2^8: probabilities of up to 256 lose nothing in 16 bits,
-      // and the output in TMEM is rescaled a few times per row instead of with every new maximum.
-      if (j == 0) {
-        m = top;
-      } else if (__any_sync(0xffffffffu, !((top - m) * p.c <= 8.f))) {
-        const float up = MaxNan(top, m);
-        const float f  = Exp2((m - up) * p.c);
-        m = up;
-        l *= f;
-#pragma unroll 1
-        for (int g = 0; g < HD / 16; ++g) {
-          uint32_t o[16];
-          TmemLoad16(t_o[i] + lanes + g * 16, o);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-          TmemStore16(t_o[i] + lanes + g * 16, o);
-        }
-      }
-      const F2 c2 = Both(p.c), nm = Both(-m * p.c);
-      F2 sum[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const F2 x = Exp2Mixed(Fma2(Pair(s[g][2 * k], s[g][2 * k + 1]), c2, nm), k);
-          sum[k & 3] = g == 0 && k < 4 ? x : Add2(sum[k & 3], x);
-          w[k] = Pack2<kBf16>(x);
-        }
-        TmemStore16(t_s[i] + lanes + g * 16, w);
-      }
-      const float2 both = SplitF2(Add2(Add2(sum[0], sum[1]), Add2(sum[2], sum[3])));
-      l += both.x + both.y;
-      TmemStoreWait();
-      TcFenceBefore();
-      __syncwarp();
-      if (lane == 0) MbarArrive(&p_full[i]);
-    }
-    if (count[i] > 0 && ok && !MbarWaitWarp(&o_full[i], 0)) {
-      if (lane == 0) atomicExch(&g_attn_error, 4);
+// A wait that remembers a failure, for warps that go on to the next piece; reports it once under `code`.
+struct Waiter {
+  int code;
+  bool ok = true;
+  __device__ __forceinline__ explicit Waiter(int c) : code(c) {}
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) {
+    if (ok && !MbarWaitWarp(bar, parity & 1)) {
+      if ((threadIdx.x & 31) == 0) atomicExch(&g_attn_error, code);
       ok = false;
     }
     TcFenceAfter();
-    if (ok) {
-      const bool live = row < len;
-      uint16_t* dst = static_cast<uint16_t*>(p.o) + b * p.so.b + row * p.so.s + h * p.so.h;
-      if (count[i] > 0) {
-        const float inv = 1.f / l;
-#pragma unroll 1
-        for (int g = 0; g < HD / 32; ++g) {
-          uint32_t o[32];
-          TmemLoad32(t_o[i] + lanes + g * 32, o);
-          if (live) StoreCols<kBf16, 32>(dst, g * 32, p.d, o, inv);
+    return ok;
+  }
+};
+
+__device__ __forceinline__ uint32_t AllocTmem(uint32_t* slot) {  // by one warp, all columns
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAddr(slot)), "r"(512u) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  return 0;
+}
+
+// ---------------------------------------------------------------- forward
+// A piece of work is 256 queries of one head as two tiles, past which the keys and values stream: while the warps of one tile
+// compute probabilities, the tensor cores run the products of the other.  Eight softmax warps per tile; a thread has half
+// of a row, 64 scores, and exchanges its maximum with the thread that has the other half.  (With a whole row per thread
+// there is nothing to exchange, but two warps per scheduler leave most issue slots empty: 32 x 512, 16 heads of 64: 87 us.)
+template <int HD>
+struct FwdCfg {
+  static constexpr int kTileBytes = (HD / 64) * kBoxBytes;
+  static constexpr int kStages    = HD == 64 ? 8 : 4;  // tiles of K and V in turn
+  static constexpr int kQBufs     = HD == 64 ? 2 : 1;  // queries of this piece of work and the next
+  static constexpr int kMaxBytes  = 2 * 2 * 2 * kTile * 4;
+  static constexpr int kSmemBytes = (2 * kQBufs + kStages) * kTileBytes + kMaxBytes + 1024 + 512;
+};
+
+struct FwdPiece {
+  int b, h, q0, len, tiles, count[2], total;
+  bool ragged;  // the last tile of V has rows to clear
+  __device__ __forceinline__ FwdPiece(const AttnParams& p, int index) {
+    // causal: the tiles with the most keys first; otherwise neighbours share a head's keys
+    const int blocks_q = TilesOf(p.s, 2 * kTile), heads = p.b * p.h;
+    const int qb = p.causal ? blocks_q - 1 - index / heads : index % blocks_q;
+    const int bh = p.causal ? index % heads : index / blocks_q;
+    b     = bh / p.h;
+    h     = bh % p.h;
+    q0    = qb * 2 * kTile;
+    len   = Uniform(SeqLen(p, b));
+    tiles = TilesOf(len, kTile);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // key tiles of either query tile
+      const int first = q0 + i * kTile;
+      count[i] = first >= len ? 0 : p.causal ? min(tiles, first / kTile + 1) : tiles;
+    }
+    total  = max(count[0], count[1]);
+    ragged = total > 0 && total == tiles && len < p.s && len % kTile != 0;
+  }
+};
+
+template <int HD, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1)
+AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
+  using Cfg = FwdCfg<HD>;
+  constexpr int S = Cfg::kStages, QB = Cfg::kQBufs;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem_q   = AlignedSmem(smem_raw);                  // [QB][2] tiles
+  uint8_t* ring     = smem_q + 2 * QB * Cfg::kTileBytes;
+  float* exchange   = reinterpret_cast<float*>(ring + S * Cfg::kTileBytes);  // [2 turns][2 tiles][2 halves][128 rows]
+  const Next next{reinterpret_cast<uint4*>(exchange + 8 * kTile), reinterpret_cast<uint64_t*>(exchange + 8 * kTile + 8),
+                  reinterpret_cast<uint64_t*>(exchange + 8 * kTile + 8) + 2};
+  uint64_t* full    = next.empty + 2;
+  uint64_t* empty   = full + S;     // both MMA warps are done with a tile of K or V
+  uint64_t* raw     = empty + S;    // a tile of V has arrived and has rows to clear before it counts as full
+  uint64_t* q_full  = raw + S;      // [QB]
+  uint64_t* q_empty = q_full + QB;  // [QB]
+  uint64_t* s_full  = q_empty + QB; // [2] scores of a tile are in TMEM
+  uint64_t* p_full  = s_full + 2;   // [2] its probabilities are
+  uint64_t* o_full  = p_full + 2;   // [2] the last product of a tile has completed
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+
+  const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    InitNext(next);
+    for (int i = 0; i < S; ++i) {
+      MbarInit(&full[i], 1);
+      MbarInit(&empty[i], 2);
+      MbarInit(&raw[i], 1);
+    }
+    for (int i = 0; i < QB; ++i) {
+      MbarInit(&q_full[i], 1);
+      MbarInit(&q_empty[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      MbarInit(&s_full[i], 1);
+      MbarInit(&p_full[i], kSoftWarps / 2);
+      MbarInit(&o_full[i], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) AllocTmem(tmem_slot);
+  TcFenceBefore();
+  __syncthreads();
+  TcFenceAfter();
+  const uint32_t tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
+  // columns: scores of either tile (their probabilities in the same place), then either output
+  const uint32_t t_s = tmem, t_o = tmem + 256;
+
+  if (warp == kTmaWarp) {
+    uint32_t e = 0, n = 0;  // tiles of K and V, and pieces with any, so far
+    bool ok = true;
+    int index = blockIdx.x;
+    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+      const FwdPiece w(p, index);
+      if (ElectOne()) {
+        ok = ok && AskNext(next, turn);
+        if (w.total > 0 && ok) {
+          const int qb = n % QB, hk = w.h / (p.h / p.hk);
+          ok = MbarWait(&q_empty[qb], ((n / QB) & 1) ^ 1);
+          uint8_t* q = smem_q + qb * 2 * Cfg::kTileBytes;
+          if (ok) {
+            MbarExpectTx(&q_full[qb], 2 * Cfg::kTileBytes);
+            TmaLoadTile<HD, kTile, kTile>(q, &maps.q, w.q0, w.h, w.b, &q_full[qb]);
+            TmaLoadTile<HD, kTile, kTile>(q + Cfg::kTileBytes, &maps.q, w.q0 + kTile, w.h, w.b, &q_full[qb]);
+          }
+          for (int k = 0; k < 2 * w.total && ok; ++k) {
+            const uint32_t at = e + k, st = at % S;
+            ok = MbarWait(&empty[st], ((at / S) & 1) ^ 1);
+            if (!ok) break;
+            uint64_t* bar = w.ragged && k == 2 * w.total - 1 ? &raw[st] : &full[st];
+            MbarExpectTx(bar, Cfg::kTileBytes);
+            TmaLoadTile<HD, kTile, kTile>(ring + st * Cfg::kTileBytes, k & 1 ? &maps.v : &maps.k, (k >> 1) * kTile, hk, w.b, bar);
+          }
         }
+        if (!ok) atomicExch(&g_attn_error, 1);
       }
-      if (!live && row < p.s) StoreZeroRow(dst, 0, p.d);
-      if (row < p.sp) p.lse[static_cast<int64_t>(bh) * p.sp + row] = live ? fmaf(m, p.c, log2f(l)) : INFINITY;
+      __syncwarp();
+      e += 2 * w.total;
+      n += w.total > 0;
+    }
+  } else if (warp == kClearWarp) {
+    uint32_t e = 0, uses = 0;  // bit st: parity of the next use of raw[st]
+    Waiter wait(2);
+    int index = blockIdx.x;
+    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+      const FwdPiece w(p, index);
+      e += 2 * w.total;
+      if (w.ragged) {
+        const uint32_t st = (e - 1) % S;
+        if (wait(&raw[st], uses >> st)) {
+          ClearRows<kTile>(ring + st * Cfg::kTileBytes, HD / 64, w.len % kTile);
+          if (lane == 0) MbarArrive(&full[st]);
+        }
+        uses ^= 1u << st;
+      }
+    }
+  } else if (warp >= kMmaWarp) {
+    const int i = warp - kMmaWarp;  // query tile
+    const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
+    const uint32_t ts = t_s + i * 128, to = t_o + i * HD;
+    uint32_t e = 0, n = 0, done = 0;  // done: tiles of probabilities so far
+    Waiter wait(3);
+    auto entry = [&](uint32_t k) { return wait(&full[k % S], k / S); };
+    auto tile  = [&](uint32_t k) { return SmemAddr(ring + (k % S) * Cfg::kTileBytes); };
+    int index = blockIdx.x;
+    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+      const FwdPiece w(p, index);
+      const int mine = w.count[i];
+      if (w.total > 0 && wait.ok) {
+        const int qb = n % QB;
+        const uint32_t q_addr = SmemAddr(smem_q + (qb * 2 + i) * Cfg::kTileBytes);
+        if (wait(&q_full[qb], n / QB) && entry(e) && ElectOne()) {
+          if (mine > 0) {
+            IssueScores<kBf16, HD, kTile>(ts, q_addr, tile(e), ksteps);
+            UmmaCommit(&s_full[i]);
+          }
+          UmmaCommit(&empty[e % S]);
+          if (mine <= 1) UmmaCommit(&q_empty[qb]);
+        }
+        for (int j = 0; j < w.total && wait.ok; ++j) {  // a tile with fewer keys than the other hands on the rest
+          const uint32_t ev = e + 2 * j + 1, ek = ev + 1;
+          if (!entry(ev) || (j + 1 < w.total && !entry(ek))) break;
+          if (j < mine) {
+            if (!wait(&p_full[i], done)) break;
+            ++done;
+            if (ElectOne()) {
+              // the probabilities lie where the next scores go: products complete in the order of their issue
+              IssueFromTmem<kBf16, kTile, kTile / 2>(to, ts, tile(ev), n_out, j > 0);
+              if (j + 1 < mine) {
+                IssueScores<kBf16, HD, kTile>(ts, q_addr, tile(ek), ksteps);
+                UmmaCommit(&s_full[i]);
+                if (j + 2 == mine) UmmaCommit(&q_empty[qb]);
+              } else {
+                UmmaCommit(&o_full[i]);
+              }
+            }
+          }
+          if (ElectOne()) {
+            UmmaCommit(&empty[ev % S]);
+            if (j + 1 < w.total) UmmaCommit(&empty[ek % S]);
+          }
+        }
+        e += 2 * w.total;
+        ++n;
+      }
+    }
+  } else {
+    const int i = warp >> 3, half = (warp >> 2) & 1;  // query tile; columns [64 half, 64 half + 64) of the scores
+    const int quarter = warp & 3;                     // TMEM lanes that this warp may access
+    const int r = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t ts = t_s + lanes + i * 128 + half * 64, to = t_o + lanes + i * HD + half * (HD / 2);
+    const int pair_bar = 1 + i * 4 + quarter;         // the two warps that share these rows
+    const F2 c2 = Both(p.c);
+    uint32_t done = 0, pieces = 0, swaps = 0;
+    Waiter wait(4);
+    // this thread's value and the one of the thread with the other half of the row
+    auto other = [&](float mine) {
+      float* at = exchange + ((swaps++ & 1) * 4 + i * 2) * kTile + r;
+      at[half * kTile] = mine;
+      NamedBarSync(pair_bar, 64);
+      return at[(half ^ 1) * kTile];
+    };
+    int index = blockIdx.x;
+    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+      const FwdPiece w(p, index);
+      const int row = w.q0 + i * kTile + r, count = i ? w.count[1] : w.count[0];
+      float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and this half's sum
+      for (int j = 0; j < count; ++j, ++done) {
+        wait(&s_full[i], done);  // on a failure the values are void, but every thread keeps meeting its barriers
+        uint32_t s[2][32];
+        TmemLoad32Async(ts, s[0]);
+        TmemLoad32Async(ts + 32, s[1]);
+        TmemLoadWait(s[0]);
+        TmemLoadWait(s[1]);
+        const int kv0 = j * kTile;
+        if (kv0 + kTile > w.len || (p.causal && kv0 + kTile - 1 > w.q0 + i * kTile)) {
+          const int limit = (p.causal ? min(w.len, row + 1) : w.len) - kv0 - half * 64;
+#pragma unroll
+          for (int k = 0; k < 64; ++k)
+            if (k >= limit) s[k >> 5][k & 31] = 0xff800000u;  // -inf
+        }
+        float part[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) part[u] = __uint_as_float(s[u >> 1][(u & 1) * 16]);
+#pragma unroll
+        for (int k = 1; k < 16; ++k)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) part[u] = MaxNan(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]));
+        float top = MaxNan(MaxNan(part[0], part[1]), MaxNan(part[2], part[3]));
+        top = MaxNan(top, other(top));
+        // a row without any key so far; and inf - inf: the row is NaN, as by the formula
+        if (top == -INFINITY) top = 0.f;
+        else if (top == INFINITY) top = __uint_as_float(0x7fc00000u);
+        // The exponents' reference may lag behind the maximum by up to 2^8: probabilities of up to 256 lose nothing in 16 bits,
+        // and the output in TMEM is rescaled a few times per row instead of with every new maximum.
+        if (j == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, !((top - m) * p.c <= 8.f))) {
+          const float up = MaxNan(top, m);
+          const float f  = Exp2((m - up) * p.c);
+          m = up;
+          l *= f;
+#pragma unroll 1
+          for (int g = 0; g < HD / 32; ++g) {
+            uint32_t o[16];
+            TmemLoad16(to + g * 16, o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            TmemStore16(to + g * 16, o);
+          }
+        }
+        const F2 nm = Both(-m * p.c);
+        F2 sum[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t v[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const F2 x = Exp2Mixed<4>(Fma2(Pair(s[g][2 * k], s[g][2 * k + 1]), c2, nm), k);
+            sum[k & 1] = g == 0 && k < 2 ? x : Add2(sum[k & 1], x);
+            v[k] = Pack2<kBf16>(x);
+          }
+          TmemStore16(ts + g * 16, v);
+        }
+        const float2 both = SplitF2(Add2(sum[0], sum[1]));
+        l += both.x + both.y;
+        TmemStoreWait();
+        TcFenceBefore();
+        __syncwarp();
+        if (lane == 0) MbarArrive(&p_full[i]);
+      }
+      const bool live = row < w.len;
+      uint16_t* dst = static_cast<uint16_t*>(p.o) + w.b * p.so.b + row * p.so.s + w.h * p.so.h;
+      if (count > 0) {
+        l += other(l);
+        wait(&o_full[i], pieces++);
+        const float inv = 1.f / l;
+        const int c0 = half * (HD / 2);
+#pragma unroll
+        for (int g = 0; g < HD / 64; ++g) {
+          uint32_t o[32];
+          TmemLoad32(to + g * 32, o);
+          if (live && wait.ok) StoreCols<kBf16, 32>(dst, c0 + g * 32, p.d, o, inv);
+        }
+        TcFenceBefore();
+      }
+      if (!live && row < p.s) StoreZeroRow(dst, half * (HD / 2), min(p.d, (half + 1) * (HD / 2)));
+      if (half == 0 && row < p.sp)
+        p.lse[(static_cast<int64_t>(w.b) * p.h + w.h) * p.sp + row] = live ? fmaf(m, p.c, log2f(l)) : INFINITY;
     }
   }
   TcFenceBefore();
   __syncthreads();
-  if (warp == kMmaWarp && total > 0) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-  }
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 // ---------------------------------------------------------------- backward
@@ -549,311 +661,356 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
   }
 }
 
-// One tile of 128 keys (kKeys) or queries (!kKeys) stays, the tiles of the other side (units) stream past it:
+// A piece of work is one tile of 128 keys (kKeys) or queries (!kKeys), which stays; the tiles of the other side (units) stream
+// past it:
 //             stays (X1, X2)   streams (Y1, Y2)   S = X1 Y1^T, dP = X2 Y2^T       accumulated
 //   kKeys     K, V             Q, dO              rows are keys: P^T and dS^T     dV += P^T dO,  dK += dS^T Q
 //   !kKeys    Q, dO            K, V               rows are queries                dQ += dS K
 // Both passes compute S and dP, seven products instead of five, and in exchange every sum has one owner: no atomics, no
 // fp32 copy of dQ in memory, and results that do not depend on the order of the blocks.
 // The softmax warps take S of a unit, then its dP; while they work on one, the tensor cores run the products that the other has
-// released and the next unit's.  Sixteen of them, four per scheduler, each with 32 rows x 32 columns.
+// released and the next unit's.  Each has 32 rows x 32 columns.
 constexpr int kUnit = 128;
 template <int HD>
 struct BwdCfg {
   static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;
   static constexpr int kStageBytes = 2 * kTileBytes;           // Y1, Y2
   static constexpr int kStages     = HD == 64 ? 4 : 2;
-  static constexpr int kSBufs      = HD == 64 ? 2 : 1;         // scores in TMEM; with 128 columns of either accumulator there is room for one
+  static constexpr int kXBufs      = HD == 64 ? 2 : 1;         // what stays, of this piece of work and the next
+  static constexpr int kSBufs      = HD == 64 ? 2 : 1;         // scores in TMEM; beside accumulators of 128 columns there is room for one
   static constexpr int kRowBytes   = 2 * kUnit * 4;            // -L and -D of a unit of queries
-  static constexpr int kSmemBytes  = 2 * kTileBytes + kStages * (kStageBytes + kRowBytes) + 1024 + 256;
+  static constexpr int kSmemBytes  = kXBufs * 2 * kTileBytes + kStages * (kStageBytes + kRowBytes) + 1024 + 512;
 };
 
-template <int HD, bool kBf16, bool kKeys>
-__device__ __forceinline__ void AttnBwdTile(const AttnMaps& maps, const AttnParams& p, int tile, int b, int head, uint8_t* smem) {
-  using Cfg = BwdCfg<HD>;
-  constexpr int kTmaWarp = kBwdWarps, kMmaWarp = kBwdWarps + 1, kClearWarp = kBwdWarps + 3;
-  uint8_t* x1     = smem;
-  uint8_t* x2     = x1 + Cfg::kTileBytes;
-  uint8_t* ring   = x2 + Cfg::kTileBytes;
-  float* ld       = reinterpret_cast<float*>(ring + Cfg::kStages * Cfg::kStageBytes);
-  uint64_t* full  = reinterpret_cast<uint64_t*>(ld + Cfg::kStages * 2 * kUnit);
-  uint64_t* empty = full + Cfg::kStages;
-  uint64_t* x_full   = empty + Cfg::kStages;
-  uint64_t* s_full   = x_full + 1;    // [2] S of a unit is in TMEM
-  uint64_t* s_done   = s_full + 2;    // [2] keys: P has taken its place; queries: S has been read
-  uint64_t* dp_full  = s_done + 2;    // dP is in TMEM
-  uint64_t* ds_full  = dp_full + 1;   // dS has taken its place
-  uint64_t* acc_full = ds_full + 1;
-  uint64_t* cleared  = acc_full + 1;  // [stages] the unit has no rows beyond the length (any more)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cleared + Cfg::kStages);
-
-  const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int group = p.h / p.hk;
-  const int x0    = tile * kTile;
-  const int len   = Uniform(SeqLen(p, b));
-  const int units = TilesOf(len, kUnit);
-  // streamed units: [first, last) of the one head, or of each head of the group
-  const int first = kKeys && p.causal ? x0 / kUnit : 0;
-  const int last  = !kKeys && p.causal ? min(units, x0 / kUnit + kTile / kUnit) : units;
-  const int per   = last - first;
-  const int total = x0 >= len ? 0 : per * (kKeys ? group : 1);
-  const bool ragged = last == units && len < p.s && len % kUnit != 0;  // a head's last unit has rows to clear
-  const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;  // of -L, -D
-  const int xhead = head, yhead = kKeys ? head * group : head / group;
-
-  if (total > 0) {
-    if (threadIdx.x == 0) {
-      for (int s = 0; s < Cfg::kStages; ++s) {
-        MbarInit(&full[s], 1);
-        MbarInit(&empty[s], 2);  // both MMA warps
-        MbarInit(&cleared[s], 1);
-      }
-      MbarInit(x_full, 1);
-      for (int i = 0; i < Cfg::kSBufs; ++i) {
-        MbarInit(&s_full[i], 1);
-        MbarInit(&s_done[i], kBwdWarps);
-      }
-      MbarInit(dp_full, 1);
-      MbarInit(ds_full, kBwdWarps);
-      MbarInit(acc_full, 2);
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == kMmaWarp) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAddr(tmem_slot)), "r"(512u)
-                   : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    TcFenceBefore();
+template <bool kKeys>
+struct BwdPiece {
+  int b, head, x0, len, first, per, total, yhead;
+  bool ragged;  // a head's last unit has rows to clear
+  __device__ __forceinline__ BwdPiece(const AttnParams& p, int index) {
+    const int tiles = p.sp / kTile, kh = kKeys ? p.hk : p.h, heads = p.b * kh;
+    // causal: the tiles with the longest streams first; otherwise neighbours share a head
+    const int tile = !p.causal ? index % tiles : kKeys ? index / heads : tiles - 1 - index / heads;
+    const int bh   = p.causal ? index % heads : index / tiles;
+    b    = bh / kh;
+    head = bh % kh;
+    x0   = tile * kTile;
+    len  = Uniform(SeqLen(p, b));
+    const int units = TilesOf(len, kUnit), group = p.h / p.hk;
+    // streamed units: [first, last) of the one head, or of each head of the group
+    first = kKeys && p.causal ? x0 / kUnit : 0;
+    const int last = !kKeys && p.causal ? min(units, x0 / kUnit + kTile / kUnit) : units;
+    per    = last - first;
+    total  = x0 >= len ? 0 : per * (kKeys ? group : 1);
+    yhead  = kKeys ? head * group : head / group;
+    ragged = total > 0 && last == units && len < p.s && len % kUnit != 0;
   }
-  __syncthreads();
-  uint32_t tmem = 0;
-  if (total > 0) {
-    TcFenceAfter();
-    tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
+};
+
+template <int HD>
+struct BwdSmem {
+  using Cfg = BwdCfg<HD>;
+  uint8_t *x, *ring;   // [XB][X1, X2], [stages][Y1, Y2]
+  float* ld;           // [stages][-L, -D]
+  Next next;
+  uint64_t *full, *empty, *raw;      // [stages] raw: a unit has arrived and has rows to clear before it counts as full
+  uint64_t *x_full, *x_empty;        // [XB]
+  uint64_t *s_full, *s_done;         // [SB] S of a unit is in TMEM; keys: P has taken its place, queries: S has been read
+  uint64_t *dp_full, *ds_full;       // dP is in TMEM; dS has taken its place
+  uint64_t *acc_full;
+  uint32_t* tmem_slot;
+  uint32_t tmem;
+  __device__ __forceinline__ explicit BwdSmem(uint8_t* smem) {
+    x          = smem;
+    ring       = x + Cfg::kXBufs * 2 * Cfg::kTileBytes;
+    ld         = reinterpret_cast<float*>(ring + Cfg::kStages * Cfg::kStageBytes);
+    next.slot  = reinterpret_cast<uint4*>(ld + Cfg::kStages * 2 * kUnit);
+    next.full  = reinterpret_cast<uint64_t*>(next.slot + 2);
+    next.empty = next.full + 2;
+    full       = next.empty + 2;
+    empty      = full + Cfg::kStages;
+    raw        = empty + Cfg::kStages;
+    x_full     = raw + Cfg::kStages;
+    x_empty    = x_full + Cfg::kXBufs;
+    s_full     = x_empty + Cfg::kXBufs;
+    s_done     = s_full + Cfg::kSBufs;
+    dp_full    = s_done + Cfg::kSBufs;
+    ds_full    = dp_full + 1;
+    acc_full   = ds_full + 1;
+    tmem_slot  = reinterpret_cast<uint32_t*>(acc_full + 1);
   }
   // columns: S, dP, the accumulators, the other S
-  const uint32_t t_s = tmem, t_dp = tmem + 128, t_acc1 = tmem + 256, t_acc2 = tmem + 256 + HD;
-  auto s_buf = [&](int u) { return Cfg::kSBufs == 1 ? 0 : u & 1; };
-  auto s_par = [&](int u) { return Cfg::kSBufs == 1 ? u & 1 : (u >> 1) & 1; };
-  auto s_col = [&](int u) { return t_s + s_buf(u) * 384; };
+  __device__ __forceinline__ uint32_t S(uint32_t u) const { return tmem + (u % Cfg::kSBufs) * 384; }
+  __device__ __forceinline__ uint32_t Dp() const { return tmem + 128; }
+  __device__ __forceinline__ uint32_t Acc(int i) const { return tmem + 256 + i * HD; }
+  __device__ __forceinline__ uint8_t* Y(uint32_t u) const { return ring + (u % Cfg::kStages) * Cfg::kStageBytes; }
+};
 
-  if (warp == kTmaWarp) {
-    if (total > 0 && ElectOne()) {
-      MbarExpectTx(x_full, 2 * Cfg::kTileBytes);
-      TmaLoadTile<HD, kTile, kUnit>(x1, kKeys ? &maps.k : &maps.q, x0, xhead, b, x_full);
-      TmaLoadTile<HD, kTile, kUnit>(x2, kKeys ? &maps.v : &maps.dout, x0, xhead, b, x_full);
-      for (int u = 0; u < total; ++u) {
-        const int st = u % Cfg::kStages;
-        if (!MbarWait(&empty[st], ((u / Cfg::kStages) & 1) ^ 1)) {
-          atomicExch(&g_attn_error, 5);
-          break;
-        }
-        const int y0 = (first + u % per) * kUnit, yh = yhead + u / per;
-        MbarExpectTx(&full[st], Cfg::kStageBytes + (kKeys ? Cfg::kRowBytes : 0));
-        uint8_t* dst = ring + st * Cfg::kStageBytes;
-        TmaLoadTile<HD, kUnit, kUnit>(dst, kKeys ? &maps.q : &maps.k, y0, yh, b, &full[st]);
-        TmaLoadTile<HD, kUnit, kUnit>(dst + Cfg::kTileBytes, kKeys ? &maps.dout : &maps.v, y0, yh, b, &full[st]);
-        if (kKeys) {
-          const int64_t at = (static_cast<int64_t>(b) * p.h + yh) * p.sp + y0;
-          BulkLoad(ld + st * 2 * kUnit, p.delta + at, kUnit * 4, &full[st]);
-          BulkLoad(ld + st * 2 * kUnit + kUnit, p.delta + plane + at, kUnit * 4, &full[st]);
-        }
-      }
+// What each kind of warp does for one piece.  u0: units so far, n: pieces with any so far.
+template <int HD, bool kKeys>
+__device__ __forceinline__ bool BwdLoad(const AttnMaps& maps, const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w,
+                                        uint32_t u0, uint32_t n) {  // one thread
+  using Cfg = BwdCfg<HD>;
+  constexpr int XB = Cfg::kXBufs, ST = Cfg::kStages;
+  const int xb = n % XB;
+  if (!MbarWait(&m.x_empty[xb], ((n / XB) & 1) ^ 1)) return false;
+  uint8_t* x = m.x + xb * 2 * Cfg::kTileBytes;
+  MbarExpectTx(&m.x_full[xb], 2 * Cfg::kTileBytes);
+  TmaLoadTile<HD, kTile, kUnit>(x, kKeys ? &maps.k : &maps.q, w.x0, w.head, w.b, &m.x_full[xb]);
+  TmaLoadTile<HD, kTile, kUnit>(x + Cfg::kTileBytes, kKeys ? &maps.v : &maps.dout, w.x0, w.head, w.b, &m.x_full[xb]);
+  const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;  // of -L, -D
+  int at = 0, yh = w.yhead;  // unit within a head
+  for (int k = 0; k < w.total; ++k) {
+    const uint32_t u = u0 + k, st = u % ST;
+    if (!MbarWait(&m.empty[st], ((u / ST) & 1) ^ 1)) return false;
+    const int y0 = (w.first + at) * kUnit;
+    uint64_t* bar = w.ragged && at == w.per - 1 ? &m.raw[st] : &m.full[st];
+    MbarExpectTx(bar, Cfg::kStageBytes + (kKeys ? Cfg::kRowBytes : 0));
+    TmaLoadTile<HD, kUnit, kUnit>(m.Y(u), kKeys ? &maps.q : &maps.k, y0, yh, w.b, bar);
+    TmaLoadTile<HD, kUnit, kUnit>(m.Y(u) + Cfg::kTileBytes, kKeys ? &maps.dout : &maps.v, y0, yh, w.b, bar);
+    if (kKeys) {
+      const float* src = p.delta + (static_cast<int64_t>(w.b) * p.h + yh) * p.sp + y0;
+      BulkLoad(m.ld + st * 2 * kUnit, src, kUnit * 4, bar);
+      BulkLoad(m.ld + st * 2 * kUnit + kUnit, src + plane, kUnit * 4, bar);
     }
-  } else if (warp == kClearWarp) {
-    for (int u = 0; ragged && u < total; ++u) {  // every unit passes here, so that the phases match those of `full`
-      const int st = u % Cfg::kStages;
-      if (!MbarWaitWarp(&full[st], (u / Cfg::kStages) & 1)) {
-        if (lane == 0) atomicExch(&g_attn_error, 6);
-        break;
-      }
-      if (u % per == per - 1) ClearRows<kUnit>(ring + st * Cfg::kStageBytes, 2 * (HD / 64), len % kUnit);
-      if (lane == 0) MbarArrive(&cleared[st]);
-    }
-  } else if (warp >= kMmaWarp) {
-    if (total > 0) {
-      const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, int parity) {
-        if (ok && !MbarWaitWarp(bar, parity)) {
-          if (lane == 0) atomicExch(&g_attn_error, 6);
-          ok = false;
-        }
-        TcFenceAfter();
-        return ok;
-      };
-      auto y1 = [&](int u) { return SmemAddr(ring + (u % Cfg::kStages) * Cfg::kStageBytes); };
-      auto y2 = [&](int u) { return y1(u) + Cfg::kTileBytes; };
-      uint64_t* ready = ragged ? cleared : full;
-      auto arrived = [&](int u) { return wait(&ready[u % Cfg::kStages], (u / Cfg::kStages) & 1); };
-      wait(x_full, 0);
-      if (warp == kMmaWarp) {  // S, and P^T dO
-        auto scores = [&](int u) {
-          IssueScores<kBf16, HD, kUnit>(s_col(u), SmemAddr(x1), y1(u), ksteps);
-          UmmaCommit(&s_full[s_buf(u)]);
-        };
-        for (int u = 0; u < min(Cfg::kSBufs, total) && arrived(u); ++u)
-          if (ElectOne()) scores(u);
-        for (int u = 0; u < total && ok; ++u) {
-          const int next = u + Cfg::kSBufs;
-          if ((next < total && !arrived(next)) || !wait(&s_done[s_buf(u)], s_par(u))) break;
-          if (ElectOne()) {
-            if (kKeys) IssueFromTmem<kBf16, kUnit, 32>(t_acc2, s_col(u), y2(u), n_out, u > 0);
-            UmmaCommit(&empty[u % Cfg::kStages]);
-            if (next < total) scores(next);  // in the place of P, which the product before it reads
-          }
-        }
-      } else {  // dP, and dS^T Q or dS K
-        auto grads = [&](int u) {
-          IssueScores<kBf16, HD, kUnit>(t_dp, SmemAddr(x2), y2(u), ksteps);
-          UmmaCommit(dp_full);
-        };
-        if (arrived(0) && ElectOne()) grads(0);
-        for (int u = 0; u < total && ok; ++u) {
-          if ((u + 1 < total && !arrived(u + 1)) || !wait(ds_full, u & 1)) break;
-          if (ElectOne()) {
-            IssueFromTmem<kBf16, kUnit, 32>(t_acc1, t_dp, y1(u), n_out, u > 0);
-            UmmaCommit(&empty[u % Cfg::kStages]);
-            if (u + 1 < total) grads(u + 1);
-          }
-        }
-      }
-      if (ok && ElectOne()) UmmaCommit(acc_full);
-    }
-  } else {
-    const int quarter = warp & 3;    // TMEM lanes
-    const int col = (warp >> 2) * 32;  // first column of this warp in a unit
-    const int row = x0 + quarter * 32 + lane;
-    const uint32_t at = (static_cast<uint32_t>(quarter * 32) << 16) + col;
-    F2 row_l{}, row_d{};  // -L, -D
-    if (!kKeys && total > 0) {  // row < sp
-      const int64_t i = (static_cast<int64_t>(b) * p.h + head) * p.sp + row;
-      row_l = Both(p.delta[i]);
-      row_d = Both(p.delta[plane + i]);
-    }
-    const F2 c2 = Both(p.c);
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, int parity) {
-      if (ok && !MbarWaitWarp(bar, parity)) {
-        if (lane == 0) atomicExch(&g_attn_error, 7);
-        ok = false;
-      }
-      TcFenceAfter();
-      return ok;
-    };
-    for (int u = 0; u < total; ++u) {
-      const int st = u % Cfg::kStages;
-      const int y0 = (first + u % per) * kUnit;
-      if (!wait(&s_full[s_buf(u)], s_par(u))) break;
-      uint32_t s[32];
-      TmemLoad32Async(s_col(u) + at, s);
-      const bool here = !kKeys || wait(&full[st], (u / Cfg::kStages) & 1);  // -L and -D
-      TmemLoadWait(s);
-      if (!here) break;
-      if (!kKeys) {
-        TcFenceBefore();
-        __syncwarp();
-        if (lane == 0) MbarArrive(&s_done[s_buf(u)]);
-      }
-      const float* ls = ld + st * 2 * kUnit + col;
-      F2 pr[16];
-#pragma unroll
-      for (int k = 0; k < 16; k += 2) {
-        F2 l0 = row_l, l1 = row_l;
-        if (kKeys) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + 2 * k);
-          l0.v = v.x;
-          l1.v = v.y;
-        }
-        pr[k]     = Exp2Mixed(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0), k);
-        pr[k + 1] = Exp2Mixed(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1), k + 1);
-      }
-      if (kKeys ? p.causal && y0 < x0 + kTile : y0 + kUnit > len || (p.causal && y0 >= x0)) {
-        // rows are keys: they count for the queries from their own position on; rows are queries: keys up to a limit
-        const int from  = kKeys ? row - y0 - col : 0;
-        const int limit = kKeys ? 32 : (p.causal ? min(len, row + 1) : len) - y0 - col;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float2 x = SplitF2(pr[k]);
-          pr[k] = MakeF2(2 * k >= from && 2 * k < limit ? x.x : 0.f, 2 * k + 1 >= from && 2 * k + 1 < limit ? x.y : 0.f);
-        }
-      }
-      if (kKeys) {
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) w[k] = Pack2<kBf16>(pr[k]);
-        TmemStore16(s_col(u) + at, w);
-        TmemStoreWait();
-        TcFenceBefore();
-        __syncwarp();
-        if (lane == 0) MbarArrive(&s_done[s_buf(u)]);
-      }
-      if (!wait(dp_full, u & 1)) break;
-      TmemLoad32(t_dp + at, s);
-      uint32_t w[16];
-#pragma unroll
-      for (int k = 0; k < 16; k += 2) {
-        F2 d0 = row_d, d1 = row_d;
-        if (kKeys) {
-          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + kUnit + 2 * k);
-          d0.v = v.x;
-          d1.v = v.y;
-        }
-        w[k]     = Pack2<kBf16>(Mul2(pr[k], Add2(Pair(s[2 * k], s[2 * k + 1]), d0)));
-        w[k + 1] = Pack2<kBf16>(Mul2(pr[k + 1], Add2(Pair(s[2 * k + 2], s[2 * k + 3]), d1)));
-      }
-      TmemStore16(t_dp + at, w);
-      TmemStoreWait();
-      TcFenceBefore();
-      __syncwarp();
-      if (lane == 0) MbarArrive(ds_full);
-    }
-    if (total > 0) wait(acc_full, 0);
-    if (ok) {
-      const bool live = row < len;
-      constexpr int kCols = HD / 4;
-      const int c0 = (warp >> 2) * kCols;
-      const uint32_t acc_at = (static_cast<uint32_t>(quarter * 32) << 16) + c0;
-#pragma unroll
-      for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
-        const Strides& st = out ? p.sdv : kKeys ? p.sdk : p.sdq;
-        uint16_t* dst = static_cast<uint16_t*>(out ? p.dv : kKeys ? p.dk : p.dq) + b * st.b + row * st.s + head * st.h;
-        if (total > 0) {
-          uint32_t o[kCols];
-          if constexpr (kCols == 32) TmemLoad32((out ? t_acc2 : t_acc1) + acc_at, o);
-          else TmemLoad16((out ? t_acc2 : t_acc1) + acc_at, o);
-          if (live) StoreCols<kBf16, kCols>(dst, c0, p.d, o, out ? 1.f : p.scale);
-        }
-        if (!live && row < p.s) StoreZeroRow(dst, c0, min(p.d, c0 + kCols));
-      }
+    if (++at == w.per) {
+      at = 0;
+      ++yh;
     }
   }
-  TcFenceBefore();
-  __syncthreads();
-  if (warp == kMmaWarp && total > 0) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  return true;
+}
+
+// uses: bit st is the parity of the next use of raw[st].
+template <int HD, bool kKeys>
+__device__ __forceinline__ void BwdClear(const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t& uses, Waiter& wait) {
+  for (int k = w.per - 1; w.ragged && k < w.total; k += w.per) {
+    const uint32_t st = (u0 + k) % BwdCfg<HD>::kStages;
+    if (!wait(&m.raw[st], uses >> st)) break;
+    uses ^= 1u << st;
+    ClearRows<kUnit>(m.Y(st), 2 * (HD / 64), w.len % kUnit);
+    if ((threadIdx.x & 31) == 0) MbarArrive(&m.full[st]);
   }
 }
 
-// Both passes in one launch, so that neither leaves a tail of idle SMs: first the blocks of the keys, whose tiles stream past
-// every query head of their group.  Causal: the tiles with the longest streams first.
-template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kBwdThreads, 1)
-AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem   = AlignedSmem(smem_raw);
-  const int tiles = p.sp / kTile;
-  int i = blockIdx.x;
-  if (i < tiles * p.b * p.hk) {
-    const int heads = p.b * p.hk;
-    const int tile  = p.causal ? i / heads : i % tiles, bh = p.causal ? i % heads : i / tiles;
-    AttnBwdTile<HD, kBf16, true>(maps, p, tile, bh / p.hk, bh % p.hk, smem);
+// Which: 0 issues S and P^T dO, 1 issues dP and dS^T Q or dS K.
+template <int HD, bool kBf16, bool kKeys, int kWhich>
+__device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
+                                       Waiter& wait) {
+  using Cfg = BwdCfg<HD>;
+  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs, XB = Cfg::kXBufs;
+  const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
+  const uint32_t xb = n % XB, x1 = SmemAddr(m.x + xb * 2 * Cfg::kTileBytes), x2 = x1 + Cfg::kTileBytes;
+  const uint32_t end = u0 + w.total;
+  auto arrived = [&](uint32_t u) { return wait(&m.full[u % ST], u / ST); };
+  wait(&m.x_full[xb], n / XB);
+  if (kWhich == 0) {
+    auto scores = [&](uint32_t u) {
+      IssueScores<kBf16, HD, kUnit>(m.S(u), x1, SmemAddr(m.Y(u)), ksteps);
+      UmmaCommit(&m.s_full[u % SB]);
+      if (u + 1 == end) UmmaCommit(&m.x_empty[xb]);
+    };
+    for (uint32_t u = u0; u < min(u0 + SB, end) && arrived(u); ++u)
+      if (ElectOne()) scores(u);
+    for (uint32_t u = u0; u < end && wait.ok; ++u) {
+      const uint32_t next = u + SB;
+      if ((next < end && !arrived(next)) || !wait(&m.s_done[u % SB], u / SB)) break;
+      if (ElectOne()) {
+        if (kKeys) IssueFromTmem<kBf16, kUnit, 32>(m.Acc(1), m.S(u), SmemAddr(m.Y(u)) + Cfg::kTileBytes, n_out, u > u0);
+        UmmaCommit(&m.empty[u % ST]);
+        if (next < end) scores(next);  // in the place of P, which the product before it reads
+      }
+    }
   } else {
-    i -= tiles * p.b * p.hk;
-    const int heads = p.b * p.h;
-    const int tile  = p.causal ? tiles - 1 - i / heads : i % tiles, bh = p.causal ? i % heads : i / tiles;
-    AttnBwdTile<HD, kBf16, false>(maps, p, tile, bh / p.h, bh % p.h, smem);
+    auto grads = [&](uint32_t u) {
+      IssueScores<kBf16, HD, kUnit>(m.Dp(), x2, SmemAddr(m.Y(u)) + Cfg::kTileBytes, ksteps);
+      UmmaCommit(m.dp_full);
+      if (u + 1 == end) UmmaCommit(&m.x_empty[xb]);
+    };
+    if (arrived(u0) && ElectOne()) grads(u0);
+    for (uint32_t u = u0; u < end && wait.ok; ++u) {
+      if ((u + 1 < end && !arrived(u + 1)) || !wait(m.ds_full, u)) break;
+      if (ElectOne()) {
+        IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(), SmemAddr(m.Y(u)), n_out, u > u0);
+        UmmaCommit(&m.empty[u % ST]);
+        if (u + 1 < end) grads(u + 1);
+      }
+    }
   }
+  if (wait.ok && ElectOne()) UmmaCommit(m.acc_full);
+}
+
+template <int HD, bool kBf16, bool kKeys>
+__device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
+                                           Waiter& wait) {
+  using Cfg = BwdCfg<HD>;
+  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quarter = warp & 3;      // TMEM lanes
+  const int col = (warp >> 2) * 32;  // first column of this warp in a unit
+  const int row = w.x0 + quarter * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+  F2 row_l{}, row_d{};  // -L, -D
+  if (!kKeys && w.total > 0) {  // row < sp
+    const float* src = p.delta + (static_cast<int64_t>(w.b) * p.h + w.head) * p.sp + row;
+    row_l = Both(*src);
+    row_d = Both(src[static_cast<int64_t>(p.b) * p.h * p.sp]);
+  }
+  const F2 c2 = Both(p.c);
+  int y0 = w.first * kUnit, y_end = (w.first + w.per) * kUnit;
+  for (uint32_t u = u0; u < u0 + w.total; ++u) {
+    const int st = u % ST;
+    if (!wait(&m.s_full[u % SB], u / SB)) break;
+    uint32_t s[32];
+    TmemLoad32Async(m.S(u) + lanes + col, s);
+    const bool here = !kKeys || wait(&m.full[st], u / ST);  // -L and -D
+    TmemLoadWait(s);
+    if (!here) break;
+    if (!kKeys) {
+      TcFenceBefore();
+      __syncwarp();
+      if (lane == 0) MbarArrive(&m.s_done[u % SB]);
+    }
+    const float* ls = m.ld + st * 2 * kUnit + col;
+    F2 pr[16];
+#pragma unroll
+    for (int k = 0; k < 16; k += 2) {
+      F2 l0 = row_l, l1 = row_l;
+      if (kKeys) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + 2 * k);
+        l0.v = v.x;
+        l1.v = v.y;
+      }
+      pr[k]     = Exp2Mixed<4>(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0), k);
+      pr[k + 1] = Exp2Mixed<4>(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1), k + 1);
+    }
+    if (kKeys ? p.causal && y0 < w.x0 + kTile : y0 + kUnit > w.len || (p.causal && y0 + kUnit > w.x0)) {
+      // rows are keys: they count for the queries from their own position on; rows are queries: keys up to a limit
+      const int from  = kKeys ? row - y0 - col : 0;
+      const int limit = kKeys ? 32 : (p.causal ? min(w.len, row + 1) : w.len) - y0 - col;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float2 x = SplitF2(pr[k]);
+        pr[k] = MakeF2(2 * k >= from && 2 * k < limit ? x.x : 0.f, 2 * k + 1 >= from && 2 * k + 1 < limit ? x.y : 0.f);
+      }
+    }
+    if (kKeys) {
+      uint32_t v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = Pack2<kBf16>(pr[k]);
+      TmemStore16(m.S(u) + lanes + col, v);
+      TmemStoreWait();
+      TcFenceBefore();
+      __syncwarp();
+      if (lane == 0) MbarArrive(&m.s_done[u % SB]);
+    }
+    if (!wait(m.dp_full, u)) break;
+    TmemLoad32(m.Dp() + lanes + col, s);
+    uint32_t v[16];
+#pragma unroll
+    for (int k = 0; k < 16; k += 2) {
+      F2 d0 = row_d, d1 = row_d;
+      if (kKeys) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(ls + kUnit + 2 * k);
+        d0.v = x.x;
+        d1.v = x.y;
+      }
+      v[k]     = Pack2<kBf16>(Mul2(pr[k], Add2(Pair(s[2 * k], s[2 * k + 1]), d0)));
+      v[k + 1] = Pack2<kBf16>(Mul2(pr[k + 1], Add2(Pair(s[2 * k + 2], s[2 * k + 3]), d1)));
+    }
+    TmemStore16(m.Dp() + lanes + col, v);
+    TmemStoreWait();
+    TcFenceBefore();
+    __syncwarp();
+    if (lane == 0) MbarArrive(m.ds_full);
+    if ((y0 += kUnit) == y_end) y0 = w.first * kUnit;  // the group's next head
+  }
+  if (w.total > 0) wait(m.acc_full, n);
+  if (!wait.ok) return;
+  const bool live = row < w.len;
+  constexpr int kCols = HD / 4;
+  const int c0 = (warp >> 2) * kCols;
+#pragma unroll
+  for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
+    const Strides& st = out ? p.sdv : kKeys ? p.sdk : p.sdq;
+    uint16_t* dst = static_cast<uint16_t*>(out ? p.dv : kKeys ? p.dk : p.dq) + w.b * st.b + row * st.s + w.head * st.h;
+    if (w.total > 0) {
+      uint32_t o[kCols];
+      if constexpr (kCols == 32) TmemLoad32(m.Acc(out) + lanes + c0, o);
+      else TmemLoad16(m.Acc(out) + lanes + c0, o);
+      if (live) StoreCols<kBf16, kCols>(dst, c0, p.d, o, out ? 1.f : p.scale);
+    }
+    if (!live && row < p.s) StoreZeroRow(dst, c0, min(p.d, c0 + kCols));
+  }
+  TcFenceBefore();
+}
+
+// Both passes in one launch, so that neither leaves a tail of idle SMs: first the pieces of the keys, whose tiles stream past
+// every query head of their group.
+template <int HD, bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1)
+AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
+  using Cfg = BwdCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  BwdSmem<HD> m(AlignedSmem(smem_raw));
+  const int warp = Uniform(threadIdx.x >> 5);
+  if (threadIdx.x == 0) {
+    InitNext(m.next);
+    for (int i = 0; i < Cfg::kStages; ++i) {
+      MbarInit(&m.full[i], 1);
+      MbarInit(&m.empty[i], 2);  // both MMA warps
+      MbarInit(&m.raw[i], 1);
+    }
+    for (int i = 0; i < Cfg::kXBufs; ++i) {
+      MbarInit(&m.x_full[i], 1);
+      MbarInit(&m.x_empty[i], 2);
+    }
+    for (int i = 0; i < Cfg::kSBufs; ++i) {
+      MbarInit(&m.s_full[i], 1);
+      MbarInit(&m.s_done[i], kSoftWarps);
+    }
+    MbarInit(m.dp_full, 1);
+    MbarInit(m.ds_full, kSoftWarps);
+    MbarInit(m.acc_full, 2);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) AllocTmem(m.tmem_slot);
+  TcFenceBefore();
+  __syncthreads();
+  TcFenceAfter();
+  m.tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(m.tmem_slot));
+
+  const int key_pieces = p.sp / kTile * p.b * p.hk;
+  uint32_t u0 = 0, n = 0;
+  Waiter wait(warp < kSoftWarps ? 7 : 6);
+  bool loading = true;
+  uint32_t uses = 0;
+  int index = blockIdx.x;
+  for (uint32_t turn = 0; index >= 0; index = TakeNext(m.next, turn), ++turn) {
+    auto work = [&](const auto& w) {
+      constexpr bool kKeys = std::is_same<decltype(w), const BwdPiece<true>&>::value;
+      if (warp < kSoftWarps) {
+        BwdSoftmax<HD, kBf16, kKeys>(p, m, w, u0, n, wait);
+      } else if (warp == kTmaWarp) {
+        if (ElectOne()) {
+          loading = loading && AskNext(m.next, turn);
+          if (w.total > 0) loading = loading && BwdLoad<HD, kKeys>(maps, p, m, w, u0, n);
+          if (!loading) atomicExch(&g_attn_error, 5);
+        }
+        __syncwarp();
+      } else if (w.total > 0 && wait.ok) {
+        if (warp == kClearWarp) BwdClear<HD, kKeys>(m, w, u0, uses, wait);
+        else if (warp == kMmaWarp) BwdMma<HD, kBf16, kKeys, 0>(p, m, w, u0, n, wait);
+        else BwdMma<HD, kBf16, kKeys, 1>(p, m, w, u0, n, wait);
+      }
+      u0 += w.total;
+      n += w.total > 0;
+    };
+    if (index < key_pieces) work(BwdPiece<true>(p, index));
+    else work(BwdPiece<false>(p, index - key_pieces));
+  }
+  TcFenceBefore();
+  __syncthreads();
+  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(m.tmem), "r"(512u) : "memory");
 }
 
 // ---------------------------------------------------------------- host side
@@ -928,7 +1085,7 @@ int LaunchFwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   int rc = AllowSmem(AttnFwdKernel<HD, kBf16>, FwdCfg<HD>::kSmemBytes, &done);
   if (rc) return rc;
   const int grid = TilesOf(p.s, 2 * kTile) * p.b * p.h;
-  AttnFwdKernel<HD, kBf16><<<grid, kFwdThreads, FwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  AttnFwdKernel<HD, kBf16><<<grid, kThreads, FwdCfg<HD>::kSmemBytes, s>>>(maps, p);
   TIPSK_LAUNCH_CHECK();
   return 0;
 }
@@ -943,7 +1100,7 @@ int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   AttnDeltaKernel<kBf16><<<static_cast<int>(rows / 32 < cap ? rows / 32 : cap), 256, 0, s>>>(p);  // sp: whole tiles
   TIPSK_LAUNCH_CHECK();
   const int grid = (p.sp / kTile) * p.b * (p.h + p.hk);
-  AttnBwdKernel<HD, kBf16><<<grid, kBwdThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  AttnBwdKernel<HD, kBf16><<<grid, kThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
   TIPSK_LAUNCH_CHECK();
   return 0;
 }
