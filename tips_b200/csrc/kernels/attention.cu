@@ -78,25 +78,83 @@ __device__ __forceinline__ int SeqLen(const AttnParams& p, int b) {
   return static_cast<int>(n < 0 ? 0 : n > p.s ? p.s : n);
 }
 
+// Barriers and tiles by their shared-memory addresses: a base and constants, where pointers would take two registers each.
+__device__ __forceinline__ void BarInit(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void BarExpect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void BarArrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void BarCommit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool BarTry(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity & 1)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ uint64_t NowNs() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// Bounded waits of a whole warp, whose lanes get one answer: false on a timeout.  A poll that fails takes issue slots from
+// the warps that compute, so the loop is short, and a warp that need not react at once (kIdle) sleeps between polls.
+template <bool kIdle>
+__device__ __forceinline__ bool BarWait(uint32_t bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (__all_sync(0xffffffffu, BarTry(bar, parity))) return true;
+    if (kIdle) __nanosleep(100);
+    if ((i & 1023) == 0) {
+      const uint64_t now = NowNs();
+      if (t0 == 0) t0 = now;
+      else if (__any_sync(0xffffffffu, now - t0 > kWaitBudgetNs)) return false;
+    }
+  }
+}
+// Of one thread, which need not react at once.
+__device__ __forceinline__ bool BarWaitOne(uint32_t bar, uint32_t parity) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 1; !BarTry(bar, parity); ++i) {
+    __nanosleep(40);
+    if ((i & 1023) == 0) {
+      const uint64_t now = NowNs();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > kWaitBudgetNs) return false;
+    }
+  }
+  return true;
+}
+
 // 64 columns x 128 rows of one head: x along d, then position, head, batch.
-__device__ __forceinline__ void TmaLoadHead(void* dst, const CUtensorMap* map, int x, int s, int h, int b, uint64_t* bar) {
+__device__ __forceinline__ void TmaLoadHead(uint32_t dst, const CUtensorMap* map, int x, int s, int h, int b, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-      ::"r"(SmemAddr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(s), "r"(h), "r"(b), "r"(SmemAddr(bar))
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(s), "r"(h), "r"(b), "r"(bar)
       : "memory");
 }
 // kRows positions of a head by boxes of kBox rows; a box of 64 columns with all its rows follows the other.
 template <int HD, int kRows, int kBox>
-__device__ __forceinline__ void TmaLoadTile(uint8_t* dst, const CUtensorMap* map, int s, int h, int b, uint64_t* bar) {
+__device__ __forceinline__ void TmaLoadTile(uint32_t dst, const CUtensorMap* map, int s, int h, int b, uint32_t bar) {
 #pragma unroll
   for (int x = 0; x < HD / 64; ++x)
 #pragma unroll
     for (int r = 0; r < kRows; r += kBox) TmaLoadHead(dst + (x * kRows + r) * 128, map, x * 64, s + r, h, b, bar);
 }
 // `bytes` (a multiple of 16) from 16-byte-aligned global memory.
-__device__ __forceinline__ void BulkLoad(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(SmemAddr(dst)),
-               "l"(src), "r"(bytes), "r"(SmemAddr(bar))
+__device__ __forceinline__ void BulkLoad(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
                : "memory");
 }
 
@@ -187,11 +245,11 @@ __device__ __forceinline__ void IssueFromTmem(uint32_t tmem_d, uint32_t tmem_a, 
 // Clears rows [first, kRows) of `boxes` boxes of kRows rows (a whole warp; the swizzle stays within a row's 128 bytes) and
 // orders the writes before the MMAs that follow.
 template <int kRows>
-__device__ __forceinline__ void ClearRows(uint8_t* tile, int boxes, int first) {
+__device__ __forceinline__ void ClearRows(uint32_t tile, int boxes, int first) {
   const int lane = threadIdx.x & 31;
   for (int x = 0; x < boxes; ++x)
     for (int i = first * 8 + lane; i < kRows * 8; i += 32)
-      *reinterpret_cast<uint4*>(tile + (x * kRows * 8 + i) * 16) = make_uint4(0, 0, 0, 0);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(tile + (x * kRows * 8 + i) * 16), "r"(0) : "memory");
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
 }
@@ -229,25 +287,33 @@ __device__ __forceinline__ F2 Add2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
-// 2^x of two values on the FMA pipe, for a share of the exponentials: ex2.approx runs at 16 per SM and clock, and a tile has
-// 16384.  x = n + f with n = rint(x) (by adding 1.5 * 2^23, whose last bits then hold n), |f| <= 0.5; 2^f by the polynomial of
-// degree 4 with the least relative error on that interval (2.6e-6, by the Remez exchange); times 2^n, made of n's bits.
-// Below -127 the result is 0 (2^-127 has a zero exponent field), a NaN stays one.
-__device__ __forceinline__ F2 Exp2Poly(F2 x) {
-  const float2 v = SplitF2(x);
-  x = MakeF2(MaxNan(v.x, -127.f), MaxNan(v.y, -127.f));
-  const F2 t = Add2(x, Both(12582912.f));
-  const F2 f = Fma2(Add2(t, Both(-12582912.f)), Both(-1.f), x);
-  F2 q = Fma2(f, Both(0.009570102207362652f), Both(0.05591785907745361f));
-  q = Fma2(q, f, Both(0.240247443318367f));
-  q = Fma2(q, f, Both(0.6931217908859253f));
-  q = Fma2(q, f, Both(0.9999992847442627f));
-  const float2 n = SplitF2(t);
-  return Mul2(q, MakeF2(__int_as_float((__float_as_int(n.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(n.y) << 23) + 0x3f800000)));
+__device__ __forceinline__ float MaxNan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x on the FMA pipe, for a share of the exponentials: ex2.approx runs at 16 per SM and clock, and a tile has 16384.
+// x = n + f with n = rint(x) (by adding 1.5 * 2^23, whose last bits then hold n), |f| <= 0.5; 2^f by the polynomial of degree 4
+// with the least relative error on that interval (2.6e-6, by the Remez exchange); times 2^n, made of n's bits.  Below -127
+// the result is 0 (2^-127 has a zero exponent field), a NaN stays one.  One value at a time: constants are immediate
+// operands then, where a pair would need them in registers.
+__device__ __forceinline__ float Exp2Poly(float x) {
+  x = MaxNan(x, -127.f);
+  const float t = x + 12582912.f;
+  const float f = x - (t - 12582912.f);
+  float q = fmaf(f, 0.009570102207362652f, 0.05591785907745361f);
+  q = fmaf(q, f, 0.240247443318367f);
+  q = fmaf(q, f, 0.6931217908859253f);
+  q = fmaf(q, f, 0.9999992847442627f);
+  return q * __int_as_float((__float_as_int(t) << 23) + 0x3f800000);
 }
 // Pair k of a run: one in kEvery by the polynomial.
 template <int kEvery>
-__device__ __forceinline__ F2 Exp2Mixed(F2 x, int k) { return k % kEvery == kEvery - 1 ? Exp2Poly(x) : Exp2Fast(x); }
+__device__ __forceinline__ F2 Exp2Mixed(F2 x, int k) {
+  if (k % kEvery != kEvery - 1) return Exp2Fast(x);
+  const float2 v = SplitF2(x);
+  return MakeF2(Exp2Poly(v.x), Exp2Poly(v.y));
+}
 __device__ __forceinline__ F2 Pair(uint32_t a, uint32_t b) { return MakeF2(__uint_as_float(a), __uint_as_float(b)); }
 template <bool kBf16>
 __device__ __forceinline__ uint32_t Pack2(F2 a) {
@@ -255,9 +321,16 @@ __device__ __forceinline__ uint32_t Pack2(F2 a) {
   return Pack2<kBf16>(x.x, x.y);
 }
 
-__device__ __forceinline__ uint8_t* AlignedSmem(uint8_t* raw) {
-  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+__device__ __forceinline__ float LoadShared(uint32_t at) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
 }
+// Four neighbouring values, 16-byte aligned, as two pairs.
+__device__ __forceinline__ void LoadPairs(uint32_t at, F2& a, F2& b) {
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a.v), "=l"(b.v) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void StoreShared(uint32_t at, float x) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory"); }
 
 // ---------------------------------------------------------------- blocks that take one piece of work after another
 // The grid has a block per piece of work, but a block that is done takes the place of one that has not started yet (cluster
@@ -265,58 +338,59 @@ __device__ __forceinline__ uint8_t* AlignedSmem(uint8_t* raw) {
 // last stores of this one, and pieces of different length still spread evenly.  Every warp runs through the same pieces.  The
 // TMA warp asks for the next one while it works on the present one; the answer lies in one of two slots.
 struct Next {
-  uint4* slot;       // [2] answers
-  uint64_t* full;    // [2]
-  uint64_t* empty;   // [2] all warps have read it
+  uint32_t at;  // two answers of 16 bytes, two barriers that they are there, two that all warps have read them
+  static constexpr int kBytes = 64;
+  __device__ __forceinline__ uint32_t Slot(uint32_t turn) const { return at + (turn & 1) * 16; }
+  __device__ __forceinline__ uint32_t Full(uint32_t turn) const { return at + 32 + (turn & 1) * 8; }
+  __device__ __forceinline__ uint32_t Empty(uint32_t turn) const { return at + 48 + (turn & 1) * 8; }
+  __device__ __forceinline__ void Init() const {
+    for (int i = 0; i < 2; ++i) {
+      BarInit(Full(i), 1);
+      BarInit(Empty(i), kWarps);
+    }
+  }
+  // One thread, at the start of piece number `turn`.
+  __device__ __forceinline__ bool Ask(uint32_t turn) const {
+    if (!BarWaitOne(Empty(turn), (turn >> 1) ^ 1)) return false;
+    BarExpect(Full(turn), 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(Slot(turn)),
+                 "r"(Full(turn))
+                 : "memory");
+    return true;
+  }
+  // A whole warp, at the end of piece number `turn`: the next piece's block index, or -1.
+  template <bool kIdle>
+  __device__ __forceinline__ int Take(uint32_t turn) const {
+    if (!BarWait<kIdle>(Full(turn), turn >> 1)) {
+      if ((threadIdx.x & 31) == 0) atomicExch(&g_attn_error, 8);
+      return -1;
+    }
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+        : "=r"(got), "=r"(x)
+        : "r"(Slot(turn))
+        : "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) BarArrive(Empty(turn));
+    return static_cast<int>(Uniform(got ? x : ~0u));
+  }
 };
-__device__ __forceinline__ void InitNext(const Next& n) {
-  for (int i = 0; i < 2; ++i) {
-    MbarInit(&n.full[i], 1);
-    MbarInit(&n.empty[i], kWarps);
-  }
-}
-// One thread, at the start of piece number `turn`.
-__device__ __forceinline__ bool AskNext(const Next& n, uint32_t turn) {
-  const int i = turn & 1;
-  if (!MbarWait(&n.empty[i], ((turn >> 1) & 1) ^ 1)) return false;
-  MbarExpectTx(&n.full[i], 16);
-  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
-                   SmemAddr(&n.slot[i])),
-               "r"(SmemAddr(&n.full[i]))
-               : "memory");
-  return true;
-}
-// A whole warp, at the end of piece number `turn`: the next piece's block index, or -1.
-__device__ __forceinline__ int TakeNext(const Next& n, uint32_t turn) {
-  const int i = turn & 1;
-  if (!MbarWaitWarp(&n.full[i], (turn >> 1) & 1)) {
-    if ((threadIdx.x & 31) == 0) atomicExch(&g_attn_error, 8);
-    return -1;
-  }
-  uint32_t got, x;
-  asm volatile(
-      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
-      "ld.shared.b128 r, [%2];\n\t"
-      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "mov.u32 %1, 0;\n\t"
-      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
-      : "=r"(got), "=r"(x)
-      : "r"(SmemAddr(&n.slot[i]))
-      : "memory");
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) MbarArrive(&n.empty[i]);
-  return static_cast<int>(Uniform(got ? x : ~0u));
-}
 
 // A wait that remembers a failure, for warps that go on to the next piece; reports it once under `code`.
-struct Waiter {
+template <bool kIdle>
+struct WaiterOf {
   int code;
   bool ok = true;
-  __device__ __forceinline__ explicit Waiter(int c) : code(c) {}
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) {
-    if (ok && !MbarWaitWarp(bar, parity & 1)) {
+  __device__ __forceinline__ explicit WaiterOf(int c) : code(c) {}
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) {
+    if (ok && !BarWait<kIdle>(bar, parity)) {
       if ((threadIdx.x & 31) == 0) atomicExch(&g_attn_error, code);
       ok = false;
     }
@@ -324,25 +398,43 @@ struct Waiter {
     return ok;
   }
 };
+using Waiter     = WaiterOf<false>;
+using IdleWaiter = WaiterOf<true>;
 
-__device__ __forceinline__ uint32_t AllocTmem(uint32_t* slot) {  // by one warp, all columns
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(SmemAddr(slot)), "r"(512u) : "memory");
+__device__ __forceinline__ void AllocTmem(uint32_t slot) {  // by one warp, all columns
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  return 0;
 }
+__device__ __forceinline__ uint32_t AlignedSmem(const uint8_t* raw) { return (SmemAddr(raw) + 1023) & ~1023u; }
 
 // ---------------------------------------------------------------- forward
 // A piece of work is 256 queries of one head as two tiles, past which the keys and values stream: while the warps of one tile
 // compute probabilities, the tensor cores run the products of the other.  Eight softmax warps per tile; a thread has half
 // of a row, 64 scores, and exchanges its maximum with the thread that has the other half.  (With a whole row per thread
 // there is nothing to exchange, but two warps per scheduler leave most issue slots empty: 32 x 512, 16 heads of 64: 87 us.)
+// With 64 output columns per tile, TMEM has room for the probabilities beside the scores, so that the next scores are
+// computed as soon as these have been read; with 128 they take the scores' place.
 template <int HD>
 struct FwdCfg {
   static constexpr int kTileBytes = (HD / 64) * kBoxBytes;
   static constexpr int kStages    = HD == 64 ? 8 : 4;  // tiles of K and V in turn
   static constexpr int kQBufs     = HD == 64 ? 2 : 1;  // queries of this piece of work and the next
-  static constexpr int kMaxBytes  = 2 * 2 * 2 * kTile * 4;
-  static constexpr int kSmemBytes = (2 * kQBufs + kStages) * kTileBytes + kMaxBytes + 1024 + 512;
+  static constexpr bool kOwnP     = HD == 64;          // probabilities beside the scores
+  // shared memory: queries [kQBufs][2], the ring, maxima [2 turns][2 tiles][2 halves][128 rows], barriers
+  static constexpr int kRing      = 2 * kQBufs * kTileBytes;
+  static constexpr int kMax       = kRing + kStages * kTileBytes;
+  static constexpr int kNext      = kMax + 2 * 2 * 2 * kTile * 4;
+  static constexpr int kFull      = kNext + Next::kBytes;
+  static constexpr int kEmpty     = kFull + 8 * kStages;   // both MMA warps are done with a tile of K or V
+  static constexpr int kRaw       = kEmpty + 8 * kStages;  // a tile of V has arrived and has rows to clear before it counts as full
+  static constexpr int kQFull     = kRaw + 8 * kStages;
+  static constexpr int kQEmpty    = kQFull + 8 * kQBufs;
+  static constexpr int kSFull     = kQEmpty + 8 * kQBufs;  // [2] scores of a tile are in TMEM
+  static constexpr int kSFree     = kSFull + 16;           // [2] they have been read
+  static constexpr int kPFull     = kSFree + 16;           // [2] the probabilities are in TMEM
+  static constexpr int kOFull     = kPFull + 16;           // [2] their product with V has completed
+  static constexpr int kTmemSlot  = kOFull + 16;
+  static constexpr int kSmemBytes = kTmemSlot + 16 + 1024;
 };
 
 struct FwdPiece {
@@ -374,72 +466,67 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   using Cfg = FwdCfg<HD>;
   constexpr int S = Cfg::kStages, QB = Cfg::kQBufs;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem_q   = AlignedSmem(smem_raw);                  // [QB][2] tiles
-  uint8_t* ring     = smem_q + 2 * QB * Cfg::kTileBytes;
-  float* exchange   = reinterpret_cast<float*>(ring + S * Cfg::kTileBytes);  // [2 turns][2 tiles][2 halves][128 rows]
-  const Next next{reinterpret_cast<uint4*>(exchange + 8 * kTile), reinterpret_cast<uint64_t*>(exchange + 8 * kTile + 8),
-                  reinterpret_cast<uint64_t*>(exchange + 8 * kTile + 8) + 2};
-  uint64_t* full    = next.empty + 2;
-  uint64_t* empty   = full + S;     // both MMA warps are done with a tile of K or V
-  uint64_t* raw     = empty + S;    // a tile of V has arrived and has rows to clear before it counts as full
-  uint64_t* q_full  = raw + S;      // [QB]
-  uint64_t* q_empty = q_full + QB;  // [QB]
-  uint64_t* s_full  = q_empty + QB; // [2] scores of a tile are in TMEM
-  uint64_t* p_full  = s_full + 2;   // [2] its probabilities are
-  uint64_t* o_full  = p_full + 2;   // [2] the last product of a tile has completed
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  const uint32_t base = AlignedSmem(smem_raw);
+  const Next next{base + Cfg::kNext};
+  auto full = [&](uint32_t k) { return base + Cfg::kFull + k % S * 8; };
+  auto empty = [&](uint32_t k) { return base + Cfg::kEmpty + k % S * 8; };
+  auto raw = [&](uint32_t k) { return base + Cfg::kRaw + k % S * 8; };
+  auto q_full = [&](uint32_t n) { return base + Cfg::kQFull + n % QB * 8; };
+  auto q_empty = [&](uint32_t n) { return base + Cfg::kQEmpty + n % QB * 8; };
+  auto q_tile = [&](uint32_t n, int i) { return base + (n % QB * 2 + i) * Cfg::kTileBytes; };
+  auto tile = [&](uint32_t k) { return base + Cfg::kRing + k % S * Cfg::kTileBytes; };
 
   const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    InitNext(next);
+    next.Init();
     for (int i = 0; i < S; ++i) {
-      MbarInit(&full[i], 1);
-      MbarInit(&empty[i], 2);
-      MbarInit(&raw[i], 1);
+      BarInit(full(i), 1);
+      BarInit(empty(i), 2);
+      BarInit(raw(i), 1);
     }
     for (int i = 0; i < QB; ++i) {
-      MbarInit(&q_full[i], 1);
-      MbarInit(&q_empty[i], 2);
+      BarInit(q_full(i), 1);
+      BarInit(q_empty(i), 2);
     }
     for (int i = 0; i < 2; ++i) {
-      MbarInit(&s_full[i], 1);
-      MbarInit(&p_full[i], kSoftWarps / 2);
-      MbarInit(&o_full[i], 1);
+      BarInit(base + Cfg::kSFull + i * 8, 1);
+      BarInit(base + Cfg::kSFree + i * 8, kSoftWarps / 2);
+      BarInit(base + Cfg::kPFull + i * 8, kSoftWarps / 2);
+      BarInit(base + Cfg::kOFull + i * 8, 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) AllocTmem(tmem_slot);
+  if (warp == kMmaWarp) AllocTmem(base + Cfg::kTmemSlot);
   TcFenceBefore();
   __syncthreads();
   TcFenceAfter();
-  const uint32_t tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(tmem_slot));
-  // columns: scores of either tile (their probabilities in the same place), then either output
+  const uint32_t tmem = Uniform(__float_as_uint(LoadShared(base + Cfg::kTmemSlot)));
+  // columns: scores of either tile, either output, and in what is left either tile's probabilities, or those in the scores' place
   const uint32_t t_s = tmem, t_o = tmem + 256;
 
   if (warp == kTmaWarp) {
     uint32_t e = 0, n = 0;  // tiles of K and V, and pieces with any, so far
     bool ok = true;
     int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+    for (uint32_t turn = 0; index >= 0; index = next.Take<true>(turn), ++turn) {
       const FwdPiece w(p, index);
       if (ElectOne()) {
-        ok = ok && AskNext(next, turn);
+        ok = ok && next.Ask(turn);
         if (w.total > 0 && ok) {
-          const int qb = n % QB, hk = w.h / (p.h / p.hk);
-          ok = MbarWait(&q_empty[qb], ((n / QB) & 1) ^ 1);
-          uint8_t* q = smem_q + qb * 2 * Cfg::kTileBytes;
+          const int hk = w.h / (p.h / p.hk);
+          ok = BarWaitOne(q_empty(n), (n / QB) ^ 1);
           if (ok) {
-            MbarExpectTx(&q_full[qb], 2 * Cfg::kTileBytes);
-            TmaLoadTile<HD, kTile, kTile>(q, &maps.q, w.q0, w.h, w.b, &q_full[qb]);
-            TmaLoadTile<HD, kTile, kTile>(q + Cfg::kTileBytes, &maps.q, w.q0 + kTile, w.h, w.b, &q_full[qb]);
+            BarExpect(q_full(n), 2 * Cfg::kTileBytes);
+            TmaLoadTile<HD, kTile, kTile>(q_tile(n, 0), &maps.q, w.q0, w.h, w.b, q_full(n));
+            TmaLoadTile<HD, kTile, kTile>(q_tile(n, 1), &maps.q, w.q0 + kTile, w.h, w.b, q_full(n));
           }
           for (int k = 0; k < 2 * w.total && ok; ++k) {
-            const uint32_t at = e + k, st = at % S;
-            ok = MbarWait(&empty[st], ((at / S) & 1) ^ 1);
+            const uint32_t at = e + k;
+            ok = BarWaitOne(empty(at), (at / S) ^ 1);
             if (!ok) break;
-            uint64_t* bar = w.ragged && k == 2 * w.total - 1 ? &raw[st] : &full[st];
-            MbarExpectTx(bar, Cfg::kTileBytes);
-            TmaLoadTile<HD, kTile, kTile>(ring + st * Cfg::kTileBytes, k & 1 ? &maps.v : &maps.k, (k >> 1) * kTile, hk, w.b, bar);
+            const uint32_t bar = w.ragged && k == 2 * w.total - 1 ? raw(at) : full(at);
+            BarExpect(bar, Cfg::kTileBytes);
+            TmaLoadTile<HD, kTile, kTile>(tile(at), k & 1 ? &maps.v : &maps.k, (k >> 1) * kTile, hk, w.b, bar);
           }
         }
         if (!ok) atomicExch(&g_attn_error, 1);
@@ -450,16 +537,16 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     }
   } else if (warp == kClearWarp) {
     uint32_t e = 0, uses = 0;  // bit st: parity of the next use of raw[st]
-    Waiter wait(2);
+    IdleWaiter wait(2);
     int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+    for (uint32_t turn = 0; index >= 0; index = next.Take<true>(turn), ++turn) {
       const FwdPiece w(p, index);
       e += 2 * w.total;
       if (w.ragged) {
         const uint32_t st = (e - 1) % S;
-        if (wait(&raw[st], uses >> st)) {
-          ClearRows<kTile>(ring + st * Cfg::kTileBytes, HD / 64, w.len % kTile);
-          if (lane == 0) MbarArrive(&full[st]);
+        if (wait(raw(st), uses >> st)) {
+          ClearRows<kTile>(tile(st), HD / 64, w.len % kTile);
+          if (lane == 0) BarArrive(full(st));
         }
         uses ^= 1u << st;
       }
@@ -467,48 +554,46 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   } else if (warp >= kMmaWarp) {
     const int i = warp - kMmaWarp;  // query tile
     const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-    const uint32_t ts = t_s + i * 128, to = t_o + i * HD;
-    uint32_t e = 0, n = 0, done = 0;  // done: tiles of probabilities so far
+    const uint32_t ts = t_s + i * 128, to = t_o + i * HD, tp = Cfg::kOwnP ? tmem + 384 + i * 64 : ts;
+    uint32_t e = 0, n = 0, done = 0, freed = 0;  // tiles of probabilities, of scores that were read, so far
     Waiter wait(3);
-    auto entry = [&](uint32_t k) { return wait(&full[k % S], k / S); };
-    auto tile  = [&](uint32_t k) { return SmemAddr(ring + (k % S) * Cfg::kTileBytes); };
+    const uint32_t s_full = base + Cfg::kSFull + i * 8, s_free = base + Cfg::kSFree + i * 8, p_full = base + Cfg::kPFull + i * 8,
+                   o_full = base + Cfg::kOFull + i * 8;
+    auto entry = [&](uint32_t k) { return wait(full(k), k / S); };
     int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+    for (uint32_t turn = 0; index >= 0; index = next.Take<false>(turn), ++turn) {
       const FwdPiece w(p, index);
-      const int mine = w.count[i];
+      const int mine = i ? w.count[1] : w.count[0];
       if (w.total > 0 && wait.ok) {
-        const int qb = n % QB;
-        const uint32_t q_addr = SmemAddr(smem_q + (qb * 2 + i) * Cfg::kTileBytes);
-        if (wait(&q_full[qb], n / QB) && entry(e) && ElectOne()) {
-          if (mine > 0) {
-            IssueScores<kBf16, HD, kTile>(ts, q_addr, tile(e), ksteps);
-            UmmaCommit(&s_full[i]);
-          }
-          UmmaCommit(&empty[e % S]);
-          if (mine <= 1) UmmaCommit(&q_empty[qb]);
-        }
-        for (int j = 0; j < w.total && wait.ok; ++j) {  // a tile with fewer keys than the other hands on the rest
-          const uint32_t ev = e + 2 * j + 1, ek = ev + 1;
-          if (!entry(ev) || (j + 1 < w.total && !entry(ek))) break;
+        const uint32_t q_addr = q_tile(n, i);
+        auto scores = [&](int j) {  // of key tile j, if it is one of this query tile's; hands on its keys
           if (j < mine) {
-            if (!wait(&p_full[i], done)) break;
-            ++done;
-            if (ElectOne()) {
-              // the probabilities lie where the next scores go: products complete in the order of their issue
-              IssueFromTmem<kBf16, kTile, kTile / 2>(to, ts, tile(ev), n_out, j > 0);
-              if (j + 1 < mine) {
-                IssueScores<kBf16, HD, kTile>(ts, q_addr, tile(ek), ksteps);
-                UmmaCommit(&s_full[i]);
-                if (j + 2 == mine) UmmaCommit(&q_empty[qb]);
-              } else {
-                UmmaCommit(&o_full[i]);
-              }
-            }
+            IssueScores<kBf16, HD, kTile>(ts, q_addr, tile(e + 2 * j), ksteps);
+            BarCommit(s_full);
           }
+          BarCommit(empty(e + 2 * j));
+          if (j + 1 == max(mine, 1)) BarCommit(q_empty(n));
+        };
+        if (wait(q_full(n), n / QB) && entry(e) && ElectOne()) scores(0);
+        for (int j = 0; j < w.total && wait.ok; ++j) {  // a tile with fewer keys than the other hands on the rest
+          const uint32_t ev = e + 2 * j + 1;
+          if (j + 1 < w.total && !entry(ev + 1)) break;
+          if (Cfg::kOwnP && j + 1 < w.total) {
+            if (j + 1 < mine && !wait(s_free, freed++)) break;
+            if (ElectOne()) scores(j + 1);
+          }
+          if (!entry(ev)) break;
+          if (j < mine && !wait(p_full, done)) break;
           if (ElectOne()) {
-            UmmaCommit(&empty[ev % S]);
-            if (j + 1 < w.total) UmmaCommit(&empty[ek % S]);
+            if (j < mine) {
+              IssueFromTmem<kBf16, kTile, Cfg::kOwnP ? kTile : kTile / 2>(to, tp, tile(ev), n_out, j > 0);
+              BarCommit(o_full);
+            }
+            BarCommit(empty(ev));
+            // in the place of the probabilities: products complete in the order of their issue
+            if (!Cfg::kOwnP && j + 1 < w.total) scores(j + 1);
           }
+          done += j < mine;
         }
         e += 2 * w.total;
         ++n;
@@ -520,29 +605,37 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     const int r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t ts = t_s + lanes + i * 128 + half * 64, to = t_o + lanes + i * HD + half * (HD / 2);
+    const uint32_t tp = Cfg::kOwnP ? tmem + 384 + lanes + i * 64 + half * 32 : ts;
     const int pair_bar = 1 + i * 4 + quarter;         // the two warps that share these rows
     const F2 c2 = Both(p.c);
-    uint32_t done = 0, pieces = 0, swaps = 0;
+    const uint32_t s_full = base + Cfg::kSFull + i * 8, s_free = base + Cfg::kSFree + i * 8, p_full = base + Cfg::kPFull + i * 8,
+                   o_full = base + Cfg::kOFull + i * 8;
+    uint32_t done = 0, swaps = 0;
     Waiter wait(4);
     // this thread's value and the one of the thread with the other half of the row
     auto other = [&](float mine) {
-      float* at = exchange + ((swaps++ & 1) * 4 + i * 2) * kTile + r;
-      at[half * kTile] = mine;
+      const uint32_t at = base + Cfg::kMax + (((swaps++ & 1) * 4 + i * 2) * kTile + r) * 4;
+      StoreShared(at + half * (kTile * 4), mine);
       NamedBarSync(pair_bar, 64);
-      return at[(half ^ 1) * kTile];
+      return LoadShared(at + (half ^ 1) * (kTile * 4));
     };
     int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = TakeNext(next, turn), ++turn) {
+    for (uint32_t turn = 0; index >= 0; index = next.Take<false>(turn), ++turn) {
       const FwdPiece w(p, index);
       const int row = w.q0 + i * kTile + r, count = i ? w.count[1] : w.count[0];
       float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and this half's sum
       for (int j = 0; j < count; ++j, ++done) {
-        wait(&s_full[i], done);  // on a failure the values are void, but every thread keeps meeting its barriers
+        wait(s_full, done);  // on a failure the values are void, but every thread keeps meeting its barriers
         uint32_t s[2][32];
         TmemLoad32Async(ts, s[0]);
         TmemLoad32Async(ts + 32, s[1]);
         TmemLoadWait(s[0]);
         TmemLoadWait(s[1]);
+        if (Cfg::kOwnP && j + 1 < count) {
+          TcFenceBefore();
+          __syncwarp();
+          if (lane == 0) BarArrive(s_free);
+        }
         const int kv0 = j * kTile;
         if (kv0 + kTile > w.len || (p.causal && kv0 + kTile - 1 > w.q0 + i * kTile)) {
           const int limit = (p.causal ? min(w.len, row + 1) : w.len) - kv0 - half * 64;
@@ -554,10 +647,12 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 #pragma unroll
         for (int u = 0; u < 4; ++u) part[u] = __uint_as_float(s[u >> 1][(u & 1) * 16]);
 #pragma unroll
-        for (int k = 1; k < 16; ++k)
+        for (int k = 1; k < 15; k += 2)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) part[u] = MaxNan(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]));
-        float top = MaxNan(MaxNan(part[0], part[1]), MaxNan(part[2], part[3]));
+          for (int u = 0; u < 4; ++u)
+            part[u] = MaxNan(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]), __uint_as_float(s[u >> 1][(u & 1) * 16 + k + 1]));
+        float top = MaxNan(MaxNan(part[0], part[1], __uint_as_float(s[0][15])), MaxNan(part[2], part[3], __uint_as_float(s[0][31])),
+                           MaxNan(__uint_as_float(s[1][15]), __uint_as_float(s[1][31])));
         top = MaxNan(top, other(top));
         // a row without any key so far; and inf - inf: the row is NaN, as by the formula
         if (top == -INFINITY) top = 0.f;
@@ -567,6 +662,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         if (j == 0) {
           m = top;
         } else if (__any_sync(0xffffffffu, !((top - m) * p.c <= 8.f))) {
+          wait(o_full, done - 1);
           const float up = MaxNan(top, m);
           const float f  = Exp2((m - up) * p.c);
           m = up;
@@ -591,20 +687,22 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
             sum[k & 1] = g == 0 && k < 2 ? x : Add2(sum[k & 1], x);
             v[k] = Pack2<kBf16>(x);
           }
-          TmemStore16(ts + g * 16, v);
+          // the last product has read the probabilities before these
+          if (Cfg::kOwnP && g == 0 && j > 0) wait(o_full, done - 1);
+          TmemStore16(tp + g * 16, v);
         }
         const float2 both = SplitF2(Add2(sum[0], sum[1]));
         l += both.x + both.y;
         TmemStoreWait();
         TcFenceBefore();
         __syncwarp();
-        if (lane == 0) MbarArrive(&p_full[i]);
+        if (lane == 0) BarArrive(p_full);
       }
       const bool live = row < w.len;
       uint16_t* dst = static_cast<uint16_t*>(p.o) + w.b * p.so.b + row * p.so.s + w.h * p.so.h;
       if (count > 0) {
         l += other(l);
-        wait(&o_full[i], pieces++);
+        wait(o_full, done - 1);
         const float inv = 1.f / l;
         const int c0 = half * (HD / 2);
 #pragma unroll
@@ -668,18 +766,39 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
 //   !kKeys    Q, dO            K, V               rows are queries                dQ += dS K
 // Both passes compute S and dP, seven products instead of five, and in exchange every sum has one owner: no atomics, no
 // fp32 copy of dQ in memory, and results that do not depend on the order of the blocks.
-// The softmax warps take S of a unit, then its dP; while they work on one, the tensor cores run the products that the other has
-// released and the next unit's.  Each has 32 rows x 32 columns.
-constexpr int kUnit = 128;
+// Units alternate between two sets of eight softmax warps (32 rows x 32 columns a warp), each with its own S and dP in TMEM.  A
+// unit goes through S, P, dP, dS in turn, and every step hands over between the tensor cores and the warps of its set; the
+// other set, half a period behind, uses the exponential unit and the issue slots meanwhile.  Units of 64 rather than 128
+// positions, as two sets of 128 columns do not fit beside the accumulators; their products S and dP take three quarters
+// of the time of twice as many columns.
+constexpr int kUnit = 64;
 template <int HD>
 struct BwdCfg {
-  static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;
-  static constexpr int kStageBytes = 2 * kTileBytes;           // Y1, Y2
-  static constexpr int kStages     = HD == 64 ? 4 : 2;
+  static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;    // what stays: X1 or X2
+  static constexpr int kUnitBytes  = kTileBytes * kUnit / kTile;
+  static constexpr int kStageBytes = 2 * kUnitBytes;           // Y1, Y2
+  static constexpr int kStages     = HD == 64 ? 8 : 4;
   static constexpr int kXBufs      = HD == 64 ? 2 : 1;         // what stays, of this piece of work and the next
-  static constexpr int kSBufs      = HD == 64 ? 2 : 1;         // scores in TMEM; beside accumulators of 128 columns there is room for one
+  static constexpr int kSBufs      = HD == 64 ? 2 : 1;         // scores of a set; beside accumulators of 128 columns there is room for one
   static constexpr int kRowBytes   = 2 * kUnit * 4;            // -L and -D of a unit of queries
-  static constexpr int kSmemBytes  = kXBufs * 2 * kTileBytes + kStages * (kStageBytes + kRowBytes) + 1024 + 512;
+  // shared memory: [kXBufs][X1, X2], the ring [kStages][Y1, Y2], [kStages][-L, -D], barriers
+  static constexpr int kRing       = kXBufs * 2 * kTileBytes;
+  static constexpr int kRows       = kRing + kStages * kStageBytes;
+  static constexpr int kNext       = kRows + kStages * kRowBytes;
+  static constexpr int kFull       = kNext + Next::kBytes;
+  static constexpr int kEmpty      = kFull + 8 * kStages;
+  static constexpr int kRaw        = kEmpty + 8 * kStages;       // a unit has arrived and has rows to clear before it counts as full
+  static constexpr int kXFull      = kRaw + 8 * kStages;
+  static constexpr int kXEmpty     = kXFull + 8 * kXBufs;
+  static constexpr int kSFull      = kXEmpty + 8 * kXBufs;       // [2 SB] S of a unit is in TMEM
+  static constexpr int kSDone      = kSFull + 16 * kSBufs;       // [2 SB] keys: P has taken its place, queries: S has been read
+  static constexpr int kDpFull     = kSDone + 16 * kSBufs;       // [2] dP is in TMEM
+  static constexpr int kDsFull     = kDpFull + 16;               // [2] dS has taken its place
+  static constexpr int kAccFull    = kDsFull + 16;               // a piece's sums are complete
+  static constexpr int kAccFree    = kAccFull + 8;               // all softmax warps have read them
+  static constexpr int kApart      = kAccFree + 8;               // the first set has made its first step
+  static constexpr int kTmemSlot   = kApart + 8;
+  static constexpr int kSmemBytes  = kTmemSlot + 16 + 1024;
 };
 
 template <bool kKeys>
@@ -698,7 +817,7 @@ struct BwdPiece {
     const int units = TilesOf(len, kUnit), group = p.h / p.hk;
     // streamed units: [first, last) of the one head, or of each head of the group
     first = kKeys && p.causal ? x0 / kUnit : 0;
-    const int last = !kKeys && p.causal ? min(units, x0 / kUnit + kTile / kUnit) : units;
+    const int last = !kKeys && p.causal ? min(units, (x0 + kTile) / kUnit) : units;
     per    = last - first;
     total  = x0 >= len ? 0 : per * (kKeys ? group : 1);
     yhead  = kKeys ? head * group : head / group;
@@ -708,41 +827,26 @@ struct BwdPiece {
 
 template <int HD>
 struct BwdSmem {
-  using Cfg = BwdCfg<HD>;
-  uint8_t *x, *ring;   // [XB][X1, X2], [stages][Y1, Y2]
-  float* ld;           // [stages][-L, -D]
-  Next next;
-  uint64_t *full, *empty, *raw;      // [stages] raw: a unit has arrived and has rows to clear before it counts as full
-  uint64_t *x_full, *x_empty;        // [XB]
-  uint64_t *s_full, *s_done;         // [SB] S of a unit is in TMEM; keys: P has taken its place, queries: S has been read
-  uint64_t *dp_full, *ds_full;       // dP is in TMEM; dS has taken its place
-  uint64_t *acc_full;
-  uint32_t* tmem_slot;
-  uint32_t tmem;
-  __device__ __forceinline__ explicit BwdSmem(uint8_t* smem) {
-    x          = smem;
-    ring       = x + Cfg::kXBufs * 2 * Cfg::kTileBytes;
-    ld         = reinterpret_cast<float*>(ring + Cfg::kStages * Cfg::kStageBytes);
-    next.slot  = reinterpret_cast<uint4*>(ld + Cfg::kStages * 2 * kUnit);
-    next.full  = reinterpret_cast<uint64_t*>(next.slot + 2);
-    next.empty = next.full + 2;
-    full       = next.empty + 2;
-    empty      = full + Cfg::kStages;
-    raw        = empty + Cfg::kStages;
-    x_full     = raw + Cfg::kStages;
-    x_empty    = x_full + Cfg::kXBufs;
-    s_full     = x_empty + Cfg::kXBufs;
-    s_done     = s_full + Cfg::kSBufs;
-    dp_full    = s_done + Cfg::kSBufs;
-    ds_full    = dp_full + 1;
-    acc_full   = ds_full + 1;
-    tmem_slot  = reinterpret_cast<uint32_t*>(acc_full + 1);
+  using C = BwdCfg<HD>;
+  uint32_t base, tmem;
+  __device__ __forceinline__ uint32_t X(uint32_t n) const { return base + n % C::kXBufs * (2 * C::kTileBytes); }
+  __device__ __forceinline__ uint32_t Y(uint32_t u) const { return base + C::kRing + u % C::kStages * C::kStageBytes; }
+  __device__ __forceinline__ uint32_t Rows(uint32_t u) const { return base + C::kRows + u % C::kStages * C::kRowBytes; }
+  __device__ __forceinline__ uint32_t Full(uint32_t u) const { return base + C::kFull + u % C::kStages * 8; }
+  __device__ __forceinline__ uint32_t Empty(uint32_t u) const { return base + C::kEmpty + u % C::kStages * 8; }
+  __device__ __forceinline__ uint32_t Raw(uint32_t u) const { return base + C::kRaw + u % C::kStages * 8; }
+  __device__ __forceinline__ uint32_t XFull(uint32_t n) const { return base + C::kXFull + n % C::kXBufs * 8; }
+  __device__ __forceinline__ uint32_t XEmpty(uint32_t n) const { return base + C::kXEmpty + n % C::kXBufs * 8; }
+  __device__ __forceinline__ uint32_t SFull(uint32_t u) const { return base + C::kSFull + u % (2 * C::kSBufs) * 8; }
+  __device__ __forceinline__ uint32_t SDone(uint32_t u) const { return base + C::kSDone + u % (2 * C::kSBufs) * 8; }
+  __device__ __forceinline__ uint32_t DpFull(uint32_t u) const { return base + C::kDpFull + (u & 1) * 8; }
+  __device__ __forceinline__ uint32_t DsFull(uint32_t u) const { return base + C::kDsFull + (u & 1) * 8; }
+  // columns: S and dP of either set, the accumulators, the other S of either set
+  __device__ __forceinline__ uint32_t S(uint32_t u) const {
+    return u % (2 * C::kSBufs) < 2 ? tmem + (u & 1) * 128 : tmem + 384 + (u & 1) * 64;
   }
-  // columns: S, dP, the accumulators, the other S
-  __device__ __forceinline__ uint32_t S(uint32_t u) const { return tmem + (u % Cfg::kSBufs) * 384; }
-  __device__ __forceinline__ uint32_t Dp() const { return tmem + 128; }
+  __device__ __forceinline__ uint32_t Dp(uint32_t u) const { return tmem + 64 + (u & 1) * 128; }
   __device__ __forceinline__ uint32_t Acc(int i) const { return tmem + 256 + i * HD; }
-  __device__ __forceinline__ uint8_t* Y(uint32_t u) const { return ring + (u % Cfg::kStages) * Cfg::kStageBytes; }
 };
 
 // What each kind of warp does for one piece.  u0: units so far, n: pieces with any so far.
@@ -751,26 +855,24 @@ __device__ __forceinline__ bool BwdLoad(const AttnMaps& maps, const AttnParams& 
                                         uint32_t u0, uint32_t n) {  // one thread
   using Cfg = BwdCfg<HD>;
   constexpr int XB = Cfg::kXBufs, ST = Cfg::kStages;
-  const int xb = n % XB;
-  if (!MbarWait(&m.x_empty[xb], ((n / XB) & 1) ^ 1)) return false;
-  uint8_t* x = m.x + xb * 2 * Cfg::kTileBytes;
-  MbarExpectTx(&m.x_full[xb], 2 * Cfg::kTileBytes);
-  TmaLoadTile<HD, kTile, kUnit>(x, kKeys ? &maps.k : &maps.q, w.x0, w.head, w.b, &m.x_full[xb]);
-  TmaLoadTile<HD, kTile, kUnit>(x + Cfg::kTileBytes, kKeys ? &maps.v : &maps.dout, w.x0, w.head, w.b, &m.x_full[xb]);
+  if (!BarWaitOne(m.XEmpty(n), (n / XB) ^ 1)) return false;
+  BarExpect(m.XFull(n), 2 * Cfg::kTileBytes);
+  TmaLoadTile<HD, kTile, kUnit>(m.X(n), kKeys ? &maps.k : &maps.q, w.x0, w.head, w.b, m.XFull(n));
+  TmaLoadTile<HD, kTile, kUnit>(m.X(n) + Cfg::kTileBytes, kKeys ? &maps.v : &maps.dout, w.x0, w.head, w.b, m.XFull(n));
   const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;  // of -L, -D
   int at = 0, yh = w.yhead;  // unit within a head
   for (int k = 0; k < w.total; ++k) {
-    const uint32_t u = u0 + k, st = u % ST;
-    if (!MbarWait(&m.empty[st], ((u / ST) & 1) ^ 1)) return false;
+    const uint32_t u = u0 + k;
+    if (!BarWaitOne(m.Empty(u), (u / ST) ^ 1)) return false;
     const int y0 = (w.first + at) * kUnit;
-    uint64_t* bar = w.ragged && at == w.per - 1 ? &m.raw[st] : &m.full[st];
-    MbarExpectTx(bar, Cfg::kStageBytes + (kKeys ? Cfg::kRowBytes : 0));
+    const uint32_t bar = w.ragged && at == w.per - 1 ? m.Raw(u) : m.Full(u);
+    BarExpect(bar, Cfg::kStageBytes + (kKeys ? Cfg::kRowBytes : 0));
     TmaLoadTile<HD, kUnit, kUnit>(m.Y(u), kKeys ? &maps.q : &maps.k, y0, yh, w.b, bar);
-    TmaLoadTile<HD, kUnit, kUnit>(m.Y(u) + Cfg::kTileBytes, kKeys ? &maps.dout : &maps.v, y0, yh, w.b, bar);
+    TmaLoadTile<HD, kUnit, kUnit>(m.Y(u) + Cfg::kUnitBytes, kKeys ? &maps.dout : &maps.v, y0, yh, w.b, bar);
     if (kKeys) {
       const float* src = p.delta + (static_cast<int64_t>(w.b) * p.h + yh) * p.sp + y0;
-      BulkLoad(m.ld + st * 2 * kUnit, src, kUnit * 4, bar);
-      BulkLoad(m.ld + st * 2 * kUnit + kUnit, src + plane, kUnit * 4, bar);
+      BulkLoad(m.Rows(u), src, kUnit * 4, bar);
+      BulkLoad(m.Rows(u) + kUnit * 4, src + plane, kUnit * 4, bar);
     }
     if (++at == w.per) {
       at = 0;
@@ -782,71 +884,75 @@ __device__ __forceinline__ bool BwdLoad(const AttnMaps& maps, const AttnParams& 
 
 // uses: bit st is the parity of the next use of raw[st].
 template <int HD, bool kKeys>
-__device__ __forceinline__ void BwdClear(const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t& uses, Waiter& wait) {
+__device__ __forceinline__ void BwdClear(const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t& uses, IdleWaiter& wait) {
   for (int k = w.per - 1; w.ragged && k < w.total; k += w.per) {
     const uint32_t st = (u0 + k) % BwdCfg<HD>::kStages;
-    if (!wait(&m.raw[st], uses >> st)) break;
+    if (!wait(m.Raw(st), uses >> st)) break;
     uses ^= 1u << st;
     ClearRows<kUnit>(m.Y(st), 2 * (HD / 64), w.len % kUnit);
-    if ((threadIdx.x & 31) == 0) MbarArrive(&m.full[st]);
+    if ((threadIdx.x & 31) == 0) BarArrive(m.Full(st));
   }
 }
 
 // Which: 0 issues S and P^T dO, 1 issues dP and dS^T Q or dS K.
-template <int HD, bool kBf16, bool kKeys, int kWhich>
+template <bool kBf16, int kWhich, int HD, bool kKeys>
 __device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
                                        Waiter& wait) {
   using Cfg = BwdCfg<HD>;
-  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs, XB = Cfg::kXBufs;
+  constexpr int ST = Cfg::kStages, SB = 2 * Cfg::kSBufs, XB = Cfg::kXBufs;
   const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-  const uint32_t xb = n % XB, x1 = SmemAddr(m.x + xb * 2 * Cfg::kTileBytes), x2 = x1 + Cfg::kTileBytes;
+  const uint32_t x1 = m.X(n), x2 = x1 + Cfg::kTileBytes;
   const uint32_t end = u0 + w.total;
-  auto arrived = [&](uint32_t u) { return wait(&m.full[u % ST], u / ST); };
-  wait(&m.x_full[xb], n / XB);
+  auto arrived = [&](uint32_t u) { return wait(m.Full(u), u / ST); };
+  wait(m.XFull(n), n / XB);
   if (kWhich == 0) {
     auto scores = [&](uint32_t u) {
-      IssueScores<kBf16, HD, kUnit>(m.S(u), x1, SmemAddr(m.Y(u)), ksteps);
-      UmmaCommit(&m.s_full[u % SB]);
-      if (u + 1 == end) UmmaCommit(&m.x_empty[xb]);
+      IssueScores<kBf16, HD, kUnit>(m.S(u), x1, m.Y(u), ksteps);
+      BarCommit(m.SFull(u));
+      if (u + 1 == end) BarCommit(m.XEmpty(n));
     };
     for (uint32_t u = u0; u < min(u0 + SB, end) && arrived(u); ++u)
       if (ElectOne()) scores(u);
     for (uint32_t u = u0; u < end && wait.ok; ++u) {
       const uint32_t next = u + SB;
-      if ((next < end && !arrived(next)) || !wait(&m.s_done[u % SB], u / SB)) break;
+      if ((next < end && !arrived(next)) || !wait(m.SDone(u), u / SB)) break;
+      if (kKeys && u == u0 && n > 0 && !wait(m.base + Cfg::kAccFree, n - 1)) break;
       if (ElectOne()) {
-        if (kKeys) IssueFromTmem<kBf16, kUnit, 32>(m.Acc(1), m.S(u), SmemAddr(m.Y(u)) + Cfg::kTileBytes, n_out, u > u0);
-        UmmaCommit(&m.empty[u % ST]);
+        if (kKeys) IssueFromTmem<kBf16, kUnit, 32>(m.Acc(1), m.S(u), m.Y(u) + Cfg::kUnitBytes, n_out, u > u0);
+        BarCommit(m.Empty(u));
         if (next < end) scores(next);  // in the place of P, which the product before it reads
       }
     }
   } else {
     auto grads = [&](uint32_t u) {
-      IssueScores<kBf16, HD, kUnit>(m.Dp(), x2, SmemAddr(m.Y(u)) + Cfg::kTileBytes, ksteps);
-      UmmaCommit(m.dp_full);
-      if (u + 1 == end) UmmaCommit(&m.x_empty[xb]);
+      IssueScores<kBf16, HD, kUnit>(m.Dp(u), x2, m.Y(u) + Cfg::kUnitBytes, ksteps);
+      BarCommit(m.DpFull(u));
+      if (u + 1 == end) BarCommit(m.XEmpty(n));
     };
-    if (arrived(u0) && ElectOne()) grads(u0);
+    for (uint32_t u = u0; u < min(u0 + 2, end) && arrived(u); ++u)
+      if (ElectOne()) grads(u);
     for (uint32_t u = u0; u < end && wait.ok; ++u) {
-      if ((u + 1 < end && !arrived(u + 1)) || !wait(m.ds_full, u)) break;
+      if ((u + 2 < end && !arrived(u + 2)) || !wait(m.DsFull(u), u / 2)) break;
+      if (u == u0 && n > 0 && !wait(m.base + Cfg::kAccFree, n - 1)) break;
       if (ElectOne()) {
-        IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(), SmemAddr(m.Y(u)), n_out, u > u0);
-        UmmaCommit(&m.empty[u % ST]);
-        if (u + 1 < end) grads(u + 1);
+        IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(u), m.Y(u), n_out, u > u0);
+        BarCommit(m.Empty(u));
+        if (u + 2 < end) grads(u + 2);
       }
     }
   }
-  if (wait.ok && ElectOne()) UmmaCommit(m.acc_full);
+  if (wait.ok && ElectOne()) BarCommit(m.base + Cfg::kAccFull);
 }
 
-template <int HD, bool kBf16, bool kKeys>
+template <bool kBf16, int HD, bool kKeys>
 __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
                                            Waiter& wait) {
   using Cfg = BwdCfg<HD>;
-  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs;
+  constexpr int ST = Cfg::kStages, SB = 2 * Cfg::kSBufs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3;      // TMEM lanes
-  const int col = (warp >> 2) * 32;  // first column of this warp in a unit
+  const int set = warp >> 3;
+  const int col = ((warp >> 2) & 1) * 32;  // first column of this warp in a unit
   const int row = w.x0 + quarter * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
   F2 row_l{}, row_d{};  // -L, -D
@@ -856,29 +962,29 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
     row_d = Both(src[static_cast<int64_t>(p.b) * p.h * p.sp]);
   }
   const F2 c2 = Both(p.c);
-  int y0 = w.first * kUnit, y_end = (w.first + w.per) * kUnit;
-  for (uint32_t u = u0; u < u0 + w.total; ++u) {
-    const int st = u % ST;
-    if (!wait(&m.s_full[u % SB], u / SB)) break;
+  int at = static_cast<int>((set ^ u0) & 1);  // unit within a head
+  if (set == 1 && u0 == 0 && w.total > 0) wait(m.base + Cfg::kApart, 0);  // half a period behind the other set, from the first piece on
+  for (uint32_t u = u0 + at; u < u0 + w.total; u += 2, at += 2) {
+    if (at >= w.per) at %= w.per;  // the group's next head
+    const int y0 = (w.first + at) * kUnit;
+    if (!wait(m.SFull(u), u / SB)) break;
     uint32_t s[32];
     TmemLoad32Async(m.S(u) + lanes + col, s);
-    const bool here = !kKeys || wait(&m.full[st], u / ST);  // -L and -D
+    const bool here = !kKeys || wait(m.Full(u), u / ST);  // -L and -D
     TmemLoadWait(s);
     if (!here) break;
     if (!kKeys) {
       TcFenceBefore();
       __syncwarp();
-      if (lane == 0) MbarArrive(&m.s_done[u % SB]);
+      if (lane == 0) BarArrive(m.SDone(u));
     }
-    const float* ls = m.ld + st * 2 * kUnit + col;
+    const uint32_t ls = m.Rows(u) + col * 4;
     F2 pr[16];
 #pragma unroll
     for (int k = 0; k < 16; k += 2) {
       F2 l0 = row_l, l1 = row_l;
       if (kKeys) {
-        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(ls + 2 * k);
-        l0.v = v.x;
-        l1.v = v.y;
+        LoadPairs(ls + 8 * k, l0, l1);
       }
       pr[k]     = Exp2Mixed<4>(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0), k);
       pr[k + 1] = Exp2Mixed<4>(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1), k + 1);
@@ -901,30 +1007,28 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       TmemStoreWait();
       TcFenceBefore();
       __syncwarp();
-      if (lane == 0) MbarArrive(&m.s_done[u % SB]);
+      if (lane == 0) BarArrive(m.SDone(u));
     }
-    if (!wait(m.dp_full, u)) break;
-    TmemLoad32(m.Dp() + lanes + col, s);
+    if (u == 0 && lane == 0) BarArrive(m.base + Cfg::kApart);
+    if (!wait(m.DpFull(u), u / 2)) break;
+    TmemLoad32(m.Dp(u) + lanes + col, s);
     uint32_t v[16];
 #pragma unroll
     for (int k = 0; k < 16; k += 2) {
       F2 d0 = row_d, d1 = row_d;
       if (kKeys) {
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(ls + kUnit + 2 * k);
-        d0.v = x.x;
-        d1.v = x.y;
+        LoadPairs(ls + kUnit * 4 + 8 * k, d0, d1);
       }
       v[k]     = Pack2<kBf16>(Mul2(pr[k], Add2(Pair(s[2 * k], s[2 * k + 1]), d0)));
       v[k + 1] = Pack2<kBf16>(Mul2(pr[k + 1], Add2(Pair(s[2 * k + 2], s[2 * k + 3]), d1)));
     }
-    TmemStore16(m.Dp() + lanes + col, v);
+    TmemStore16(m.Dp(u) + lanes + col, v);
     TmemStoreWait();
     TcFenceBefore();
     __syncwarp();
-    if (lane == 0) MbarArrive(m.ds_full);
-    if ((y0 += kUnit) == y_end) y0 = w.first * kUnit;  // the group's next head
+    if (lane == 0) BarArrive(m.DsFull(u));
   }
-  if (w.total > 0) wait(m.acc_full, n);
+  if (w.total > 0) wait(m.base + Cfg::kAccFull, n);
   if (!wait.ok) return;
   const bool live = row < w.len;
   constexpr int kCols = HD / 4;
@@ -941,7 +1045,11 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
     }
     if (!live && row < p.s) StoreZeroRow(dst, c0, min(p.d, c0 + kCols));
   }
-  TcFenceBefore();
+  if (w.total > 0) {
+    TcFenceBefore();
+    __syncwarp();
+    if (lane == 0) BarArrive(m.base + Cfg::kAccFree);
+  }
 }
 
 // Both passes in one launch, so that neither leaves a tail of idle SMs: first the pieces of the keys, whose tiles stream past
@@ -951,62 +1059,81 @@ __global__ void __launch_bounds__(kThreads, 1)
 AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   using Cfg = BwdCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
-  BwdSmem<HD> m(AlignedSmem(smem_raw));
+  BwdSmem<HD> m{AlignedSmem(smem_raw), 0};
+  const Next next{m.base + Cfg::kNext};
   const int warp = Uniform(threadIdx.x >> 5);
   if (threadIdx.x == 0) {
-    InitNext(m.next);
+    next.Init();
     for (int i = 0; i < Cfg::kStages; ++i) {
-      MbarInit(&m.full[i], 1);
-      MbarInit(&m.empty[i], 2);  // both MMA warps
-      MbarInit(&m.raw[i], 1);
+      BarInit(m.Full(i), 1);
+      BarInit(m.Empty(i), 2);  // both MMA warps
+      BarInit(m.Raw(i), 1);
     }
     for (int i = 0; i < Cfg::kXBufs; ++i) {
-      MbarInit(&m.x_full[i], 1);
-      MbarInit(&m.x_empty[i], 2);
+      BarInit(m.XFull(i), 1);
+      BarInit(m.XEmpty(i), 2);
     }
-    for (int i = 0; i < Cfg::kSBufs; ++i) {
-      MbarInit(&m.s_full[i], 1);
-      MbarInit(&m.s_done[i], kSoftWarps);
+    for (int i = 0; i < 2 * Cfg::kSBufs; ++i) {
+      BarInit(m.SFull(i), 1);
+      BarInit(m.SDone(i), kSoftWarps / 2);
     }
-    MbarInit(m.dp_full, 1);
-    MbarInit(m.ds_full, kSoftWarps);
-    MbarInit(m.acc_full, 2);
+    for (int i = 0; i < 2; ++i) {
+      BarInit(m.DpFull(i), 1);
+      BarInit(m.DsFull(i), kSoftWarps / 2);
+    }
+    BarInit(m.base + Cfg::kAccFull, 2);
+    BarInit(m.base + Cfg::kAccFree, kSoftWarps);
+    BarInit(m.base + Cfg::kApart, kSoftWarps / 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) AllocTmem(m.tmem_slot);
+  if (warp == kMmaWarp) AllocTmem(m.base + Cfg::kTmemSlot);
   TcFenceBefore();
   __syncthreads();
   TcFenceAfter();
-  m.tmem = Uniform(*reinterpret_cast<volatile uint32_t*>(m.tmem_slot));
+  m.tmem = Uniform(__float_as_uint(LoadShared(m.base + Cfg::kTmemSlot)));
 
+  // what a kind of warp does for each piece, until there is none: `step` gets the piece, the units and the pieces with any before it
   const int key_pieces = p.sp / kTile * p.b * p.hk;
-  uint32_t u0 = 0, n = 0;
-  Waiter wait(warp < kSoftWarps ? 7 : 6);
-  bool loading = true;
-  uint32_t uses = 0;
-  int index = blockIdx.x;
-  for (uint32_t turn = 0; index >= 0; index = TakeNext(m.next, turn), ++turn) {
-    auto work = [&](const auto& w) {
-      constexpr bool kKeys = std::is_same<decltype(w), const BwdPiece<true>&>::value;
-      if (warp < kSoftWarps) {
-        BwdSoftmax<HD, kBf16, kKeys>(p, m, w, u0, n, wait);
-      } else if (warp == kTmaWarp) {
-        if (ElectOne()) {
-          loading = loading && AskNext(m.next, turn);
-          if (w.total > 0) loading = loading && BwdLoad<HD, kKeys>(maps, p, m, w, u0, n);
-          if (!loading) atomicExch(&g_attn_error, 5);
-        }
-        __syncwarp();
-      } else if (w.total > 0 && wait.ok) {
-        if (warp == kClearWarp) BwdClear<HD, kKeys>(m, w, u0, uses, wait);
-        else if (warp == kMmaWarp) BwdMma<HD, kBf16, kKeys, 0>(p, m, w, u0, n, wait);
-        else BwdMma<HD, kBf16, kKeys, 1>(p, m, w, u0, n, wait);
+  auto pieces = [&](auto idle, auto&& step) {
+    uint32_t u0 = 0, n = 0;
+    int index = blockIdx.x;
+    for (uint32_t turn = 0; index >= 0; index = next.Take<decltype(idle)::value>(turn), ++turn) {
+      auto work = [&](const auto& w) {
+        step(w, turn, u0, n);
+        u0 += w.total;
+        n += w.total > 0;
+      };
+      if (index < key_pieces) work(BwdPiece<true>(p, index));
+      else work(BwdPiece<false>(p, index - key_pieces));
+    }
+  };
+  if (warp == kTmaWarp) {
+    bool ok = true;
+    pieces(std::true_type{}, [&](const auto& w, uint32_t turn, uint32_t u0, uint32_t n) {
+      if (ElectOne()) {
+        ok = ok && next.Ask(turn);
+        if (w.total > 0) ok = ok && BwdLoad(maps, p, m, w, u0, n);
+        if (!ok) atomicExch(&g_attn_error, 5);
       }
-      u0 += w.total;
-      n += w.total > 0;
-    };
-    if (index < key_pieces) work(BwdPiece<true>(p, index));
-    else work(BwdPiece<false>(p, index - key_pieces));
+      __syncwarp();
+    });
+  } else if (warp == kClearWarp) {
+    uint32_t uses = 0;
+    IdleWaiter wait(6);
+    pieces(std::true_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t) { BwdClear(m, w, u0, uses, wait); });
+  } else if (warp == kMmaWarp) {
+    Waiter wait(6);
+    pieces(std::false_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t n) {
+      if (w.total > 0 && wait.ok) BwdMma<kBf16, 0>(p, m, w, u0, n, wait);
+    });
+  } else if (warp == kMmaWarp + 1) {
+    Waiter wait(6);
+    pieces(std::false_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t n) {
+      if (w.total > 0 && wait.ok) BwdMma<kBf16, 1>(p, m, w, u0, n, wait);
+    });
+  } else {
+    Waiter wait(7);
+    pieces(std::false_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t n) { BwdSoftmax<kBf16>(p, m, w, u0, n, wait); });
   }
   TcFenceBefore();
   __syncthreads();
