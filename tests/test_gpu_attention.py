@@ -152,15 +152,17 @@ def test_the_same_bits_twice_on_other_streams_and_in_graphs():
     for name in first:
         assert torch.equal(first[name], other[name]), name
     # two graphs with their own outputs; replayed on other inputs, then in turn
-    from tips_b200.ops.attention import _attention_bwd, _attention_fwd
+    from tips_b200.ops.attention import _attention_bwd, _attention_fwd, _view
     bufs = [t.detach().clone() for t in (q, k, v, do)]
+    views = [_view(t) for t in bufs[:3]]
+    shape = (2, 500, 4, 2, 64)
     graphs = []
     for _ in range(2):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            out, lse, a, b, c = _attention_fwd(*bufs[:3], n, 0.125, False)
-            grads = [torch.empty_like(t) for t in (a, b, c)]
-            _attention_bwd(bufs[3], a, b, c, out, lse, n, 0.125, False, *grads)
+            out, lse = _attention_fwd(bufs[0], shape, *views, n, 0.125, False)
+            grads = [torch.empty_like(t) for t in bufs[:3]]
+            _attention_bwd(bufs[3], shape, *views, out, lse, n, 0.125, False, *(_view(t) for t in grads))
         graphs.append((g, dict(zip(("out", "dq", "dk", "dv"), (out, *grads)))))
     for t, x in zip(bufs, make(2, 500, 4, 2, 64, torch.bfloat16, seed=11)):
         t.copy_(x)

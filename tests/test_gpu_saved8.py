@@ -63,7 +63,7 @@ def test_activation_backward(rows, cols, dtype):
     # and reciprocal at 2^-22 of factors up to 3); fp16's least half step is 2^-25
     slack = 4e-6 * dy.double().abs()
     for bias_dtype in DTYPES + [None]:
-        dz, db = act_bwd8(dy, p.q, p.e, bias_dtype)
+        dz, db = act_bwd8(dy, p.buf, bias_dtype)
         assert dz.dtype == dtype and ((dz.double() - want).abs() <= u * want.abs() + slack + 2.0 ** -25).all()
         if bias_dtype is None:
             assert db is None
@@ -71,8 +71,8 @@ def test_activation_backward(rows, cols, dtype):
         # sums of the unrounded values in 32 bits: 2^-24 per addition, at most rows of them in a row
         off = (slack + rows * 2.0 ** -24 * want.abs()).sum(0) + torch.finfo(bias_dtype).eps / 2 * want.sum(0).abs() + 2.0 ** -25
         assert db.dtype == bias_dtype and ((db.double() - want.sum(0)).abs() <= off).all()
-        assert torch.equal(db, act_bwd8(dy, p.q, p.e, bias_dtype)[1])
-    same_dy, db = act_bwd8(dy, None, None, torch.float32)
+        assert torch.equal(db, act_bwd8(dy, p.buf, bias_dtype)[1])
+    same_dy, db = act_bwd8(dy, None, torch.float32)
     assert same_dy.data_ptr() == dy.data_ptr()
     off = rows * 2.0 ** -24 * dy.double().abs().sum(0) + 2.0 ** -24 * dy.double().sum(0).abs()
     assert ((db.double() - dy.double().sum(0)).abs() <= off).all()

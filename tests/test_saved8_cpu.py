@@ -41,7 +41,8 @@ def test_definition():
 def test_shapes_and_the_last_block(shape):
     x = torch.randn(shape, generator=torch.Generator().manual_seed(1))
     p = pack8(x)
-    assert p.shape == x.shape and p.nbytes == x.numel() + (x.numel() + 31) // 32
+    assert p.shape == x.shape and p.q.numel() == x.numel() and p.e.numel() == (x.numel() + 31) // 32
+    assert x.numel() * 33 / 32 <= p.nbytes < x.numel() * 33 / 32 + 17
     y = p.unpack()
     assert y.shape == x.shape and y.dtype == x.dtype
     flat = x.reshape(-1).tolist()

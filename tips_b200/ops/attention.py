@@ -87,30 +87,19 @@ def _check_lengths(lengths, b: int, device) -> None:
         raise ValueError(f"lengths are on {lengths.device}, the inputs on {device}")
 
 
-def _check_attention(q, k, v, lengths, scale) -> float:
-    """Checks the arguments of `attention` and returns the scale to use."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [batch, seq, heads, head_size], got {tuple(t.shape)}")
-        if t.dtype != q.dtype or t.device != q.device:
-            raise TypeError(f"q, k and v must share dtype and device: {name} is {t.dtype} on {t.device}, q {q.dtype} on {q.device}")
-    b, s, h, d = q.shape
-    if k.shape != v.shape or k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
-        raise ValueError(f"k and v must be [{b}, {s}, kv_heads, {d}] like q, got {tuple(k.shape)} and {tuple(v.shape)}")
-    hk = k.shape[2]
-    if h == 0 or hk == 0 or h % hk != 0:
+def _check_attention(t, s, h, hk, d, lengths, scale) -> float:
+    """Checks sizes, type and the other arguments of an attention over a tensor like `t` and returns the scale to use."""
+    if h <= 0 or hk <= 0 or h % hk != 0:
         raise ValueError(f"{h} heads cannot share {hk} key and value heads evenly")
-    if d == 0:
+    if d <= 0:
         raise ValueError("the head size must be positive")
-    _check_lengths(lengths, b, q.device)
-    if scale is None:
-        scale = 1.0 / math.sqrt(d)
-    scale = float(scale)
+    _check_lengths(lengths, t.shape[0], t.device)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    if q.is_cuda:
-        if q.dtype not in (torch.bfloat16, torch.float16):
-            raise TypeError(f"attention on a GPU takes bfloat16 or float16, got {q.dtype}")
+    if t.is_cuda:
+        if t.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"attention on a GPU takes bfloat16 or float16, got {t.dtype}")
         if d % 8 != 0 or d > 128:
             raise ValueError(f"attention on a GPU takes head sizes that are multiples of 8 up to 128, got {d}")
     return scale
@@ -119,90 +108,105 @@ def _check_attention(q, k, v, lengths, scale) -> float:
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy where the kernels cannot read it in place: they need a contiguous last axis, positive strides of whole
     16 bytes and a 16-byte-aligned start."""
-    st = t.stride()
-    if t.data_ptr() % 16 == 0 and st[3] == 1 and all(x > 0 and x % 8 == 0 for x in st[:3]):
+    sb, ss, sh, sd = t.stride()
+    if sd == 1 and t.data_ptr() % 16 == 0 and sb > 0 and ss > 0 and sh > 0 and (sb | ss | sh) % 8 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(*tensors):
-    return base.i64_array([x for t in tensors for x in t.stride()[:3]])
+def _view(t: torch.Tensor):
+    """(address, strides) of a [batch, seq, heads, d] tensor as the launchers take them."""
+    return t.data_ptr(), t.stride()[:3]
 
 
-def _attention_fwd(q, k, v, lengths, scale, causal):
-    """(out, lse, and q, k, v as the kernel read them) for CUDA tensors."""
-    b, s, h, d = q.shape
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    out = torch.empty(b, s, h, d, dtype=q.dtype, device=q.device)
-    lse = torch.empty(b, h, -(-s // 128) * 128, dtype=torch.float32, device=q.device)
-    if out.numel() == 0:
-        return out, lse, q, k, v
-    with torch.cuda.device(q.device):
-        base.check(base.K().tipsk_attention_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), base.ptr(lengths),
-            int(lengths is not None and lengths.dtype == torch.int64), b, s, h, k.shape[2], d, base.code(q),
-            _strides(q, k, v, out), scale, int(causal), base.stream()), "attention_fwd")
-    return out, lse, q, k, v
+def _packed_views(t: torch.Tensor, h: int, hk: int, d: int):
+    """The same of the q, k and v heads of a contiguous [batch, seq, (h + 2 hk) * d] tensor, without making views."""
+    at, row, step = t.data_ptr(), (h + 2 * hk) * d, d * t.element_size()
+    st = (t.shape[1] * row, row, d)
+    return (at, st), (at + h * step, st), (at + (h + hk) * step, st)
 
 
-def _attention_bwd(dout, q, k, v, out, lse, lengths, scale, causal, dq, dk, dv):
-    """Writes the gradients into dq, dk, dv (views whose last axis is contiguous)."""
-    b, s, h, d = q.shape
-    if out.numel() == 0:
+def _strides(*views):
+    return base.i64_array([x for _, st in views for x in st])
+
+
+def _attention_fwd(like, shape, q, k, v, lengths, scale, causal):
+    """(out, lse) for the views q, k, v of CUDA tensors like `like`; shape = (b, s, h, hk, d)."""
+    b, s, h, hk, d = shape
+    out = torch.empty(b, s, h, d, dtype=like.dtype, device=like.device)
+    lse = torch.empty(b, h, -(-s // 128) * 128, dtype=torch.float32, device=like.device)
+    if out.numel():
+        with base.device_of(like):
+            base.check(base.K().tipsk_attention_fwd(
+                q[0], k[0], v[0], out.data_ptr(), lse.data_ptr(), base.ptr(lengths),
+                int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(like),
+                _strides(q, k, v, _view(out)), scale, int(causal), base.stream()), "attention_fwd")
+    return out, lse
+
+
+def _attention_bwd(dout, shape, q, k, v, out, lse, lengths, scale, causal, dq, dk, dv):
+    """Writes the gradients into the views dq, dk, dv."""
+    b, s, h, hk, d = shape
+    if not out.numel():
         return
     dout = _rows16(dout)
     delta = torch.empty(2, *lse.shape, dtype=torch.float32, device=lse.device)
-    with torch.cuda.device(q.device):
+    with base.device_of(out):
         base.check(base.K().tipsk_attention_bwd(
-            dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), base.ptr(lengths),
-            int(lengths is not None and lengths.dtype == torch.int64), b, s, h, k.shape[2], d, base.code(q),
-            _strides(q, k, v, out, dout, dq, dk, dv), scale, int(causal), base.stream()), "attention_bwd")
+            dout.data_ptr(), q[0], k[0], v[0], out.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq[0], dk[0], dv[0],
+            base.ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(out),
+            _strides(q, k, v, _view(out), _view(dout), dq, dk, dv), scale, int(causal), base.stream()), "attention_bwd")
     base.count_launches(1)
 
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, scale, causal):
-        out, lse, q, k, v = _attention_fwd(q, k, v, lengths, scale, causal)
+        shape = (*q.shape[:3], k.shape[2], q.shape[3])
+        q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        out, lse = _attention_fwd(q, shape, _view(q), _view(k), _view(v), lengths, scale, causal)
         ctx.save_for_backward(q, k, v, out, lse, lengths)
-        ctx.scale, ctx.causal = scale, causal
+        ctx.meta = (shape, scale, causal)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, lengths = ctx.saved_tensors
+        shape, scale, causal = ctx.meta
+        # a saved-tensor hook may have changed the layout
+        q, k, v, out, lse = _rows16(q), _rows16(k), _rows16(v), _rows16(out), lse.contiguous()
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _attention_bwd(dout, q, k, v, out, lse, lengths, ctx.scale, ctx.causal, dq, dk, dv)
+        _attention_bwd(dout, shape, _view(q), _view(k), _view(v), out, lse, lengths, scale, causal, _view(dq), _view(dk), _view(dv))
         return dq, dk, dv, None, None, None
 
 
-def _split_heads(t: torch.Tensor, h: int, hk: int):
-    """q, k, v views [b, s, heads, d] of a packed [b, s, (h + 2 hk) * d] tensor."""
-    b, s, width = t.shape
-    x = t.view(b, s, h + 2 * hk, width // (h + 2 * hk))
-    return x[:, :, :h], x[:, :, h:h + hk], x[:, :, h + hk:]
+def _packed16(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 class _PackedOwnAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, h, hk, lengths, scale, causal):
-        qkv = qkv.contiguous()
-        q, k, v = _split_heads(qkv, h, hk)
-        out, lse, _, _, _ = _attention_fwd(q, k, v, lengths, scale, causal)
+        qkv = _packed16(qkv)
+        b, s, width = qkv.shape
+        shape = (b, s, h, hk, width // (h + 2 * hk))
+        out, lse = _attention_fwd(qkv, shape, *_packed_views(qkv, h, hk, shape[4]), lengths, scale, causal)
         ctx.save_for_backward(qkv, out, lse, lengths)
-        ctx.meta = (h, hk, scale, causal)
-        return out.view(*qkv.shape[:2], -1)
+        ctx.meta = (shape, scale, causal)
+        return out.view(b, s, h * shape[4])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         qkv, out, lse, lengths = ctx.saved_tensors
-        h, hk, scale, causal = ctx.meta
-        q, k, v = (_rows16(t) for t in _split_heads(qkv, h, hk))
+        shape, scale, causal = ctx.meta
+        _, _, h, hk, d = shape
+        qkv, out, lse = _packed16(qkv), _rows16(out), lse.contiguous()
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _attention_bwd(dy.reshape(out.shape), q, k, v, out, lse, lengths, scale, causal, *_split_heads(dqkv, h, hk))
+        _attention_bwd(dy.reshape(out.shape), shape, *_packed_views(qkv, h, hk, d), out, lse, lengths, scale, causal,
+                       *_packed_views(dqkv, h, hk, d))
         return dqkv, None, None, None, None, None
 
 
@@ -244,7 +248,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     gradient in the backward pass, are rounded to the inputs' type as operands of the products.  Gradients do not depend on
     the order of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
     do not see it, as 0 * inf does in the formula.  `lengths` may not change between forward and backward."""
-    scale = _check_attention(q, k, v, lengths, scale)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [batch, seq, heads, head_size], got {tuple(t.shape)}")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise TypeError(f"q, k and v must share dtype and device: {name} is {t.dtype} on {t.device}, q {q.dtype} on {q.device}")
+    b, s, h, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
+        raise ValueError(f"k and v must be [{b}, {s}, kv_heads, {d}] like q, got {tuple(k.shape)} and {tuple(v.shape)}")
+    scale = _check_attention(q, s, h, k.shape[2], d, lengths, scale)
     if not q.is_cuda:
         return _plain_attention(q, k, v, lengths, scale, causal)
     if lengths is not None:
@@ -262,10 +274,11 @@ def packed_attention(qkv: torch.Tensor, heads: int, causal: bool = False, kv_hea
         hk = heads if kv_heads is None else kv_heads
         if qkv.dim() != 3 or heads <= 0 or hk <= 0 or qkv.shape[2] == 0 or qkv.shape[2] % (heads + 2 * hk) != 0:
             raise ValueError(f"qkv must be [batch, seq, ({heads} + 2 * {hk}) * head_size], got {tuple(qkv.shape)}")
-        q, k, v = _split_heads(qkv.contiguous(), heads, hk)
-        scale = _check_attention(q.detach(), k.detach(), v.detach(), lengths, scale)
+        b, s, width = qkv.shape
+        scale = _check_attention(qkv, s, heads, hk, width // (heads + 2 * hk), lengths, scale)
         if not qkv.is_cuda:
-            return _plain_attention(q, k, v, lengths, scale, causal).reshape(*qkv.shape[:2], -1)
+            x = qkv.view(b, s, heads + 2 * hk, -1) if b and s else qkv.new_empty(b, s, heads + 2 * hk, width // (heads + 2 * hk))
+            return _plain_attention(*x.split([heads, hk, hk], 2), lengths, scale, causal).reshape(b, s, -1)
         if lengths is not None:
             lengths = lengths.contiguous()
         return _PackedOwnAttentionFn.apply(qkv, heads, hk, lengths, scale, bool(causal))

@@ -53,6 +53,22 @@ def stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *a):
+        return None
+
+
+_HERE = _Here()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which launches go to the device of a CUDA tensor (nothing to do when it is the current one)."""
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
 def comm_stream() -> int:
     """Current stream for the collective launchers, where a null handle means "the library's own stream":
     the legacy default stream is passed as its explicit handle instead."""

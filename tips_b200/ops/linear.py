@@ -149,17 +149,15 @@ class _Linear8Fn(torch.autograd.Function):
         x2 = x.reshape(-1, x.shape[-1])
         if not x2.is_contiguous():
             x2 = x2.contiguous()
-        gelu = _ACT[act] == 2
-        xq = xe = pq = pe = None
-        if gelu:
+        x8 = pre8 = None
+        if _ACT[act] == 2 and any(ctx.needs_input_grad[:3]):
             y, pre = gemm_tn(x2, weight, bias, act, want_pre=True)
-            if any(ctx.needs_input_grad[:3]):
-                pq, pe = saved8._pack(pre)
+            pre8 = saved8._pack(pre)
         else:
             y = gemm_tn(x2, weight, bias, act)
         if ctx.needs_input_grad[1]:
-            xq, xe = saved8._pack(x2)
-        ctx.save_for_backward(weight, xq, xe, pq, pe)
+            x8 = saved8._pack(x2)
+        ctx.save_for_backward(weight, x8, pre8)
         ctx.x_dtype, ctx.bias_dtype = x.dtype, None if bias is None else bias.dtype
         ctx.in_shape = x.shape
         return y.view(*x.shape[:-1], weight.shape[0])
@@ -171,18 +169,18 @@ class _Linear8Fn(torch.autograd.Function):
 
 
 def _linear8_backward(ctx, dy, d_alias):
-    weight, xq, xe, pq, pe = ctx.saved_tensors  # pq, pe: None without an activation
+    weight, x8, pre8 = ctx.saved_tensors  # pre8: None without an activation
     n, k = weight.shape
     dz = dy.reshape(-1, n)
     if not dz.is_contiguous():
         dz = dz.contiguous()
     want_bias = ctx.bias_dtype if ctx.needs_input_grad[2] else None
-    dz, db = saved8.act_bwd8(dz, pq, pe, want_bias)
+    dz, db = saved8.act_bwd8(dz, pre8, want_bias)
     dx = dw = None
     if ctx.needs_input_grad[0]:
         dx = _input_grad(dz, weight, d_alias).view(ctx.in_shape)
     if ctx.needs_input_grad[1]:
-        dw = _weight_grad(dz, saved8._unpack(xq, xe, (dz.shape[0], k), ctx.x_dtype), weight.dtype).to(weight.dtype)
+        dw = _weight_grad(dz, saved8._unpack(x8, (dz.shape[0], k), ctx.x_dtype), weight.dtype).to(weight.dtype)
     return dx, dw, db, None
 
 

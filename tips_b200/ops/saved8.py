@@ -13,6 +13,8 @@ The reference keeps no activations of its own (it trains TensorFlow models).
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import base
@@ -32,7 +34,18 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def _pack_plain(x: torch.Tensor):
+def _exponents_at(n: int) -> int:
+    """Where the exponents start in the buffer of n values: behind them, on 16 bytes."""
+    return -(-n // 16) * 16
+
+
+def _parts(buf: torch.Tensor, n: int):
+    """The int8 values and step exponents in a buffer of n values."""
+    at = _exponents_at(n)
+    return buf[:n], buf[at:at - (-n // BLOCK)]
+
+
+def _pack_plain(x: torch.Tensor, buf: torch.Tensor) -> None:
     n = x.numel()
     flat = torch.zeros(-(-n // BLOCK) * BLOCK, dtype=torch.float32)
     flat[:n] = x.reshape(-1)
@@ -43,36 +56,41 @@ def _pack_plain(x: torch.Tensor):
     e = torch.where(part == 0, torch.full_like(e, -126), e)
     step = ((e + 127) << 23).view(torch.float32)
     q = torch.where(finite, torch.round(flat / step).clamp(-127, 127), -128.0)
-    return q.to(torch.int8).view(-1)[:n].clone(), e.to(torch.int8).view(-1)
+    values, exponents = _parts(buf, n)
+    values.copy_(q.view(-1)[:n])
+    exponents.copy_(e.view(-1))
 
 
-def _unpack_plain(q: torch.Tensor, e: torch.Tensor, dtype) -> torch.Tensor:
-    step = ((e.to(torch.int32) + 127) << 23).view(torch.float32).repeat_interleave(BLOCK)[:q.numel()]
+def _unpack_plain(buf: torch.Tensor, n: int, dtype) -> torch.Tensor:
+    q, e = _parts(buf, n)
+    step = ((e.to(torch.int32) + 127) << 23).view(torch.float32).repeat_interleave(BLOCK)[:n]
     return torch.where(q == -128, float("nan"), q.float() * step).to(dtype)
 
 
-def _pack(x: torch.Tensor):
-    """(q, e) of a tensor: int8 values and step exponents, flat."""
-    if not x.is_cuda:
-        return _pack_plain(x)
-    x = _aligned(x)
+def _pack(x: torch.Tensor) -> torch.Tensor:
+    """The 8-bit form of a tensor as one int8 buffer: the values, and from _exponents_at on a step exponent per block."""
     n = x.numel()
-    q = torch.empty(n, dtype=torch.int8, device=x.device)
-    e = torch.empty(-(-n // BLOCK), dtype=torch.int8, device=x.device)
+    at = _exponents_at(n)
+    buf = torch.empty(at - (-n // BLOCK), dtype=torch.int8, device=x.device)
+    if not x.is_cuda:
+        _pack_plain(x, buf)
+    elif n:
+        x = _aligned(x)
+        with base.device_of(x):
+            q = buf.data_ptr()
+            base.check(base.K().tipsk_pack8(x.data_ptr(), q, q + at, n, base.code(x), base.stream()), "pack8")
+    return buf
+
+
+def _unpack(buf: torch.Tensor, shape, dtype) -> torch.Tensor:
+    if not buf.is_cuda:
+        return _unpack_plain(buf, math.prod(shape), dtype).view(shape)
+    y = torch.empty(shape, dtype=dtype, device=buf.device)
+    n = y.numel()
     if n:
-        with torch.cuda.device(x.device):
-            base.check(base.K().tipsk_pack8(x.data_ptr(), q.data_ptr(), e.data_ptr(), n, base.code(x), base.stream()), "pack8")
-    return q, e
-
-
-def _unpack(q: torch.Tensor, e: torch.Tensor, shape, dtype) -> torch.Tensor:
-    if not q.is_cuda:
-        return _unpack_plain(q, e, dtype).view(shape)
-    y = torch.empty(shape, dtype=dtype, device=q.device)
-    if y.numel():
-        with torch.cuda.device(q.device):
-            base.check(base.K().tipsk_unpack8(q.data_ptr(), e.data_ptr(), y.data_ptr(), y.numel(), base.code(y), base.stream()),
-                       "unpack8")
+        with base.device_of(y):
+            q = buf.data_ptr()
+            base.check(base.K().tipsk_unpack8(q, q + _exponents_at(n), y.data_ptr(), n, base.code(y), base.stream()), "unpack8")
     return y
 
 
@@ -80,52 +98,62 @@ class Packed8:
     """A tensor in 8 bits: `q` (int8, one per value, -128 for NaN), `e` (int8, one per block of 32: the step is 2**e),
     `shape` and `dtype` of what was packed."""
 
-    __slots__ = ("q", "e", "shape", "dtype")
+    __slots__ = ("buf", "shape", "dtype")
 
-    def __init__(self, q, e, shape, dtype):
-        self.q, self.e, self.shape, self.dtype = q, e, torch.Size(shape), dtype
+    def __init__(self, buf, shape, dtype):
+        self.buf, self.shape, self.dtype = buf, torch.Size(shape), dtype
+
+    @property
+    def q(self) -> torch.Tensor:
+        return _parts(self.buf, self.shape.numel())[0]
+
+    @property
+    def e(self) -> torch.Tensor:
+        return _parts(self.buf, self.shape.numel())[1]
 
     @property
     def nbytes(self) -> int:
-        return self.q.numel() + self.e.numel()
+        return self.buf.numel()
 
     def unpack(self, dtype: torch.dtype | None = None) -> torch.Tensor:
         """The stored values, in `dtype` (default: that of the packed tensor).  fp16 rounds values below 2**-14 once more,
         and values beyond its range become infinite."""
         dtype = self.dtype if dtype is None else dtype
         _check(dtype, "unpack")
-        return _unpack(self.q, self.e, self.shape, dtype)
+        return _unpack(self.buf, self.shape, dtype)
 
 
 def pack8(x: torch.Tensor) -> Packed8:
     """The 8-bit form of a float32, bfloat16 or float16 tensor (any strides; no gradient flows through it)."""
     _check(x.dtype, "pack8")
     x = x.detach()
-    return Packed8(*_pack(x), x.shape, x.dtype)
+    return Packed8(_pack(x), x.shape, x.dtype)
 
 
-def act_bwd8(dy: torch.Tensor, q, e, bias_dtype=None):
-    """(dz, column sums of dz or None) for dy [rows, cols], with dz = dy * gelu'(z) for z stored as (q, e), or dy without them."""
+def act_bwd8(dy: torch.Tensor, z: torch.Tensor | None, bias_dtype=None):
+    """(dz, column sums of dz or None) for dy [rows, cols], with dz = dy * gelu'(z) for z in 8 bits (the buffer of `_pack`), or
+    dy itself without it."""
     rows, cols = dy.shape
-    if q is None and bias_dtype is None:
+    if z is None and bias_dtype is None:
         return dy, None
     if dy.is_cuda and cols % 8 == 0 and dy.dtype in _DTYPES and rows and cols:
         dy = _aligned(dy)
         lib = base.K()
-        with torch.cuda.device(dy.device):
-            dz = None if q is None else torch.empty_like(dy)
+        with base.device_of(dy):
+            dz = None if z is None else torch.empty_like(dy)
             db = part = None
             if bias_dtype is not None:
                 db = torch.empty(cols, dtype=bias_dtype, device=dy.device)
-                part = torch.empty(lib.tipsk_act_bwd8_parts(rows, cols), cols, dtype=torch.float32, device=dy.device)
+                part = torch.empty(lib.tipsk_act_bwd8_parts(rows, cols) * cols, dtype=torch.float32, device=dy.device)
                 base.count_launches(1)
-            base.check(lib.tipsk_act_bwd8(dy.data_ptr(), base.ptr(q), base.ptr(e), base.ptr(dz), base.ptr(db),
-                                          0 if db is None else base.code(db), base.ptr(part), rows, cols, base.code(dy),
-                                          base.stream()), "act_bwd8")
+            q = base.ptr(z)
+            base.check(lib.tipsk_act_bwd8(dy.data_ptr(), q, None if q is None else q + _exponents_at(rows * cols), base.ptr(dz),
+                                          base.ptr(db), 0 if db is None else base.code(db), base.ptr(part), rows, cols,
+                                          base.code(dy), base.stream()), "act_bwd8")
         return (dy if dz is None else dz), db
     dz = dy.float()
-    if q is not None:
-        z = _unpack(q, e, dy.shape, torch.float32)
-        dz = dz * (0.5 * (1 + torch.erf(z * 0.7071067811865476)) + z * torch.exp(-0.5 * z * z) * 0.3989422804014327)
+    if z is not None:
+        v = _unpack(z, dy.shape, torch.float32)
+        dz = dz * (0.5 * (1 + torch.erf(v * 0.7071067811865476)) + v * torch.exp(-0.5 * v * v) * 0.3989422804014327)
         dy = dz.to(dy.dtype)
     return dy, None if bias_dtype is None else dz.sum(0).to(bias_dtype)
