@@ -21,6 +21,7 @@
 // The reference contains no attention; this serves the BERT-shaped encoder.
 #include <cuda.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <type_traits>
@@ -724,38 +725,45 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 }
 
 // ---------------------------------------------------------------- backward
-// D_i = dO_i . O_i, eight lanes per row; the heads of a position are neighbours, so contiguous tensors are read in order.
-// Writes [2][b, h, sp]: -L and -D, the addends as the main kernel uses them.
+// D_i = dO_i . O_i, eight lanes per row.  A block takes 32 positions of eight heads: it reads runs of heads, which are neighbours
+// in a contiguous tensor, and writes runs of positions.  Writes [2][b, h, sp]: -L and -D, the addends as the main kernel uses them.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ AttnParams p) {
-  const int64_t rows = static_cast<int64_t>(p.b) * p.sp * p.h;
-  const int part = threadIdx.x & 7;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * 32; r0 < rows; r0 += static_cast<int64_t>(gridDim.x) * 32) {
-    const int64_t r = r0 + (threadIdx.x >> 3);
-    const int h     = static_cast<int>(r % p.h);
-    const int i     = static_cast<int>(r / p.h % p.sp);
-    const int64_t b = r / p.h / p.sp;
-    float sum = 0.f;
-    if (r < rows && i < SeqLen(p, static_cast<int>(b))) {
-      const uint16_t* o  = static_cast<const uint16_t*>(p.o) + b * p.so.b + i * p.so.s + h * p.so.h;
-      const uint16_t* g  = static_cast<const uint16_t*>(p.dout) + b * p.sdo.b + i * p.sdo.s + h * p.sdo.h;
-      for (int c = part * 8; c < p.d; c += 64) {
-        const uint4 x = *reinterpret_cast<const uint4*>(o + c), y = *reinterpret_cast<const uint4*>(g + c);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+  __shared__ float sums[8][33];
+  const int b = blockIdx.z, h0 = blockIdx.y * 8, len = SeqLen(p, b);
+  const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;
+  const int h = (threadIdx.x >> 3) & 7, part = threadIdx.x & 7;
+  const uint16_t* out  = static_cast<const uint16_t*>(p.o) + b * p.so.b + (h0 + h) * p.so.h + part * 8;
+  const uint16_t* grad = static_cast<const uint16_t*>(p.dout) + b * p.sdo.b + (h0 + h) * p.sdo.h + part * 8;
+  for (int i0 = blockIdx.x * 32; i0 < p.sp; i0 += gridDim.x * 32) {
+#pragma unroll 4
+    for (int t = 0; t < 8; ++t) {
+      const int j = t * 4 + (threadIdx.x >> 6), i = i0 + j;
+      float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 u = Unpack2<kBf16>(xs[k]), v = Unpack2<kBf16>(ys[k]);
-          sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+      for (int k = 0; k < 2; ++k)
+        if (i < len && h0 + h < p.h && part * 8 + k * 64 < p.d) {
+          const uint4 x = *reinterpret_cast<const uint4*>(out + i * p.so.s + k * 64);
+          const uint4 y = *reinterpret_cast<const uint4*>(grad + i * p.sdo.s + k * 64);
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float2 a = Unpack2<kBf16>(xs[v]), c = Unpack2<kBf16>(ys[v]);
+            sum = fmaf(a.x, c.x, fmaf(a.y, c.y, sum));
+          }
         }
-      }
-    }
 #pragma unroll
-    for (int k = 4; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-    if (part == 0 && r < rows) {
-      const int64_t at = (b * p.h + h) * p.sp + i;
-      p.delta[at]        = -p.lse[at];
-      p.delta[rows + at] = -sum;
+      for (int k = 4; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+      if (part == 0) sums[h][j] = sum;
     }
+    __syncthreads();
+    const int hw = threadIdx.x >> 5, j = threadIdx.x & 31;
+    if (h0 + hw < p.h) {  // i0 + j < sp, a multiple of 32
+      const int64_t at = (static_cast<int64_t>(b) * p.h + h0 + hw) * p.sp + i0 + j;
+      p.delta[at]         = -p.lse[at];
+      p.delta[plane + at] = -sums[hw][j];
+    }
+    __syncthreads();
   }
 }
 
@@ -1187,8 +1195,9 @@ int CheckSizes(int b, int s, int h, int hk, int d, int dtype, float scale) {
   TIPSK_REQUIRE(b > 0 && s > 0 && h > 0 && hk > 0 && h % hk == 0, "attention: empty shape, or heads that kv_heads does not divide");
   TIPSK_REQUIRE(d > 0 && d <= 128 && d % 8 == 0, "attention: the head size must be a multiple of 8 up to 128");
   TIPSK_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), "attention: scale must be positive and finite");
-  TIPSK_REQUIRE(s <= (1 << 30) && static_cast<int64_t>(b) * (h + hk) * TilesOf(s, kTile) < (int64_t{1} << 31),
-                "attention: too many tiles for one launch");
+  TIPSK_REQUIRE(b <= 65535 && s <= (1 << 30) && h <= (1 << 18) &&
+                    static_cast<int64_t>(b) * (h + hk) * TilesOf(s, kTile) < (int64_t{1} << 31),
+                "attention: too many rows for one launch");
   return 0;
 }
 
@@ -1222,9 +1231,7 @@ int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   int rc = AllowSmem(AttnBwdKernel<HD, kBf16>, BwdCfg<HD>::kSmemBytes, &done);
   if (rc) return rc;
-  const int64_t rows = static_cast<int64_t>(p.b) * p.sp * p.h;
-  const int64_t cap  = static_cast<int64_t>(NumSMs()) * 16;
-  AttnDeltaKernel<kBf16><<<static_cast<int>(rows / 32 < cap ? rows / 32 : cap), 256, 0, s>>>(p);  // sp: whole tiles
+  AttnDeltaKernel<kBf16><<<dim3(std::min(p.sp / 32, 4096), TilesOf(p.h, 8), p.b), 256, 0, s>>>(p);
   TIPSK_LAUNCH_CHECK();
   const int grid = (p.sp / kTile) * p.b * (p.h + p.hk);
   AttnBwdKernel<HD, kBf16><<<grid, kThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);

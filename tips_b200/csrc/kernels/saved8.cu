@@ -34,74 +34,125 @@ __device__ __forceinline__ uint32_t Quantise(float x, float inv) {
   const int q = __float2int_rn(fminf(fmaxf(x * inv, -127.f), 127.f));
   return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u ? static_cast<uint32_t>(q) & 0xffu : 0x80u;
 }
+// The same of four finite values that need no clamp, |x| inv <= 127.5: adding 1.5 * 2^23 rounds to a whole number, ties to even,
+// whose two's complement stands in the sum's last byte.
+__device__ __forceinline__ uint32_t Quantise4(const float* x, float inv) {
+  constexpr float kRound = 12582912.f;
+  const uint32_t a = __float_as_uint(fmaf(x[0], inv, kRound)), b = __float_as_uint(fmaf(x[1], inv, kRound));
+  const uint32_t c = __float_as_uint(fmaf(x[2], inv, kRound)), d = __float_as_uint(fmaf(x[3], inv, kRound));
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 __device__ __forceinline__ float Dequantise(int q, float step) { return q == -128 ? __uint_as_float(0x7fc00000u) : q * step; }
+// Four stored values.  Without a NaN among them: the byte, with its sign bit flipped, becomes the last bits of 2^23 + q + 128.
+__device__ __forceinline__ void Dequantise4(uint32_t w, float step, float* x) {
+  const uint32_t u = w ^ 0x80808080u;  // 0 where q is -128
+  if (((u - 0x01010101u) & ~u & 0x80808080u) == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + j)) - 8388736.f) * step;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = Dequantise(static_cast<int8_t>(w >> (8 * j)), step);
+  }
+}
 
-// Sixteen values per thread, so two lanes share a block.
+// Eight values per thread, so four lanes share a block and a warp's loads and stores are contiguous; U groups of eight in flight.
+// A block whose values are all finite, and not so large that the step is clamped, takes a short path of about four
+// instructions a value.  Bound by HBM.
 template <typename T>
 __global__ void __launch_bounds__(256) Pack8Kernel(const T* __restrict__ x, int8_t* __restrict__ q, int8_t* __restrict__ e, int64_t n) {
-  constexpr int N = 16 / sizeof(T), kLoads = 16 / N;
-  const int64_t groups = (n + 31) / 32 * 2;  // both lanes of a block take part, whatever the tail holds
+  constexpr int N = 16 / sizeof(T), U = 4;
+  const int64_t groups = (n + 31) / 32 * 4;  // all lanes of a block take part, whatever the tail holds
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
-  const int64_t rounds = (groups + stride - 1) / stride;
-  for (int64_t k = 0; k < rounds; ++k) {  // every lane makes the same number of rounds: the shuffle needs them all
-    const int64_t g  = k * stride + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t at = g * 16;
-    float v[16];
-    if (at + 16 <= n) {
+  // every lane makes the same number of rounds: the exchange needs them all
+  for (int64_t g0 = static_cast<int64_t>(blockIdx.x) * 256; g0 < groups; g0 += U * stride) {
+    float v[U][8];
 #pragma unroll
-      for (int u = 0; u < kLoads; ++u) {
-        const Vec16<T> w = LoadVec(x + at + u * N);
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (g0 + u * stride + threadIdx.x) * 8;
+      if (at + 8 <= n) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[u * N + j] = ToFloat<T>(w.v[j]);
+        for (int k = 0; k < 8; k += N) {
+          const Vec16<T> w = LoadVec(x + at + k);
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[u][k + j] = ToFloat<T>(w.v[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = at + j < n ? ToFloat<T>(x[at + j]) : 0.f;
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = at + j < n ? ToFloat<T>(x[at + j]) : 0.f;
     }
-    uint32_t amax = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) amax = max(amax, FiniteBits(v[j]));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    const int ex    = StepExponent(amax);
-    const float inv = PowerOfTwo(-ex);
-    uint32_t w[4];
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (g0 + u * stride + threadIdx.x) * 8;
+      // as whole numbers, magnitudes compare like the values, and what is not finite is above all that is
+      uint32_t amax = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w[j] = Quantise(v[4 * j], inv) | Quantise(v[4 * j + 1], inv) << 8 | Quantise(v[4 * j + 2], inv) << 16 |
-             Quantise(v[4 * j + 3], inv) << 24;
-    if (at + 16 <= n) {
-      *reinterpret_cast<uint4*>(q + at) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+      for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[u][j]) & 0x7fffffffu);
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const bool finite = amax < 0x7f800000u;
+      if (!__all_sync(0xffffffffu, finite)) {
+        amax = 0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (at + j < n) q[at + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
+        for (int j = 0; j < 8; ++j) amax = max(amax, FiniteBits(v[u][j]));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      }
+      const int ex    = StepExponent(amax);
+      const float inv = PowerOfTwo(-ex);
+      uint32_t w[2];
+      if (finite && ex < 121) {
+        w[0] = Quantise4(&v[u][0], inv);
+        w[1] = Quantise4(&v[u][4], inv);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          w[j] = Quantise(v[u][4 * j], inv) | Quantise(v[u][4 * j + 1], inv) << 8 | Quantise(v[u][4 * j + 2], inv) << 16 |
+                 Quantise(v[u][4 * j + 3], inv) << 24;
+      }
+      if (at + 8 <= n) {
+        *reinterpret_cast<uint2*>(q + at) = make_uint2(w[0], w[1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (at + j < n) q[at + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
+      }
+      if ((threadIdx.x & 3) == 0 && at < n) e[at / kBlock8] = static_cast<int8_t>(ex);
     }
-    if ((threadIdx.x & 1) == 0 && at < n) e[at / kBlock8] = static_cast<int8_t>(ex);
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) Unpack8Kernel(const int8_t* __restrict__ q, const int8_t* __restrict__ e, T* __restrict__ y, int64_t n) {
-  constexpr int N = 16 / sizeof(T);
+  constexpr int N = 16 / sizeof(T), U = 4;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g * 16 < n; g += stride) {
-    const int64_t at = g * 16;
-    const float step = PowerOfTwo(e[at / kBlock8]);
-    if (at + 16 <= n) {
-      const uint4 w = *reinterpret_cast<const uint4*>(q + at);
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+  for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g * 8 < n; g += U * stride) {
+    uint2 w[U];
+    int ex[U];
 #pragma unroll
-      for (int u = 0; u < 16 / N; ++u) {
-        Vec16<T> o;
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (g + u * stride) * 8;
+      if (at < n) ex[u] = e[at / kBlock8];
+      if (at + 8 <= n) w[u] = *reinterpret_cast<const uint2*>(q + at);
+    }
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const int i = u * N + j;
-          o.v[j] = FromFloat<T>(Dequantise(static_cast<int8_t>(ws[i / 4] >> (8 * (i % 4))), step));
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = (g + u * stride) * 8;
+      if (at + 8 <= n) {
+        const float step = PowerOfTwo(ex[u]);
+        float v[8];
+        Dequantise4(w[u].x, step, v);
+        Dequantise4(w[u].y, step, v + 4);
+#pragma unroll
+        for (int k = 0; k < 8; k += N) {
+          Vec16<T> o;
+#pragma unroll
+          for (int j = 0; j < N; ++j) o.v[j] = FromFloat<T>(v[k + j]);
+          StoreVec(y + at + k, o);
         }
-        StoreVec(y + at + u * N, o);
+      } else {
+        for (int j = 0; at + j < n; ++j) y[at + j] = FromFloat<T>(Dequantise(q[at + j], PowerOfTwo(ex[u])));
       }
-    } else {
-      for (int j = 0; at + j < n; ++j) y[at + j] = FromFloat<T>(Dequantise(q[at + j], step));
     }
   }
 }
@@ -111,41 +162,56 @@ __global__ void __launch_bounds__(256) Unpack8Kernel(const int8_t* __restrict__ 
 // multiples of 8 values), every block a share of the rows; the shares' sums go to partial [gridDim.y][cols] and are added in
 // their order by ColumnSumKernel, so a result does not depend on the order of the blocks.
 template <typename T, bool kGelu>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 ActBwd8Kernel(const T* __restrict__ dy, const int8_t* __restrict__ q, const int8_t* __restrict__ e, T* __restrict__ dz,
-               float* __restrict__ partial, int64_t rows, int cols) {
-  constexpr int N = 8;
+              float* __restrict__ partial, int64_t rows, int cols) {
+  constexpr int N = 8, U = sizeof(T) == 4 ? 1 : 2;  // rows in flight
   __shared__ float red[8][32][N + 1];
   const int vc = blockIdx.x * 32 + threadIdx.x;
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
   if (vc < cols / N) {
-    for (int64_t r = static_cast<int64_t>(blockIdx.y) * 8 + threadIdx.y; r < rows; r += static_cast<int64_t>(gridDim.y) * 8) {
-      const int64_t off = r * cols + static_cast<int64_t>(vc) * N;
-      alignas(16) T g[N], o[N];
+    const int64_t step = static_cast<int64_t>(gridDim.y) * 8;
+    for (int64_t r = static_cast<int64_t>(blockIdx.y) * 8 + threadIdx.y; r < rows; r += U * step) {
+      alignas(16) T g[U][N];
+      uint2 w[U];
+      float s[U];
 #pragma unroll
-      for (int k = 0; k < N; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(&g[k]) = *reinterpret_cast<const uint4*>(dy + off + k);
-      if (!kGelu) {
+      for (int u = 0; u < U; ++u)
+        if (r + u * step < rows) {
+          const int64_t off = (r + u * step) * cols + static_cast<int64_t>(vc) * N;
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += ToFloat<T>(g[k]);
-        continue;
+          for (int k = 0; k < N; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(&g[u][k]) = *reinterpret_cast<const uint4*>(dy + off + k);
+          if (kGelu) {
+            w[u] = *reinterpret_cast<const uint2*>(q + off);
+            s[u] = PowerOfTwo(e[off / kBlock8]);
+          }
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (r + u * step >= rows) continue;
+        if (!kGelu) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] += ToFloat<T>(g[u][k]);
+          continue;
+        }
+        float z[N];
+        Dequantise4(w[u].x, s[u], z);
+        Dequantise4(w[u].y, s[u], z + 4);
+        alignas(16) T o[N];
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+          const float2 v = SplitF2(Mul2(MakeF2(ToFloat<T>(g[u][k]), ToFloat<T>(g[u][k + 1])), GeluGrad2(MakeF2(z[k], z[k + 1]))));
+          acc[k] += v.x;
+          acc[k + 1] += v.y;
+          o[k]     = FromFloat<T>(v.x);
+          o[k + 1] = FromFloat<T>(v.y);
+        }
+        const int64_t off = (r + u * step) * cols + static_cast<int64_t>(vc) * N;
+#pragma unroll
+        for (int k = 0; k < N; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(dz + off + k) = *reinterpret_cast<uint4*>(&o[k]);
       }
-      const float step = PowerOfTwo(e[off / kBlock8]);
-      const uint2 w    = *reinterpret_cast<const uint2*>(q + off);
-#pragma unroll
-      for (int k = 0; k < N; k += 2) {
-        const uint32_t word = k < 4 ? w.x : w.y;
-        const F2 z = MakeF2(Dequantise(static_cast<int8_t>(word >> (8 * (k & 3))), step),
-                            Dequantise(static_cast<int8_t>(word >> (8 * (k & 3) + 8)), step));
-        const float2 v = SplitF2(Mul2(MakeF2(ToFloat<T>(g[k]), ToFloat<T>(g[k + 1])), GeluGrad2(z)));
-        acc[k] += v.x;
-        acc[k + 1] += v.y;
-        o[k]     = FromFloat<T>(v.x);
-        o[k + 1] = FromFloat<T>(v.y);
-      }
-#pragma unroll
-      for (int k = 0; k < N; k += 16 / sizeof(T)) *reinterpret_cast<uint4*>(dz + off + k) = *reinterpret_cast<uint4*>(&o[k]);
     }
   }
   if (!partial) return;
@@ -195,7 +261,7 @@ int tipsk_pack8(const void* x, void* q, void* e, int64_t n, int dtype, void* str
   TIPSK_REQUIRE(n > 0 && (dtype == kF32 || dtype == kBF16 || dtype == kF16), "pack8: fp32, bf16 or fp16 and at least one value");
   TIPSK_REQUIRE(Aligned16(x) && Aligned16(q), "pack8: the values must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int grid = Blocks((n + 31) / 32 * 2, 8);
+  const int grid = Blocks((n + 31) / 32 * 4, 8);
   int8_t *qq = static_cast<int8_t*>(q), *ee = static_cast<int8_t*>(e);
   if (dtype == kF32) Pack8Kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(x), qq, ee, n);
   else if (dtype == kBF16) Pack8Kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), qq, ee, n);
@@ -209,7 +275,7 @@ int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, v
   TIPSK_REQUIRE(n > 0 && (dtype == kF32 || dtype == kBF16 || dtype == kF16), "unpack8: fp32, bf16 or fp16 and at least one value");
   TIPSK_REQUIRE(Aligned16(y) && Aligned16(q), "unpack8: the values must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int grid = Blocks((n + 15) / 16, 8);
+  const int grid = Blocks((n + 7) / 8, 8);
   const int8_t *qq = static_cast<const int8_t*>(q), *ee = static_cast<const int8_t*>(e);
   if (dtype == kF32) Unpack8Kernel<float><<<grid, 256, 0, s>>>(qq, ee, static_cast<float*>(y), n);
   else if (dtype == kBF16) Unpack8Kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(qq, ee, static_cast<__nv_bfloat16*>(y), n);
@@ -220,7 +286,7 @@ int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, v
 
 /* Shares of the rows of tipsk_act_bwd8, for its workspace. */
 int tipsk_act_bwd8_parts(int64_t rows, int cols) {
-  const int64_t tiles = (cols + 255) / 256, fill = (static_cast<int64_t>(NumSMs()) * 8 + tiles - 1) / tiles;
+  const int64_t tiles = (cols + 255) / 256, fill = (static_cast<int64_t>(NumSMs()) * 4 + tiles - 1) / tiles;
   const int64_t most  = (rows + 7) / 8;
   return static_cast<int>(fill < most ? fill : most);
 }

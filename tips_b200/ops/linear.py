@@ -180,7 +180,7 @@ def _linear8_backward(ctx, dy, d_alias):
     if ctx.needs_input_grad[0]:
         dx = _input_grad(dz, weight, d_alias).view(ctx.in_shape)
     if ctx.needs_input_grad[1]:
-        dw = _weight_grad(dz, saved8._unpack(x8, (dz.shape[0], k), ctx.x_dtype), weight.dtype).to(weight.dtype)
+        dw = _weight_grad8(dz, saved8._unpack(x8, (dz.shape[0], k), ctx.x_dtype), weight.dtype).to(weight.dtype)
     return dx, dw, db, None
 
 
@@ -196,6 +196,23 @@ class _Linear8PassFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, d_alias):
         return _linear8_backward(ctx, dy, d_alias)
+
+
+def _weight_grad8(dz: torch.Tensor, x2: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """dz^T @ x2 for operands of any row count: `_weight_grad` where it reads both in place, and otherwise the CTA-pair GEMM,
+    whose tensor maps end where the rows do, or for narrow operands transposed copies with zeros up to whole 16 bytes."""
+    m, n = dz.shape
+    k = x2.shape[1]
+    if not (dz.is_cuda and dz.dtype == x2.dtype == torch.bfloat16 and m) or (n % 64 == 0 and k % 64 == 0 and m >= 16):
+        return _weight_grad(dz, x2, dtype)
+    if n >= 64 and k >= 64 and _supported(dz, x2) and n % 8 == 0 and k % 8 == 0:
+        dw = torch.empty(n, k, dtype=torch.bfloat16, device=dz.device)
+        if not _split(2, dz, x2, dw, None, None, n, k, m, 0, False):
+            base.check(base.K().tipsk_gemm_bf16_tt(dz.data_ptr(), x2.data_ptr(), dw.data_ptr(), n, k, m, n, k, k,
+                                                   base.stream()), "gemm_bf16_tt")
+        return dw
+    pad = -m % 8
+    return gemm_tn(F.pad(dz.t(), (0, pad)).contiguous(), F.pad(x2.t(), (0, pad)).contiguous())
 
 
 def _input_grad(dz: torch.Tensor, weight: torch.Tensor, d_alias: torch.Tensor | None) -> torch.Tensor:
