@@ -336,51 +336,77 @@ __device__ __forceinline__ void StoreShared(uint32_t at, float x) { asm volatile
 // ---------------------------------------------------------------- blocks that take one piece of work after another
 // The grid has a block per piece of work, but a block that is done takes the place of one that has not started yet (cluster
 // launch control): its barriers, its TMEM and its pipelines stay up, loads and scores of the next piece run under the
-// last stores of this one, and pieces of different length still spread evenly.  Every warp runs through the same pieces.  The
-// TMA warp asks for the next one while it works on the present one; the answer lies in one of two slots.
-struct Next {
-  uint32_t at;  // two answers of 16 bytes, two barriers that they are there, two that all warps have read them
-  static constexpr int kBytes = 64;
-  __device__ __forceinline__ uint32_t Slot(uint32_t turn) const { return at + (turn & 1) * 16; }
-  __device__ __forceinline__ uint32_t Full(uint32_t turn) const { return at + 32 + (turn & 1) * 8; }
-  __device__ __forceinline__ uint32_t Empty(uint32_t turn) const { return at + 48 + (turn & 1) * 8; }
+// last stores of this one, and pieces of different length still spread evenly.  The thread that issues TMA loads asks for the
+// next piece while it works on the present one, works out what the piece consists of, and leaves that in one of two slots
+// in shared memory for the other warps, which run through the same pieces.
+struct Pieces {
+  uint32_t at;  // two slots of eight words, an answer of 16 bytes, barriers: slots written [2], slots read [2], answer
+  static constexpr int kBytes = 64 + 16 + 48;
+  __device__ __forceinline__ uint32_t Slot(uint32_t turn) const { return at + (turn & 1) * 32; }
+  __device__ __forceinline__ uint32_t Answer() const { return at + 64; }
+  __device__ __forceinline__ uint32_t Full(uint32_t turn) const { return at + 80 + (turn & 1) * 8; }
+  __device__ __forceinline__ uint32_t Empty(uint32_t turn) const { return at + 96 + (turn & 1) * 8; }
+  __device__ __forceinline__ uint32_t Answered() const { return at + 112; }
   __device__ __forceinline__ void Init() const {
     for (int i = 0; i < 2; ++i) {
       BarInit(Full(i), 1);
-      BarInit(Empty(i), kWarps);
+      BarInit(Empty(i), kWarps - 1);
+    }
+    BarInit(Answered(), 1);
+  }
+  // By the thread that leads: `describe` turns a block index into eight words, the last not negative, and `load` starts the loads of
+  // a piece; both come from the piece's type.  False on a timeout.
+  template <typename Describe, typename Load>
+  __device__ __forceinline__ bool Lead(Describe&& describe, Load&& load) const {
+    int index = blockIdx.x;
+    for (uint32_t turn = 0;; ++turn) {
+      int w[8];
+      if (index >= 0) describe(index, w);
+      else w[7] = -1;
+      if (!BarWaitOne(Empty(turn), (turn >> 1) ^ 1)) return false;
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(Slot(turn)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(Slot(turn) + 16), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+      BarArrive(Full(turn));
+      if (index < 0) return true;
+      BarExpect(Answered(), 16);
+      asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(Answer()),
+                   "r"(Answered())
+                   : "memory");
+      bool ok = load(w);
+      ok      = BarWaitOne(Answered(), turn) && ok;
+      uint32_t got, x;
+      asm volatile(
+          "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+          "ld.shared.b128 r, [%2];\n\t"
+          "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t"
+          "mov.u32 %1, 0;\n\t"
+          "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+          : "=r"(got), "=r"(x)
+          : "r"(Answer())
+          : "memory");
+      if (!ok) return false;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next answer is written to the same place
+      index = got ? static_cast<int>(x) : -1;
     }
   }
-  // One thread, at the start of piece number `turn`.
-  __device__ __forceinline__ bool Ask(uint32_t turn) const {
-    if (!BarWaitOne(Empty(turn), (turn >> 1) ^ 1)) return false;
-    BarExpect(Full(turn), 16);
-    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(Slot(turn)),
-                 "r"(Full(turn))
-                 : "memory");
-    return true;
-  }
-  // A whole warp, at the end of piece number `turn`: the next piece's block index, or -1.
+  // By every other warp, from turn 0 on: the piece's words, the same in all lanes; false when there are no more.
   template <bool kIdle>
-  __device__ __forceinline__ int Take(uint32_t turn) const {
+  __device__ __forceinline__ bool Take(uint32_t turn, int (&w)[8]) const {
     if (!BarWait<kIdle>(Full(turn), turn >> 1)) {
       if ((threadIdx.x & 31) == 0) atomicExch(&g_attn_error, 8);
-      return -1;
+      return false;
     }
-    uint32_t got, x;
-    asm volatile(
-        "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
-        "ld.shared.b128 r, [%2];\n\t"
-        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t"
-        "mov.u32 %1, 0;\n\t"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
-        : "=r"(got), "=r"(x)
-        : "r"(Slot(turn))
-        : "memory");
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(Slot(turn)) : "memory");
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "r"(Slot(turn) + 16)
+                 : "memory");
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = Uniform(w[k]);
     if ((threadIdx.x & 31) == 0) BarArrive(Empty(turn));
-    return static_cast<int>(Uniform(got ? x : ~0u));
+    return w[7] >= 0;
   }
 };
 
@@ -425,7 +451,7 @@ struct FwdCfg {
   static constexpr int kRing      = 2 * kQBufs * kTileBytes;
   static constexpr int kMax       = kRing + kStages * kTileBytes;
   static constexpr int kNext      = kMax + 2 * 2 * 2 * kTile * 4;
-  static constexpr int kFull      = kNext + Next::kBytes;
+  static constexpr int kFull      = kNext + Pieces::kBytes;
   static constexpr int kEmpty     = kFull + 8 * kStages;   // both MMA warps are done with a tile of K or V
   static constexpr int kRaw       = kEmpty + 8 * kStages;  // a tile of V has arrived and has rows to clear before it counts as full
   static constexpr int kQFull     = kRaw + 8 * kStages;
@@ -439,25 +465,28 @@ struct FwdCfg {
 };
 
 struct FwdPiece {
-  int b, h, q0, len, tiles, count[2], total;
+  int b, h, q0, len, count0, count1, total;
   bool ragged;  // the last tile of V has rows to clear
-  __device__ __forceinline__ FwdPiece(const AttnParams& p, int index) {
+  __device__ __forceinline__ explicit FwdPiece(const int (&w)[8])
+      : b(w[0]), h(w[1]), q0(w[2]), len(w[3]), count0(w[4]), count1(w[5]), total(w[6]), ragged(w[7] != 0) {}
+  __device__ __forceinline__ static void Describe(const AttnParams& p, int index, int (&w)[8]) {
     // causal: the tiles with the most keys first; otherwise neighbours share a head's keys
     const int blocks_q = TilesOf(p.s, 2 * kTile), heads = p.b * p.h;
     const int qb = p.causal ? blocks_q - 1 - index / heads : index % blocks_q;
     const int bh = p.causal ? index % heads : index / blocks_q;
-    b     = bh / p.h;
-    h     = bh % p.h;
-    q0    = qb * 2 * kTile;
-    len   = Uniform(SeqLen(p, b));
-    tiles = TilesOf(len, kTile);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {  // key tiles of either query tile
-      const int first = q0 + i * kTile;
-      count[i] = first >= len ? 0 : p.causal ? min(tiles, first / kTile + 1) : tiles;
-    }
-    total  = max(count[0], count[1]);
-    ragged = total > 0 && total == tiles && len < p.s && len % kTile != 0;
+    const int b = bh / p.h, q0 = qb * 2 * kTile, len = SeqLen(p, b), tiles = TilesOf(len, kTile);
+    // key tiles of either query tile
+    const int count0 = q0 >= len ? 0 : p.causal ? min(tiles, q0 / kTile + 1) : tiles;
+    const int count1 = q0 + kTile >= len ? 0 : p.causal ? min(tiles, q0 / kTile + 2) : tiles;
+    const int total = max(count0, count1);
+    w[0] = b;
+    w[1] = bh % p.h;
+    w[2] = q0;
+    w[3] = len;
+    w[4] = count0;
+    w[5] = count1;
+    w[6] = total;
+    w[7] = total > 0 && total == tiles && len < p.s && len % kTile != 0;
   }
 };
 
@@ -468,7 +497,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   constexpr int S = Cfg::kStages, QB = Cfg::kQBufs;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = AlignedSmem(smem_raw);
-  const Next next{base + Cfg::kNext};
+  const Pieces pieces{base + Cfg::kNext};
   auto full = [&](uint32_t k) { return base + Cfg::kFull + k % S * 8; };
   auto empty = [&](uint32_t k) { return base + Cfg::kEmpty + k % S * 8; };
   auto raw = [&](uint32_t k) { return base + Cfg::kRaw + k % S * 8; };
@@ -479,7 +508,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 
   const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    next.Init();
+    pieces.Init();
     for (int i = 0; i < S; ++i) {
       BarInit(full(i), 1);
       BarInit(empty(i), 2);
@@ -505,43 +534,34 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   // columns: scores of either tile, either output, and in what is left either tile's probabilities, or those in the scores' place
   const uint32_t t_s = tmem, t_o = tmem + 256;
 
+  int words[8];
   if (warp == kTmaWarp) {
-    uint32_t e = 0, n = 0;  // tiles of K and V, and pieces with any, so far
-    bool ok = true;
-    int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = next.Take<true>(turn), ++turn) {
-      const FwdPiece w(p, index);
-      if (ElectOne()) {
-        ok = ok && next.Ask(turn);
-        if (w.total > 0 && ok) {
-          const int hk = w.h / (p.h / p.hk);
-          ok = BarWaitOne(q_empty(n), (n / QB) ^ 1);
-          if (ok) {
-            BarExpect(q_full(n), 2 * Cfg::kTileBytes);
-            TmaLoadTile<HD, kTile, kTile>(q_tile(n, 0), &maps.q, w.q0, w.h, w.b, q_full(n));
-            TmaLoadTile<HD, kTile, kTile>(q_tile(n, 1), &maps.q, w.q0 + kTile, w.h, w.b, q_full(n));
-          }
-          for (int k = 0; k < 2 * w.total && ok; ++k) {
-            const uint32_t at = e + k;
-            ok = BarWaitOne(empty(at), (at / S) ^ 1);
-            if (!ok) break;
-            const uint32_t bar = w.ragged && k == 2 * w.total - 1 ? raw(at) : full(at);
-            BarExpect(bar, Cfg::kTileBytes);
-            TmaLoadTile<HD, kTile, kTile>(tile(at), k & 1 ? &maps.v : &maps.k, (k >> 1) * kTile, hk, w.b, bar);
-          }
+    if (ElectOne()) {
+      uint32_t e = 0, n = 0;  // tiles of K and V, and pieces with any, so far
+      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { FwdPiece::Describe(p, index, v); }, [&](const int (&v)[8]) {
+        const FwdPiece w(v);
+        if (w.total == 0) return true;
+        if (!BarWaitOne(q_empty(n), (n / QB) ^ 1)) return false;
+        BarExpect(q_full(n), 2 * Cfg::kTileBytes);
+        TmaLoadTile<HD, kTile, kTile>(q_tile(n, 0), &maps.q, w.q0, w.h, w.b, q_full(n));
+        TmaLoadTile<HD, kTile, kTile>(q_tile(n, 1), &maps.q, w.q0 + kTile, w.h, w.b, q_full(n));
+        ++n;
+        const int hk = w.h / (p.h / p.hk);
+        for (int k = 0; k < 2 * w.total; ++k, ++e) {
+          if (!BarWaitOne(empty(e), (e / S) ^ 1)) return false;
+          const uint32_t bar = w.ragged && k == 2 * w.total - 1 ? raw(e) : full(e);
+          BarExpect(bar, Cfg::kTileBytes);
+          TmaLoadTile<HD, kTile, kTile>(tile(e), k & 1 ? &maps.v : &maps.k, (k >> 1) * kTile, hk, w.b, bar);
         }
-        if (!ok) atomicExch(&g_attn_error, 1);
-      }
-      __syncwarp();
-      e += 2 * w.total;
-      n += w.total > 0;
+        return true;
+      });
+      if (!ok) atomicExch(&g_attn_error, 1);
     }
   } else if (warp == kClearWarp) {
     uint32_t e = 0, uses = 0;  // bit st: parity of the next use of raw[st]
     IdleWaiter wait(2);
-    int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = next.Take<true>(turn), ++turn) {
-      const FwdPiece w(p, index);
+    for (uint32_t turn = 0; pieces.Take<true>(turn, words); ++turn) {
+      const FwdPiece w(words);
       e += 2 * w.total;
       if (w.ragged) {
         const uint32_t st = (e - 1) % S;
@@ -561,10 +581,9 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     const uint32_t s_full = base + Cfg::kSFull + i * 8, s_free = base + Cfg::kSFree + i * 8, p_full = base + Cfg::kPFull + i * 8,
                    o_full = base + Cfg::kOFull + i * 8;
     auto entry = [&](uint32_t k) { return wait(full(k), k / S); };
-    int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = next.Take<false>(turn), ++turn) {
-      const FwdPiece w(p, index);
-      const int mine = i ? w.count[1] : w.count[0];
+    for (uint32_t turn = 0; pieces.Take<false>(turn, words); ++turn) {
+      const FwdPiece w(words);
+      const int mine = i ? w.count1 : w.count0;
       if (w.total > 0 && wait.ok) {
         const uint32_t q_addr = q_tile(n, i);
         auto scores = [&](int j) {  // of key tile j, if it is one of this query tile's; hands on its keys
@@ -620,10 +639,9 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
       NamedBarSync(pair_bar, 64);
       return LoadShared(at + (half ^ 1) * (kTile * 4));
     };
-    int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = next.Take<false>(turn), ++turn) {
-      const FwdPiece w(p, index);
-      const int row = w.q0 + i * kTile + r, count = i ? w.count[1] : w.count[0];
+    for (uint32_t turn = 0; pieces.Take<false>(turn, words); ++turn) {
+      const FwdPiece w(words);
+      const int row = w.q0 + i * kTile + r, count = i ? w.count1 : w.count0;
       float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and this half's sum
       for (int j = 0; j < count; ++j, ++done) {
         wait(s_full, done);  // on a failure the values are void, but every thread keeps meeting its barriers
@@ -792,8 +810,9 @@ struct BwdCfg {
   // shared memory: [kXBufs][X1, X2], the ring [kStages][Y1, Y2], [kStages][-L, -D], barriers
   static constexpr int kRing       = kXBufs * 2 * kTileBytes;
   static constexpr int kRows       = kRing + kStages * kStageBytes;
-  static constexpr int kNext       = kRows + kStages * kRowBytes;
-  static constexpr int kFull       = kNext + Next::kBytes;
+  static constexpr int kXRows      = kRows + kStages * kRowBytes;  // [kXBufs] -L and -D of the tile of queries that stays
+  static constexpr int kNext       = kXRows + kXBufs * 2 * kTile * 4;
+  static constexpr int kFull       = kNext + Pieces::kBytes;
   static constexpr int kEmpty      = kFull + 8 * kStages;
   static constexpr int kRaw        = kEmpty + 8 * kStages;       // a unit has arrived and has rows to clear before it counts as full
   static constexpr int kXFull      = kRaw + 8 * kStages;
@@ -809,28 +828,38 @@ struct BwdCfg {
   static constexpr int kSmemBytes  = kTmemSlot + 16 + 1024;
 };
 
-template <bool kKeys>
-struct BwdPiece {
-  int b, head, x0, len, first, per, total, yhead;
-  bool ragged;  // a head's last unit has rows to clear
-  __device__ __forceinline__ BwdPiece(const AttnParams& p, int index) {
-    const int tiles = p.sp / kTile, kh = kKeys ? p.hk : p.h, heads = p.b * kh;
-    // causal: the tiles with the longest streams first; otherwise neighbours share a head
-    const int tile = !p.causal ? index % tiles : kKeys ? index / heads : tiles - 1 - index / heads;
-    const int bh   = p.causal ? index % heads : index / tiles;
-    b    = bh / kh;
-    head = bh % kh;
-    x0   = tile * kTile;
-    len  = Uniform(SeqLen(p, b));
-    const int units = TilesOf(len, kUnit), group = p.h / p.hk;
+struct BwdWords {  // what stands in a slot
+  int b, head, x0, len, first, per, total;
+  bool ragged, keys;  // a head's last unit has rows to clear; keys stay
+  __device__ __forceinline__ explicit BwdWords(const int (&w)[8])
+      : b(w[0]), head(w[1]), x0(w[2]), len(w[3]), first(w[4]), per(w[5]), total(w[6]), ragged(w[7] & 1), keys(w[7] & 2) {}
+  // First the pieces of the keys, whose tiles stream past every query head of their group; causal: the tiles with the longest
+  // streams first; otherwise neighbours share a head.
+  __device__ __forceinline__ static void Describe(const AttnParams& p, int index, int (&w)[8]) {
+    const int tiles = p.sp / kTile, group = p.h / p.hk, key_pieces = tiles * p.b * p.hk;
+    const bool keys = index < key_pieces;
+    if (!keys) index -= key_pieces;
+    const int kh = keys ? p.hk : p.h, heads = p.b * kh;
+    const int tile = !p.causal ? index % tiles : keys ? index / heads : tiles - 1 - index / heads;
+    const int bh = p.causal ? index % heads : index / tiles, b = bh / kh, x0 = tile * kTile;
+    const int len = SeqLen(p, b), units = TilesOf(len, kUnit);
     // streamed units: [first, last) of the one head, or of each head of the group
-    first = kKeys && p.causal ? x0 / kUnit : 0;
-    const int last = !kKeys && p.causal ? min(units, (x0 + kTile) / kUnit) : units;
-    per    = last - first;
-    total  = x0 >= len ? 0 : per * (kKeys ? group : 1);
-    yhead  = kKeys ? head * group : head / group;
-    ragged = total > 0 && last == units && len < p.s && len % kUnit != 0;
+    const int first = keys && p.causal ? x0 / kUnit : 0;
+    const int last  = !keys && p.causal ? min(units, (x0 + kTile) / kUnit) : units;
+    const int total = x0 >= len ? 0 : (last - first) * (keys ? group : 1);
+    w[0] = b;
+    w[1] = bh % kh;
+    w[2] = x0;
+    w[3] = len;
+    w[4] = first;
+    w[5] = last - first;
+    w[6] = total;
+    w[7] = (total > 0 && last == units && len < p.s && len % kUnit != 0 ? 1 : 0) | (keys ? 2 : 0);
   }
+};
+template <bool kKeys>
+struct BwdPiece : BwdWords {
+  using BwdWords::BwdWords;
 };
 
 template <int HD>
@@ -840,6 +869,7 @@ struct BwdSmem {
   __device__ __forceinline__ uint32_t X(uint32_t n) const { return base + n % C::kXBufs * (2 * C::kTileBytes); }
   __device__ __forceinline__ uint32_t Y(uint32_t u) const { return base + C::kRing + u % C::kStages * C::kStageBytes; }
   __device__ __forceinline__ uint32_t Rows(uint32_t u) const { return base + C::kRows + u % C::kStages * C::kRowBytes; }
+  __device__ __forceinline__ uint32_t XRows(uint32_t n) const { return base + C::kXRows + n % C::kXBufs * (2 * kTile * 4); }
   __device__ __forceinline__ uint32_t Full(uint32_t u) const { return base + C::kFull + u % C::kStages * 8; }
   __device__ __forceinline__ uint32_t Empty(uint32_t u) const { return base + C::kEmpty + u % C::kStages * 8; }
   __device__ __forceinline__ uint32_t Raw(uint32_t u) const { return base + C::kRaw + u % C::kStages * 8; }
@@ -864,11 +894,17 @@ __device__ __forceinline__ bool BwdLoad(const AttnMaps& maps, const AttnParams& 
   using Cfg = BwdCfg<HD>;
   constexpr int XB = Cfg::kXBufs, ST = Cfg::kStages;
   if (!BarWaitOne(m.XEmpty(n), (n / XB) ^ 1)) return false;
-  BarExpect(m.XFull(n), 2 * Cfg::kTileBytes);
+  BarExpect(m.XFull(n), 2 * Cfg::kTileBytes + (kKeys ? 0 : 2 * kTile * 4));
   TmaLoadTile<HD, kTile, kUnit>(m.X(n), kKeys ? &maps.k : &maps.q, w.x0, w.head, w.b, m.XFull(n));
   TmaLoadTile<HD, kTile, kUnit>(m.X(n) + Cfg::kTileBytes, kKeys ? &maps.v : &maps.dout, w.x0, w.head, w.b, m.XFull(n));
   const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;  // of -L, -D
-  int at = 0, yh = w.yhead;  // unit within a head
+  if (!kKeys) {
+    const float* src = p.delta + (static_cast<int64_t>(w.b) * p.h + w.head) * p.sp + w.x0;
+    BulkLoad(m.XRows(n), src, kTile * 4, m.XFull(n));
+    BulkLoad(m.XRows(n) + kTile * 4, src + plane, kTile * 4, m.XFull(n));
+  }
+  const int group = p.h / p.hk;
+  int at = 0, yh = kKeys ? w.head * group : w.head / group;  // unit within a head
   for (int k = 0; k < w.total; ++k) {
     const uint32_t u = u0 + k;
     if (!BarWaitOne(m.Empty(u), (u / ST) ^ 1)) return false;
@@ -910,6 +946,8 @@ __device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m
   constexpr int ST = Cfg::kStages, SB = 2 * Cfg::kSBufs, XB = Cfg::kXBufs;
   const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
   const uint32_t x1 = m.X(n), x2 = x1 + Cfg::kTileBytes;
+  u0 = Uniform(u0);
+  n  = Uniform(n);
   const uint32_t end = u0 + w.total;
   auto arrived = [&](uint32_t u) { return wait(m.Full(u), u / ST); };
   wait(m.XFull(n), n / XB);
@@ -964,10 +1002,14 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
   const int row = w.x0 + quarter * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
   F2 row_l{}, row_d{};  // -L, -D
-  if (!kKeys && w.total > 0) {  // row < sp
-    const float* src = p.delta + (static_cast<int64_t>(w.b) * p.h + w.head) * p.sp + row;
-    row_l = Both(*src);
-    row_d = Both(src[static_cast<int64_t>(p.b) * p.h * p.sp]);
+  if (w.total > 0) {
+    if (!kKeys) {
+      wait(m.XFull(n), n / Cfg::kXBufs);
+      row_l = Both(LoadShared(m.XRows(n) + (quarter * 32 + lane) * 4));
+      row_d = Both(LoadShared(m.XRows(n) + (kTile + quarter * 32 + lane) * 4));
+    }
+    __syncwarp();
+    if (lane == 0) BarArrive(m.XEmpty(n));
   }
   const F2 c2 = Both(p.c);
   int at = static_cast<int>((set ^ u0) & 1);  // unit within a head
@@ -1060,18 +1102,17 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
   }
 }
 
-// Both passes in one launch, so that neither leaves a tail of idle SMs: first the pieces of the keys, whose tiles stream past
-// every query head of their group.
+// Both passes in one launch, so that neither leaves a tail of idle SMs.
 template <int HD, bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
 AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   using Cfg = BwdCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<HD> m{AlignedSmem(smem_raw), 0};
-  const Next next{m.base + Cfg::kNext};
+  const Pieces pieces{m.base + Cfg::kNext};
   const int warp = Uniform(threadIdx.x >> 5);
   if (threadIdx.x == 0) {
-    next.Init();
+    pieces.Init();
     for (int i = 0; i < Cfg::kStages; ++i) {
       BarInit(m.Full(i), 1);
       BarInit(m.Empty(i), 2);  // both MMA warps
@@ -1079,7 +1120,7 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     }
     for (int i = 0; i < Cfg::kXBufs; ++i) {
       BarInit(m.XFull(i), 1);
-      BarInit(m.XEmpty(i), 2);
+      BarInit(m.XEmpty(i), 2 + kSoftWarps);
     }
     for (int i = 0; i < 2 * Cfg::kSBufs; ++i) {
       BarInit(m.SFull(i), 1);
@@ -1100,48 +1141,53 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   TcFenceAfter();
   m.tmem = Uniform(__float_as_uint(LoadShared(m.base + Cfg::kTmemSlot)));
 
-  // what a kind of warp does for each piece, until there is none: `step` gets the piece, the units and the pieces with any before it
-  const int key_pieces = p.sp / kTile * p.b * p.hk;
-  auto pieces = [&](auto idle, auto&& step) {
-    uint32_t u0 = 0, n = 0;
-    int index = blockIdx.x;
-    for (uint32_t turn = 0; index >= 0; index = next.Take<decltype(idle)::value>(turn), ++turn) {
-      auto work = [&](const auto& w) {
-        step(w, turn, u0, n);
-        u0 += w.total;
-        n += w.total > 0;
-      };
-      if (index < key_pieces) work(BwdPiece<true>(p, index));
-      else work(BwdPiece<false>(p, index - key_pieces));
-    }
+  uint32_t u0 = 0, n = 0;  // units, and pieces with any, so far
+  // what a warp does for a piece
+  auto each = [&](const int (&v)[8], auto&& step) {
+    const BwdWords w(v);
+    bool ok = true;
+    if (w.keys) ok = step(BwdPiece<true>(v));
+    else ok = step(BwdPiece<false>(v));
+    u0 += w.total;
+    n += w.total > 0;
+    return ok;
+  };
+  auto follow = [&](auto idle, auto&& step) {
+    int v[8];
+    for (uint32_t turn = 0; pieces.Take<decltype(idle)::value>(turn, v); ++turn) each(v, step);
   };
   if (warp == kTmaWarp) {
-    bool ok = true;
-    pieces(std::true_type{}, [&](const auto& w, uint32_t turn, uint32_t u0, uint32_t n) {
-      if (ElectOne()) {
-        ok = ok && next.Ask(turn);
-        if (w.total > 0) ok = ok && BwdLoad(maps, p, m, w, u0, n);
-        if (!ok) atomicExch(&g_attn_error, 5);
-      }
-      __syncwarp();
-    });
+    if (ElectOne()) {
+      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { BwdWords::Describe(p, index, v); }, [&](const int (&v)[8]) {
+        return each(v, [&](const auto& w) { return w.total == 0 || BwdLoad(maps, p, m, w, u0, n); });
+      });
+      if (!ok) atomicExch(&g_attn_error, 5);
+    }
   } else if (warp == kClearWarp) {
     uint32_t uses = 0;
     IdleWaiter wait(6);
-    pieces(std::true_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t) { BwdClear(m, w, u0, uses, wait); });
+    follow(std::true_type{}, [&](const auto& w) {
+      BwdClear(m, w, u0, uses, wait);
+      return true;
+    });
   } else if (warp == kMmaWarp) {
     Waiter wait(6);
-    pieces(std::false_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t n) {
+    follow(std::false_type{}, [&](const auto& w) {
       if (w.total > 0 && wait.ok) BwdMma<kBf16, 0>(p, m, w, u0, n, wait);
+      return true;
     });
   } else if (warp == kMmaWarp + 1) {
     Waiter wait(6);
-    pieces(std::false_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t n) {
+    follow(std::false_type{}, [&](const auto& w) {
       if (w.total > 0 && wait.ok) BwdMma<kBf16, 1>(p, m, w, u0, n, wait);
+      return true;
     });
   } else {
     Waiter wait(7);
-    pieces(std::false_type{}, [&](const auto& w, uint32_t, uint32_t u0, uint32_t n) { BwdSoftmax<kBf16>(p, m, w, u0, n, wait); });
+    follow(std::false_type{}, [&](const auto& w) {
+      BwdSoftmax<kBf16>(p, m, w, u0, n, wait);
+      return true;
+    });
   }
   TcFenceBefore();
   __syncthreads();
