@@ -42,6 +42,7 @@ constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kClearWarp = kSo
 constexpr int kWarps   = kSoftWarps + 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFwdPoly = 4, kBwdPoly = 4;  // one pair of exponentials in so many by a polynomial
 
 __device__ int32_t g_attn_error;  // one per device
 
@@ -702,7 +703,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
           uint32_t v[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const F2 x = Exp2Mixed<4>(Fma2(Pair(s[g][2 * k], s[g][2 * k + 1]), c2, nm), k);
+            const F2 x = Exp2Mixed<kFwdPoly>(Fma2(Pair(s[g][2 * k], s[g][2 * k + 1]), c2, nm), k);
             sum[k & 1] = g == 0 && k < 2 ? x : Add2(sum[k & 1], x);
             v[k] = Pack2<kBf16>(x);
           }
@@ -792,20 +793,21 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
 //   !kKeys    Q, dO            K, V               rows are queries                dQ += dS K
 // Both passes compute S and dP, seven products instead of five, and in exchange every sum has one owner: no atomics, no
 // fp32 copy of dQ in memory, and results that do not depend on the order of the blocks.
-// Units alternate between two sets of eight softmax warps (32 rows x 32 columns a warp), each with its own S and dP in TMEM.  A
-// unit goes through S, P, dP, dS in turn, and every step hands over between the tensor cores and the warps of its set; the
-// other set, half a period behind, uses the exponential unit and the issue slots meanwhile.  Units of 64 rather than 128
-// positions, as two sets of 128 columns do not fit beside the accumulators; their products S and dP take three quarters
-// of the time of twice as many columns.
-constexpr int kUnit = 64;
+// A unit goes through S, P, dP, dS in turn, and every step hands over between the tensor cores and the softmax warps, each of
+// which has 32 rows x 32 columns.  With 64 accumulator columns a unit has 128 positions and all sixteen warps, and the next
+// unit's scores are ready in a second place when they are needed.  With 128 there is no second place; units have 64 positions and
+// alternate between two sets of eight warps, each with its own S and dP: while one waits for the tensor cores, the other
+// computes.  (Products of 64 columns take three quarters of the time of 128.)
 template <int HD>
 struct BwdCfg {
   static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;    // what stays: X1 or X2
-  static constexpr int kUnitBytes  = kTileBytes * kUnit / kTile;
+  static constexpr int kSets       = HD == 64 ? 1 : 2;
+  static constexpr int kUnit       = kTile / kSets;            // positions of a streamed unit
+  static constexpr int kUnitBytes  = kTileBytes / kSets;
   static constexpr int kStageBytes = 2 * kUnitBytes;           // Y1, Y2
-  static constexpr int kStages     = HD == 64 ? 8 : 4;
+  static constexpr int kStages     = 4;
   static constexpr int kXBufs      = HD == 64 ? 2 : 1;         // what stays, of this piece of work and the next
-  static constexpr int kSBufs      = HD == 64 ? 2 : 1;         // scores of a set; beside accumulators of 128 columns there is room for one
+  static constexpr int kSBufs      = 2;                        // places for scores in TMEM: two of the one set, one of either
   static constexpr int kRowBytes   = 2 * kUnit * 4;            // -L and -D of a unit of queries
   // shared memory: [kXBufs][X1, X2], the ring [kStages][Y1, Y2], [kStages][-L, -D], barriers
   static constexpr int kRing       = kXBufs * 2 * kTileBytes;
@@ -817,14 +819,14 @@ struct BwdCfg {
   static constexpr int kRaw        = kEmpty + 8 * kStages;       // a unit has arrived and has rows to clear before it counts as full
   static constexpr int kXFull      = kRaw + 8 * kStages;
   static constexpr int kXEmpty     = kXFull + 8 * kXBufs;
-  static constexpr int kSFull      = kXEmpty + 8 * kXBufs;       // [2 SB] S of a unit is in TMEM
-  static constexpr int kSDone      = kSFull + 16 * kSBufs;       // [2 SB] keys: P has taken its place, queries: S has been read
-  static constexpr int kDpFull     = kSDone + 16 * kSBufs;       // [2] dP is in TMEM
-  static constexpr int kDsFull     = kDpFull + 16;               // [2] dS has taken its place
-  static constexpr int kAccFull    = kDsFull + 16;               // a piece's sums are complete
+  static constexpr int kSFull      = kXEmpty + 8 * kXBufs;       // [SB] S of a unit is in TMEM
+  static constexpr int kSDone      = kSFull + 8 * kSBufs;        // [SB] keys: P has taken its place, queries: S has been read
+  static constexpr int kDpFull     = kSDone + 8 * kSBufs;        // [sets] dP is in TMEM
+  static constexpr int kDsFull     = kDpFull + 8 * kSets;        // [sets] dS has taken its place
+  static constexpr int kTurn       = kDsFull + 8 * kSets;        // [sets] a unit's exponentials are done
+  static constexpr int kAccFull    = kTurn + 8 * kSets;          // a piece's sums are complete
   static constexpr int kAccFree    = kAccFull + 8;               // all softmax warps have read them
-  static constexpr int kApart      = kAccFree + 8;               // the first set has made its first step
-  static constexpr int kTmemSlot   = kApart + 8;
+  static constexpr int kTmemSlot   = kAccFree + 8;
   static constexpr int kSmemBytes  = kTmemSlot + 16 + 1024;
 };
 
@@ -835,6 +837,7 @@ struct BwdWords {  // what stands in a slot
       : b(w[0]), head(w[1]), x0(w[2]), len(w[3]), first(w[4]), per(w[5]), total(w[6]), ragged(w[7] & 1), keys(w[7] & 2) {}
   // First the pieces of the keys, whose tiles stream past every query head of their group; causal: the tiles with the longest
   // streams first; otherwise neighbours share a head.
+  template <int kUnit>
   __device__ __forceinline__ static void Describe(const AttnParams& p, int index, int (&w)[8]) {
     const int tiles = p.sp / kTile, group = p.h / p.hk, key_pieces = tiles * p.b * p.hk;
     const bool keys = index < key_pieces;
@@ -875,15 +878,14 @@ struct BwdSmem {
   __device__ __forceinline__ uint32_t Raw(uint32_t u) const { return base + C::kRaw + u % C::kStages * 8; }
   __device__ __forceinline__ uint32_t XFull(uint32_t n) const { return base + C::kXFull + n % C::kXBufs * 8; }
   __device__ __forceinline__ uint32_t XEmpty(uint32_t n) const { return base + C::kXEmpty + n % C::kXBufs * 8; }
-  __device__ __forceinline__ uint32_t SFull(uint32_t u) const { return base + C::kSFull + u % (2 * C::kSBufs) * 8; }
-  __device__ __forceinline__ uint32_t SDone(uint32_t u) const { return base + C::kSDone + u % (2 * C::kSBufs) * 8; }
-  __device__ __forceinline__ uint32_t DpFull(uint32_t u) const { return base + C::kDpFull + (u & 1) * 8; }
-  __device__ __forceinline__ uint32_t DsFull(uint32_t u) const { return base + C::kDsFull + (u & 1) * 8; }
-  // columns: S and dP of either set, the accumulators, the other S of either set
-  __device__ __forceinline__ uint32_t S(uint32_t u) const {
-    return u % (2 * C::kSBufs) < 2 ? tmem + (u & 1) * 128 : tmem + 384 + (u & 1) * 64;
-  }
-  __device__ __forceinline__ uint32_t Dp(uint32_t u) const { return tmem + 64 + (u & 1) * 128; }
+  __device__ __forceinline__ uint32_t SFull(uint32_t u) const { return base + C::kSFull + u % C::kSBufs * 8; }
+  __device__ __forceinline__ uint32_t SDone(uint32_t u) const { return base + C::kSDone + u % C::kSBufs * 8; }
+  __device__ __forceinline__ uint32_t DpFull(uint32_t u) const { return base + C::kDpFull + u % C::kSets * 8; }
+  __device__ __forceinline__ uint32_t DsFull(uint32_t u) const { return base + C::kDsFull + u % C::kSets * 8; }
+  __device__ __forceinline__ uint32_t Turn(uint32_t u) const { return base + C::kTurn + u % C::kSets * 8; }
+  // columns: S and dP, of one set or of either, then the accumulators and the one set's second S
+  __device__ __forceinline__ uint32_t S(uint32_t u) const { return tmem + (u & 1) * (C::kSets == 1 ? 384 : 128); }
+  __device__ __forceinline__ uint32_t Dp(uint32_t u) const { return C::kSets == 1 ? tmem + 128 : tmem + 64 + (u & 1) * 128; }
   __device__ __forceinline__ uint32_t Acc(int i) const { return tmem + 256 + i * HD; }
 };
 
@@ -892,7 +894,7 @@ template <int HD, bool kKeys>
 __device__ __forceinline__ bool BwdLoad(const AttnMaps& maps, const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w,
                                         uint32_t u0, uint32_t n) {  // one thread
   using Cfg = BwdCfg<HD>;
-  constexpr int XB = Cfg::kXBufs, ST = Cfg::kStages;
+  constexpr int XB = Cfg::kXBufs, ST = Cfg::kStages, kUnit = Cfg::kUnit;
   if (!BarWaitOne(m.XEmpty(n), (n / XB) ^ 1)) return false;
   BarExpect(m.XFull(n), 2 * Cfg::kTileBytes + (kKeys ? 0 : 2 * kTile * 4));
   TmaLoadTile<HD, kTile, kUnit>(m.X(n), kKeys ? &maps.k : &maps.q, w.x0, w.head, w.b, m.XFull(n));
@@ -933,7 +935,7 @@ __device__ __forceinline__ void BwdClear(const BwdSmem<HD>& m, const BwdPiece<kK
     const uint32_t st = (u0 + k) % BwdCfg<HD>::kStages;
     if (!wait(m.Raw(st), uses >> st)) break;
     uses ^= 1u << st;
-    ClearRows<kUnit>(m.Y(st), 2 * (HD / 64), w.len % kUnit);
+    ClearRows<BwdCfg<HD>::kUnit>(m.Y(st), 2 * (HD / 64), w.len % BwdCfg<HD>::kUnit);
     if ((threadIdx.x & 31) == 0) BarArrive(m.Full(st));
   }
 }
@@ -943,7 +945,7 @@ template <bool kBf16, int kWhich, int HD, bool kKeys>
 __device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
                                        Waiter& wait) {
   using Cfg = BwdCfg<HD>;
-  constexpr int ST = Cfg::kStages, SB = 2 * Cfg::kSBufs, XB = Cfg::kXBufs;
+  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs, XB = Cfg::kXBufs, NS = Cfg::kSets, kUnit = Cfg::kUnit;
   const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
   const uint32_t x1 = m.X(n), x2 = x1 + Cfg::kTileBytes;
   u0 = Uniform(u0);
@@ -975,15 +977,15 @@ __device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m
       BarCommit(m.DpFull(u));
       if (u + 1 == end) BarCommit(m.XEmpty(n));
     };
-    for (uint32_t u = u0; u < min(u0 + 2, end) && arrived(u); ++u)
+    for (uint32_t u = u0; u < min(u0 + NS, end) && arrived(u); ++u)
       if (ElectOne()) grads(u);
     for (uint32_t u = u0; u < end && wait.ok; ++u) {
-      if ((u + 2 < end && !arrived(u + 2)) || !wait(m.DsFull(u), u / 2)) break;
+      if ((u + NS < end && !arrived(u + NS)) || !wait(m.DsFull(u), u / NS)) break;
       if (u == u0 && n > 0 && !wait(m.base + Cfg::kAccFree, n - 1)) break;
       if (ElectOne()) {
         IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(u), m.Y(u), n_out, u > u0);
         BarCommit(m.Empty(u));
-        if (u + 2 < end) grads(u + 2);
+        if (u + NS < end) grads(u + NS);
       }
     }
   }
@@ -994,11 +996,11 @@ template <bool kBf16, int HD, bool kKeys>
 __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
                                            Waiter& wait) {
   using Cfg = BwdCfg<HD>;
-  constexpr int ST = Cfg::kStages, SB = 2 * Cfg::kSBufs;
+  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs, NS = Cfg::kSets, kUnit = Cfg::kUnit;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3;      // TMEM lanes
-  const int set = warp >> 3;
-  const int col = ((warp >> 2) & 1) * 32;  // first column of this warp in a unit
+  const int set = NS == 1 ? 0 : warp >> 3;
+  const int col = ((warp >> 2) & (4 / NS - 1)) * 32;  // first column of this warp in a unit
   const int row = w.x0 + quarter * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
   F2 row_l{}, row_d{};  // -L, -D
@@ -1012,9 +1014,8 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
     if (lane == 0) BarArrive(m.XEmpty(n));
   }
   const F2 c2 = Both(p.c);
-  int at = static_cast<int>((set ^ u0) & 1);  // unit within a head
-  if (set == 1 && u0 == 0 && w.total > 0) wait(m.base + Cfg::kApart, 0);  // half a period behind the other set, from the first piece on
-  for (uint32_t u = u0 + at; u < u0 + w.total; u += 2, at += 2) {
+  int at = NS == 1 ? 0 : static_cast<int>((set ^ u0) & 1);  // unit within a head
+  for (uint32_t u = u0 + at; u < u0 + w.total; u += NS, at += NS) {
     if (at >= w.per) at %= w.per;  // the group's next head
     const int y0 = (w.first + at) * kUnit;
     if (!wait(m.SFull(u), u / SB)) break;
@@ -1028,6 +1029,9 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       __syncwarp();
       if (lane == 0) BarArrive(m.SDone(u));
     }
+    // the sets take turns at the exponentials: side by side they would share the unit for them, wait for the tensor cores at
+    // the same time, and stay in step
+    if (NS > 1 && u > 0 && !wait(m.Turn(u - 1), (u - 1) / NS)) break;
     const uint32_t ls = m.Rows(u) + col * 4;
     F2 pr[16];
 #pragma unroll
@@ -1036,8 +1040,12 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       if (kKeys) {
         LoadPairs(ls + 8 * k, l0, l1);
       }
-      pr[k]     = Exp2Mixed<4>(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0), k);
-      pr[k + 1] = Exp2Mixed<4>(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1), k + 1);
+      pr[k]     = Exp2Mixed<kBwdPoly>(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0), k);
+      pr[k + 1] = Exp2Mixed<kBwdPoly>(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1), k + 1);
+    }
+    if (NS > 1) {
+      __syncwarp();
+      if (lane == 0) BarArrive(m.Turn(u));
     }
     if (kKeys ? p.causal && y0 < w.x0 + kTile : y0 + kUnit > w.len || (p.causal && y0 + kUnit > w.x0)) {
       // rows are keys: they count for the queries from their own position on; rows are queries: keys up to a limit
@@ -1059,8 +1067,7 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       __syncwarp();
       if (lane == 0) BarArrive(m.SDone(u));
     }
-    if (u == 0 && lane == 0) BarArrive(m.base + Cfg::kApart);
-    if (!wait(m.DpFull(u), u / 2)) break;
+    if (!wait(m.DpFull(u), u / NS)) break;
     TmemLoad32(m.Dp(u) + lanes + col, s);
     uint32_t v[16];
 #pragma unroll
@@ -1122,17 +1129,17 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
       BarInit(m.XFull(i), 1);
       BarInit(m.XEmpty(i), 2 + kSoftWarps);
     }
-    for (int i = 0; i < 2 * Cfg::kSBufs; ++i) {
+    for (int i = 0; i < Cfg::kSBufs; ++i) {
       BarInit(m.SFull(i), 1);
-      BarInit(m.SDone(i), kSoftWarps / 2);
+      BarInit(m.SDone(i), kSoftWarps / Cfg::kSets);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < Cfg::kSets; ++i) {
       BarInit(m.DpFull(i), 1);
-      BarInit(m.DsFull(i), kSoftWarps / 2);
+      BarInit(m.DsFull(i), kSoftWarps / Cfg::kSets);
+      BarInit(m.Turn(i), kSoftWarps / Cfg::kSets);
     }
     BarInit(m.base + Cfg::kAccFull, 2);
     BarInit(m.base + Cfg::kAccFree, kSoftWarps);
-    BarInit(m.base + Cfg::kApart, kSoftWarps / 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) AllocTmem(m.base + Cfg::kTmemSlot);
@@ -1158,7 +1165,7 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   };
   if (warp == kTmaWarp) {
     if (ElectOne()) {
-      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { BwdWords::Describe(p, index, v); }, [&](const int (&v)[8]) {
+      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { BwdWords::Describe<Cfg::kUnit>(p, index, v); }, [&](const int (&v)[8]) {
         return each(v, [&](const auto& w) { return w.total == 0 || BwdLoad(maps, p, m, w, u0, n); });
       });
       if (!ok) atomicExch(&g_attn_error, 5);
@@ -1340,11 +1347,12 @@ int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const vo
   TIPSK_REQUIRE(reinterpret_cast<uintptr_t>(lse) % 16 == 0 && reinterpret_cast<uintptr_t>(delta) % 16 == 0,
                 "attention: lse and delta must be 16-byte aligned");
   TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.sdo), "attention: strides must be positive");
+  const int box = d <= 64 ? BwdCfg<64>::kUnit : BwdCfg<128>::kUnit;
   AttnMaps maps;
-  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, kUnit))) return rc;
-  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, kUnit))) return rc;
-  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, kUnit))) return rc;
-  if ((rc = HeadMap(&maps.dout, dout, dtype, b, s, h, d, p.sdo, kUnit))) return rc;
+  if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, box))) return rc;
+  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, box))) return rc;
+  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, box))) return rc;
+  if ((rc = HeadMap(&maps.dout, dout, dtype, b, s, h, d, p.sdo, box))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == kBF16) return d <= 64 ? LaunchBwd<64, true>(maps, p, st) : LaunchBwd<128, true>(maps, p, st);
   return d <= 64 ? LaunchBwd<64, false>(maps, p, st) : LaunchBwd<128, false>(maps, p, st);
