@@ -42,7 +42,7 @@ constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kClearWarp = kSo
 constexpr int kWarps   = kSoftWarps + 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFwdPoly = 4, kBwdPoly = 4;  // one pair of exponentials in so many by a polynomial
+constexpr int kFwdPoly = 4;  // forward, one pair of exponentials in so many by a polynomial
 
 __device__ int32_t g_attn_error;  // one per device
 
@@ -68,6 +68,7 @@ struct AttnParams {
 
 struct AttnMaps {
   CUtensorMap q, k, v, dout;
+  CUtensorMap out, dq, dk, dv;  // written: boxes of 128 positions
 };
 
 // A value that all lanes of a warp hold, as the compiler can tell: what is computed from it stays in uniform registers, from
@@ -269,6 +270,37 @@ __device__ __forceinline__ void StoreCols(uint16_t* row, int col0, int d, const 
     *reinterpret_cast<uint4*>(row + col0 + g * 8) = v;
   }
 }
+// The same of a row into a staged tile, whose boxes of 64 columns and 128 rows have the swizzled layout that a TMA store reads;
+// rows that are not live are zero.
+template <bool kBf16, int kCols>
+__device__ __forceinline__ void StageCols(uint32_t tile, int r, int col0, const uint32_t (&acc)[kCols], float factor, bool live) {
+#pragma unroll
+  for (int g = 0; g < kCols / 8; ++g) {
+    uint32_t v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v[k] = live ? Pack2<kBf16>(__uint_as_float(acc[g * 8 + 2 * k]) * factor, __uint_as_float(acc[g * 8 + 2 * k + 1]) * factor) : 0u;
+    const int c = col0 + g * 8;
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + (c >> 6) * kBoxBytes + r * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4)),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
+  }
+}
+// A staged tile into memory, by one thread: what lies beyond the tensor's positions and columns is not written.
+template <int HD>
+__device__ __forceinline__ void TmaStoreTile(uint32_t tile, const CUtensorMap* map, int s, int h, int b) {
+#pragma unroll
+  for (int x = 0; x < HD / 64; ++x)
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x * 64), "r"(s), "r"(h), "r"(b), "r"(tile + x * kBoxBytes)
+                 : "memory");
+}
+// Until this thread's stores have read their tiles.
+__device__ __forceinline__ void StoresRead() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
 __device__ __forceinline__ void StoreZeroRow(uint16_t* row, int c0, int c1) {
   for (int c = c0; c < c1; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
 }
@@ -448,6 +480,8 @@ struct FwdCfg {
   static constexpr int kStages    = HD == 64 ? 8 : 4;  // tiles of K and V in turn
   static constexpr int kQBufs     = HD == 64 ? 2 : 1;  // queries of this piece of work and the next
   static constexpr bool kOwnP     = HD == 64;          // probabilities beside the scores
+  // outputs leave by TMA through the place of their queries, where the next piece has another
+  static constexpr bool kStaged   = kQBufs == 2;
   // shared memory: queries [kQBufs][2], the ring, maxima [2 turns][2 tiles][2 halves][128 rows], barriers
   static constexpr int kRing      = 2 * kQBufs * kTileBytes;
   static constexpr int kMax       = kRing + kStages * kTileBytes;
@@ -461,7 +495,8 @@ struct FwdCfg {
   static constexpr int kSFree     = kSFull + 16;           // [2] they have been read
   static constexpr int kPFull     = kSFree + 16;           // [2] the probabilities are in TMEM
   static constexpr int kOFull     = kPFull + 16;           // [2] their product with V has completed
-  static constexpr int kTmemSlot  = kOFull + 16;
+  static constexpr int kOStaged   = kOFull + 16;           // [2] a piece's output is in shared memory
+  static constexpr int kTmemSlot  = kOStaged + 16;
   static constexpr int kSmemBytes = kTmemSlot + 16 + 1024;
 };
 
@@ -517,13 +552,14 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     }
     for (int i = 0; i < QB; ++i) {
       BarInit(q_full(i), 1);
-      BarInit(q_empty(i), 2);
+      BarInit(q_empty(i), Cfg::kStaged ? 4 : 2);  // both MMA warps are done with their tile, and have stored what took its place
     }
     for (int i = 0; i < 2; ++i) {
       BarInit(base + Cfg::kSFull + i * 8, 1);
       BarInit(base + Cfg::kSFree + i * 8, kSoftWarps / 2);
       BarInit(base + Cfg::kPFull + i * 8, kSoftWarps / 2);
       BarInit(base + Cfg::kOFull + i * 8, 1);
+      BarInit(base + Cfg::kOStaged + i * 8, kSoftWarps / 2);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -582,6 +618,24 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     const uint32_t s_full = base + Cfg::kSFull + i * 8, s_free = base + Cfg::kSFree + i * 8, p_full = base + Cfg::kPFull + i * 8,
                    o_full = base + Cfg::kOFull + i * 8;
     auto entry = [&](uint32_t k) { return wait(full(k), k / S); };
+    // The output of an earlier piece is stored when this piece's scores are on their way.
+    uint32_t owed = 0, stored = 0;  // pieces whose store is owed (at most one), pieces stored with any output
+    int owed_b = 0, owed_h = 0, owed_row = 0;
+    bool owed_any = false;
+    auto settle = [&] {
+      if (!Cfg::kStaged || owed == 0) return;
+      if (owed_any && !wait(base + Cfg::kOStaged + i * 8, stored)) return;
+      if (ElectOne()) {
+        if (owed_any) {
+          TmaStoreTile<HD>(q_tile(n - 1, i), &maps.out, owed_row, owed_h, owed_b);
+          StoresRead();
+        }
+        BarArrive(q_empty(n - 1));
+      }
+      __syncwarp();
+      stored += owed_any;
+      owed = 0;
+    };
     for (uint32_t turn = 0; pieces.Take<false>(turn, words); ++turn) {
       const FwdPiece w(words);
       const int mine = i ? w.count1 : w.count0;
@@ -596,6 +650,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
           if (j + 1 == max(mine, 1)) BarCommit(q_empty(n));
         };
         if (wait(q_full(n), n / QB) && entry(e) && ElectOne()) scores(0);
+        settle();
         for (int j = 0; j < w.total && wait.ok; ++j) {  // a tile with fewer keys than the other hands on the rest
           const uint32_t ev = e + 2 * j + 1;
           if (j + 1 < w.total && !entry(ev + 1)) break;
@@ -618,8 +673,15 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         }
         e += 2 * w.total;
         ++n;
+        owed     = 1;
+        owed_any = mine > 0;
+        owed_b   = w.b;
+        owed_h   = w.h;
+        owed_row = w.q0 + i * kTile;
       }
     }
+    if (wait.ok) settle();
+    if (Cfg::kStaged && ElectOne()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
     const int i = warp >> 3, half = (warp >> 2) & 1;  // query tile; columns [64 half, 64 half + 64) of the scores
     const int quarter = warp & 3;                     // TMEM lanes that this warp may access
@@ -631,7 +693,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     const F2 c2 = Both(p.c);
     const uint32_t s_full = base + Cfg::kSFull + i * 8, s_free = base + Cfg::kSFree + i * 8, p_full = base + Cfg::kPFull + i * 8,
                    o_full = base + Cfg::kOFull + i * 8;
-    uint32_t done = 0, swaps = 0;
+    uint32_t done = 0, swaps = 0, pieces_done = 0;
     Waiter wait(4);
     // this thread's value and the one of the thread with the other half of the row
     auto other = [&](float mine) {
@@ -729,11 +791,18 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         for (int g = 0; g < HD / 64; ++g) {
           uint32_t o[32];
           TmemLoad32(to + g * 32, o);
-          if (live && wait.ok) StoreCols<kBf16, 32>(dst, c0 + g * 32, p.d, o, inv);
+          if (Cfg::kStaged) StageCols<kBf16, 32>(q_tile(pieces_done, i), r, c0 + g * 32, o, inv, live);
+          else if (live && wait.ok) StoreCols<kBf16, 32>(dst, c0 + g * 32, p.d, o, inv);
         }
         TcFenceBefore();
+        if (Cfg::kStaged) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) BarArrive(base + Cfg::kOStaged + i * 8);
+        }
       }
-      if (!live && row < p.s) StoreZeroRow(dst, half * (HD / 2), min(p.d, (half + 1) * (HD / 2)));
+      pieces_done += w.total > 0;
+      if ((!Cfg::kStaged || count == 0) && !live && row < p.s) StoreZeroRow(dst, half * (HD / 2), min(p.d, (half + 1) * (HD / 2)));
       if (half == 0 && row < p.sp)
         p.lse[(static_cast<int64_t>(w.b) * p.h + w.h) * p.sp + row] = live ? fmaf(m, p.c, log2f(l)) : INFINITY;
     }
@@ -825,7 +894,7 @@ struct BwdCfg {
   static constexpr int kDsFull     = kDpFull + 8 * kSets;        // [sets] dS has taken its place
   static constexpr int kTurn       = kDsFull + 8 * kSets;        // [sets] a unit's exponentials are done
   static constexpr int kAccFull    = kTurn + 8 * kSets;          // a piece's sums are complete
-  static constexpr int kAccFree    = kAccFull + 8;               // all softmax warps have read them
+  static constexpr int kAccFree    = kAccFull + 8;               // all softmax warps have read them, and staged them for the store
   static constexpr int kTmemSlot   = kAccFree + 8;
   static constexpr int kSmemBytes  = kTmemSlot + 16 + 1024;
 };
@@ -940,10 +1009,31 @@ __device__ __forceinline__ void BwdClear(const BwdSmem<HD>& m, const BwdPiece<kK
   }
 }
 
+// Stores of a piece whose sums are, or will be, staged: the warp that issues S makes them when the next piece's first scores are
+// on their way, while the softmax warps work on these.
+struct Owed {
+  int b = -1, head, x0;
+  bool keys;
+  uint32_t n;
+};
+template <int HD>
+__device__ __forceinline__ void BwdSettle(const AttnMaps& maps, const BwdSmem<HD>& m, Owed& o, Waiter& wait) {
+  using Cfg = BwdCfg<HD>;
+  if (o.b < 0 || !wait(m.base + Cfg::kAccFree, o.n)) return;
+  if (ElectOne()) {
+    TmaStoreTile<HD>(m.X(o.n), o.keys ? &maps.dk : &maps.dq, o.x0, o.head, o.b);
+    if (o.keys) TmaStoreTile<HD>(m.X(o.n) + Cfg::kTileBytes, &maps.dv, o.x0, o.head, o.b);
+    StoresRead();
+    BarArrive(m.XEmpty(o.n));
+  }
+  __syncwarp();
+  o.b = -1;
+}
+
 // Which: 0 issues S and P^T dO, 1 issues dP and dS^T Q or dS K.
 template <bool kBf16, int kWhich, int HD, bool kKeys>
-__device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
-                                       Waiter& wait) {
+__device__ __forceinline__ void BwdMma(const AttnMaps& maps, const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w,
+                                       uint32_t u0, uint32_t n, Owed& owed, Waiter& wait) {
   using Cfg = BwdCfg<HD>;
   constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs, XB = Cfg::kXBufs, NS = Cfg::kSets, kUnit = Cfg::kUnit;
   const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
@@ -952,6 +1042,7 @@ __device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m
   n  = Uniform(n);
   const uint32_t end = u0 + w.total;
   auto arrived = [&](uint32_t u) { return wait(m.Full(u), u / ST); };
+  if (kWhich == 0 && XB == 1) BwdSettle(maps, m, owed, wait);  // this piece's X comes to the same place
   wait(m.XFull(n), n / XB);
   if (kWhich == 0) {
     auto scores = [&](uint32_t u) {
@@ -961,10 +1052,11 @@ __device__ __forceinline__ void BwdMma(const AttnParams& p, const BwdSmem<HD>& m
     };
     for (uint32_t u = u0; u < min(u0 + SB, end) && arrived(u); ++u)
       if (ElectOne()) scores(u);
+    BwdSettle(maps, m, owed, wait);
+    owed = Owed{w.b, w.head, w.x0, kKeys, n};
     for (uint32_t u = u0; u < end && wait.ok; ++u) {
       const uint32_t next = u + SB;
       if ((next < end && !arrived(next)) || !wait(m.SDone(u), u / SB)) break;
-      if (kKeys && u == u0 && n > 0 && !wait(m.base + Cfg::kAccFree, n - 1)) break;
       if (ElectOne()) {
         if (kKeys) IssueFromTmem<kBf16, kUnit, 32>(m.Acc(1), m.S(u), m.Y(u) + Cfg::kUnitBytes, n_out, u > u0);
         BarCommit(m.Empty(u));
@@ -1010,8 +1102,6 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       row_l = Both(LoadShared(m.XRows(n) + (quarter * 32 + lane) * 4));
       row_d = Both(LoadShared(m.XRows(n) + (kTile + quarter * 32 + lane) * 4));
     }
-    __syncwarp();
-    if (lane == 0) BarArrive(m.XEmpty(n));
   }
   const F2 c2 = Both(p.c);
   int at = NS == 1 ? 0 : static_cast<int>((set ^ u0) & 1);  // unit within a head
@@ -1040,8 +1130,8 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       if (kKeys) {
         LoadPairs(ls + 8 * k, l0, l1);
       }
-      pr[k]     = Exp2Mixed<kBwdPoly>(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0), k);
-      pr[k + 1] = Exp2Mixed<kBwdPoly>(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1), k + 1);
+      pr[k]     = Exp2Fast(Fma2(Pair(s[2 * k], s[2 * k + 1]), c2, l0));
+      pr[k + 1] = Exp2Fast(Fma2(Pair(s[2 * k + 2], s[2 * k + 3]), c2, l1));
     }
     if (NS > 1) {
       __syncwarp();
@@ -1089,23 +1179,26 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
   if (!wait.ok) return;
   const bool live = row < w.len;
   constexpr int kCols = HD / 4;
-  const int c0 = (warp >> 2) * kCols;
+  const int c0 = (warp >> 2) * kCols, r = quarter * 32 + lane;
+  if (w.total > 0) {  // dK (dQ) into the place of X1, dV of X2
 #pragma unroll
-  for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
-    const Strides& st = out ? p.sdv : kKeys ? p.sdk : p.sdq;
-    uint16_t* dst = static_cast<uint16_t*>(out ? p.dv : kKeys ? p.dk : p.dq) + w.b * st.b + row * st.s + w.head * st.h;
-    if (w.total > 0) {
+    for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
       uint32_t o[kCols];
       if constexpr (kCols == 32) TmemLoad32(m.Acc(out) + lanes + c0, o);
       else TmemLoad16(m.Acc(out) + lanes + c0, o);
-      if (live) StoreCols<kBf16, kCols>(dst, c0, p.d, o, out ? 1.f : p.scale);
+      StageCols<kBf16, kCols>(m.X(n) + out * Cfg::kTileBytes, r, c0, o, out ? 1.f : p.scale, live);
     }
-    if (!live && row < p.s) StoreZeroRow(dst, c0, min(p.d, c0 + kCols));
-  }
-  if (w.total > 0) {
     TcFenceBefore();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) BarArrive(m.base + Cfg::kAccFree);
+  } else if (row < p.s) {
+#pragma unroll
+    for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
+      const Strides& st = out ? p.sdv : kKeys ? p.sdk : p.sdq;
+      StoreZeroRow(static_cast<uint16_t*>(out ? p.dv : kKeys ? p.dk : p.dq) + w.b * st.b + row * st.s + w.head * st.h, c0,
+                   min(p.d, c0 + kCols));
+    }
   }
 }
 
@@ -1127,7 +1220,7 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     }
     for (int i = 0; i < Cfg::kXBufs; ++i) {
       BarInit(m.XFull(i), 1);
-      BarInit(m.XEmpty(i), 2 + kSoftWarps);
+      BarInit(m.XEmpty(i), 3);  // both MMA warps are done with it, and the sums that took its place are stored
     }
     for (int i = 0; i < Cfg::kSBufs; ++i) {
       BarInit(m.SFull(i), 1);
@@ -1179,14 +1272,18 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     });
   } else if (warp == kMmaWarp) {
     Waiter wait(6);
+    Owed owed;
     follow(std::false_type{}, [&](const auto& w) {
-      if (w.total > 0 && wait.ok) BwdMma<kBf16, 0>(p, m, w, u0, n, wait);
+      if (w.total > 0 && wait.ok) BwdMma<kBf16, 0>(maps, p, m, w, u0, n, owed, wait);
       return true;
     });
+    if (wait.ok) BwdSettle(maps, m, owed, wait);
+    if (ElectOne()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else if (warp == kMmaWarp + 1) {
     Waiter wait(6);
+    Owed none;
     follow(std::false_type{}, [&](const auto& w) {
-      if (w.total > 0 && wait.ok) BwdMma<kBf16, 1>(p, m, w, u0, n, wait);
+      if (w.total > 0 && wait.ok) BwdMma<kBf16, 1>(maps, p, m, w, u0, n, none, wait);
       return true;
     });
   } else {
@@ -1312,12 +1409,13 @@ int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, 
   p.lse = lse;
   TIPSK_REQUIRE(Aligned(q, sq) && Aligned(k, sk) && Aligned(v, sv) && Aligned(out, p.so),
                 "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");
-  TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv), "attention: strides of q, k and v must be positive");
+  TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.so), "attention: strides must be positive");
   AttnMaps maps;
   if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, kTile))) return rc;
   if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, kTile))) return rc;
   if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, kTile))) return rc;
-  maps.dout = maps.q;  // not read
+  if ((rc = HeadMap(&maps.out, out, dtype, b, s, h, d, p.so, kTile))) return rc;
+  maps.dout = maps.dq = maps.dk = maps.dv = maps.q;  // not used
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == kBF16) return d <= 64 ? LaunchFwd<64, true>(maps, p, st) : LaunchFwd<128, true>(maps, p, st);
   return d <= 64 ? LaunchFwd<64, false>(maps, p, st) : LaunchFwd<128, false>(maps, p, st);
@@ -1346,13 +1444,19 @@ int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const vo
                 "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");
   TIPSK_REQUIRE(reinterpret_cast<uintptr_t>(lse) % 16 == 0 && reinterpret_cast<uintptr_t>(delta) % 16 == 0,
                 "attention: lse and delta must be 16-byte aligned");
-  TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.sdo), "attention: strides must be positive");
+  TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.sdo) && Mappable(p.sdq) && Mappable(p.sdk) &&
+                    Mappable(p.sdv),
+                "attention: strides must be positive");
   const int box = d <= 64 ? BwdCfg<64>::kUnit : BwdCfg<128>::kUnit;
   AttnMaps maps;
   if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, box))) return rc;
   if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, box))) return rc;
   if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, box))) return rc;
   if ((rc = HeadMap(&maps.dout, dout, dtype, b, s, h, d, p.sdo, box))) return rc;
+  if ((rc = HeadMap(&maps.dq, dq, dtype, b, s, h, d, p.sdq, kTile))) return rc;
+  if ((rc = HeadMap(&maps.dk, dk, dtype, b, s, hk, d, p.sdk, kTile))) return rc;
+  if ((rc = HeadMap(&maps.dv, dv, dtype, b, s, hk, d, p.sdv, kTile))) return rc;
+  maps.out = maps.q;  // not used
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == kBF16) return d <= 64 ? LaunchBwd<64, true>(maps, p, st) : LaunchBwd<128, true>(maps, p, st);
   return d <= 64 ? LaunchBwd<64, false>(maps, p, st) : LaunchBwd<128, false>(maps, p, st);
