@@ -110,6 +110,28 @@ def test_linear(rows, k, n, act):
         assert a.dtype == bf and ((a.double() - t).abs() <= o + slack * m + u * t.abs()).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(16384, 4096, 1024), (9600, 4096, 64), (5000, 4128, 72), (16384, 1056, 256)])
+def test_pre_activation_packed_by_the_gemm(m, n, k):
+    """The bytes are those of packing the 16-bit pre-activation, with infinities and NaN among them; ragged rows and columns."""
+    from tips_b200.ops import base
+    from tips_b200.ops.linear import _gemm_pre8
+    from tips_b200.ops.saved8 import _pack, _parts
+    g = torch.Generator(device=DEV)
+    g.manual_seed(m + n)
+    bf = torch.bfloat16
+    a, b = torch.randn(m, k, generator=g, device=DEV).to(bf), torch.randn(n, k, generator=g, device=DEV).to(bf)
+    bias = torch.randn(n, generator=g, device=DEV).to(bf)
+    a[7, 3], a[m - 1, 0], b[n - 1, 1], bias[5] = math.inf, math.nan, -math.inf, 3e38
+    a[100:200] *= 1e-30
+    assert base.K().tipsk_gemm_pre8_fits(m, n, k)
+    y, buf = _gemm_pre8(a, b, bias, "gelu")
+    want, pre = gemm_tn(a, b, bias, "gelu", want_pre=True)
+    assert gemm_status() == 0
+    assert torch.equal(y.nan_to_num(nan=-7.0), want.nan_to_num(nan=-7.0))
+    for x, z in zip(_parts(buf, m * n), _parts(_pack(pre), m * n)):
+        assert torch.equal(x, z)
+
+
 def test_passthrough_and_dtypes():
     """The residual gradient is added into the input's; fp32 and fp16 layers take the same arguments."""
     g = torch.Generator(device=DEV)

@@ -27,6 +27,7 @@
 #include <tuple>
 
 #include "kernels/common.cuh"
+#include "kernels/pack8.cuh"
 #include "kernels/tcgen05.cuh"
 #include "kernels/tips_kernels.h"
 
@@ -46,6 +47,7 @@ struct GemmParams {
   int bias_vec;                // 1: bias is 16-byte aligned, so eight values can be read with one load
   float* partial;              // pair kernel, K split over several tiles: [splits][m][n] fp32 partial products
   int splits;
+  int8_t* exps;                // pair kernel, value before the activation in 8 bits: step exponents, one per 32 columns
 };
 
 // Eight consecutive bias values as floats (zeros without a bias): one 16-byte load when the bias is 16-byte aligned
@@ -497,7 +499,7 @@ GemmTnPersistentKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
 // Bound by the tensor cores.  Measured against the single-CTA kernels it took over from (us, M x N x K): 16384 x 4096 x
 // 1024 with bias 100 : 114 (1377 TFLOP/s), the same with GELU and the second output 139 : 307 (159 with two staging boxes), 1232 x 30528 x 1024 71 : 105;
 // A and B MN-major (a weight gradient) 4096 x 1024 x 16384 92 : 114, 30528 x 1024 x 1232 57 : 128.
-template <bool kPre>
+template <bool kPre, bool kPre8 = false>
 struct PairCfgOf {
   static constexpr int kBN            = 256;
   static constexpr int kStages        = kPre ? 4 : 5;
@@ -508,25 +510,58 @@ struct PairCfgOf {
   static constexpr int kGroupBoxes    = kPre ? 3 : 2;           // staging boxes of an epilogue group, used in turn
   static constexpr int kStagingBytes  = 2 * kGroupBoxes * kBoxBytes;
   static constexpr int kTmemCols      = 512;
-  static constexpr int kThreads       = 320;                    // TMA warp, MMA warp, eight epilogue warps
+  static constexpr int kEpiWarps      = kPre8 ? 16 : 8;
+  static constexpr int kThreads       = (2 + kEpiWarps) * 32;   // TMA warp, MMA warp, epilogue warps
   static constexpr int kSmemBytes     = kStages * kStageBytes + kStagingBytes + 1024 + 256;
 };
 
 using PairCfg = PairCfgOf<false>;
 
-// What the epilogue of the pair kernel writes: the bf16 result, also the value before the activation, or fp32 partials.
-constexpr int kOutPlain = 0, kOutPre = 1, kOutPartial = 2;
+// What the epilogue of the pair kernel writes: the bf16 result, also the value before the activation in bf16 or, rounded to bf16
+// first, in 8 bits, or fp32 partials.
+constexpr int kOutPlain = 0, kOutPre = 1, kOutPartial = 2, kOutPre8 = 3;
+
+// 32 bf16 values of a row, which are a block of the 8-bit form, into 32 bytes; returns the step's exponent.
+__device__ __forceinline__ int PackBlock(const uint32_t (&pairs)[16], uint32_t (&q)[8]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) amax = max(amax, max((pairs[j] << 16) & 0x7fffffffu, pairs[j] & 0x7fff0000u));
+  const bool finite = amax < 0x7f800000u;
+  if (!finite) {
+    amax = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      amax = max(amax, max(FiniteBits(__uint_as_float(pairs[j] << 16)), FiniteBits(__uint_as_float(pairs[j] & 0xffff0000u))));
+  }
+  const int e     = StepExponent(amax);
+  const float inv = PowerOfTwo(-e);
+  if (__all_sync(0xffffffffu, finite && e < 121)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x[4] = {__uint_as_float(pairs[2 * j] << 16), __uint_as_float(pairs[2 * j] & 0xffff0000u),
+                          __uint_as_float(pairs[2 * j + 1] << 16), __uint_as_float(pairs[2 * j + 1] & 0xffff0000u)};
+      q[j] = Quantise4(x, inv);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      q[j] = Quantise(__uint_as_float(pairs[2 * j] << 16), inv) | Quantise(__uint_as_float(pairs[2 * j] & 0xffff0000u), inv) << 8 |
+             Quantise(__uint_as_float(pairs[2 * j + 1] << 16), inv) << 16 |
+             Quantise(__uint_as_float(pairs[2 * j + 1] & 0xffff0000u), inv) << 24;
+  }
+  return e;
+}
 
 __host__ __device__ __forceinline__ int SplitBegin(int k_blocks, int split, int splits) {
   return static_cast<int>(static_cast<int64_t>(k_blocks) * split / splits);
 }
 
 template <bool kAMn, bool kBMn, int kOut>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfgOf<false, kOut == kOutPre8>::kThreads), 1)
 GemmPairKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                const __grid_constant__ CUtensorMap tmap_c, const __grid_constant__ CUtensorMap tmap_pre, GemmParams p) {
-  constexpr bool kPre = kOut == kOutPre, kSplit = kOut == kOutPartial;
-  using Cfg = PairCfgOf<kPre>;
+  constexpr bool kPre8 = kOut == kOutPre8, kPre = kOut == kOutPre || kPre8, kSplit = kOut == kOutPartial;
+  using Cfg = PairCfgOf<kPre, kPre8>;
   constexpr int BN = Cfg::kBN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem    = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -554,7 +589,7 @@ GemmPairKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     }
     for (int b = 0; b < 2; ++b) {
       MbarInit(&tmem_full[b], 1);
-      MbarInit(&tmem_empty[b], 16);  // eight epilogue warps of each CTA
+      MbarInit(&tmem_empty[b], 2 * Cfg::kEpiWarps);  // the epilogue warps of both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -649,6 +684,73 @@ GemmPairKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         if (ok && ElectOne()) UmmaCommitPair(&tmem_full[buf]);
       }
     }
+  } else if constexpr (kPre8) {
+    // Four groups of four warps, each with a box of 64 columns.  GELU and the 8-bit form take about 26 instructions a value, most
+    // of them waiting for one another: eight warps took 200 us for 16384 x 4096 x 1024, and the product with the
+    // 16-bit value and a pass that packs it 139 + 42.
+    const int q = warp & 3, g = (warp - 2) >> 2, r = q * 32 + lane;
+    const bool issuer = ((warp - 2) & 3) == 0 && lane == 0;
+    uint8_t* box  = staging + g * (Cfg::kStagingBytes / 4);
+    uint8_t* qbox = box + Cfg::kBoxBytes;
+    int local = 0;
+    bool ok = true;
+    for (int tile = pair; tile < num_tiles; tile += pairs, ++local) {
+      const int m0 = (tile / tiles_n) * 2 * kBM + cta * kBM, n0 = (tile % tiles_n) * BN + g * 64;
+      const int buf = local & 1;
+      if (ok && !MbarWait(&tmem_full[buf], (local >> 1) & 1)) {
+        if (lane == 0) atomicExch(p.error, 3);
+        ok = false;
+      }
+      TcFenceAfter();
+      if (issuer) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      NamedBarSync(1 + g, 128);
+      const uint32_t tsrc = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + static_cast<uint32_t>(buf * BN + g * 64);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (!ok) continue;
+        uint32_t acc[32];
+        TmemLoad32(tsrc + half * 32, acc);
+        if (half == 1) {  // this warp's share of the accumulator is drained
+          TcFenceBefore();
+          __syncwarp();
+          if (lane == 0) MbarArriveLeader(&tmem_empty[buf]);
+        }
+        const int col0 = n0 + half * 32;
+        uint32_t before[16];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float bv[8];
+          LoadBias8(p, col0 + u * 8, bv);
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = __uint_as_float(acc[u * 8 + 2 * j]) + bv[2 * j], y = __uint_as_float(acc[u * 8 + 2 * j + 1]) + bv[2 * j + 1];
+            const float2 z = GemmAct2(x, y, p.act);
+            const __nv_bfloat162 pr = __floats2bfloat162_rn(x, y), ob = __floats2bfloat162_rn(z.x, z.y);
+            before[u * 4 + j] = *reinterpret_cast<const uint32_t*>(&pr);
+            o[j] = *reinterpret_cast<const uint32_t*>(&ob);
+          }
+          *reinterpret_cast<uint4*>(box + r * 128 + (((half * 4 + u) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        uint32_t q8[8];
+        const int e = PackBlock(before, q8);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)  // rows of 64 bytes, 64-byte swizzle
+          *reinterpret_cast<uint4*>(qbox + r * 64 + (((half * 2 + u) ^ ((r >> 1) & 3)) << 4)) =
+              make_uint4(q8[u * 4], q8[u * 4 + 1], q8[u * 4 + 2], q8[u * 4 + 3]);
+        if (m0 + r < p.m && col0 < p.n) p.exps[(static_cast<int64_t>(m0 + r) * p.n + col0) / kBlock8] = static_cast<int8_t>(e);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      NamedBarSync(1 + g, 128);
+      if (issuer) {
+        if (ok && n0 < p.n && m0 < p.m) {
+          TmaStoreOrAdd2D(&tmap_c, n0, m0, box, 0);
+          TmaStoreOrAdd2D(&tmap_pre, n0, m0, qbox, 0);
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    }
+    if (issuer) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
     // Two groups of four warps: group g drains columns [128 g, 128 g + 128) as two boxes of 64.
     const int q = warp & 3;                // TMEM lane quarter
@@ -813,6 +915,21 @@ int MakeTmap(CUtensorMap* out, const void* base, int64_t rows, int64_t cols, int
   return 0;
 }
 
+// Row-major [rows, cols] matrix of bytes without gaps; boxes of 64 bytes x 128 rows, 64-byte swizzle.
+int MakeByteTmap(CUtensorMap* out, const void* base, int64_t rows, int64_t cols) {
+  EncodeFn enc = GetEncodeFn();
+  if (!enc) return SetError(-7, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[2]    = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols)};
+  cuuint32_t box[2]     = {64, static_cast<cuuint32_t>(kBM)};
+  cuuint32_t estr[2]    = {1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return SetError(-7, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return 0;
+}
+
 int32_t* GemmErrorWord() {
   static int32_t* word = nullptr;
   if (!word) {
@@ -860,7 +977,7 @@ int LaunchGemmPersistent(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
 template <bool kAMn, bool kBMn, int kOut>
 int LaunchPair(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const CUtensorMap& tp,
                const GemmParams& p, cudaStream_t s) {
-  using Cfg = PairCfgOf<kOut == kOutPre>;
+  using Cfg = PairCfgOf<kOut == kOutPre || kOut == kOutPre8, kOut == kOutPre8>;
   static std::atomic<int> resident{0};
   int pairs = resident.load(std::memory_order_acquire);
   if (pairs == 0) {
@@ -979,6 +1096,38 @@ int tipsk_gemm_bf16(const void* a, const void* b, void* c, const void* bias, voi
     case 256: return LaunchGemm<256>(ta, tb, tc, tp, p, s);
     default: return LaunchGemm<128>(ta, tb, tc, tp, p, s);
   }
+}
+
+/* 1 when tipsk_gemm_bf16_pre8 is the way to run a product: the CTA-pair kernel takes it and a row is whole blocks of 32. */
+int tipsk_gemm_pre8_fits(int m, int n, int k) {
+  return m > 0 && n > 0 && k > 0 && n % kBlock8 == 0 && PreferPair(m, n, k) ? 1 : 0;
+}
+
+/* tipsk_gemm_bf16 that leaves the value before the activation in 8 bits, from its rounding to bf16: q[m * n] and e[m * n / 32] as
+ * tipsk_pack8 writes them.  C is contiguous. */
+int tipsk_gemm_bf16_pre8(const void* a, const void* b, void* c, const void* bias, void* q, void* e, int m, int n, int k, int lda,
+                         int ldb, int act, void* stream) {
+  TIPSK_REQUIRE(tipsk_gemm_pre8_fits(m, n, k) && lda % 8 == 0 && ldb % 8 == 0, "gemm_pre8: unsupported shape");
+  TIPSK_REQUIRE(reinterpret_cast<uintptr_t>(c) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && e != nullptr,
+                "gemm_pre8: outputs must be 16-byte aligned");
+  GemmParams p{};
+  p.c     = static_cast<__nv_bfloat16*>(c);
+  p.bias  = static_cast<const __nv_bfloat16*>(bias);
+  p.exps  = static_cast<int8_t*>(e);
+  p.error = GemmErrorWord();
+  TIPSK_REQUIRE(p.error != nullptr, "gemm: cannot allocate the error word");
+  p.m = m; p.n = n; p.k = k; p.ldc = n; p.act = act; p.tma_store = 1;
+  p.bias_vec = (bias != nullptr && reinterpret_cast<uintptr_t>(bias) % 16 == 0) ? 1 : 0;
+  CUtensorMap ta, tb, tc, tq;
+  int rc = MakeTmap(&ta, a, m, k, lda, kBM);
+  if (rc) return rc;
+  rc = MakeTmap(&tb, b, n, k, ldb, PairCfg::kBN / 2);
+  if (rc) return rc;
+  rc = MakeTmap(&tc, c, m, n, n, kBM);
+  if (rc) return rc;
+  rc = MakeByteTmap(&tq, q, m, n);
+  if (rc) return rc;
+  return LaunchPair<false, false, kOutPre8>(ta, tb, tc, tq, p, static_cast<cudaStream_t>(stream));
 }
 
 /* C[m,n] = A[m,k] * B[k,n]: B row-major with the contraction over its rows (no transposed copy is made; the MMA

@@ -1,47 +1,13 @@
-// Activations kept for the backward pass in 8 bits.
-//
-// A tensor is taken as one run of values in blocks of 32.  The values of a block share a power-of-two step 2^e and are stored as
-// whole multiples of it:
-//   e = the least integer with rint(amax 2^-e) <= 127, clamped to [-126, 121];   q = clamp(rint(x 2^-e), -127, 127)
-// where amax is the largest finite |x| of the block.  A value that is not finite is stored as q = -128 and stands for NaN.
-// Scaling by a power of two rounds nothing, so the only rounding is rint, off by at most half a step, amax / 127 at
-// most: for a normally distributed block 0.8 % of its root mean square.  And a stored value has at most 7 significant
-// bits, so bf16 holds it exactly: reading it back into the tensor cores' type costs no further rounding.
-// A block takes 32 + 1 bytes.
+// Activations kept for the backward pass in 8 bits (the form: pack8.cuh).  The GEMM writes it too, from its accumulators.
 //
 // The reference keeps no activations (it trains TensorFlow models); these serve the linear layers of the encoder.
 #include "kernels/common.cuh"
+#include "kernels/pack8.cuh"
 #include "kernels/tips_kernels.h"
 
 namespace tipsk {
 namespace {
 
-constexpr int kBlock8 = 32;  // values that share a step
-
-// e of a block from the bits of its amax: amax = 1.M 2^(E - 127) needs E - 133, one more if 1.M 64 rounds to 128
-// (1.M >= 127.5 / 64, M >= 0x7f0000).  Zero and subnormal values end in the lower clamp.
-__device__ __forceinline__ int StepExponent(uint32_t amax_bits) {
-  const int e = static_cast<int>((amax_bits + 0x10000u) >> 23) - 133;
-  return e < -126 ? -126 : e > 121 ? 121 : e;
-}
-__device__ __forceinline__ float PowerOfTwo(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
-__device__ __forceinline__ uint32_t FiniteBits(float x) {
-  const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
-  return a < 0x7f800000u ? a : 0u;
-}
-// One value as its byte; inv = 2^-e.
-__device__ __forceinline__ uint32_t Quantise(float x, float inv) {
-  const int q = __float2int_rn(fminf(fmaxf(x * inv, -127.f), 127.f));
-  return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u ? static_cast<uint32_t>(q) & 0xffu : 0x80u;
-}
-// The same of four finite values that need no clamp, |x| inv <= 127.5: adding 1.5 * 2^23 rounds to a whole number, ties to even,
-// whose two's complement stands in the sum's last byte.
-__device__ __forceinline__ uint32_t Quantise4(const float* x, float inv) {
-  constexpr float kRound = 12582912.f;
-  const uint32_t a = __float_as_uint(fmaf(x[0], inv, kRound)), b = __float_as_uint(fmaf(x[1], inv, kRound));
-  const uint32_t c = __float_as_uint(fmaf(x[2], inv, kRound)), d = __float_as_uint(fmaf(x[3], inv, kRound));
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
 __device__ __forceinline__ float Dequantise(int q, float step) { return q == -128 ? __uint_as_float(0x7fc00000u) : q * step; }
 // Four stored values.  Without a NaN among them: the byte, with its sign bit flipped, becomes the last bits of 2^23 + q + 128.
 __device__ __forceinline__ void Dequantise4(uint32_t w, float step, float* x) {
@@ -55,70 +21,58 @@ __device__ __forceinline__ void Dequantise4(uint32_t w, float step, float* x) {
   }
 }
 
-// Eight values per thread, so four lanes share a block and a warp's loads and stores are contiguous; U groups of eight in flight.
-// A block whose values are all finite, and not so large that the step is clamped, takes a short path of about four
-// instructions a value.  Bound by HBM.
+// A block of 32 values per thread, so nothing is exchanged.  A block whose values are all finite, and not so large that the step is
+// clamped, takes a short path of about four instructions a value.  Bound by HBM.
 template <typename T>
 __global__ void __launch_bounds__(256) Pack8Kernel(const T* __restrict__ x, int8_t* __restrict__ q, int8_t* __restrict__ e, int64_t n) {
-  constexpr int N = 16 / sizeof(T), U = 4;
-  const int64_t groups = (n + 31) / 32 * 4;  // all lanes of a block take part, whatever the tail holds
+  constexpr int N = 16 / sizeof(T);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
-  // every lane makes the same number of rounds: the exchange needs them all
-  for (int64_t g0 = static_cast<int64_t>(blockIdx.x) * 256; g0 < groups; g0 += U * stride) {
-    float v[U][8];
+  for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g * kBlock8 < n; g += stride) {
+    const int64_t at = g * kBlock8;
+    float v[kBlock8];
+    const bool whole = at + kBlock8 <= n;
+    if (whole) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (g0 + u * stride + threadIdx.x) * 8;
-      if (at + 8 <= n) {
+      for (int k = 0; k < kBlock8; k += N) {
+        const Vec16<T> w = LoadVec(x + at + k);
 #pragma unroll
-        for (int k = 0; k < 8; k += N) {
-          const Vec16<T> w = LoadVec(x + at + k);
-#pragma unroll
-          for (int j = 0; j < N; ++j) v[u][k + j] = ToFloat<T>(w.v[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[u][j] = at + j < n ? ToFloat<T>(x[at + j]) : 0.f;
+        for (int j = 0; j < N; ++j) v[k + j] = ToFloat<T>(w.v[j]);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kBlock8; ++j) v[j] = at + j < n ? ToFloat<T>(x[at + j]) : 0.f;
     }
+    // as whole numbers, magnitudes compare like the values, and what is not finite is above all that is
+    uint32_t amax = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t at = (g0 + u * stride + threadIdx.x) * 8;
-      // as whole numbers, magnitudes compare like the values, and what is not finite is above all that is
-      uint32_t amax = 0;
+    for (int j = 0; j < kBlock8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+    const bool finite = amax < 0x7f800000u;
+    if (!finite) {
+      amax = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[u][j]) & 0x7fffffffu);
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      const bool finite = amax < 0x7f800000u;
-      if (!__all_sync(0xffffffffu, finite)) {
-        amax = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, FiniteBits(v[u][j]));
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-      }
-      const int ex    = StepExponent(amax);
-      const float inv = PowerOfTwo(-ex);
-      uint32_t w[2];
-      if (finite && ex < 121) {
-        w[0] = Quantise4(&v[u][0], inv);
-        w[1] = Quantise4(&v[u][4], inv);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          w[j] = Quantise(v[u][4 * j], inv) | Quantise(v[u][4 * j + 1], inv) << 8 | Quantise(v[u][4 * j + 2], inv) << 16 |
-                 Quantise(v[u][4 * j + 3], inv) << 24;
-      }
-      if (at + 8 <= n) {
-        *reinterpret_cast<uint2*>(q + at) = make_uint2(w[0], w[1]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (at + j < n) q[at + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
-      }
-      if ((threadIdx.x & 3) == 0 && at < n) e[at / kBlock8] = static_cast<int8_t>(ex);
+      for (int j = 0; j < kBlock8; ++j) amax = max(amax, FiniteBits(v[j]));
     }
+    const int ex    = StepExponent(amax);
+    const float inv = PowerOfTwo(-ex);
+    uint32_t w[kBlock8 / 4];
+    if (finite && ex < 121) {
+#pragma unroll
+      for (int j = 0; j < kBlock8 / 4; ++j) w[j] = Quantise4(&v[4 * j], inv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kBlock8 / 4; ++j)
+        w[j] = Quantise(v[4 * j], inv) | Quantise(v[4 * j + 1], inv) << 8 | Quantise(v[4 * j + 2], inv) << 16 |
+               Quantise(v[4 * j + 3], inv) << 24;
+    }
+    if (whole) {
+      *reinterpret_cast<uint4*>(q + at)      = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(q + at + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kBlock8; ++j)
+        if (at + j < n) q[at + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j % 4)));
+    }
+    e[g] = static_cast<int8_t>(ex);
   }
 }
 
@@ -261,7 +215,7 @@ int tipsk_pack8(const void* x, void* q, void* e, int64_t n, int dtype, void* str
   TIPSK_REQUIRE(n > 0 && (dtype == kF32 || dtype == kBF16 || dtype == kF16), "pack8: fp32, bf16 or fp16 and at least one value");
   TIPSK_REQUIRE(Aligned16(x) && Aligned16(q), "pack8: the values must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int grid = Blocks((n + 31) / 32 * 4, 8);
+  const int grid = Blocks((n + 31) / 32, 8);
   int8_t *qq = static_cast<int8_t*>(q), *ee = static_cast<int8_t*>(e);
   if (dtype == kF32) Pack8Kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(x), qq, ee, n);
   else if (dtype == kBF16) Pack8Kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), qq, ee, n);

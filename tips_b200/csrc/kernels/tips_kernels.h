@@ -220,6 +220,9 @@ int tipsk_gemm_splits(int m, int n, int k);
 int tipsk_gemm_bf16_split(int kind, const void* a, const void* b, void* c, const void* bias, void* pre, float* partial,
                           int splits, int m, int n, int k, int lda, int ldb, int ldc, int act, int accumulate,
                           void* stream);
+int tipsk_gemm_pre8_fits(int m, int n, int k);
+int tipsk_gemm_bf16_pre8(const void* a, const void* b, void* c, const void* bias, void* q, void* e, int m, int n, int k, int lda,
+                         int ldb, int act, void* stream);
 int tipsk_gemm_bf16_tt(const void* a, const void* b, void* c, int m, int n, int k, int lda, int ldb, int ldc,
                        void* stream);
 int tipsk_gemm_status(void);

@@ -141,6 +141,23 @@ class _LinearFn(torch.autograd.Function):
         return _linear_backward(ctx, dy, None)
 
 
+def _gemm_pre8(a, b, bias, act):
+    """(act(a @ b.T + bias), the value before the activation in 8 bits), the latter from the GEMM's epilogue where the CTA-pair kernel
+    runs the product."""
+    m, k = a.shape
+    n = b.shape[0]
+    if not (_supported(a, b) and base.K().tipsk_gemm_pre8_fits(m, n, k)):
+        y, pre = gemm_tn(a, b, bias, act, want_pre=True)
+        return y, saved8._pack(pre)
+    c = torch.empty(m, n, dtype=torch.bfloat16, device=a.device)
+    buf, at = saved8._buffer(m * n, a.device)
+    bb = None if bias is None else bias.to(torch.bfloat16).contiguous()
+    base.check(base.K().tipsk_gemm_bf16_pre8(a.data_ptr(), b.data_ptr(), c.data_ptr(), base.ptr(bb), buf.data_ptr(),
+                                             buf.data_ptr() + at, m, n, k, a.stride(0), b.stride(0), _ACT[act], base.stream()),
+               "gemm_bf16_pre8")
+    return c, buf
+
+
 class _Linear8Fn(torch.autograd.Function):
     """linear(x) that keeps x and, with GELU, the value before the activation in 8 bits (ops/saved8.py)."""
 
@@ -151,8 +168,7 @@ class _Linear8Fn(torch.autograd.Function):
             x2 = x2.contiguous()
         x8 = pre8 = None
         if _ACT[act] == 2 and any(ctx.needs_input_grad[:3]):
-            y, pre = gemm_tn(x2, weight, bias, act, want_pre=True)
-            pre8 = saved8._pack(pre)
+            y, pre8 = _gemm_pre8(x2, weight, bias, act)
         else:
             y = gemm_tn(x2, weight, bias, act)
         if ctx.needs_input_grad[1]:
