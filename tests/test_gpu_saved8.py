@@ -13,6 +13,12 @@ DEV = "cuda"
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
+def within(got, want, bound):
+    """NaN where NaN is wanted (a pre-activation beyond fp16), and elsewhere within the bound."""
+    nan = want.isnan()
+    return bool((got.isnan() == nan).all() and (((got.double() - want).abs() <= bound) | nan).all())
+
+
 def same(x):
     """pack8 on the GPU gives the CPU's bytes, and unpack its values in every type."""
     a, b = pack8(x), pack8(x.cpu())
@@ -50,12 +56,15 @@ def test_long_tensor():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,cols", [(1, 8), (7, 24), (33, 264), (1000, 512), (4097, 40), (3, 4104), (5, 13)])
+# the largest take the slope from a table
+@pytest.mark.parametrize("rows,cols", [(1, 8), (7, 24), (33, 264), (1000, 512), (4097, 40), (3, 4104), (5, 13), (40000, 72), (5000, 2048)])
 def test_activation_backward(rows, cols, dtype):
     g = torch.Generator(device=DEV)
     g.manual_seed(rows)
     dy = torch.randn(rows, cols, generator=g, device=DEV).to(dtype)
-    p = pack8((torch.randn(rows, cols, generator=g, device=DEV) * 2).to(dtype))
+    z = torch.randn(rows, cols, generator=g, device=DEV) * 2
+    z[::3] *= torch.exp(torch.randn(z[::3].shape, generator=g, device=DEV) * 4)  # steps of any size
+    p = pack8(z.to(dtype))
     z = p.unpack(torch.float32).double()
     want = dy.double() * (0.5 * (1 + torch.erf(z / math.sqrt(2))) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi))
     u = torch.finfo(dtype).eps / 2
@@ -64,14 +73,14 @@ def test_activation_backward(rows, cols, dtype):
     slack = 4e-6 * dy.double().abs()
     for bias_dtype in DTYPES + [None]:
         dz, db = act_bwd8(dy, p.buf, bias_dtype)
-        assert dz.dtype == dtype and ((dz.double() - want).abs() <= u * want.abs() + slack + 2.0 ** -25).all()
+        assert dz.dtype == dtype and within(dz, want, u * want.abs() + slack + 2.0 ** -25)
         if bias_dtype is None:
             assert db is None
             continue
         # sums of the unrounded values in 32 bits: 2^-24 per addition, at most rows of them in a row
         off = (slack + rows * 2.0 ** -24 * want.abs()).sum(0) + torch.finfo(bias_dtype).eps / 2 * want.sum(0).abs() + 2.0 ** -25
-        assert db.dtype == bias_dtype and ((db.double() - want.sum(0)).abs() <= off).all()
-        assert torch.equal(db, act_bwd8(dy, p.buf, bias_dtype)[1])
+        assert db.dtype == bias_dtype and within(db, want.sum(0), off)
+        assert torch.equal(db.nan_to_num(nan=-7.0), act_bwd8(dy, p.buf, bias_dtype)[1].nan_to_num(nan=-7.0))
     same_dy, db = act_bwd8(dy, None, torch.float32)
     assert same_dy.data_ptr() == dy.data_ptr()
     off = rows * 2.0 ** -24 * dy.double().abs().sum(0) + 2.0 ** -24 * dy.double().sum(0).abs()
