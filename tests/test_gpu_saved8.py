@@ -123,7 +123,7 @@ def test_linear(rows, k, n, act):
 def test_pre_activation_packed_by_the_gemm(m, n, k):
     """The bytes are those of packing the 16-bit pre-activation, with infinities and NaN among them; ragged rows and columns."""
     from tips_b200.ops import base
-    from tips_b200.ops.linear import _gemm_pre8
+    from tips_b200.ops.linear import _linear8_forward
     from tips_b200.ops.saved8 import _pack, _parts
     g = torch.Generator(device=DEV)
     g.manual_seed(m + n)
@@ -133,7 +133,7 @@ def test_pre_activation_packed_by_the_gemm(m, n, k):
     a[7, 3], a[m - 1, 0], b[n - 1, 1], bias[5] = math.inf, math.nan, -math.inf, 3e38
     a[100:200] *= 1e-30
     assert base.K().tipsk_gemm_pre8_fits(m, n, k)
-    y, buf = _gemm_pre8(a, b, bias, "gelu")
+    y, _, buf = _linear8_forward(a, b, bias, "gelu", False, True)
     want, pre = gemm_tn(a, b, bias, "gelu", want_pre=True)
     assert gemm_status() == 0
     assert torch.equal(y.nan_to_num(nan=-7.0), want.nan_to_num(nan=-7.0))

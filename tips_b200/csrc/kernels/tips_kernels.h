@@ -247,6 +247,14 @@ int tipsk_act_bwd8_parts(int64_t rows, int cols);
 int tipsk_act_bwd8(const void* dy, const void* q, const void* e, void* dz, void* dbias, int bias_dtype, float* partial,
                    int64_t rows, int cols, int dtype, void* stream);
 
+/* ---- a linear layer with its activations in 8 bits, one call per pass (linear8.cu) ---- */
+int64_t tipsk_linear8_fwd_ws(int m, int n, int k, int want_pre);
+int64_t tipsk_linear8_bwd_ws(int m, int n, int k, int gelu, int want_dw, int want_db);
+int tipsk_linear8_fwd(const void* x, const void* w, const void* bias, void* y, void* x8, void* pre8, void* ws, int m, int n, int k,
+                      int ldw, int act, void* stream);
+int tipsk_linear8_bwd(const void* dy, const void* w, const void* x8, const void* pre8, void* dx, void* dw, void* db, int db_dtype,
+                      void* ws, int m, int n, int k, int ldw, int accumulate, void* stream);
+
 /* ---- 3x3 / stride 2 / pad 1 max pooling on NHWC (pool.cu); idx holds the argmax position 0..8 per output ---- */
 /* Global average pooling on NHWC (x [n, hw, c] -> y [n, c]) and its backward (pool.cu). */
 int tipsk_global_avgpool_fwd(const void* x, void* y, int n, int hw, int c, int dtype, void* stream);

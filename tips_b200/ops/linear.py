@@ -141,21 +141,32 @@ class _LinearFn(torch.autograd.Function):
         return _linear_backward(ctx, dy, None)
 
 
-def _gemm_pre8(a, b, bias, act):
-    """(act(a @ b.T + bias), the value before the activation in 8 bits), the latter from the GEMM's epilogue where the CTA-pair kernel
-    runs the product."""
-    m, k = a.shape
-    n = b.shape[0]
-    if not (_supported(a, b) and base.K().tipsk_gemm_pre8_fits(m, n, k)):
-        y, pre = gemm_tn(a, b, bias, act, want_pre=True)
-        return y, saved8._pack(pre)
-    c = torch.empty(m, n, dtype=torch.bfloat16, device=a.device)
-    buf, at = saved8._buffer(m * n, a.device)
-    bb = None if bias is None else bias.to(torch.bfloat16).contiguous()
-    base.check(base.K().tipsk_gemm_bf16_pre8(a.data_ptr(), b.data_ptr(), c.data_ptr(), base.ptr(bb), buf.data_ptr(),
-                                             buf.data_ptr() + at, m, n, k, a.stride(0), b.stride(0), _ACT[act], base.stream()),
-               "gemm_bf16_pre8")
-    return c, buf
+def _linear8_fits(x2: torch.Tensor, weight: torch.Tensor) -> bool:
+    """Whether the layer runs as one call per pass."""
+    n, k = weight.shape
+    return _supported(x2, weight) and n >= 64 and k >= 64 and n % 8 == 0 and k % 8 == 0 and x2.shape[0] > 0
+
+
+def _linear8_forward(x2, weight, bias, act, want_x8, want_pre8):
+    """(act(x2 @ weight.T + bias), x2 in 8 bits, the value before the activation in 8 bits) with None for what is not wanted."""
+    m, k = x2.shape
+    n = weight.shape[0]
+    if not _linear8_fits(x2, weight):
+        y = gemm_tn(x2, weight, bias, act, want_pre=want_pre8)
+        y, pre8 = (y[0], saved8._pack(y[1])) if want_pre8 else (y, None)
+        return y, saved8._pack(x2) if want_x8 else None, pre8
+    lib = base.K()
+    with base.device_of(x2):
+        y = torch.empty(m, n, dtype=torch.bfloat16, device=x2.device)
+        x8 = saved8._buffer(m * k, x2.device) if want_x8 else None
+        pre8 = saved8._buffer(m * n, x2.device) if want_pre8 else None
+        bb = None if bias is None else bias.to(torch.bfloat16).contiguous()
+        need = lib.tipsk_linear8_fwd_ws(m, n, k, int(want_pre8))
+        ws = torch.empty(need, dtype=torch.uint8, device=x2.device) if need else None
+        base.check(lib.tipsk_linear8_fwd(x2.data_ptr(), weight.data_ptr(), base.ptr(bb), y.data_ptr(), base.ptr(x8), base.ptr(pre8),
+                                         base.ptr(ws), m, n, k, weight.stride(0), _ACT[act], base.stream()), "linear8_fwd")
+    base.count_launches(int(want_x8) + int(want_pre8))
+    return y, x8, pre8
 
 
 class _Linear8Fn(torch.autograd.Function):
@@ -166,13 +177,8 @@ class _Linear8Fn(torch.autograd.Function):
         x2 = x.reshape(-1, x.shape[-1])
         if not x2.is_contiguous():
             x2 = x2.contiguous()
-        x8 = pre8 = None
-        if _ACT[act] == 2 and any(ctx.needs_input_grad[:3]):
-            y, pre8 = _gemm_pre8(x2, weight, bias, act)
-        else:
-            y = gemm_tn(x2, weight, bias, act)
-        if ctx.needs_input_grad[1]:
-            x8 = saved8._pack(x2)
+        need = ctx.needs_input_grad
+        y, x8, pre8 = _linear8_forward(x2, weight, bias, act, need[1], _ACT[act] == 2 and (need[0] or need[1] or need[2]))
         ctx.save_for_backward(weight, x8, pre8)
         ctx.x_dtype, ctx.bias_dtype = x.dtype, None if bias is None else bias.dtype
         ctx.in_shape = x.shape
@@ -190,14 +196,29 @@ def _linear8_backward(ctx, dy, d_alias):
     dz = dy.reshape(-1, n)
     if not dz.is_contiguous():
         dz = dz.contiguous()
-    want_bias = ctx.bias_dtype if ctx.needs_input_grad[2] else None
-    dz, db = saved8.act_bwd8(dz, pre8, want_bias)
-    dx = dw = None
-    if ctx.needs_input_grad[0]:
-        dx = _input_grad(dz, weight, d_alias).view(ctx.in_shape)
-    if ctx.needs_input_grad[1]:
-        dw = _weight_grad8(dz, saved8._unpack(x8, (dz.shape[0], k), ctx.x_dtype), weight.dtype).to(weight.dtype)
-    return dx, dw, db, None
+    want_dx, want_dw = ctx.needs_input_grad[:2]
+    want_db = ctx.bias_dtype if ctx.needs_input_grad[2] else None
+    m = dz.shape[0]
+    if not (_linear8_fits(dz, weight) and weight.dtype == ctx.x_dtype and want_db in (None, *saved8._DTYPES)):
+        dz, db = saved8.act_bwd8(dz, pre8, want_db)
+        dx = _input_grad(dz, weight, d_alias).view(ctx.in_shape) if want_dx else None
+        dw = None
+        if want_dw:
+            dw = _weight_grad8(dz, saved8._unpack(x8, (m, k), ctx.x_dtype), weight.dtype).to(weight.dtype)
+        return dx, dw, db, None
+    lib = base.K()
+    with base.device_of(dz):
+        into = _accumulator(d_alias, k) if want_dx else None
+        dx = (torch.empty(m, k, dtype=torch.bfloat16, device=dz.device) if into is None else into) if want_dx else None
+        dw = torch.empty(n, k, dtype=torch.bfloat16, device=dz.device) if want_dw else None
+        db = torch.empty(n, dtype=want_db, device=dz.device) if want_db is not None else None
+        need = lib.tipsk_linear8_bwd_ws(m, n, k, int(pre8 is not None), int(want_dw), int(db is not None))
+        ws = torch.empty(need, dtype=torch.uint8, device=dz.device) if need else None
+        base.check(lib.tipsk_linear8_bwd(dz.data_ptr(), weight.data_ptr(), base.ptr(x8), base.ptr(pre8), base.ptr(dx), base.ptr(dw),
+                                         base.ptr(db), 0 if db is None else base.code(db), base.ptr(ws), m, n, k, weight.stride(0),
+                                         int(into is not None), base.stream()), "linear8_bwd")
+    base.count_launches(3)
+    return None if dx is None else dx.view(ctx.in_shape), dw, db, None
 
 
 class _Linear8PassFn(torch.autograd.Function):
@@ -215,30 +236,29 @@ class _Linear8PassFn(torch.autograd.Function):
 
 
 def _weight_grad8(dz: torch.Tensor, x2: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """dz^T @ x2 for operands of any row count: `_weight_grad` where it reads both in place, and otherwise the CTA-pair GEMM,
-    whose tensor maps end where the rows do, or for narrow operands transposed copies with zeros up to whole 16 bytes."""
+    """dz^T @ x2 where the layer does not run as one call: `_weight_grad` where it reads both operands in place, and otherwise
+    transposed copies, whose rows are filled up with zeros to the whole 16 bytes that the GEMM reads."""
     m, n = dz.shape
     k = x2.shape[1]
     if not (dz.is_cuda and dz.dtype == x2.dtype == torch.bfloat16 and m) or (n % 64 == 0 and k % 64 == 0 and m >= 16):
         return _weight_grad(dz, x2, dtype)
-    if n >= 64 and k >= 64 and _supported(dz, x2) and n % 8 == 0 and k % 8 == 0:
-        dw = torch.empty(n, k, dtype=torch.bfloat16, device=dz.device)
-        if not _split(2, dz, x2, dw, None, None, n, k, m, 0, False):
-            base.check(base.K().tipsk_gemm_bf16_tt(dz.data_ptr(), x2.data_ptr(), dw.data_ptr(), n, k, m, n, k, k,
-                                                   base.stream()), "gemm_bf16_tt")
-        return dw
     pad = -m % 8
     return gemm_tn(F.pad(dz.t(), (0, pad)).contiguous(), F.pad(x2.t(), (0, pad)).contiguous())
 
 
+def _accumulator(d_alias: torch.Tensor | None, k: int) -> torch.Tensor | None:
+    """The gradient of another consumer of a layer's input as a matrix that the GEMM can add to."""
+    if d_alias is None:
+        return None
+    into = d_alias.reshape(-1, k)
+    if not (into.is_contiguous() and into.dtype == torch.bfloat16 and into.data_ptr() % 16 == 0):
+        into = into.contiguous()
+    return into
+
+
 def _input_grad(dz: torch.Tensor, weight: torch.Tensor, d_alias: torch.Tensor | None) -> torch.Tensor:
     """dz @ weight as [rows, k]; with `d_alias` (the gradient of another consumer of the input) added into it by the GEMM."""
-    into = None
-    if d_alias is not None:
-        into = d_alias.reshape(-1, weight.shape[1])
-        if not (into.is_contiguous() and into.dtype == torch.bfloat16 and into.data_ptr() % 16 == 0):
-            into = into.contiguous()
-    return gemm_nn(dz, weight, into=into)
+    return gemm_nn(dz, weight, into=_accumulator(d_alias, weight.shape[1]))
 
 
 def _linear_backward(ctx, dy, d_alias):

@@ -67,16 +67,16 @@ def _unpack_plain(buf: torch.Tensor, n: int, dtype) -> torch.Tensor:
     return torch.where(q == -128, float("nan"), q.float() * step).to(dtype)
 
 
-def _buffer(n: int, device):
-    """An int8 buffer for n values, and where its exponents start."""
-    at = _exponents_at(n)
-    return torch.empty(at - (-n // BLOCK), dtype=torch.int8, device=device), at
+def _buffer(n: int, device) -> torch.Tensor:
+    """An int8 buffer for the 8-bit form of n values."""
+    return torch.empty(_exponents_at(n) - (-n // BLOCK), dtype=torch.int8, device=device)
 
 
 def _pack(x: torch.Tensor) -> torch.Tensor:
     """The 8-bit form of a tensor as one int8 buffer: the values, and from _exponents_at on a step exponent per block."""
     n = x.numel()
-    buf, at = _buffer(n, x.device)
+    at = _exponents_at(n)
+    buf = _buffer(n, x.device)
     if not x.is_cuda:
         _pack_plain(x, buf)
     elif n:
