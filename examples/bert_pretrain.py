@@ -1,7 +1,8 @@
 """Data-parallel masked-language-model pre-training of a BERT-large-shaped encoder on synthetic tokens: tcgen05 GEMMs
 with fused bias / GELU epilogues, layer norms with the residual add inside, fused AdamW on flat buffers, gradient
 buckets reduced over NVLink while the backward pass is still running.  With --fused-update the optimizer step runs
-inside the allreduce kernel and every rank keeps 1/N of the AdamW state.  Needs CUDA.
+inside the allreduce kernel and every rank keeps 1/N of the AdamW state.  With --padded the sequences have different lengths and the
+attention skips the padding; with --save8 the linear layers keep their activations in 8 bits.  Needs CUDA.
 
     python -m torch.distributed.run --nproc-per-node 8 examples/bert_pretrain.py --steps 50 --fused-update
 """
@@ -29,6 +30,8 @@ def main():
     ap.add_argument("--warmup-steps", type=int, default=10)
     ap.add_argument("--fused-update", action="store_true")
     ap.add_argument("--checkpoint", default="", help="file that rank 0 writes at the end")
+    ap.add_argument("--save8", action="store_true", help="keep the linear layers' activations for the backward pass in 8 bits")
+    ap.add_argument("--padded", action="store_true", help="sequences of random length, padded to --seq")
     a = ap.parse_args()
     if not torch.cuda.is_available():
         raise SystemExit("this example needs a CUDA device")
@@ -36,12 +39,19 @@ def main():
     rank, size = tips.rank(), tips.size()
     dev = torch.device("cuda", torch.cuda.current_device())
     torch.manual_seed(1234)
-    model = bert_large(device=dev, layers=a.layers, max_seq=a.seq).train()
+    model = bert_large(device=dev, layers=a.layers, max_seq=a.seq, save8=a.save8).train()
     opt = tips.DistributedOptimizer(FusedAdamW(model.parameters(), lr=a.lr, weight_decay=0.01),
                                     fused_update=a.fused_update if size > 1 else None)
     tips.broadcast_parameters(model.state_dict(), root_rank=0, optimizer=opt)
     # three host batches in pinned memory, copied while the previous step computes
-    host = [tuple(t.pin_memory() for t in synthetic_mlm_batch(a.batch, a.seq, 30522, seed=31 * rank + i)) for i in range(3)]
+    host = []
+    for i in range(3):
+        ids, pos, labels = synthetic_mlm_batch(a.batch, a.seq, 30522, seed=31 * rank + i)
+        lengths = torch.full((a.batch,), a.seq)
+        if a.padded:
+            lengths = torch.randint(a.seq // 4, a.seq + 1, (a.batch,), generator=torch.Generator().manual_seed(31 * rank + i))
+            labels = labels.masked_fill(pos >= lengths[:, None], -100)  # masked positions in the padding do not count
+        host.append(tuple(t.pin_memory() for t in (ids, pos, labels, lengths)))
     copy_stream = torch.cuda.Stream()
     nxt = [t.to(dev, non_blocking=True) for t in host[0]]
     t0 = None
@@ -49,12 +59,12 @@ def main():
         if step == 5:
             torch.cuda.synchronize()
             t0 = time.time()
-        ids, pos, labels = nxt
+        ids, pos, labels, lengths = nxt
         with torch.cuda.stream(copy_stream):
             nxt = [t.to(dev, non_blocking=True) for t in host[(step + 1) % 3]]
         for g in opt.param_groups:                      # linear warm-up; the fused kernels read lr every step
             g["lr"] = a.lr * min(1.0, (step + 1) / max(1, a.warmup_steps))
-        loss = model.loss(ids, pos, labels)
+        loss = model.loss(ids, pos, labels, lengths=lengths if a.padded else None)
         loss.backward()
         opt.step()
         torch.cuda.current_stream().wait_stream(copy_stream)

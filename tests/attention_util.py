@@ -11,8 +11,9 @@ def reference(q, k, v, dout, causal=False, lengths=None, scale=None, store=None)
     With u the half step of `store` and t its smallest half step (underflow), to first order and with sums of absolute values:
         |P~ - P| <= u P + t                           O: (u P + t) |V| + u |O| + t
         D~ = dO . O~ with the stored O~               dD <= |dO| . bound(O)
-        dS~ = P (dP - D~) rounded                     e = u |dS| + t + P dD
-        dQ: scale e |K| + u |dQ| + t                  dK alike with e^T |Q|, dV: (u P + t)^T |dO| + u |dV| + t
+        dS~ = P (dP - D~) rounded                     e = u |dS| + t / f + P dD
+        dQ: scale e |K| + u |dQ| + t                  dK alike with e^T |Q|, dV: (u P + t / 2^10)^T |dO| + u |dV| + t
+    where fp16 holds the backward pass's P times 2^10 and dS times a power of two f with 2^14 <= f 2 d max|dO| max|V| < 2^15
     plus `slack` of the sums of absolute values for the accumulation in 32 bits (2^-24 per term, up to some thousand terms in
     no fixed order), exponentials (2^-22) and exponents (a score of up to 64 in units of log2, rounded, is off by 2^-18)."""
     b, s, h, d = q.shape
@@ -47,8 +48,11 @@ def reference(q, k, v, dout, causal=False, lengths=None, scale=None, store=None)
     pe = (u + slack) * p + t * valid
     oe = pe @ vd.abs() + u * out.abs() + t
     mag = p * (do.abs() @ vd.abs().mT + (do.abs() * out.abs()).sum(-1, keepdim=True))
-    e = u * ds.abs() + slack * mag + t * valid + p * (do.abs() * oe).sum(-1, keepdim=True)
-    bound = {"out": oe, "dq": e @ kd.abs() * scale, "dk": fold(e.mT @ qd.abs()) * scale, "dv": fold(pe.mT @ do.abs())}
+    most = 2 * d * do.abs().reshape(b, hk, -1).amax(-1) * vd.abs().reshape(b, hk, -1).amax(-1)
+    f = (2.0 ** 14 / most.clamp_min(1e-30)).repeat_interleave(h // hk, 1)[:, :, None, None]
+    e = u * ds.abs() + slack * mag + t / f * valid + p * (do.abs() * oe).sum(-1, keepdim=True)
+    pb = (u + slack) * p + t / 1024 * valid
+    bound = {"out": oe, "dq": e @ kd.abs() * scale, "dk": fold(e.mT @ qd.abs()) * scale, "dv": fold(pb.mT @ do.abs())}
     bound = {name: x.transpose(1, 2) for name, x in bound.items()}
     for name in ("dq", "dk", "dv"):
         bound[name] = bound[name] + u * want[name].abs() + t

@@ -25,8 +25,8 @@ def run(q, k, v, do, **kw):
 
 
 def status():
-    from tips_b200.ops import base
-    return base.K().tipsk_attention_status()
+    from tips_b200.ops.attention import attention_status
+    return attention_status()
 
 
 @pytest.mark.parametrize("causal", [False, True])
@@ -65,6 +65,23 @@ def test_scale_and_large_scores():
     """Scores of some hundred: the running maximum carries the row."""
     q, k, v, do = make(2, 400, 2, 2, 64, torch.bfloat16, seed=3, amp=2.0)
     check(run(q, k, v, do, scale=0.5, causal=True), *reference(q, k, v, do, True, scale=0.5))
+
+
+@pytest.mark.parametrize("of_do,of_v", [(1e-5, 1.0), (3e3, 1.0), (1.0, 500.0), (1e-4, 1e-3), (0.0, 1.0), (200.0, 200.0)])
+@pytest.mark.parametrize("d", [64, 96])
+def test_fp16_gradients_of_any_size(d, of_do, of_v):
+    """Gradients near fp16's smallest numbers, and products far beyond its largest, on their way to results within its range; one
+    of the heads that share a key head has far smaller gradients."""
+    q, k, v, do = make(2, 300, 4, 2, d, torch.float16, seed=21)
+    with torch.no_grad():
+        v.mul_(of_v)
+        do.mul_(of_do)
+        do[:, :, 1] *= 2.0 ** -6
+        k.mul_(min(1.0, 1.0 / (of_do * of_v + 1e-9)))  # results stay finite
+        q.mul_(min(1.0, 1.0 / (of_do * of_v + 1e-9)))
+    want, bound = reference(q, k, v, do)
+    assert max(float(x.abs().max()) for x in want.values()) < 6e4
+    check(run(q, k, v, do), want, bound)
 
 
 def test_rising_scores_rescale_the_output():

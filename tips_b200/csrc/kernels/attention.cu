@@ -60,10 +60,10 @@ struct AttnParams {
   int causal;
   float scale, c;       // c = scale * log2(e)
   float* lse;           // [b, h, sp]
-  float* delta;         // [2][b, h, sp]
+  float* delta;         // [2][b, h, sp], and for fp16 [2][b, hk]
   void *o, *dq, *dk, *dv;
-  const void* dout;
-  Strides so, sdo, sdq, sdk, sdv;
+  const void *dout, *v;
+  Strides so, sdo, sdq, sdk, sdv, sv;
 };
 
 struct AttnMaps {
@@ -813,16 +813,28 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 }
 
 // ---------------------------------------------------------------- backward
+// fp16 has few exponents: gradients are scaled by whole powers of two on their way through it.  P, at most 1, is held times 2^10,
+// so that the probabilities of long sequences stay clear of its smallest numbers; dS times 2^k, with k from the largest |dO| of the
+// heads that share a key and value head and the largest |V|: |dS| <= 2 d max|dO| max|V|, and 2^k times that is below 2^15.
+constexpr int kHalfP = 10;
+__device__ __forceinline__ float TwoTo(int k) { return __int_as_float((k + 127) << 23); }
+
 // D_i = dO_i . O_i, eight lanes per row.  A block takes 32 positions of eight heads: it reads runs of heads, which are neighbours
 // in a contiguous tensor, and writes runs of positions.  Writes [2][b, h, sp]: -L and -D, the addends as the main kernel uses them.
+// For fp16 further blocks read V, and the largest magnitudes go to [2][b, hk] behind that, cleared before.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ AttnParams p) {
   __shared__ float sums[8][33];
-  const int b = blockIdx.z, h0 = blockIdx.y * 8, len = SeqLen(p, b);
+  const int b = blockIdx.z, len = SeqLen(p, b), runs = TilesOf(p.h, 8);
   const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;
   const int h = (threadIdx.x >> 3) & 7, part = threadIdx.x & 7;
+  const bool values = !kBf16 && static_cast<int>(blockIdx.y) >= runs;
+  const int h0 = (blockIdx.y - (values ? runs : 0)) * 8, heads = values ? p.hk : p.h;
   const uint16_t* out  = static_cast<const uint16_t*>(p.o) + b * p.so.b + (h0 + h) * p.so.h + part * 8;
-  const uint16_t* grad = static_cast<const uint16_t*>(p.dout) + b * p.sdo.b + (h0 + h) * p.sdo.h + part * 8;
+  const uint16_t* grad = values ? static_cast<const uint16_t*>(p.v) + b * p.sv.b + (h0 + h) * p.sv.h + part * 8
+                                : static_cast<const uint16_t*>(p.dout) + b * p.sdo.b + (h0 + h) * p.sdo.h + part * 8;
+  const int64_t step = values ? p.sv.s : p.sdo.s;
+  uint32_t largest = 0;  // of the magnitudes that this thread has read, as fp32 bits
   for (int i0 = blockIdx.x * 32; i0 < p.sp; i0 += gridDim.x * 32) {
 #pragma unroll 4
     for (int t = 0; t < 8; ++t) {
@@ -830,14 +842,16 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (i < len && h0 + h < p.h && part * 8 + k * 64 < p.d) {
-          const uint4 x = *reinterpret_cast<const uint4*>(out + i * p.so.s + k * 64);
-          const uint4 y = *reinterpret_cast<const uint4*>(grad + i * p.sdo.s + k * 64);
+        if (i < len && h0 + h < heads && part * 8 + k * 64 < p.d) {
+          const uint4 y = *reinterpret_cast<const uint4*>(grad + i * step + k * 64);
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (!values) x = *reinterpret_cast<const uint4*>(out + i * p.so.s + k * 64);
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const float2 a = Unpack2<kBf16>(xs[v]), c = Unpack2<kBf16>(ys[v]);
             sum = fmaf(a.x, c.x, fmaf(a.y, c.y, sum));
+            if (!kBf16) largest = max(largest, max(__float_as_uint(c.x) & 0x7fffffffu, __float_as_uint(c.y) & 0x7fffffffu));
           }
         }
 #pragma unroll
@@ -846,13 +860,30 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
     }
     __syncthreads();
     const int hw = threadIdx.x >> 5, j = threadIdx.x & 31;
-    if (h0 + hw < p.h) {  // i0 + j < sp, a multiple of 32
+    if (!values && h0 + hw < p.h) {  // i0 + j < sp, a multiple of 32
       const int64_t at = (static_cast<int64_t>(b) * p.h + h0 + hw) * p.sp + i0 + j;
-      p.delta[at]         = -p.lse[at];
+      p.delta[at]         = (kBf16 ? 0.f : kHalfP) - p.lse[at];
       p.delta[plane + at] = -sums[hw][j];
     }
     __syncthreads();
   }
+  if (!kBf16) {
+#pragma unroll
+    for (int k = 4; k > 0; k >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, k));
+    if (part == 0 && h0 + h < heads && largest)  // a maximum does not depend on the order
+      atomicMax(reinterpret_cast<uint32_t*>(p.delta + 2 * plane) + (values ? p.b * p.hk : 0) + b * p.hk +
+                    (values ? h0 + h : (h0 + h) / (p.h / p.hk)),
+                largest);
+  }
+}
+
+// The k of a key and value head's dS.
+__device__ __forceinline__ int GradExponent(const AttnParams& p, int b, int hk) {
+  const float* most = p.delta + 2 * static_cast<int64_t>(p.b) * p.h * p.sp + b * p.hk + hk;
+  const uint32_t bits = __float_as_uint(2.f * p.d * most[0] * most[p.b * p.hk]);
+  if (bits == 0 || bits >= 0x7f800000u) return 0;  // no gradient, or one that is not finite anyway
+  const int k = 14 - (static_cast<int>(bits >> 23) - 127);
+  return k < -100 ? -100 : k > 100 ? 100 : k;
 }
 
 // A piece of work is one tile of 128 keys (kKeys) or queries (!kKeys), which stays; the tiles of the other side (units) stream
@@ -902,11 +933,13 @@ struct BwdCfg {
 struct BwdWords {  // what stands in a slot
   int b, head, x0, len, first, per, total;
   bool ragged, keys;  // a head's last unit has rows to clear; keys stay
+  int exponent;       // of the factor of dS, for fp16
   __device__ __forceinline__ explicit BwdWords(const int (&w)[8])
-      : b(w[0]), head(w[1]), x0(w[2]), len(w[3]), first(w[4]), per(w[5]), total(w[6]), ragged(w[7] & 1), keys(w[7] & 2) {}
+      : b(w[0]), head(w[1]), x0(w[2]), len(w[3]), first(w[4]), per(w[5]), total(w[6]), ragged(w[7] & 1), keys(w[7] & 2),
+        exponent((w[7] >> 8) - 128) {}
   // First the pieces of the keys, whose tiles stream past every query head of their group; causal: the tiles with the longest
   // streams first; otherwise neighbours share a head.
-  template <int kUnit>
+  template <int kUnit, bool kBf16>
   __device__ __forceinline__ static void Describe(const AttnParams& p, int index, int (&w)[8]) {
     const int tiles = p.sp / kTile, group = p.h / p.hk, key_pieces = tiles * p.b * p.hk;
     const bool keys = index < key_pieces;
@@ -927,6 +960,7 @@ struct BwdWords {  // what stands in a slot
     w[5] = last - first;
     w[6] = total;
     w[7] = (total > 0 && last == units && len < p.s && len % kUnit != 0 ? 1 : 0) | (keys ? 2 : 0);
+    if (!kBf16) w[7] |= (GradExponent(p, b, keys ? w[1] : w[1] / group) + 128) << 8;
   }
 };
 template <bool kKeys>
@@ -1103,7 +1137,7 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       row_d = Both(LoadShared(m.XRows(n) + (kTile + quarter * 32 + lane) * 4));
     }
   }
-  const F2 c2 = Both(p.c);
+  const F2 c2 = Both(p.c), grad2 = Both(kBf16 ? 1.f : TwoTo(w.exponent - kHalfP));
   int at = NS == 1 ? 0 : static_cast<int>((set ^ u0) & 1);  // unit within a head
   for (uint32_t u = u0 + at; u < u0 + w.total; u += NS, at += NS) {
     if (at >= w.per) at %= w.per;  // the group's next head
@@ -1166,8 +1200,13 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       if (kKeys) {
         LoadPairs(ls + kUnit * 4 + 8 * k, d0, d1);
       }
-      v[k]     = Pack2<kBf16>(Mul2(pr[k], Add2(Pair(s[2 * k], s[2 * k + 1]), d0)));
-      v[k + 1] = Pack2<kBf16>(Mul2(pr[k + 1], Add2(Pair(s[2 * k + 2], s[2 * k + 3]), d1)));
+      F2 g0 = Mul2(pr[k], Add2(Pair(s[2 * k], s[2 * k + 1]), d0)), g1 = Mul2(pr[k + 1], Add2(Pair(s[2 * k + 2], s[2 * k + 3]), d1));
+      if (!kBf16) {
+        g0 = Mul2(g0, grad2);
+        g1 = Mul2(g1, grad2);
+      }
+      v[k]     = Pack2<kBf16>(g0);
+      v[k + 1] = Pack2<kBf16>(g1);
     }
     TmemStore16(m.Dp(u) + lanes + col, v);
     TmemStoreWait();
@@ -1186,7 +1225,8 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       uint32_t o[kCols];
       if constexpr (kCols == 32) TmemLoad32(m.Acc(out) + lanes + c0, o);
       else TmemLoad16(m.Acc(out) + lanes + c0, o);
-      StageCols<kBf16, kCols>(m.X(n) + out * Cfg::kTileBytes, r, c0, o, out ? 1.f : p.scale, live);
+      StageCols<kBf16, kCols>(m.X(n) + out * Cfg::kTileBytes, r, c0, o,
+                              out ? (kBf16 ? 1.f : TwoTo(-kHalfP)) : kBf16 ? p.scale : p.scale * TwoTo(-w.exponent), live);
     }
     TcFenceBefore();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1258,7 +1298,7 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   };
   if (warp == kTmaWarp) {
     if (ElectOne()) {
-      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { BwdWords::Describe<Cfg::kUnit>(p, index, v); }, [&](const int (&v)[8]) {
+      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { BwdWords::Describe<Cfg::kUnit, kBf16>(p, index, v); }, [&](const int (&v)[8]) {
         return each(v, [&](const auto& w) { return w.total == 0 || BwdLoad(maps, p, m, w, u0, n); });
       });
       if (!ok) atomicExch(&g_attn_error, 5);
@@ -1345,7 +1385,8 @@ int CheckSizes(int b, int s, int h, int hk, int d, int dtype, float scale) {
   TIPSK_REQUIRE(b > 0 && s > 0 && h > 0 && hk > 0 && h % hk == 0, "attention: empty shape, or heads that kv_heads does not divide");
   TIPSK_REQUIRE(d > 0 && d <= 128 && d % 8 == 0, "attention: the head size must be a multiple of 8 up to 128");
   TIPSK_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), "attention: scale must be positive and finite");
-  TIPSK_REQUIRE(b <= 65535 && s <= (1 << 30) && h <= (1 << 18) &&
+  // a tile's stream past a group's heads has to end well within the kernels' bounded waits
+  TIPSK_REQUIRE(b <= 65535 && h <= (1 << 18) && static_cast<int64_t>(s) * (h / hk) <= (1 << 26) &&
                     static_cast<int64_t>(b) * (h + hk) * TilesOf(s, kTile) < (int64_t{1} << 31),
                 "attention: too many rows for one launch");
   return 0;
@@ -1381,7 +1422,12 @@ int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   int rc = AllowSmem(AttnBwdKernel<HD, kBf16>, BwdCfg<HD>::kSmemBytes, &done);
   if (rc) return rc;
-  AttnDeltaKernel<kBf16><<<dim3(std::min(p.sp / 32, 4096), TilesOf(p.h, 8), p.b), 256, 0, s>>>(p);
+  int runs = TilesOf(p.h, 8);
+  if (!kBf16) {
+    runs += TilesOf(p.hk, 8);
+    TIPSK_CUDA(cudaMemsetAsync(p.delta + 2 * static_cast<int64_t>(p.b) * p.h * p.sp, 0, static_cast<size_t>(2) * p.b * p.hk * 4, s));
+  }
+  AttnDeltaKernel<kBf16><<<dim3(std::min(p.sp / 32, 4096), runs, p.b), 256, 0, s>>>(p);
   TIPSK_LAUNCH_CHECK();
   const int grid = (p.sp / kTile) * p.b * (p.h + p.hk);
   AttnBwdKernel<HD, kBf16><<<grid, kThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
@@ -1439,6 +1485,8 @@ int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const vo
   p.lse   = const_cast<float*>(lse);
   p.delta = delta;
   p.dq = dq; p.dk = dk; p.dv = dv;
+  p.v  = v;
+  p.sv = sv;
   TIPSK_REQUIRE(Aligned(q, sq) && Aligned(k, sk) && Aligned(v, sv) && Aligned(out, p.so) && Aligned(dout, p.sdo) &&
                     Aligned(dq, p.sdq) && Aligned(dk, p.sdk) && Aligned(dv, p.sdv),
                 "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");

@@ -150,7 +150,7 @@ def _attention_bwd(dout, shape, q, k, v, out, lse, lengths, scale, causal, dq, d
     if not out.numel():
         return
     dout = _rows16(dout)
-    delta = torch.empty(2, *lse.shape, dtype=torch.float32, device=lse.device)
+    delta = torch.empty(2 * lse.numel() + 2 * b * hk, dtype=torch.float32, device=lse.device)
     with base.device_of(out):
         base.check(base.K().tipsk_attention_bwd(
             dout.data_ptr(), q[0], k[0], v[0], out.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq[0], dk[0], dv[0],
@@ -210,6 +210,11 @@ class _PackedOwnAttentionFn(torch.autograd.Function):
         return dqkv, None, None, None, None, None
 
 
+def attention_status() -> int:
+    """0 when no attention launch on the current device since the last call reported a bounded-wait timeout (synchronises)."""
+    return int(base.K().tipsk_attention_status())
+
+
 def _plain_attention(q, k, v, lengths, scale, causal):
     """The formula, for CPU tensors."""
     b, s, h, d = q.shape
@@ -245,7 +250,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
 
     On a GPU: bfloat16 or float16, d a multiple of 8 up to 128, any strides (inputs whose last axis is not contiguous, or
     whose rows do not start on 16 bytes, are copied).  The softmax is held in fp32; the probabilities, and their
-    gradient in the backward pass, are rounded to the inputs' type as operands of the products.  Gradients do not depend on
+    gradient in the backward pass, are rounded to the inputs' type as operands of the products (for float16 at a scale that keeps
+    them within its range).  Gradients do not depend on
     the order of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
     do not see it, as 0 * inf does in the formula.  `lengths` may not change between forward and backward."""
     for name, t in (("q", q), ("k", k), ("v", v)):

@@ -347,6 +347,8 @@ def linear_passthrough(x, weight, bias=None, act=None, save8=False):
 class Linear(nn.Module):
     """`save8`: keep the activations for the backward pass in 8 bits (see `linear`)."""
 
+    save8 = False
+
     def __init__(self, in_features, out_features, bias=True, act=None, save8=False):
         super().__init__()
         self.in_features, self.out_features, self.act, self.save8 = in_features, out_features, act, save8
