@@ -64,13 +64,23 @@ def test_the_library_refuses_before_it_reads():
                                        a["scale"], 0, None)
 
     for kw in (dict(d=0), dict(d=12), dict(d=136), dict(hk=3), dict(h=0), dict(hk=0), dict(b=0), dict(s=0), dict(dtype=0),
-               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=3e38), dict(s=1 << 30, b=1 << 10),
+               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=3e38), dict(s=1 << 30, b=1 << 10), dict(h=1 << 18, hk=1 << 18),
                dict(at=4100)):
         assert call(**kw) == -2, kw
     for i, x in ((1, 132), (3, 0), (8, -64), (11, 4)):
         bad = (ctypes.c_int64 * 12)(*strides)
         bad[i] = x
         assert call(strides=bad) == -2, (i, x)
+
+
+def test_types_on_the_cpu():
+    """64-bit inputs are computed in 64 bits; whole numbers are refused."""
+    torch.manual_seed(3)
+    q, k, v = (torch.randn(2, 7, n, 8, dtype=torch.float64, requires_grad=True) for n in (4, 2, 2))
+    n = torch.tensor([7, 3])
+    assert torch.autograd.gradcheck(lambda *t: attention(*t, causal=True, lengths=n), (q, k, v))
+    with pytest.raises(TypeError):
+        attention(*(torch.ones(1, 2, 1, 8, dtype=torch.int32),) * 3)
 
 
 def test_encoder_on_a_padded_batch():

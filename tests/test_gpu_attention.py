@@ -201,6 +201,78 @@ def test_infinities_in_valid_places_are_not_hidden():
     assert not got["dq"].isfinite().all()
 
 
+def test_scores_of_minus_infinity():
+    """Keys whose scores are -inf, as many as a whole tile holds, do not count, wherever they stand."""
+    from tips_b200.ops.attention import attention
+    for first in (True, False):
+        q, k, v, _ = make(2, 300, 4, 2, 64, torch.bfloat16, seed=13)
+        with torch.no_grad():
+            q[..., 0] = -1.0
+            k[..., 0] = 0.5
+            hidden = slice(0, 140) if first else slice(100, 300)
+            k[:, hidden, :, 0] = math.inf
+            got = attention(q, k, v)
+            seen = slice(140, 300) if first else slice(0, 100)
+            x = (q.double().transpose(1, 2) @ k[:, seen].double().transpose(1, 2).repeat_interleave(2, 1).mT) / 8
+            p, vd = torch.softmax(x, -1), v[:, seen].double().transpose(1, 2).repeat_interleave(2, 1)
+            want = (p @ vd).transpose(1, 2)
+            # the probabilities and the output are rounded once each; 2^-14 for what is held in 32 bits
+            bound = (2.0 ** -8 + 2.0 ** -14) * (p @ vd.abs()).transpose(1, 2) + 2.0 ** -8 * want.abs()
+        assert ((got.double() - want).abs() <= bound).all()
+
+
+def test_fp16_many_small_probabilities():
+    """One key takes nearly all of every row's weight; thousands of others, each 2^-26 of it, make up the output."""
+    from tips_b200.ops.attention import attention
+    s, d = 8192, 64
+    q, k, v = (torch.zeros(1, s, 1, d, device=DEV, dtype=torch.float16) for _ in range(3))
+    q[..., 0] = 1.0
+    k[:, 0, :, 0] = 18.0  # e^-18: 2^-25.97
+    v[:, 1:] = 1000.0
+    got = attention(q, k, v, scale=1.0).double()
+    p = math.exp(-18.0)
+    want = 1000.0 * (s - 1) * p / (1 + (s - 1) * p)
+    # a probability held times 2^7 is off by fp16's smallest half step, 2^-25, at most; a half step of the output; 2^-14 for 32 bits
+    assert float((got - want).abs().max()) <= 1000.0 * (s - 1) * 2.0 ** -32 + (2.0 ** -11 + 2.0 ** -14) * want
+
+
+def test_offsets_beyond_32_bits():
+    """Sequences of a batch that lie more than 2^31 elements apart, every tensor in one buffer of 4.3 GB."""
+    b, s, h, d = 2, 150, 2, 64
+    step = 2 ** 31 + 64
+    buf = torch.zeros(step + 4 * s * h * d, device=DEV, dtype=torch.bfloat16)
+    q, k, v, do = make(b, s, h, h, d, torch.bfloat16, seed=14)
+    far = [buf.as_strided((b, s, h, d), (step, h * d, d, 1), i * s * h * d) for i in range(4)]
+    for t, x in zip(far, (q, k, v, do)):
+        t.copy_(x.detach())
+    n = torch.tensor([150, 99], device=DEV)
+    want = run(q, k, v, do, lengths=n)
+    got = run(*(t.detach().requires_grad_() for t in far[:3]), far[3], lengths=n)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+
+
+def test_fp16_backward_in_a_graph():
+    """The largest magnitudes that scale fp16's gradients are found anew in every replay."""
+    from tips_b200.ops.attention import _attention_bwd, _attention_fwd, _view
+    shape = (2, 300, 4, 2, 64)
+    bufs = [t.detach().clone() for t in make(*shape, torch.float16, seed=15)]
+    views = [_view(t) for t in bufs[:3]]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = _attention_fwd(bufs[0], shape, *views, None, 0.125, True)
+        grads = [torch.empty_like(t) for t in bufs[:3]]
+        _attention_bwd(bufs[3], shape, *views, out, lse, None, 0.125, True, *(_view(t) for t in grads))
+    for amp in (100.0, 1e-3, 1.0):
+        for t, x in zip(bufs, make(*shape, torch.float16, seed=16)):
+            t.copy_(x.detach())
+        bufs[3].mul_(amp)
+        want = run(*(t.clone().requires_grad_() for t in bufs[:3]), bufs[3], causal=True)
+        g.replay()
+        for name, x in zip(("out", "dq", "dk", "dv"), (out, *grads)):
+            assert torch.equal(x, want[name]), (name, amp)
+
+
 def test_refusals_on_a_gpu():
     from tips_b200.ops.attention import attention, packed_attention
     q, k, v, _ = make(1, 16, 2, 2, 64, torch.bfloat16)

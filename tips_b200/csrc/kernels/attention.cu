@@ -43,6 +43,9 @@ constexpr int kWarps   = kSoftWarps + 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kFwdPoly = 4;  // forward, one pair of exponentials in so many by a polynomial
+// fp16 has few exponents: forward, probabilities are held times 2^7 (so up to 2^15, see the lag of the maximum), which keeps those
+// of the many small ones of a long row that 2^-25 of the largest would have lost.
+constexpr float kHalfShift = 7.f;
 
 __device__ int32_t g_attn_error;  // one per device
 
@@ -736,8 +739,9 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         float top = MaxNan(MaxNan(part[0], part[1], __uint_as_float(s[0][15])), MaxNan(part[2], part[3], __uint_as_float(s[0][31])),
                            MaxNan(__uint_as_float(s[1][15]), __uint_as_float(s[1][31])));
         top = MaxNan(top, other(top));
-        // a row without any key so far; and inf - inf: the row is NaN, as by the formula
-        if (top == -INFINITY) top = 0.f;
+        // a row whose scores are -inf so far: any finite reference below the scores to come; and inf - inf: the row is NaN, as by the
+        // formula
+        if (top == -INFINITY) top = -1e30f;
         else if (top == INFINITY) top = __uint_as_float(0x7fc00000u);
         // The exponents' reference may lag behind the maximum by up to 2^8: probabilities of up to 256 lose nothing in 16 bits,
         // and the output in TMEM is rescaled a few times per row instead of with every new maximum.
@@ -758,7 +762,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
             TmemStore16(to + g * 16, o);
           }
         }
-        const F2 nm = Both(-m * p.c);
+        const F2 nm = Both(fmaf(-m, p.c, kBf16 ? 0.f : kHalfShift));
         F2 sum[2];
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
@@ -804,7 +808,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
       pieces_done += w.total > 0;
       if ((!Cfg::kStaged || count == 0) && !live && row < p.s) StoreZeroRow(dst, half * (HD / 2), min(p.d, (half + 1) * (HD / 2)));
       if (half == 0 && row < p.sp)
-        p.lse[(static_cast<int64_t>(w.b) * p.h + w.h) * p.sp + row] = live ? fmaf(m, p.c, log2f(l)) : INFINITY;
+        p.lse[(static_cast<int64_t>(w.b) * p.h + w.h) * p.sp + row] = live ? fmaf(m, p.c, log2f(l) - (kBf16 ? 0.f : kHalfShift)) : INFINITY;
     }
   }
   TcFenceBefore();
@@ -1386,7 +1390,7 @@ int CheckSizes(int b, int s, int h, int hk, int d, int dtype, float scale) {
   TIPSK_REQUIRE(d > 0 && d <= 128 && d % 8 == 0, "attention: the head size must be a multiple of 8 up to 128");
   TIPSK_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), "attention: scale must be positive and finite");
   // a tile's stream past a group's heads has to end well within the kernels' bounded waits
-  TIPSK_REQUIRE(b <= 65535 && h <= (1 << 18) && static_cast<int64_t>(s) * (h / hk) <= (1 << 26) &&
+  TIPSK_REQUIRE(b <= 65535 && h <= (1 << 17) && static_cast<int64_t>(s) * (h / hk) <= (1 << 26) &&
                     static_cast<int64_t>(b) * (h + hk) * TilesOf(s, kTile) < (int64_t{1} << 31),
                 "attention: too many rows for one launch");
   return 0;

@@ -93,6 +93,8 @@ def _check_attention(t, s, h, hk, d, lengths, scale) -> float:
         raise ValueError(f"{h} heads cannot share {hk} key and value heads evenly")
     if d <= 0:
         raise ValueError("the head size must be positive")
+    if not t.dtype.is_floating_point:
+        raise TypeError(f"attention takes floating-point tensors, got {t.dtype}")
     _check_lengths(lengths, t.shape[0], t.device)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
@@ -219,7 +221,7 @@ def _plain_attention(q, k, v, lengths, scale, causal):
     """The formula, for CPU tensors."""
     b, s, h, d = q.shape
     group = h // k.shape[2]
-    qf, kf, vf = (t.float().transpose(1, 2) for t in (q, k, v))
+    qf, kf, vf = ((t if t.dtype == torch.float64 else t.float()).transpose(1, 2) for t in (q, k, v))
     kf, vf = kf.repeat_interleave(group, 1), vf.repeat_interleave(group, 1)
     pos = torch.arange(s, device=q.device)
     rows = torch.ones(b, s, dtype=torch.bool, device=q.device)
