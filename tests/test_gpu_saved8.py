@@ -163,6 +163,53 @@ def test_passthrough_and_dtypes():
             assert t.dtype == dtype and (t.double() - v.double()).norm() <= 2.0 ** -5 * v.double().norm()
 
 
+@pytest.mark.parametrize("save8", [False, True])
+def test_passthrough_of_a_sum_with_its_input(save8):
+    """The layer's output and its input's alias get one and the same gradient, which the input's is added into."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(6)
+    bf = torch.bfloat16
+    x, w, dy = (torch.randn(*s, generator=g, device=DEV).to(bf) for s in ((700, 256), (256, 256), (700, 256)))
+    x.requires_grad_()
+    w.requires_grad_()
+    y, alias = linear_passthrough(x, w, None, None, save8)
+    got = torch.autograd.grad(y + alias, (x, w), dy)
+    plain = torch.autograd.grad(linear(x, w, None, None, save8), (x, w), dy)
+    assert ((got[0].double() - plain[0].double() - dy.double()).abs()
+            <= 2.0 ** -8 * (plain[0].double().abs() + got[0].double().abs()) + 2.0 ** -12).all()
+    if save8:
+        assert torch.equal(got[1], plain[1])
+    else:
+        # without save8 the 700 products of an element are added in no fixed order, so that two runs may differ: each sum by
+        # 700 * 2^-24 of the sum of absolute values, and by a half step of bf16, 2^-8, when it is rounded
+        bound = 2.0 ** -8 * (got[1].double().abs() + plain[1].double().abs()) + 2 * 700 * 2.0 ** -24 * (dy.double().abs().t() @ x.detach().double().abs())
+        assert ((got[1].double() - plain[1].double()).abs() <= bound).all()
+
+
+def test_bias_of_another_type():
+    x, w = torch.randn(64, 128, device=DEV).to(torch.bfloat16), torch.randn(256, 128, device=DEV).to(torch.bfloat16)
+    dy = torch.randn(64, 256, device=DEV).to(torch.bfloat16)
+    for dtype in (torch.float32, torch.float64, torch.float16):
+        b = torch.randn(256, device=DEV).to(torch.bfloat16).to(dtype).requires_grad_()
+        (db,) = torch.autograd.grad(linear(x, w, b, None, save8=True), b, dy)
+        assert db.dtype == dtype
+        # sums of 64 addends in 32 bits, rounded to the bias's type
+        bound = 64 * 2.0 ** -24 * dy.double().abs().sum(0) + max(torch.finfo(dtype).eps, 2.0 ** -23) / 2 * dy.double().sum(0).abs()
+        assert ((db.double() - dy.double().sum(0)).abs() <= bound).all()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values: the last ones keep their places."""
+    n = 2 ** 31 + 2 ** 20 + 40
+    x = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    tail = torch.randn(2 ** 20 + 40, device=DEV).to(torch.bfloat16)
+    x[2 ** 31:] = tail
+    p, small = pack8(x), pack8(tail)
+    assert torch.equal(p.q[2 ** 31:], small.q) and torch.equal(p.e[2 ** 26:], small.e)
+    y = p.unpack()
+    assert torch.equal(y[2 ** 31:], small.unpack()) and not y[:2 ** 31:4097].any()
+
+
 def test_graph_and_stream():
     x = torch.randn(513, 96, device=DEV).to(torch.bfloat16)
     want = pack8(x).unpack()

@@ -208,7 +208,7 @@ def _linear8_backward(ctx, dy, d_alias):
         return dx, dw, db, None
     lib = base.K()
     with base.device_of(dz):
-        into = _accumulator(d_alias, k) if want_dx else None
+        into = _accumulator(d_alias, k, dz) if want_dx else None
         dx = (torch.empty(m, k, dtype=torch.bfloat16, device=dz.device) if into is None else into) if want_dx else None
         dw = torch.empty(n, k, dtype=torch.bfloat16, device=dz.device) if want_dw else None
         db = torch.empty(n, dtype=want_db, device=dz.device) if want_db is not None else None
@@ -217,7 +217,7 @@ def _linear8_backward(ctx, dy, d_alias):
         base.check(lib.tipsk_linear8_bwd(dz.data_ptr(), weight.data_ptr(), base.ptr(x8), base.ptr(pre8), base.ptr(dx), base.ptr(dw),
                                          base.ptr(db), 0 if db is None else base.code(db), base.ptr(ws), m, n, k, weight.stride(0),
                                          int(into is not None), base.stream()), "linear8_bwd")
-    base.count_launches(3)
+    base.count_launches(int(pre8 is not None or want_db is not None) + int(want_db is not None) + int(want_dx) + 2 * int(want_dw) - 1)
     return None if dx is None else dx.view(ctx.in_shape), dw, db, None
 
 
@@ -246,19 +246,20 @@ def _weight_grad8(dz: torch.Tensor, x2: torch.Tensor, dtype: torch.dtype) -> tor
     return gemm_tn(F.pad(dz.t(), (0, pad)).contiguous(), F.pad(x2.t(), (0, pad)).contiguous())
 
 
-def _accumulator(d_alias: torch.Tensor | None, k: int) -> torch.Tensor | None:
-    """The gradient of another consumer of a layer's input as a matrix that the GEMM can add to."""
+def _accumulator(d_alias: torch.Tensor | None, k: int, dz: torch.Tensor) -> torch.Tensor | None:
+    """The gradient of another consumer of a layer's input as a matrix that the GEMM can add to, while it reads dz."""
     if d_alias is None:
         return None
     into = d_alias.reshape(-1, k)
-    if not (into.is_contiguous() and into.dtype == torch.bfloat16 and into.data_ptr() % 16 == 0):
-        into = into.contiguous()
+    # a sum of the layer's output and its input hands both the same gradient
+    if not (into.is_contiguous() and into.data_ptr() % 16 == 0) or into.untyped_storage().data_ptr() == dz.untyped_storage().data_ptr():
+        into = into.clone(memory_format=torch.contiguous_format)
     return into
 
 
 def _input_grad(dz: torch.Tensor, weight: torch.Tensor, d_alias: torch.Tensor | None) -> torch.Tensor:
     """dz @ weight as [rows, k]; with `d_alias` (the gradient of another consumer of the input) added into it by the GEMM."""
-    return gemm_nn(dz, weight, into=_accumulator(d_alias, weight.shape[1]))
+    return gemm_nn(dz, weight, into=_accumulator(d_alias, weight.shape[1], dz))
 
 
 def _linear_backward(ctx, dy, d_alias):

@@ -141,6 +141,9 @@ def act_bwd8(dy: torch.Tensor, z: torch.Tensor | None, bias_dtype=None):
     rows, cols = dy.shape
     if z is None and bias_dtype is None:
         return dy, None
+    if bias_dtype not in (None, *_DTYPES):
+        dz, db = act_bwd8(dy, z, torch.float32)
+        return dz, db.to(bias_dtype)
     if dy.is_cuda and cols % 8 == 0 and dy.dtype in _DTYPES and rows and cols:
         dy = _aligned(dy)
         lib = base.K()
