@@ -2,7 +2,7 @@
 little larger than L2, holds well under a GB on the device and exits by itself in seconds.
 
     python -m tips_b200.bench.profile_case {bn_fwd,bn_bwd,gemm,gemm_gelu,gemm_wgrad,ln,sgd,ps_pull,ps_push,conv1x1,conv3x3,conv_dgrad,conv_wgrad,
-                                           adam,ln_bwd,ln_bwd_groups,bias_act_bwd,softmax_xent,maxpool}
+                                           adam,ln_bwd,ln_bwd_groups,bias_act_bwd,softmax_xent,maxpool,attention,attention_gqa,linear8}
 """
 from __future__ import annotations
 
@@ -102,6 +102,21 @@ def main(argv=None):
         dy = torch.randn_like(y)
         for _ in range(reps):
             torch.autograd.grad(y, x, dy, retain_graph=True)
+    elif case in ("attention", "attention_gqa"):
+        from tips_b200.ops.attention import attention
+        # the encoder's heads; a causal batch with few key heads of 128
+        b, s, h, hk, d = (32, 512, 16, 16, 64) if case == "attention" else (2, 4096, 16, 4, 128)
+        q, k, v = (torch.randn(b, s, n, d, device=dev).to(torch.bfloat16).requires_grad_() for n in (h, hk, hk))
+        dy = torch.randn_like(q)
+        for _ in range(reps):
+            torch.autograd.grad(attention(q, k, v, causal=case == "attention_gqa"), (q, k, v), dy)
+    elif case == "linear8":
+        from tips_b200.ops.linear import Linear
+        lin = Linear(1024, 4096, act="gelu", save8=True).to(dev).to(torch.bfloat16)
+        x = torch.randn(16384, 1024, device=dev).to(torch.bfloat16).requires_grad_()
+        dy = torch.randn(16384, 4096, device=dev).to(torch.bfloat16)
+        for _ in range(reps):
+            torch.autograd.grad(lin(x), (x, lin.weight, lin.bias), dy)
     elif case == "softmax_xent":
         from tips_b200.ops.pointwise import softmax_cross_entropy
         logits = torch.randn(16384, 30528, device=dev).to(torch.bfloat16).requires_grad_()

@@ -42,7 +42,7 @@ constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kClearWarp = kSo
 constexpr int kWarps   = kSoftWarps + 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFwdPoly = 4;  // forward, one pair of exponentials in so many by a polynomial
+constexpr int kFwdPoly = 8;  // forward, one pair of exponentials in so many by a polynomial (one in 4: 57 us where 8 takes 54, none: 56)
 // fp16 has few exponents: forward, probabilities are held times 2^7 (so up to 2^15, see the lag of the maximum), which keeps those
 // of the many small ones of a long row that 2^-25 of the largest would have lost.
 constexpr float kHalfShift = 7.f;
@@ -187,17 +187,6 @@ __device__ __forceinline__ void TmemStore16(uint32_t taddr, const uint32_t (&r)[
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void TmemStore32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
 __device__ __forceinline__ void TmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -367,7 +356,6 @@ __device__ __forceinline__ float LoadShared(uint32_t at) {
 __device__ __forceinline__ void LoadPairs(uint32_t at, F2& a, F2& b) {
   asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(a.v), "=l"(b.v) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void StoreShared(uint32_t at, float x) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory"); }
 
 // ---------------------------------------------------------------- blocks that take one piece of work after another
 // The grid has a block per piece of work, but a block that is done takes the place of one that has not started yet (cluster
@@ -383,10 +371,10 @@ struct Pieces {
   __device__ __forceinline__ uint32_t Full(uint32_t turn) const { return at + 80 + (turn & 1) * 8; }
   __device__ __forceinline__ uint32_t Empty(uint32_t turn) const { return at + 96 + (turn & 1) * 8; }
   __device__ __forceinline__ uint32_t Answered() const { return at + 112; }
-  __device__ __forceinline__ void Init() const {
+  __device__ __forceinline__ void Init(int followers) const {  // warps that follow
     for (int i = 0; i < 2; ++i) {
       BarInit(Full(i), 1);
-      BarInit(Empty(i), kWarps - 1);
+      BarInit(Empty(i), followers);
     }
     BarInit(Answered(), 1);
   }
@@ -464,59 +452,65 @@ struct WaiterOf {
 using Waiter     = WaiterOf<false>;
 using IdleWaiter = WaiterOf<true>;
 
-__device__ __forceinline__ void AllocTmem(uint32_t slot) {  // by one warp, all columns
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(512u) : "memory");
+__device__ __forceinline__ void AllocTmem(uint32_t slot, uint32_t columns) {  // by one warp
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t AlignedSmem(const uint8_t* raw) { return (SmemAddr(raw) + 1023) & ~1023u; }
 
 // ---------------------------------------------------------------- forward
-// A piece of work is 256 queries of one head as two tiles, past which the keys and values stream: while the warps of one tile
-// compute probabilities, the tensor cores run the products of the other.  Eight softmax warps per tile; a thread has half
-// of a row, 64 scores, and exchanges its maximum with the thread that has the other half.  (With a whole row per thread
-// there is nothing to exchange, but two warps per scheduler leave most issue slots empty: 32 x 512, 16 heads of 64: 87 us.)
-// With 64 output columns per tile, TMEM has room for the probabilities beside the scores, so that the next scores are
-// computed as soon as these have been read; with 128 they take the scores' place.
+// A piece of work is 256 queries of one head as two tiles, past which the keys and values stream in units.  A thread has a row of a
+// tile, so maximum and sum need no exchange; a tile's probabilities take the place of its scores, and the next scores follow the
+// product with V, so that one barrier tells that both are done.  While one tile waits for its products, others compute:
+// with 64 output columns, units of 64 keys leave TMEM for two blocks per SM, four tiles that run apart from each other
+// (32 x 512, 16 heads of 64: 54 us; one block with units of 128, next scores beside the probabilities, and a row shared
+// by two threads: 61).  With 128 one block fills TMEM, units have 128 keys, and one warp issues the products of both tiles, which
+// makes them take turns (8192, 16 heads of 128 that share 4, causal: 231 us = 1190 TFLOP/s; with a warp for each tile 248).
+// Bound by the exponentials (with 64 columns the unit for them is busy four fifths of the time) and by issue slots beside them.
 template <int HD>
 struct FwdCfg {
   static constexpr int kTileBytes = (HD / 64) * kBoxBytes;
-  static constexpr int kStages    = HD == 64 ? 8 : 4;  // tiles of K and V in turn
+  static constexpr int kUnit      = HD == 64 ? 64 : 128;
+  static constexpr int kUnitBytes = kUnit * HD * 2;
+  static constexpr int kBlocks    = HD == 64 ? 2 : 1;  // per SM
+  static constexpr int kStages    = 4;  // units of K and V in turn
   static constexpr int kQBufs     = HD == 64 ? 2 : 1;  // queries of this piece of work and the next
-  static constexpr bool kOwnP     = HD == 64;          // probabilities beside the scores
   // outputs leave by TMA through the place of their queries, where the next piece has another
   static constexpr bool kStaged   = kQBufs == 2;
-  // shared memory: queries [kQBufs][2], the ring, maxima [2 turns][2 tiles][2 halves][128 rows], barriers
+  static constexpr int kSoftWarps = 8;                 // four for each tile
+  static constexpr int kTmaWarp   = kSoftWarps, kMmaWarp = kSoftWarps + 1;
+  static constexpr int kThreads   = (kSoftWarps + 2) * 32;
+  static constexpr int kColumns   = 2 * (kUnit + HD);  // of TMEM: scores and output of either tile
+  // shared memory: queries [kQBufs][2], the ring, barriers
   static constexpr int kRing      = 2 * kQBufs * kTileBytes;
-  static constexpr int kMax       = kRing + kStages * kTileBytes;
-  static constexpr int kNext      = kMax + 2 * 2 * 2 * kTile * 4;
+  static constexpr int kNext      = kRing + kStages * kUnitBytes;
   static constexpr int kFull      = kNext + Pieces::kBytes;
-  static constexpr int kEmpty     = kFull + 8 * kStages;   // both MMA warps are done with a tile of K or V
-  static constexpr int kRaw       = kEmpty + 8 * kStages;  // a tile of V has arrived and has rows to clear before it counts as full
-  static constexpr int kQFull     = kRaw + 8 * kStages;
+  static constexpr int kEmpty     = kFull + 8 * kStages;
+  static constexpr int kQFull     = kEmpty + 8 * kStages;
   static constexpr int kQEmpty    = kQFull + 8 * kQBufs;
-  static constexpr int kSFull     = kQEmpty + 8 * kQBufs;  // [2] scores of a tile are in TMEM
-  static constexpr int kSFree     = kSFull + 16;           // [2] they have been read
-  static constexpr int kPFull     = kSFree + 16;           // [2] the probabilities are in TMEM
-  static constexpr int kOFull     = kPFull + 16;           // [2] their product with V has completed
-  static constexpr int kOStaged   = kOFull + 16;           // [2] a piece's output is in shared memory
+  static constexpr int kSFull     = kQEmpty + 8 * kQBufs;  // [2] scores of a tile are in TMEM, and the products before are done
+  static constexpr int kPFull     = kSFull + 16;           // [2] the probabilities are in TMEM
+  static constexpr int kOFull     = kPFull + 16;           // [2] a piece's output is complete
+  static constexpr int kOStaged   = kOFull + 16;           // [2] it is in shared memory
   static constexpr int kTmemSlot  = kOStaged + 16;
   static constexpr int kSmemBytes = kTmemSlot + 16 + 1024;
 };
 
 struct FwdPiece {
   int b, h, q0, len, count0, count1, total;
-  bool ragged;  // the last tile of V has rows to clear
+  bool ragged;  // the last unit of V has rows to clear
   __device__ __forceinline__ explicit FwdPiece(const int (&w)[8])
       : b(w[0]), h(w[1]), q0(w[2]), len(w[3]), count0(w[4]), count1(w[5]), total(w[6]), ragged(w[7] != 0) {}
+  template <int kUnit>
   __device__ __forceinline__ static void Describe(const AttnParams& p, int index, int (&w)[8]) {
     // causal: the tiles with the most keys first; otherwise neighbours share a head's keys
     const int blocks_q = TilesOf(p.s, 2 * kTile), heads = p.b * p.h;
     const int qb = p.causal ? blocks_q - 1 - index / heads : index % blocks_q;
     const int bh = p.causal ? index % heads : index / blocks_q;
-    const int b = bh / p.h, q0 = qb * 2 * kTile, len = SeqLen(p, b), tiles = TilesOf(len, kTile);
-    // key tiles of either query tile
-    const int count0 = q0 >= len ? 0 : p.causal ? min(tiles, q0 / kTile + 1) : tiles;
-    const int count1 = q0 + kTile >= len ? 0 : p.causal ? min(tiles, q0 / kTile + 2) : tiles;
+    const int b = bh / p.h, q0 = qb * 2 * kTile, len = SeqLen(p, b), units = TilesOf(len, kUnit);
+    // units of keys of either query tile
+    const int count0 = q0 >= len ? 0 : p.causal ? min(units, (q0 + kTile) / kUnit) : units;
+    const int count1 = q0 + kTile >= len ? 0 : p.causal ? min(units, (q0 + 2 * kTile) / kUnit) : units;
     const int total = max(count0, count1);
     w[0] = b;
     w[1] = bh % p.h;
@@ -525,60 +519,56 @@ struct FwdPiece {
     w[4] = count0;
     w[5] = count1;
     w[6] = total;
-    w[7] = total > 0 && total == tiles && len < p.s && len % kTile != 0;
+    w[7] = total > 0 && total == units && len < p.s && len % kUnit != 0;
   }
 };
 
 template <int HD, bool kBf16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(FwdCfg<HD>::kThreads, FwdCfg<HD>::kBlocks)
 AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   using Cfg = FwdCfg<HD>;
-  constexpr int S = Cfg::kStages, QB = Cfg::kQBufs;
+  constexpr int S = Cfg::kStages, QB = Cfg::kQBufs, kUnit = Cfg::kUnit;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = AlignedSmem(smem_raw);
   const Pieces pieces{base + Cfg::kNext};
   auto full = [&](uint32_t k) { return base + Cfg::kFull + k % S * 8; };
   auto empty = [&](uint32_t k) { return base + Cfg::kEmpty + k % S * 8; };
-  auto raw = [&](uint32_t k) { return base + Cfg::kRaw + k % S * 8; };
   auto q_full = [&](uint32_t n) { return base + Cfg::kQFull + n % QB * 8; };
   auto q_empty = [&](uint32_t n) { return base + Cfg::kQEmpty + n % QB * 8; };
   auto q_tile = [&](uint32_t n, int i) { return base + (n % QB * 2 + i) * Cfg::kTileBytes; };
-  auto tile = [&](uint32_t k) { return base + Cfg::kRing + k % S * Cfg::kTileBytes; };
+  auto unit = [&](uint32_t k) { return base + Cfg::kRing + k % S * Cfg::kUnitBytes; };
 
   const int warp = Uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    pieces.Init();
+    pieces.Init(Cfg::kSoftWarps + 1);
     for (int i = 0; i < S; ++i) {
       BarInit(full(i), 1);
-      BarInit(empty(i), 2);
-      BarInit(raw(i), 1);
+      BarInit(empty(i), 1);
     }
     for (int i = 0; i < QB; ++i) {
       BarInit(q_full(i), 1);
-      BarInit(q_empty(i), Cfg::kStaged ? 4 : 2);  // both MMA warps are done with their tile, and have stored what took its place
+      BarInit(q_empty(i), Cfg::kStaged ? 2 : 1);  // the products are done with the queries, and what took their place is stored
     }
     for (int i = 0; i < 2; ++i) {
       BarInit(base + Cfg::kSFull + i * 8, 1);
-      BarInit(base + Cfg::kSFree + i * 8, kSoftWarps / 2);
-      BarInit(base + Cfg::kPFull + i * 8, kSoftWarps / 2);
+      BarInit(base + Cfg::kPFull + i * 8, Cfg::kSoftWarps / 2);
       BarInit(base + Cfg::kOFull + i * 8, 1);
-      BarInit(base + Cfg::kOStaged + i * 8, kSoftWarps / 2);
+      BarInit(base + Cfg::kOStaged + i * 8, Cfg::kSoftWarps / 2);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) AllocTmem(base + Cfg::kTmemSlot);
+  if (warp == Cfg::kMmaWarp) AllocTmem(base + Cfg::kTmemSlot, Cfg::kColumns);
   TcFenceBefore();
   __syncthreads();
   TcFenceAfter();
   const uint32_t tmem = Uniform(__float_as_uint(LoadShared(base + Cfg::kTmemSlot)));
-  // columns: scores of either tile, either output, and in what is left either tile's probabilities, or those in the scores' place
-  const uint32_t t_s = tmem, t_o = tmem + 256;
+  const uint32_t t_s = tmem, t_o = tmem + 2 * kUnit;  // scores of either tile, in their place the probabilities; either output
 
-  int words[8];
-  if (warp == kTmaWarp) {
+  int words[8] = {};
+  if (warp == Cfg::kTmaWarp) {
     if (ElectOne()) {
-      uint32_t e = 0, n = 0;  // tiles of K and V, and pieces with any, so far
-      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { FwdPiece::Describe(p, index, v); }, [&](const int (&v)[8]) {
+      uint32_t e = 0, n = 0;  // units of K and V, and pieces with any, so far
+      const bool ok = pieces.Lead([&](int index, int (&v)[8]) { FwdPiece::Describe<kUnit>(p, index, v); }, [&](const int (&v)[8]) {
         const FwdPiece w(v);
         if (w.total == 0) return true;
         if (!BarWaitOne(q_empty(n), (n / QB) ^ 1)) return false;
@@ -589,156 +579,120 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         const int hk = w.h / (p.h / p.hk);
         for (int k = 0; k < 2 * w.total; ++k, ++e) {
           if (!BarWaitOne(empty(e), (e / S) ^ 1)) return false;
-          const uint32_t bar = w.ragged && k == 2 * w.total - 1 ? raw(e) : full(e);
-          BarExpect(bar, Cfg::kTileBytes);
-          TmaLoadTile<HD, kTile, kTile>(tile(e), k & 1 ? &maps.v : &maps.k, (k >> 1) * kTile, hk, w.b, bar);
+          BarExpect(full(e), Cfg::kUnitBytes);
+          TmaLoadTile<HD, kUnit, kUnit>(unit(e), k & 1 ? &maps.v : &maps.k, (k >> 1) * kUnit, hk, w.b, full(e));
         }
         return true;
       });
       if (!ok) atomicExch(&g_attn_error, 1);
     }
-  } else if (warp == kClearWarp) {
-    uint32_t e = 0, uses = 0;  // bit st: parity of the next use of raw[st]
-    IdleWaiter wait(2);
-    for (uint32_t turn = 0; pieces.Take<true>(turn, words); ++turn) {
-      const FwdPiece w(words);
-      e += 2 * w.total;
-      if (w.ragged) {
-        const uint32_t st = (e - 1) % S;
-        if (wait(raw(st), uses >> st)) {
-          ClearRows<kTile>(tile(st), HD / 64, w.len % kTile);
-          if (lane == 0) BarArrive(full(st));
-        }
-        uses ^= 1u << st;
-      }
-    }
-  } else if (warp >= kMmaWarp) {
-    const int i = warp - kMmaWarp;  // query tile
+  } else if (warp == Cfg::kMmaWarp) {
     const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-    const uint32_t ts = t_s + i * 128, to = t_o + i * HD, tp = Cfg::kOwnP ? tmem + 384 + i * 64 : ts;
-    uint32_t e = 0, n = 0, done = 0, freed = 0;  // tiles of probabilities, of scores that were read, so far
+    uint32_t e = 0, n = 0, done[2] = {0, 0}, staged[2] = {0, 0};  // done, staged: units and pieces of a tile so far
     Waiter wait(3);
-    const uint32_t s_full = base + Cfg::kSFull + i * 8, s_free = base + Cfg::kSFree + i * 8, p_full = base + Cfg::kPFull + i * 8,
-                   o_full = base + Cfg::kOFull + i * 8;
-    auto entry = [&](uint32_t k) { return wait(full(k), k / S); };
-    // The output of an earlier piece is stored when this piece's scores are on their way.
-    uint32_t owed = 0, stored = 0;  // pieces whose store is owed (at most one), pieces stored with any output
-    int owed_b = 0, owed_h = 0, owed_row = 0;
-    bool owed_any = false;
+    auto s_full = [&](int i) { return base + Cfg::kSFull + i * 8; };
+    // The output of an earlier piece is stored when this piece's first scores are on their way.
+    FwdPiece owed(words);
+    owed.total = 0;
     auto settle = [&] {
-      if (!Cfg::kStaged || owed == 0) return;
-      if (owed_any && !wait(base + Cfg::kOStaged + i * 8, stored)) return;
+      if (!Cfg::kStaged || owed.total == 0) return;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if ((i ? owed.count1 : owed.count0) == 0) continue;
+        if (!wait(base + Cfg::kOStaged + i * 8, staged[i]++)) return;
+        if (ElectOne()) TmaStoreTile<HD>(q_tile(n - 1, i), &maps.out, owed.q0 + i * kTile, owed.h, owed.b);
+      }
       if (ElectOne()) {
-        if (owed_any) {
-          TmaStoreTile<HD>(q_tile(n - 1, i), &maps.out, owed_row, owed_h, owed_b);
-          StoresRead();
-        }
+        StoresRead();
         BarArrive(q_empty(n - 1));
       }
       __syncwarp();
-      stored += owed_any;
-      owed = 0;
+      owed.total = 0;
     };
     for (uint32_t turn = 0; pieces.Take<false>(turn, words); ++turn) {
       const FwdPiece w(words);
-      const int mine = i ? w.count1 : w.count0;
-      if (w.total > 0 && wait.ok) {
-        const uint32_t q_addr = q_tile(n, i);
-        auto scores = [&](int j) {  // of key tile j, if it is one of this query tile's; hands on its keys
-          if (j < mine) {
-            IssueScores<kBf16, HD, kTile>(ts, q_addr, tile(e + 2 * j), ksteps);
-            BarCommit(s_full);
-          }
-          BarCommit(empty(e + 2 * j));
-          if (j + 1 == max(mine, 1)) BarCommit(q_empty(n));
-        };
-        if (wait(q_full(n), n / QB) && entry(e) && ElectOne()) scores(0);
-        settle();
-        for (int j = 0; j < w.total && wait.ok; ++j) {  // a tile with fewer keys than the other hands on the rest
-          const uint32_t ev = e + 2 * j + 1;
-          if (j + 1 < w.total && !entry(ev + 1)) break;
-          if (Cfg::kOwnP && j + 1 < w.total) {
-            if (j + 1 < mine && !wait(s_free, freed++)) break;
-            if (ElectOne()) scores(j + 1);
-          }
-          if (!entry(ev)) break;
-          if (j < mine && !wait(p_full, done)) break;
-          if (ElectOne()) {
-            if (j < mine) {
-              IssueFromTmem<kBf16, kTile, Cfg::kOwnP ? kTile : kTile / 2>(to, tp, tile(ev), n_out, j > 0);
-              BarCommit(o_full);
-            }
-            BarCommit(empty(ev));
-            // in the place of the probabilities: products complete in the order of their issue
-            if (!Cfg::kOwnP && j + 1 < w.total) scores(j + 1);
-          }
-          done += j < mine;
-        }
-        e += 2 * w.total;
-        ++n;
-        owed     = 1;
-        owed_any = mine > 0;
-        owed_b   = w.b;
-        owed_h   = w.h;
-        owed_row = w.q0 + i * kTile;
+      if (w.total == 0 || !wait.ok) continue;
+      const int count[2] = {w.count0, w.count1};
+      auto scores = [&](int i, int j) {  // tile i, unit j
+        IssueScores<kBf16, HD, kUnit>(t_s + i * kUnit, q_tile(n, i), unit(e + 2 * j), ksteps);
+        BarCommit(s_full(i));
+      };
+      auto entry = [&](uint32_t k) { return wait(full(k), k / S); };
+      if (wait(q_full(n), n / QB) && entry(e) && ElectOne()) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (count[i] > 0) scores(i, 0);
+        BarCommit(empty(e));
+        if (w.total == 1) BarCommit(q_empty(n));
       }
+      __syncwarp();
+      settle();
+      for (int j = 0; j < w.total && wait.ok; ++j) {
+        const uint32_t ev = e + 2 * j + 1;
+        if (!entry(ev)) break;
+        if (w.ragged && j + 1 == w.total) ClearRows<kUnit>(unit(ev), HD / 64, w.len % kUnit);
+        if (j + 1 < w.total && !entry(ev + 1)) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (j >= count[i] || !wait(base + Cfg::kPFull + i * 8, done[i]++)) continue;
+          if (ElectOne()) {
+            IssueFromTmem<kBf16, kUnit, kUnit>(t_o + i * HD, t_s + i * kUnit, unit(ev), n_out, j > 0);
+            if (j + 1 < count[i]) scores(i, j + 1);  // products complete in the order of their issue
+            else BarCommit(base + Cfg::kOFull + i * 8);
+          }
+          __syncwarp();
+        }
+        if (!wait.ok) break;
+        if (ElectOne()) {
+          BarCommit(empty(ev));
+          if (j + 1 < w.total) BarCommit(empty(ev + 1));
+          if (j + 2 == w.total) BarCommit(q_empty(n));
+        }
+        __syncwarp();
+      }
+      e += 2 * w.total;
+      ++n;
+      owed = w;
     }
     if (wait.ok) settle();
     if (Cfg::kStaged && ElectOne()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
-    const int i = warp >> 3, half = (warp >> 2) & 1;  // query tile; columns [64 half, 64 half + 64) of the scores
-    const int quarter = warp & 3;                     // TMEM lanes that this warp may access
+    const int i = warp >> 2, quarter = warp & 3;  // query tile, TMEM lanes that this warp may access
     const int r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t ts = t_s + lanes + i * 128 + half * 64, to = t_o + lanes + i * HD + half * (HD / 2);
-    const uint32_t tp = Cfg::kOwnP ? tmem + 384 + lanes + i * 64 + half * 32 : ts;
-    const int pair_bar = 1 + i * 4 + quarter;         // the two warps that share these rows
+    const uint32_t ts = t_s + lanes + i * kUnit, to = t_o + lanes + i * HD;
     const F2 c2 = Both(p.c);
-    const uint32_t s_full = base + Cfg::kSFull + i * 8, s_free = base + Cfg::kSFree + i * 8, p_full = base + Cfg::kPFull + i * 8,
-                   o_full = base + Cfg::kOFull + i * 8;
-    uint32_t done = 0, swaps = 0, pieces_done = 0;
+    const uint32_t s_full = base + Cfg::kSFull + i * 8, p_full = base + Cfg::kPFull + i * 8;
+    uint32_t done = 0, pieces_done = 0, outputs = 0;
     Waiter wait(4);
-    // this thread's value and the one of the thread with the other half of the row
-    auto other = [&](float mine) {
-      const uint32_t at = base + Cfg::kMax + (((swaps++ & 1) * 4 + i * 2) * kTile + r) * 4;
-      StoreShared(at + half * (kTile * 4), mine);
-      NamedBarSync(pair_bar, 64);
-      return LoadShared(at + (half ^ 1) * (kTile * 4));
-    };
     for (uint32_t turn = 0; pieces.Take<false>(turn, words); ++turn) {
       const FwdPiece w(words);
       const int row = w.q0 + i * kTile + r, count = i ? w.count1 : w.count0;
-      float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and this half's sum
+      float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and the sum
       for (int j = 0; j < count; ++j, ++done) {
-        wait(s_full, done);  // on a failure the values are void, but every thread keeps meeting its barriers
-        uint32_t s[2][32];
-        TmemLoad32Async(ts, s[0]);
-        TmemLoad32Async(ts + 32, s[1]);
-        TmemLoadWait(s[0]);
-        TmemLoadWait(s[1]);
-        if (Cfg::kOwnP && j + 1 < count) {
-          TcFenceBefore();
-          __syncwarp();
-          if (lane == 0) BarArrive(s_free);
-        }
-        const int kv0 = j * kTile;
-        if (kv0 + kTile > w.len || (p.causal && kv0 + kTile - 1 > w.q0 + i * kTile)) {
-          const int limit = (p.causal ? min(w.len, row + 1) : w.len) - kv0 - half * 64;
+        if (!wait(s_full, done)) break;
+        uint32_t s[kUnit / 32][32];
 #pragma unroll
-          for (int k = 0; k < 64; ++k)
+        for (int g = 0; g < kUnit / 32; ++g) TmemLoad32Async(ts + g * 32, s[g]);
+#pragma unroll
+        for (int g = 0; g < kUnit / 32; ++g) TmemLoadWait(s[g]);
+        const int kv0 = j * kUnit;
+        if (kv0 + kUnit > w.len || (p.causal && kv0 + kUnit - 1 > w.q0 + i * kTile)) {
+          const int limit = (p.causal ? min(w.len, row + 1) : w.len) - kv0;
+#pragma unroll
+          for (int k = 0; k < kUnit; ++k)
             if (k >= limit) s[k >> 5][k & 31] = 0xff800000u;  // -inf
         }
         float part[4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) part[u] = __uint_as_float(s[u >> 1][(u & 1) * 16]);
+        for (int u = 0; u < 4; ++u) {
+          constexpr int kRun = kUnit / 4;
+          auto at = [&](int k) { return __uint_as_float(s[(u * kRun + k) >> 5][(u * kRun + k) & 31]); };
+          part[u] = MaxNan(at(0), at(1));
 #pragma unroll
-        for (int k = 1; k < 15; k += 2)
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            part[u] = MaxNan(part[u], __uint_as_float(s[u >> 1][(u & 1) * 16 + k]), __uint_as_float(s[u >> 1][(u & 1) * 16 + k + 1]));
-        float top = MaxNan(MaxNan(part[0], part[1], __uint_as_float(s[0][15])), MaxNan(part[2], part[3], __uint_as_float(s[0][31])),
-                           MaxNan(__uint_as_float(s[1][15]), __uint_as_float(s[1][31])));
-        top = MaxNan(top, other(top));
+          for (int k = 2; k < kRun; k += 2) part[u] = MaxNan(part[u], at(k), at(k + 1));
+        }
+        float top = MaxNan(MaxNan(part[0], part[1], part[2]), part[3]);
         // a row whose scores are -inf so far: any finite reference below the scores to come; and inf - inf: the row is NaN, as by the
         // formula
         if (top == -INFINITY) top = -1e30f;
@@ -748,13 +702,12 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         if (j == 0) {
           m = top;
         } else if (__any_sync(0xffffffffu, !((top - m) * p.c <= 8.f))) {
-          wait(o_full, done - 1);
           const float up = MaxNan(top, m);
           const float f  = Exp2((m - up) * p.c);
           m = up;
           l *= f;
 #pragma unroll 1
-          for (int g = 0; g < HD / 32; ++g) {
+          for (int g = 0; g < HD / 16; ++g) {  // the products before these scores are done
             uint32_t o[16];
             TmemLoad16(to + g * 16, o);
 #pragma unroll
@@ -765,7 +718,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         const F2 nm = Both(fmaf(-m, p.c, kBf16 ? 0.f : kHalfShift));
         F2 sum[2];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < kUnit / 32; ++g) {
           uint32_t v[16];
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
@@ -773,9 +726,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
             sum[k & 1] = g == 0 && k < 2 ? x : Add2(sum[k & 1], x);
             v[k] = Pack2<kBf16>(x);
           }
-          // the last product has read the probabilities before these
-          if (Cfg::kOwnP && g == 0 && j > 0) wait(o_full, done - 1);
-          TmemStore16(tp + g * 16, v);
+          TmemStore16(ts + g * 16, v);
         }
         const float2 both = SplitF2(Add2(sum[0], sum[1]));
         l += both.x + both.y;
@@ -787,16 +738,14 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
       const bool live = row < w.len;
       uint16_t* dst = static_cast<uint16_t*>(p.o) + w.b * p.so.b + row * p.so.s + w.h * p.so.h;
       if (count > 0) {
-        l += other(l);
-        wait(o_full, done - 1);
+        wait(base + Cfg::kOFull + i * 8, outputs++);
         const float inv = 1.f / l;
-        const int c0 = half * (HD / 2);
 #pragma unroll
-        for (int g = 0; g < HD / 64; ++g) {
+        for (int g = 0; g < HD / 32; ++g) {
           uint32_t o[32];
           TmemLoad32(to + g * 32, o);
-          if (Cfg::kStaged) StageCols<kBf16, 32>(q_tile(pieces_done, i), r, c0 + g * 32, o, inv, live);
-          else if (live && wait.ok) StoreCols<kBf16, 32>(dst, c0 + g * 32, p.d, o, inv);
+          if (Cfg::kStaged) StageCols<kBf16, 32>(q_tile(pieces_done, i), r, g * 32, o, inv, live);
+          else if (live && wait.ok) StoreCols<kBf16, 32>(dst, g * 32, p.d, o, inv);
         }
         TcFenceBefore();
         if (Cfg::kStaged) {
@@ -806,14 +755,15 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         }
       }
       pieces_done += w.total > 0;
-      if ((!Cfg::kStaged || count == 0) && !live && row < p.s) StoreZeroRow(dst, half * (HD / 2), min(p.d, (half + 1) * (HD / 2)));
-      if (half == 0 && row < p.sp)
+      if ((!Cfg::kStaged || count == 0) && !live && row < p.s) StoreZeroRow(dst, 0, p.d);
+      if (row < p.sp)
         p.lse[(static_cast<int64_t>(w.b) * p.h + w.h) * p.sp + row] = live ? fmaf(m, p.c, log2f(l) - (kBf16 ? 0.f : kHalfShift)) : INFINITY;
     }
   }
   TcFenceBefore();
   __syncthreads();
-  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (warp == Cfg::kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(static_cast<uint32_t>(Cfg::kColumns)) : "memory");
 }
 
 // ---------------------------------------------------------------- backward
@@ -1256,7 +1206,7 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   const Pieces pieces{m.base + Cfg::kNext};
   const int warp = Uniform(threadIdx.x >> 5);
   if (threadIdx.x == 0) {
-    pieces.Init();
+    pieces.Init(kWarps - 1);
     for (int i = 0; i < Cfg::kStages; ++i) {
       BarInit(m.Full(i), 1);
       BarInit(m.Empty(i), 2);  // both MMA warps
@@ -1279,7 +1229,7 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     BarInit(m.base + Cfg::kAccFree, kSoftWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) AllocTmem(m.base + Cfg::kTmemSlot);
+  if (warp == kMmaWarp) AllocTmem(m.base + Cfg::kTmemSlot, 512);
   TcFenceBefore();
   __syncthreads();
   TcFenceAfter();
@@ -1416,7 +1366,7 @@ int LaunchFwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   int rc = AllowSmem(AttnFwdKernel<HD, kBf16>, FwdCfg<HD>::kSmemBytes, &done);
   if (rc) return rc;
   const int grid = TilesOf(p.s, 2 * kTile) * p.b * p.h;
-  AttnFwdKernel<HD, kBf16><<<grid, kThreads, FwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  AttnFwdKernel<HD, kBf16><<<grid, FwdCfg<HD>::kThreads, FwdCfg<HD>::kSmemBytes, s>>>(maps, p);
   TIPSK_LAUNCH_CHECK();
   return 0;
 }
@@ -1462,8 +1412,9 @@ int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, 
   TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.so), "attention: strides must be positive");
   AttnMaps maps;
   if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, kTile))) return rc;
-  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, kTile))) return rc;
-  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, kTile))) return rc;
+  const int unit = d <= 64 ? FwdCfg<64>::kUnit : FwdCfg<128>::kUnit;
+  if ((rc = HeadMap(&maps.k, k, dtype, b, s, hk, d, sk, unit))) return rc;
+  if ((rc = HeadMap(&maps.v, v, dtype, b, s, hk, d, sv, unit))) return rc;
   if ((rc = HeadMap(&maps.out, out, dtype, b, s, h, d, p.so, kTile))) return rc;
   maps.dout = maps.dq = maps.dk = maps.dv = maps.q;  // not used
   cudaStream_t st = static_cast<cudaStream_t>(stream);
