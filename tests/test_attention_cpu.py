@@ -60,7 +60,7 @@ def test_the_library_refuses_before_it_reads():
 
     def call(at=4096, strides=strides, **kw):
         a = {**ok, **kw}
-        return lib.tipsk_attention_fwd(at, at, at, at, at, None, 0, a["b"], a["s"], a["h"], a["hk"], a["d"], a["dtype"], strides,
+        return lib.tipsk_attention_fwd(at, at, at, at, at, None, None, 0, a["b"], a["s"], a["h"], a["hk"], a["d"], a["dtype"], strides,
                                        a["scale"], 0, None)
 
     for kw in (dict(d=0), dict(d=12), dict(d=136), dict(hk=3), dict(h=0), dict(hk=0), dict(b=0), dict(s=0), dict(dtype=0),

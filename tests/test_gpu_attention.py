@@ -84,6 +84,21 @@ def test_fp16_gradients_of_any_size(d, of_do, of_v):
     check(run(q, k, v, do), want, bound)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("s,d", [(5, 64), (48, 40), (130, 128)])
+def test_short_rows_lose_nothing_in_their_difference(s, d, dtype):
+    """dP - D is small where rows are short.  Of the two roundings that a gradient dQ or dK cannot do without, of dS and of the
+    result, each leaves u sqrt(1/3 * 3/(8 ln 2)) = 0.425 u in the 2-norm (uniform over half a step, magnitudes spread evenly over an
+    octave): together 0.60 u, and 0.64 u allows for the sample.  The rounding of O by itself would leave as much again in the shortest."""
+    q, k, v, do = make(8, s, 16, 8, d, dtype, seed=31)
+    got = run(q, k, v, do, causal=True)
+    want, _ = reference(q, k, v, do, True)
+    u = torch.finfo(dtype).eps / 2
+    for name in ("dq", "dk"):
+        off = float((got[name].double() - want[name]).norm() / want[name].norm())
+        assert off <= 0.64 * u, (name, off / u)
+
+
 def test_rising_scores_rescale_the_output():
     """Every key tile raises the maximum of every row."""
     q, k, v, do = make(1, 700, 2, 1, 64, torch.bfloat16, seed=4)

@@ -4,6 +4,9 @@
 //   S = scale Q K^T,  L_i = log sum_j exp S_ij,  P = exp(S - L) where valid and 0 elsewhere,  O = P V
 //   dV = P^T dO,  dP = dO V^T,  D_i = dO_i . O_i,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
 //
+// D is a difference's other half: in short rows the rounding of O to 16 bits would show in it (a causal batch of 48 positions: dQ off by
+// 2.6e-3 where everything else leaves 2.4e-3).  There the forward pass also leaves what the rounding dropped, in 8 bits, for D.
+//
 // Nothing of size s x s reaches memory: the forward pass keeps a running maximum and sum per row and leaves L, the backward
 // pass computes P again from S and L.  Exponentials are taken to base 2 (scale and log2 e in one factor), L is kept in
 // units of log2.  Rows that the mask leaves empty (i >= len) get O = 0, L = +inf, and gradients of 0.
@@ -64,6 +67,7 @@ struct AttnParams {
   float scale, c;       // c = scale * log2(e)
   float* lse;           // [b, h, sp]
   float* delta;         // [2][b, h, sp], and for fp16 [2][b, hk]
+  uint8_t* rest;        // [b, s, h, d]: what rounding dropped of O, times RestScale, as e5m2; null: not kept
   void *o, *dq, *dk, *dv;
   const void *dout, *v;
   Strides so, sdo, sdq, sdk, sdv, sv;
@@ -261,6 +265,31 @@ __device__ __forceinline__ void StoreCols(uint16_t* row, int col0, int d, const 
     v.w = Pack2<kBf16>(__uint_as_float(acc[g * 8 + 6]) * factor, __uint_as_float(acc[g * 8 + 7]) * factor);
     *reinterpret_cast<uint4*>(row + col0 + g * 8) = v;
   }
+}
+// What the rounding of O to 16 bits drops is at most 2^-9 |O| (bf16) or 2^-12 |O|; e5m2 has 3 bits of it between 2^-14 and 2^15.
+template <bool kBf16>
+__device__ __forceinline__ constexpr float RestScale() { return kBf16 ? 256.f : 2048.f; }
+template <bool kBf16, int kCols>
+__device__ __forceinline__ void StoreRest(uint8_t* row, int col0, int d, const uint32_t (&acc)[kCols], float factor) {
+#pragma unroll
+  for (int g = 0; g < kCols / 8; ++g) {
+    if (col0 + g * 8 >= d) break;
+    uint32_t r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a = __uint_as_float(acc[g * 8 + 2 * k]) * factor, b = __uint_as_float(acc[g * 8 + 2 * k + 1]) * factor;
+      const float2 kept = Unpack2<kBf16>(Pack2<kBf16>(a, b));
+      uint16_t pair;
+      asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(pair) : "f"((b - kept.y) * RestScale<kBf16>()), "f"((a - kept.x) * RestScale<kBf16>()));
+      r[k] = pair;
+    }
+    *reinterpret_cast<uint2*>(row + col0 + g * 8) = make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
+  }
+}
+__device__ __forceinline__ float2 UnpackE5m2(uint32_t pair) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(pair)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 // The same of a row into a staged tile, whose boxes of 64 columns and 128 rows have the swizzled layout that a TMA store reads;
 // rows that are not live are zero.
@@ -746,6 +775,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
           TmemLoad32(to + g * 32, o);
           if (Cfg::kStaged) StageCols<kBf16, 32>(q_tile(pieces_done, i), r, g * 32, o, inv, live);
           else if (live && wait.ok) StoreCols<kBf16, 32>(dst, g * 32, p.d, o, inv);
+          if (p.rest && live && wait.ok) StoreRest<kBf16, 32>(p.rest + ((static_cast<int64_t>(w.b) * p.s + row) * p.h + w.h) * p.d, g * 32, p.d, o, inv);
         }
         TcFenceBefore();
         if (Cfg::kStaged) {
@@ -773,7 +803,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
 constexpr int kHalfP = 10;
 __device__ __forceinline__ float TwoTo(int k) { return __int_as_float((k + 127) << 23); }
 
-// D_i = dO_i . O_i, eight lanes per row.  A block takes 32 positions of eight heads: it reads runs of heads, which are neighbours
+// D_i = dO_i . O_i, with what rounding dropped of O, eight lanes per row.  A block takes 32 positions of eight heads: it reads runs of heads, which are neighbours
 // in a contiguous tensor, and writes runs of positions.  Writes [2][b, h, sp]: -L and -D, the addends as the main kernel uses them.
 // For fp16 further blocks read V, and the largest magnitudes go to [2][b, hk] behind that, cleared before.
 template <bool kBf16>
@@ -799,12 +829,16 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
         if (i < len && h0 + h < heads && part * 8 + k * 64 < p.d) {
           const uint4 y = *reinterpret_cast<const uint4*>(grad + i * step + k * 64);
           uint4 x = make_uint4(0, 0, 0, 0);
-          if (!values) x = *reinterpret_cast<const uint4*>(out + i * p.so.s + k * 64);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+          uint2 z = make_uint2(0, 0);
+          if (!values) {
+            x = *reinterpret_cast<const uint4*>(out + i * p.so.s + k * 64);
+            if (p.rest) z = *reinterpret_cast<const uint2*>(p.rest + ((static_cast<int64_t>(b) * p.s + i) * p.h + h0 + h) * p.d + part * 8 + k * 64);
+          }
+          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.x >> 16, z.y, z.y >> 16};
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const float2 a = Unpack2<kBf16>(xs[v]), c = Unpack2<kBf16>(ys[v]);
-            sum = fmaf(a.x, c.x, fmaf(a.y, c.y, sum));
+            const float2 a = Unpack2<kBf16>(xs[v]), c = Unpack2<kBf16>(ys[v]), e = UnpackE5m2(zs[v]);
+            sum = fmaf(fmaf(e.x, 1 / RestScale<kBf16>(), a.x), c.x, fmaf(fmaf(e.y, 1 / RestScale<kBf16>(), a.y), c.y, sum));
             if (!kBf16) largest = max(largest, max(__float_as_uint(c.x) & 0x7fffffffu, __float_as_uint(c.y) & 0x7fffffffu));
           }
         }
@@ -1396,8 +1430,9 @@ using namespace tipsk;
 
 extern "C" {
 
-/* O = softmax(scale Q K^T + mask) V and L.  host_strides: q, k, v, out. */
-int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const void* lengths, int len64,
+/* O = softmax(scale Q K^T + mask) V and L [b, h, s rounded up to 128].  rest (optional): [b, s, h, d] bytes, what the
+ * rounding of O dropped, for the backward pass to take.  host_strides: q, k, v, out. */
+int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const void* lengths, int len64,
                         int b, int s, int h, int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal,
                         void* stream) {
   int rc = CheckSizes(b, s, h, hk, d, dtype, scale);
@@ -1405,10 +1440,12 @@ int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, 
   const Strides sq = Take(host_strides, 0), sk = Take(host_strides, 1), sv = Take(host_strides, 2);
   AttnParams p = MakeParams(lengths, len64, b, s, h, hk, d, scale, causal);
   p.so  = Take(host_strides, 3);
-  p.o   = out;
-  p.lse = lse;
+  p.o    = out;
+  p.lse  = lse;
+  p.rest = static_cast<uint8_t*>(rest);
   TIPSK_REQUIRE(Aligned(q, sq) && Aligned(k, sk) && Aligned(v, sv) && Aligned(out, p.so),
                 "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");
+  TIPSK_REQUIRE(reinterpret_cast<uintptr_t>(rest) % 8 == 0, "attention: rest must be 8-byte aligned");
   TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.so), "attention: strides must be positive");
   AttnMaps maps;
   if ((rc = HeadMap(&maps.q, q, dtype, b, s, h, d, sq, kTile))) return rc;
@@ -1422,9 +1459,9 @@ int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, 
   return d <= 64 ? LaunchFwd<64, false>(maps, p, st) : LaunchFwd<128, false>(maps, p, st);
 }
 
-/* Gradients from dO, the inputs, O and L of the forward pass.  host_strides: q, k, v, out, dout, dq, dk, dv. */
+/* Gradients from dO, the inputs, O, L and (optional) rest of the forward pass.  host_strides: q, k, v, out, dout, dq, dk, dv. */
 int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
-                        float* delta, void* dq, void* dk, void* dv, const void* lengths, int len64, int b, int s, int h,
+                        const void* rest, float* delta, void* dq, void* dk, void* dv, const void* lengths, int len64, int b, int s, int h,
                         int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal, void* stream) {
   int rc = CheckSizes(b, s, h, hk, d, dtype, scale);
   if (rc) return rc;
@@ -1439,14 +1476,16 @@ int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const vo
   p.dout  = dout;
   p.lse   = const_cast<float*>(lse);
   p.delta = delta;
+  p.rest  = static_cast<uint8_t*>(const_cast<void*>(rest));
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.v  = v;
   p.sv = sv;
   TIPSK_REQUIRE(Aligned(q, sq) && Aligned(k, sk) && Aligned(v, sv) && Aligned(out, p.so) && Aligned(dout, p.sdo) &&
                     Aligned(dq, p.sdq) && Aligned(dk, p.sdk) && Aligned(dv, p.sdv),
                 "attention: tensors must be 16-byte aligned with strides of whole 16 bytes");
-  TIPSK_REQUIRE(reinterpret_cast<uintptr_t>(lse) % 16 == 0 && reinterpret_cast<uintptr_t>(delta) % 16 == 0,
-                "attention: lse and delta must be 16-byte aligned");
+  TIPSK_REQUIRE(reinterpret_cast<uintptr_t>(lse) % 16 == 0 && reinterpret_cast<uintptr_t>(delta) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(rest) % 8 == 0,
+                "attention: lse and delta must be 16-byte aligned, rest 8-byte aligned");
   TIPSK_REQUIRE(Mappable(sq) && Mappable(sk) && Mappable(sv) && Mappable(p.sdo) && Mappable(p.sdq) && Mappable(p.sdk) &&
                     Mappable(p.sdv),
                 "attention: strides must be positive");

@@ -232,10 +232,10 @@ int tipsk_gemm_status(void);
  * multiples of 8; the last axis is contiguous.  lengths: [b] int32 (len64 = 0) or int64, or null: positions from a
  * sequence's length on neither count nor receive anything but zeros.  lse: fp32 [b, h, s rounded up to 128]; delta: a
  * workspace of twice that and 2 b hk values more. ---- */
-int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const void* lengths, int len64,
+int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const void* lengths, int len64,
                         int b, int s, int h, int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal,
                         void* stream);
-int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* rest,
                         float* delta, void* dq, void* dk, void* dv, const void* lengths, int len64, int b, int s, int h,
                         int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal, void* stream);
 int tipsk_attention_status(void);

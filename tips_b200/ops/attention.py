@@ -132,30 +132,47 @@ def _strides(*views):
     return base.i64_array([x for _, st in views for x in st])
 
 
-def _attention_fwd(like, shape, q, k, v, lengths, scale, causal):
-    """(out, lse) for the views q, k, v of CUDA tensors like `like`; shape = (b, s, h, hk, d)."""
+def _lse_bytes(shape) -> int:
+    b, s, h, _, _ = shape
+    return b * h * (-(-s // 128) * 128) * 4
+
+
+def _keeps_rest(shape, causal) -> bool:
+    """Whether a forward pass keeps what the rounding of its output drops.  It shows in dQ and dK where rows are short (16 positions,
+    causal, bf16: they are off by 2.8e-3 without and 2.4e-3 with it; from 512 keys a row on 2.4e-3 either way), and costs
+    more than it is worth where they are not (32 x 512, 16 heads of 64, forward: 54 us without, 66 with it)."""
+    return shape[1] < (1024 if causal else 512)
+
+
+def _attention_fwd(like, shape, q, k, v, lengths, scale, causal, grad=True):
+    """(out, stats) for the views q, k, v of CUDA tensors like `like`; shape = (b, s, h, hk, d).  `stats`: bytes of the rows'
+    log-sums and, for a backward pass to come, what rounding dropped of `out` where it is kept."""
     b, s, h, hk, d = shape
     out = torch.empty(b, s, h, d, dtype=like.dtype, device=like.device)
-    lse = torch.empty(b, h, -(-s // 128) * 128, dtype=torch.float32, device=like.device)
+    at = _lse_bytes(shape)
+    keep = grad and _keeps_rest(shape, causal)
+    stats = torch.empty(at + b * s * h * d if keep else at, dtype=torch.uint8, device=like.device)
     if out.numel():
         with base.device_of(like):
             base.check(base.K().tipsk_attention_fwd(
-                q[0], k[0], v[0], out.data_ptr(), lse.data_ptr(), base.ptr(lengths),
+                q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if keep else None, base.ptr(lengths),
                 int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(like),
                 _strides(q, k, v, _view(out)), scale, int(causal), base.stream()), "attention_fwd")
-    return out, lse
+    return out, stats
 
 
-def _attention_bwd(dout, shape, q, k, v, out, lse, lengths, scale, causal, dq, dk, dv):
+def _attention_bwd(dout, shape, q, k, v, out, stats, lengths, scale, causal, dq, dk, dv):
     """Writes the gradients into the views dq, dk, dv."""
     b, s, h, hk, d = shape
     if not out.numel():
         return
     dout = _rows16(dout)
-    delta = torch.empty(2 * lse.numel() + 2 * b * hk, dtype=torch.float32, device=lse.device)
+    at = _lse_bytes(shape)
+    delta = torch.empty(at // 2 + 2 * b * hk, dtype=torch.float32, device=out.device)
     with base.device_of(out):
         base.check(base.K().tipsk_attention_bwd(
-            dout.data_ptr(), q[0], k[0], v[0], out.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq[0], dk[0], dv[0],
+            dout.data_ptr(), q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if _keeps_rest(shape, causal) else None,
+            delta.data_ptr(), dq[0], dk[0], dv[0],
             base.ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(out),
             _strides(q, k, v, _view(out), _view(dout), dq, dk, dv), scale, int(causal), base.stream()), "attention_bwd")
     base.count_launches(1)
@@ -163,24 +180,24 @@ def _attention_bwd(dout, shape, q, k, v, out, lse, lengths, scale, causal, dq, d
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, lengths, scale, causal):
+    def forward(ctx, q, k, v, lengths, scale, causal, grad):
         shape = (*q.shape[:3], k.shape[2], q.shape[3])
         q, k, v = _rows16(q), _rows16(k), _rows16(v)
-        out, lse = _attention_fwd(q, shape, _view(q), _view(k), _view(v), lengths, scale, causal)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        out, stats = _attention_fwd(q, shape, _view(q), _view(k), _view(v), lengths, scale, causal, grad)
+        ctx.save_for_backward(q, k, v, out, stats, lengths)
         ctx.meta = (shape, scale, causal)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, lengths = ctx.saved_tensors
+        q, k, v, out, stats, lengths = ctx.saved_tensors
         shape, scale, causal = ctx.meta
         # a saved-tensor hook may have changed the layout
-        q, k, v, out, lse = _rows16(q), _rows16(k), _rows16(v), _rows16(out), lse.contiguous()
+        q, k, v, out, stats = _rows16(q), _rows16(k), _rows16(v), _rows16(out), _packed16(stats)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _attention_bwd(dout, shape, _view(q), _view(k), _view(v), out, lse, lengths, scale, causal, _view(dq), _view(dk), _view(dv))
-        return dq, dk, dv, None, None, None
+        _attention_bwd(dout, shape, _view(q), _view(k), _view(v), out, stats, lengths, scale, causal, _view(dq), _view(dk), _view(dv))
+        return dq, dk, dv, None, None, None, None
 
 
 def _packed16(t: torch.Tensor) -> torch.Tensor:
@@ -190,26 +207,26 @@ def _packed16(t: torch.Tensor) -> torch.Tensor:
 
 class _PackedOwnAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, h, hk, lengths, scale, causal):
+    def forward(ctx, qkv, h, hk, lengths, scale, causal, grad):
         qkv = _packed16(qkv)
         b, s, width = qkv.shape
         shape = (b, s, h, hk, width // (h + 2 * hk))
-        out, lse = _attention_fwd(qkv, shape, *_packed_views(qkv, h, hk, shape[4]), lengths, scale, causal)
-        ctx.save_for_backward(qkv, out, lse, lengths)
+        out, stats = _attention_fwd(qkv, shape, *_packed_views(qkv, h, hk, shape[4]), lengths, scale, causal, grad)
+        ctx.save_for_backward(qkv, out, stats, lengths)
         ctx.meta = (shape, scale, causal)
         return out.view(b, s, h * shape[4])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        qkv, out, lse, lengths = ctx.saved_tensors
+        qkv, out, stats, lengths = ctx.saved_tensors
         shape, scale, causal = ctx.meta
         _, _, h, hk, d = shape
-        qkv, out, lse = _packed16(qkv), _rows16(out), lse.contiguous()
+        qkv, out, stats = _packed16(qkv), _rows16(out), _packed16(stats)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _attention_bwd(dy.reshape(out.shape), shape, *_packed_views(qkv, h, hk, d), out, lse, lengths, scale, causal,
+        _attention_bwd(dy.reshape(out.shape), shape, *_packed_views(qkv, h, hk, d), out, stats, lengths, scale, causal,
                        *_packed_views(dqkv, h, hk, d))
-        return dqkv, None, None, None, None, None
+        return dqkv, None, None, None, None, None, None
 
 
 def attention_status() -> int:
@@ -269,7 +286,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
         return _plain_attention(q, k, v, lengths, scale, causal)
     if lengths is not None:
         lengths = lengths.contiguous()
-    return _AttentionFn.apply(q, k, v, lengths, scale, bool(causal))
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    return _AttentionFn.apply(q, k, v, lengths, scale, bool(causal), grad)
 
 
 def packed_attention(qkv: torch.Tensor, heads: int, causal: bool = False, kv_heads: int | None = None,
@@ -289,7 +307,7 @@ def packed_attention(qkv: torch.Tensor, heads: int, causal: bool = False, kv_hea
             return _plain_attention(*x.split([heads, hk, hk], 2), lengths, scale, causal).reshape(b, s, -1)
         if lengths is not None:
             lengths = lengths.contiguous()
-        return _PackedOwnAttentionFn.apply(qkv, heads, hk, lengths, scale, bool(causal))
+        return _PackedOwnAttentionFn.apply(qkv, heads, hk, lengths, scale, bool(causal), torch.is_grad_enabled() and qkv.requires_grad)
     b, s, three_h = qkv.shape
     d = three_h // 3 // heads
     if _fast_ok(qkv, d) and qkv.is_contiguous():
