@@ -11,7 +11,7 @@
 // pass computes P again from S and L.  Exponentials are taken to base 2 (scale and log2 e in one factor), L is kept in
 // units of log2.  Rows that the mask leaves empty (i >= len) get O = 0, L = +inf, and gradients of 0.
 //
-// All products run as tcgen05.mma on 128 x 128 tiles with fp32 accumulators in TMEM.  A tile of probabilities goes back to
+// All products run as tcgen05.mma on tiles of 128 rows with fp32 accumulators in TMEM.  A tile of probabilities goes back to
 // TMEM in 16 bits and is the A operand of the next product from there; tiles of Q, K, V and dO come by TMA in the
 // 128-byte-swizzled layout, which serves as a K-major operand (contraction over d) and as an MN-major one (contraction over
 // tokens) alike.  Head sizes up to 128 run on tiles of 64 or 128 columns; TMA fills what lies beyond d with zeros.
@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kTile        = 128;  // rows of a tile of queries or keys
 constexpr int kBoxBytes    = kTile * 128;  // 128 rows of 64 16-bit values
-// Softmax warps, and behind them one that issues TMA loads, two that issue MMAs (a wait costs such a warp as much time as an
+// Backward: softmax warps, and behind them one that issues TMA loads, two that issue MMAs (a wait costs such a warp as much time as an
 // MMA or two, so each gets half of the products) and one that clears rows beyond a sequence's length.
 constexpr int kSoftWarps = 16;
 constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kClearWarp = kSoftWarps + 3;
@@ -322,8 +322,23 @@ __device__ __forceinline__ void StoresRead() {
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
-__device__ __forceinline__ void StoreZeroRow(uint16_t* row, int c0, int c1) {
-  for (int c = c0; c < c1; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+// Rows [first, last) of one head to zero, by a warp, neighbouring lanes within a row.
+__device__ __forceinline__ void StoreZeroRows(void* tensor, const Strides& st, int b, int h, int first, int last, int d) {
+  uint16_t* base = static_cast<uint16_t*>(tensor) + b * st.b + h * st.h;
+  const int vecs = d >> 3;
+  int row = first, c = threadIdx.x & 31;
+  while (c >= vecs) {
+    c -= vecs;
+    ++row;
+  }
+  while (row < last) {
+    *reinterpret_cast<uint4*>(base + row * st.s + c * 8) = make_uint4(0, 0, 0, 0);
+    c += 32;
+    while (c >= vecs) {
+      c -= vecs;
+      ++row;
+    }
+  }
 }
 
 __device__ __forceinline__ float Exp2(float x) {
@@ -785,7 +800,10 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         }
       }
       pieces_done += w.total > 0;
-      if ((!Cfg::kStaged || count == 0) && !live && row < p.s) StoreZeroRow(dst, 0, p.d);
+      if (!Cfg::kStaged || count == 0) {  // rows beyond the sequence
+        const int first = w.q0 + i * kTile + quarter * 32;
+        StoreZeroRows(p.o, p.so, w.b, w.h, max(first, w.len), min(first + 32, p.s), p.d);
+      }
       if (row < p.sp)
         p.lse[(static_cast<int64_t>(w.b) * p.h + w.h) * p.sp + row] = live ? fmaf(m, p.c, log2f(l) - (kBf16 ? 0.f : kHalfShift)) : INFINITY;
     }
@@ -806,6 +824,8 @@ __device__ __forceinline__ float TwoTo(int k) { return __int_as_float((k + 127) 
 // D_i = dO_i . O_i, with what rounding dropped of O, eight lanes per row.  A block takes 32 positions of eight heads: it reads runs of heads, which are neighbours
 // in a contiguous tensor, and writes runs of positions.  Writes [2][b, h, sp]: -L and -D, the addends as the main kernel uses them.
 // For fp16 further blocks read V, and the largest magnitudes go to [2][b, hk] behind that, cleared before.
+// Bound by HBM: 32 x 512, 16 heads of 64, 67 MB read in 20 us from a cold L2 (3.4 TB/s; 10 us at HBM's rate, which so short a
+// launch does not reach), 13 us behind the forward pass.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ AttnParams p) {
   __shared__ float sums[8][33];
@@ -885,7 +905,12 @@ __device__ __forceinline__ int GradExponent(const AttnParams& p, int b, int hk) 
 // which has 32 rows x 32 columns.  With 64 accumulator columns a unit has 128 positions and all sixteen warps, and the next
 // unit's scores are ready in a second place when they are needed.  With 128 there is no second place; units have 64 positions and
 // alternate between two sets of eight warps, each with its own S and dP: while one waits for the tensor cores, the other
-// computes.  (Products of 64 columns take three quarters of the time of 128.)
+// computes.  (Products of 64 columns take three quarters of the time of 128.)  Two blocks per SM with units of 64, which serve the forward
+// pass, gain nothing here (32 x 512, 16 heads of 64: 183 us where this takes 186; 4 x 2048: 273 and 269), and one warp for all
+// products makes the sets of 128 columns wait for one another (8192, 16 heads that share 4, causal: 1143 us where two take 790).
+// D included: 32 x 512, 16 heads of 64: 186 us = 463 TFLOP/s counting five products; 4 x 2048: 269 us = 640; 8192 positions, 16 heads
+// of 128 that share 4, causal: 790 us = 870.  Bound by the way from one unit to the next: S, exponentials, dP, dS and the
+// products' latencies follow one another, with the tensor cores busy a third of the time, the exponentials' unit half.
 template <int HD>
 struct BwdCfg {
   static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;    // what stays: X1 or X2
@@ -1220,13 +1245,12 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) BarArrive(m.base + Cfg::kAccFree);
-  } else if (row < p.s) {
+  } else {
+    const int first = w.x0 + warp * (kTile / kSoftWarps);
 #pragma unroll
-    for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
-      const Strides& st = out ? p.sdv : kKeys ? p.sdk : p.sdq;
-      StoreZeroRow(static_cast<uint16_t*>(out ? p.dv : kKeys ? p.dk : p.dq) + w.b * st.b + row * st.s + w.head * st.h, c0,
-                   min(p.d, c0 + kCols));
-    }
+    for (int out = 0; out < (kKeys ? 2 : 1); ++out)
+      StoreZeroRows(out ? p.dv : kKeys ? p.dk : p.dq, out ? p.sdv : kKeys ? p.sdk : p.sdq, w.b, w.head, first,
+                    min(first + kTile / kSoftWarps, p.s), p.d);
   }
 }
 

@@ -687,7 +687,7 @@ GemmPairKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
   } else if constexpr (kPre8) {
     // Four groups of four warps, each with a box of 64 columns.  GELU and the 8-bit form take about 26 instructions a value, most
     // of them waiting for one another: eight warps took 200 us for 16384 x 4096 x 1024, and the product with the
-    // 16-bit value and a pass that packs it 139 + 42.
+    // 16-bit value and a pass that packs it 139 + 42; sixteen take 136.
     const int q = warp & 3, g = (warp - 2) >> 2, r = q * 32 + lane;
     const bool issuer = ((warp - 2) & 3) == 0 && lane == 0;
     uint8_t* box  = staging + g * (Cfg::kStagingBytes / 4);
