@@ -510,7 +510,9 @@ __device__ __forceinline__ uint32_t AlignedSmem(const uint8_t* raw) { return (Sm
 // (32 x 512, 16 heads of 64: 54 us; one block with units of 128, next scores beside the probabilities, and a row shared
 // by two threads: 61).  With 128 one block fills TMEM, units have 128 keys, and one warp issues the products of both tiles, which
 // makes them take turns (8192, 16 heads of 128 that share 4, causal: 231 us = 1190 TFLOP/s; with a warp for each tile 248).
-// Bound by the exponentials (with 64 columns the unit for them is busy four fifths of the time) and by issue slots beside them.
+// Bound, within a long piece of 64 columns, by the unit for exponentials, which is busy four fifths of the time, and by issue slots
+// beside it; at 512 positions also by the start and the end of a piece.  With 128 columns by the way from a tile's scores through its
+// probabilities and products to its next scores (3300 clocks, of which the tensor cores work 2050 for both tiles).
 template <int HD>
 struct FwdCfg {
   static constexpr int kTileBytes = (HD / 64) * kBoxBytes;
