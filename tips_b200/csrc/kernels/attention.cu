@@ -507,9 +507,9 @@ __device__ __forceinline__ uint32_t AlignedSmem(const uint8_t* raw) { return (Sm
 // tile, so maximum and sum need no exchange; a tile's probabilities take the place of its scores, and the next scores follow the
 // product with V, so that one barrier tells that both are done.  While one tile waits for its products, others compute:
 // with 64 output columns, units of 64 keys leave TMEM for two blocks per SM, four tiles that run apart from each other
-// (32 x 512, 16 heads of 64: 54 us; one block with units of 128, next scores beside the probabilities, and a row shared
+// (32 x 512, 16 heads of 64: 53 us; one block with units of 128, next scores beside the probabilities, and a row shared
 // by two threads: 61).  With 128 one block fills TMEM, units have 128 keys, and one warp issues the products of both tiles, which
-// makes them take turns (8192, 16 heads of 128 that share 4, causal: 231 us = 1190 TFLOP/s; with a warp for each tile 248).
+// makes them take turns (8192, 16 heads of 128 that share 4, causal: 225 us = 1220 TFLOP/s; with a warp for each tile 248).
 // Bound, within a long piece of 64 columns, by the unit for exponentials, which is busy four fifths of the time, and by issue slots
 // beside it; at 512 positions also by the start and the end of a piece.  With 128 columns by the way from a tile's scores through its
 // probabilities and products to its next scores (3300 clocks, of which the tensor cores work 2050 for both tiles).
@@ -703,7 +703,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     if (wait.ok) settle();
     if (Cfg::kStaged && ElectOne()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
-    const int i = warp >> 2, quarter = warp & 3;  // query tile, TMEM lanes that this warp may access
+    const int i = warp / 4, quarter = warp & 3;  // query tile, TMEM lanes that this warp may access
     const int r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t ts = t_s + lanes + i * kUnit, to = t_o + lanes + i * HD;
@@ -716,7 +716,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
       const int row = w.q0 + i * kTile + r, count = i ? w.count1 : w.count0;
       float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and the sum
       for (int j = 0; j < count; ++j, ++done) {
-        if (!wait(s_full, done)) break;
+        wait(s_full, done);  // on a failure the values are void, and nothing is stored
         uint32_t s[kUnit / 32][32];
 #pragma unroll
         for (int g = 0; g < kUnit / 32; ++g) TmemLoad32Async(ts + g * 32, s[g]);
