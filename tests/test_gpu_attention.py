@@ -85,18 +85,22 @@ def test_fp16_gradients_of_any_size(d, of_do, of_v):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("s,d", [(5, 64), (48, 40), (130, 128)])
-def test_short_rows_lose_nothing_in_their_difference(s, d, dtype):
-    """dP - D is small where rows are short.  Of the two roundings that a gradient dQ or dK cannot do without, of dS and of the
-    result, each leaves u sqrt(1/3 * 3/(8 ln 2)) = 0.425 u in the 2-norm (uniform over half a step, magnitudes spread evenly over an
-    octave): together 0.60 u, and 0.64 u allows for the sample.  The rounding of O by itself would leave as much again in the shortest."""
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("s,d", [(5, 64), (48, 40), (128, 128)])
+def test_short_rows_lose_nothing_in_their_difference(s, d, causal, dtype):
+    """Rows of up to 128 keys hold D and dS more exactly than in 16 bits.  What is left is the rounding of dQ and dK themselves, r = u
+    sqrt(1/3 * 3/(8 ln 2)) = 0.425 u in the 2-norm (uniform over half a step, magnitudes spread evenly over an octave), and that of the
+    forward pass's probabilities, which reaches D by O.  It moves D by sum_j dP_j eps_j P_j with eps of size r: of n keys of like weight P
+    and dP of size a by r P a sqrt(n); dQ by that times sum_j P K_j, of size P sqrt(n) |K|, with P = 1 / n, against dQ's own P a sqrt(n)
+    |K|: by r / sqrt(n).  With 5 keys both together make 0.466 u, and 0.49 u allows for the sample.  The rounding of dS alone would make
+    it 0.63 u with 5 keys and 0.60 u with many."""
     q, k, v, do = make(8, s, 16, 8, d, dtype, seed=31)
-    got = run(q, k, v, do, causal=True)
-    want, _ = reference(q, k, v, do, True)
+    got = run(q, k, v, do, causal=causal)
+    want, _ = reference(q, k, v, do, causal)
     u = torch.finfo(dtype).eps / 2
     for name in ("dq", "dk"):
         off = float((got[name].double() - want[name]).norm() / want[name].norm())
-        assert off <= 0.64 * u, (name, off / u)
+        assert off <= 0.49 * u, (name, off / u)
 
 
 def test_rising_scores_rescale_the_output():

@@ -4,8 +4,11 @@
 //   S = scale Q K^T,  L_i = log sum_j exp S_ij,  P = exp(S - L) where valid and 0 elsewhere,  O = P V
 //   dV = P^T dO,  dP = dO V^T,  D_i = dO_i . O_i,  dS = P (dP - D),  dQ = scale dS K,  dK = scale dS^T Q
 //
-// D is a difference's other half: in short rows the rounding of O to 16 bits would show in it (a causal batch of 48 positions: dQ off by
-// 2.6e-3 where everything else leaves 2.4e-3).  There the forward pass also leaves what the rounding dropped, in 8 bits, for D.
+// Where rows have few keys, roundings to 16 bits show that average out elsewhere (and in a causal batch such rows make up most
+// of dK).  So for rows of up to 128 keys, those of the first tile of queries if the batch is causal or the sequence ends there, the
+// forward pass also leaves what the rounding of O dropped, in 8 bits, for D, which is a difference's other half.  And where no
+// sequence has more than 128 positions, dS enters its products as a sum of two 16-bit values.  In the 2-norm, bf16, causal: 48 positions,
+// dQ and dK off by 1.75e-3, of which the rounding of the result is 1.66e-3, instead of 2.6e-3; 8192 positions, dK 2.4e-3 instead of 2.5e-3.
 //
 // Nothing of size s x s reaches memory: the forward pass keeps a running maximum and sum per row and leaves L, the backward
 // pass computes P again from S and L.  Exponentials are taken to base 2 (scale and log2 e in one factor), L is kept in
@@ -67,7 +70,7 @@ struct AttnParams {
   float scale, c;       // c = scale * log2(e)
   float* lse;           // [b, h, sp]
   float* delta;         // [2][b, h, sp], and for fp16 [2][b, hk]
-  uint8_t* rest;        // [b, s, h, d]: what rounding dropped of O, times RestScale, as e5m2; null: not kept
+  uint8_t* rest;        // [b, min(s, 128), h, d]: what rounding dropped of O, times RestScale, as e5m2; null: not kept
   void *o, *dq, *dk, *dv;
   const void *dout, *v;
   Strides so, sdo, sdq, sdk, sdv, sv;
@@ -82,6 +85,11 @@ struct AttnMaps {
 // which tcgen05.mma takes its operands, and branches on it do not diverge.
 __device__ __forceinline__ uint32_t Uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
+// Whether the rows of the first tile of a sequence of `len` positions have few keys.
+__device__ __forceinline__ bool FewKeys(const AttnParams& p, int len) { return p.causal || len <= kTile; }
+__device__ __forceinline__ int64_t RestAt(const AttnParams& p, int b, int row, int h) {
+  return ((static_cast<int64_t>(b) * min(p.s, kTile) + row) * p.h + h) * p.d;
+}
 __device__ __forceinline__ int SeqLen(const AttnParams& p, int b) {
   if (p.lengths == nullptr) return p.s;
   const int64_t n = p.len64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
@@ -389,6 +397,13 @@ template <bool kBf16>
 __device__ __forceinline__ uint32_t Pack2(F2 a) {
   const float2 x = SplitF2(a);
   return Pack2<kBf16>(x.x, x.y);
+}
+
+// What rounding to `kept` dropped of a pair, in 16 bits.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t PackRest(F2 a, uint32_t kept) {
+  const float2 x = SplitF2(a), y = Unpack2<kBf16>(kept);
+  return Pack2<kBf16>(x.x - y.x, x.y - y.y);
 }
 
 __device__ __forceinline__ float LoadShared(uint32_t at) {
@@ -786,13 +801,14 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
       if (count > 0) {
         wait(base + Cfg::kOFull + i * 8, outputs++);
         const float inv = 1.f / l;
+        const bool rest = p.rest && w.q0 + i * kTile == 0 && FewKeys(p, w.len);
 #pragma unroll
         for (int g = 0; g < HD / 32; ++g) {
           uint32_t o[32];
           TmemLoad32(to + g * 32, o);
           if (Cfg::kStaged) StageCols<kBf16, 32>(q_tile(pieces_done, i), r, g * 32, o, inv, live);
           else if (live && wait.ok) StoreCols<kBf16, 32>(dst, g * 32, p.d, o, inv);
-          if (p.rest && live && wait.ok) StoreRest<kBf16, 32>(p.rest + ((static_cast<int64_t>(w.b) * p.s + row) * p.h + w.h) * p.d, g * 32, p.d, o, inv);
+          if (rest && live && wait.ok) StoreRest<kBf16, 32>(p.rest + RestAt(p, w.b, row, w.h), g * 32, p.d, o, inv);
         }
         TcFenceBefore();
         if (Cfg::kStaged) {
@@ -854,7 +870,7 @@ __global__ void __launch_bounds__(256) AttnDeltaKernel(const __grid_constant__ A
           uint2 z = make_uint2(0, 0);
           if (!values) {
             x = *reinterpret_cast<const uint4*>(out + i * p.so.s + k * 64);
-            if (p.rest) z = *reinterpret_cast<const uint2*>(p.rest + ((static_cast<int64_t>(b) * p.s + i) * p.h + h0 + h) * p.d + part * 8 + k * 64);
+            if (p.rest && i < kTile && FewKeys(p, len)) z = *reinterpret_cast<const uint2*>(p.rest + RestAt(p, b, i, h0 + h) + part * 8 + k * 64);
           }
           const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.x >> 16, z.y, z.y >> 16};
 #pragma unroll
@@ -1080,7 +1096,7 @@ __device__ __forceinline__ void BwdSettle(const AttnMaps& maps, const BwdSmem<HD
 }
 
 // Which: 0 issues S and P^T dO, 1 issues dP and dS^T Q or dS K.
-template <bool kBf16, int kWhich, int HD, bool kKeys>
+template <bool kBf16, bool kFine, int kWhich, int HD, bool kKeys>
 __device__ __forceinline__ void BwdMma(const AttnMaps& maps, const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w,
                                        uint32_t u0, uint32_t n, Owed& owed, Waiter& wait) {
   using Cfg = BwdCfg<HD>;
@@ -1125,6 +1141,7 @@ __device__ __forceinline__ void BwdMma(const AttnMaps& maps, const AttnParams& p
       if (u == u0 && n > 0 && !wait(m.base + Cfg::kAccFree, n - 1)) break;
       if (ElectOne()) {
         IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(u), m.Y(u), n_out, u > u0);
+        if (kFine) IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(u) + 16, m.Y(u), n_out, true);
         BarCommit(m.Empty(u));
         if (u + NS < end) grads(u + NS);
       }
@@ -1133,7 +1150,7 @@ __device__ __forceinline__ void BwdMma(const AttnMaps& maps, const AttnParams& p
   if (wait.ok && ElectOne()) BarCommit(m.base + Cfg::kAccFull);
 }
 
-template <bool kBf16, int HD, bool kKeys>
+template <bool kBf16, bool kFine, int HD, bool kKeys>
 __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
                                            Waiter& wait) {
   using Cfg = BwdCfg<HD>;
@@ -1208,7 +1225,7 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
     }
     if (!wait(m.DpFull(u), u / NS)) break;
     TmemLoad32(m.Dp(u) + lanes + col, s);
-    uint32_t v[16];
+    uint32_t v[16], low[16];
 #pragma unroll
     for (int k = 0; k < 16; k += 2) {
       F2 d0 = row_d, d1 = row_d;
@@ -1222,8 +1239,13 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
       }
       v[k]     = Pack2<kBf16>(g0);
       v[k + 1] = Pack2<kBf16>(g1);
+      if (kFine) {
+        low[k]     = PackRest<kBf16>(g0, v[k]);
+        low[k + 1] = PackRest<kBf16>(g1, v[k + 1]);
+      }
     }
     TmemStore16(m.Dp(u) + lanes + col, v);
+    if (kFine) TmemStore16(m.Dp(u) + lanes + col + 16, low);
     TmemStoreWait();
     TcFenceBefore();
     __syncwarp();
@@ -1256,8 +1278,9 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
   }
 }
 
-// Both passes in one launch, so that neither leaves a tail of idle SMs.
-template <int HD, bool kBf16>
+// Both passes in one launch, so that neither leaves a tail of idle SMs.  kFine: dS as a sum of two values (a branch in the loop
+// instead costs long sequences 4 %).
+template <int HD, bool kBf16, bool kFine>
 __global__ void __launch_bounds__(kThreads, 1)
 AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   using Cfg = BwdCfg<HD>;
@@ -1328,7 +1351,7 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     Waiter wait(6);
     Owed owed;
     follow(std::false_type{}, [&](const auto& w) {
-      if (w.total > 0 && wait.ok) BwdMma<kBf16, 0>(maps, p, m, w, u0, n, owed, wait);
+      if (w.total > 0 && wait.ok) BwdMma<kBf16, kFine, 0>(maps, p, m, w, u0, n, owed, wait);
       return true;
     });
     if (wait.ok) BwdSettle(maps, m, owed, wait);
@@ -1337,13 +1360,13 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     Waiter wait(6);
     Owed none;
     follow(std::false_type{}, [&](const auto& w) {
-      if (w.total > 0 && wait.ok) BwdMma<kBf16, 1>(maps, p, m, w, u0, n, none, wait);
+      if (w.total > 0 && wait.ok) BwdMma<kBf16, kFine, 1>(maps, p, m, w, u0, n, none, wait);
       return true;
     });
   } else {
     Waiter wait(7);
     follow(std::false_type{}, [&](const auto& w) {
-      BwdSoftmax<kBf16>(p, m, w, u0, n, wait);
+      BwdSoftmax<kBf16, kFine>(p, m, w, u0, n, wait);
       return true;
     });
   }
@@ -1431,10 +1454,10 @@ int LaunchFwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   return 0;
 }
 
-template <int HD, bool kBf16>
+template <int HD, bool kBf16, bool kFine>
 int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
-  int rc = AllowSmem(AttnBwdKernel<HD, kBf16>, BwdCfg<HD>::kSmemBytes, &done);
+  int rc = AllowSmem(AttnBwdKernel<HD, kBf16, kFine>, BwdCfg<HD>::kSmemBytes, &done);
   if (rc) return rc;
   int runs = TilesOf(p.h, 8);
   if (!kBf16) {
@@ -1444,9 +1467,13 @@ int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   AttnDeltaKernel<kBf16><<<dim3(std::min(p.sp / 32, 4096), runs, p.b), 256, 0, s>>>(p);
   TIPSK_LAUNCH_CHECK();
   const int grid = (p.sp / kTile) * p.b * (p.h + p.hk);
-  AttnBwdKernel<HD, kBf16><<<grid, kThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  AttnBwdKernel<HD, kBf16, kFine><<<grid, kThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
   TIPSK_LAUNCH_CHECK();
   return 0;
+}
+template <int HD, bool kBf16>
+int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
+  return p.s <= kTile ? LaunchBwd<HD, kBf16, true>(maps, p, s) : LaunchBwd<HD, kBf16, false>(maps, p, s);
 }
 
 }  // namespace
@@ -1456,8 +1483,8 @@ using namespace tipsk;
 
 extern "C" {
 
-/* O = softmax(scale Q K^T + mask) V and L [b, h, s rounded up to 128].  rest (optional): [b, s, h, d] bytes, what the
- * rounding of O dropped, for the backward pass to take.  host_strides: q, k, v, out. */
+/* O = softmax(scale Q K^T + mask) V and L [b, h, s rounded up to 128].  rest (optional): [b, min(s, 128), h, d]
+ * bytes, what the rounding of O dropped in rows of few keys, for the backward pass to take.  host_strides: q, k, v, out. */
 int tipsk_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest, const void* lengths, int len64,
                         int b, int s, int h, int hk, int d, int dtype, const int64_t* host_strides, float scale, int causal,
                         void* stream) {

@@ -137,25 +137,23 @@ def _lse_bytes(shape) -> int:
     return b * h * (-(-s // 128) * 128) * 4
 
 
-def _keeps_rest(shape, causal) -> bool:
-    """Whether a forward pass keeps what the rounding of its output drops.  It shows in dQ and dK where rows are short (16 positions,
-    causal, bf16: they are off by 2.8e-3 without and 2.4e-3 with it; from 512 keys a row on 2.4e-3 either way), and costs
-    more than it is worth where they are not (32 x 512, 16 heads of 64, forward: 54 us without, 66 with it)."""
-    return shape[1] < (1024 if causal else 512)
+def _rest_bytes(shape, lengths, causal) -> int:
+    """Bytes for what the rounding of the output drops in rows of up to 128 keys, if there can be any."""
+    b, s, h, _, d = shape
+    return b * min(s, 128) * h * d if causal or lengths is not None or s <= 128 else 0
 
 
 def _attention_fwd(like, shape, q, k, v, lengths, scale, causal, grad=True):
     """(out, stats) for the views q, k, v of CUDA tensors like `like`; shape = (b, s, h, hk, d).  `stats`: bytes of the rows'
-    log-sums and, for a backward pass to come, what rounding dropped of `out` where it is kept."""
+    log-sums and, for a backward pass to come, what rounding dropped of `out` in rows of few keys."""
     b, s, h, hk, d = shape
     out = torch.empty(b, s, h, d, dtype=like.dtype, device=like.device)
-    at = _lse_bytes(shape)
-    keep = grad and _keeps_rest(shape, causal)
-    stats = torch.empty(at + b * s * h * d if keep else at, dtype=torch.uint8, device=like.device)
+    at, rest = _lse_bytes(shape), _rest_bytes(shape, lengths, causal) if grad else 0
+    stats = torch.empty(at + rest, dtype=torch.uint8, device=like.device)
     if out.numel():
         with base.device_of(like):
             base.check(base.K().tipsk_attention_fwd(
-                q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if keep else None, base.ptr(lengths),
+                q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if rest else None, base.ptr(lengths),
                 int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(like),
                 _strides(q, k, v, _view(out)), scale, int(causal), base.stream()), "attention_fwd")
     return out, stats
@@ -171,7 +169,7 @@ def _attention_bwd(dout, shape, q, k, v, out, stats, lengths, scale, causal, dq,
     delta = torch.empty(at // 2 + 2 * b * hk, dtype=torch.float32, device=out.device)
     with base.device_of(out):
         base.check(base.K().tipsk_attention_bwd(
-            dout.data_ptr(), q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if _keeps_rest(shape, causal) else None,
+            dout.data_ptr(), q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if _rest_bytes(shape, lengths, causal) else None,
             delta.data_ptr(), dq[0], dk[0], dv[0],
             base.ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(out),
             _strides(q, k, v, _view(out), _view(dout), dq, dk, dv), scale, int(causal), base.stream()), "attention_bwd")
