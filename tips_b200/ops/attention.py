@@ -268,8 +268,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     On a GPU: bfloat16 or float16, d a multiple of 8 up to 128, any strides (inputs whose last axis is not contiguous, or
     whose rows do not start on 16 bytes, are copied).  The softmax is held in fp32; the probabilities, and their
     gradient in the backward pass, are rounded to the inputs' type as operands of the products (for float16 at a scale that keeps
-    them within its range).  Gradients do not depend on
-    the order of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
+    them within its range; the gradient as a sum of two values where seq is at most 128).  Gradients do not depend on the order
+    of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
     do not see it, as 0 * inf does in the formula.  `lengths` may not change between forward and backward."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
