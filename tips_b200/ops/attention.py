@@ -121,6 +121,14 @@ def _view(t: torch.Tensor):
     return t.data_ptr(), t.stride()[:3]
 
 
+def _heads_view(t: torch.Tensor, shape):
+    """The same of the query heads in a tensor of that shape, or in a contiguous [batch, seq, heads * d] one."""
+    if t.dim() == 4:
+        return _view(t)
+    _, s, h, _, d = shape
+    return t.data_ptr(), (s * h * d, h * d, d)
+
+
 def _packed_views(t: torch.Tensor, h: int, hk: int, d: int):
     """The same of the q, k and v heads of a contiguous [batch, seq, (h + 2 hk) * d] tensor, without making views."""
     at, row, step = t.data_ptr(), (h + 2 * hk) * d, d * t.element_size()
@@ -143,11 +151,11 @@ def _rest_bytes(shape, lengths, causal) -> int:
     return b * min(s, 128) * h * d if causal or lengths is not None or s <= 128 else 0
 
 
-def _attention_fwd(like, shape, q, k, v, lengths, scale, causal, grad=True):
-    """(out, stats) for the views q, k, v of CUDA tensors like `like`; shape = (b, s, h, hk, d).  `stats`: bytes of the rows'
+def _attention_fwd(like, shape, q, k, v, lengths, scale, causal, grad=True, flat=False):
+    """(out, stats) for the views q, k, v of CUDA tensors like `like`; shape = (b, s, h, hk, d), `flat`: out is [b, s, h * d].  `stats`: bytes of the rows'
     log-sums and, for a backward pass to come, what rounding dropped of `out` in rows of few keys."""
     b, s, h, hk, d = shape
-    out = torch.empty(b, s, h, d, dtype=like.dtype, device=like.device)
+    out = torch.empty((b, s, h * d) if flat else (b, s, h, d), dtype=like.dtype, device=like.device)
     at, rest = _lse_bytes(shape), _rest_bytes(shape, lengths, causal) if grad else 0
     stats = torch.empty(at + rest, dtype=torch.uint8, device=like.device)
     if out.numel():
@@ -155,7 +163,7 @@ def _attention_fwd(like, shape, q, k, v, lengths, scale, causal, grad=True):
             base.check(base.K().tipsk_attention_fwd(
                 q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if rest else None, base.ptr(lengths),
                 int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(like),
-                _strides(q, k, v, _view(out)), scale, int(causal), base.stream()), "attention_fwd")
+                _strides(q, k, v, _heads_view(out, shape)), scale, int(causal), base.stream()), "attention_fwd")
     return out, stats
 
 
@@ -164,7 +172,7 @@ def _attention_bwd(dout, shape, q, k, v, out, stats, lengths, scale, causal, dq,
     b, s, h, hk, d = shape
     if not out.numel():
         return
-    dout = _rows16(dout)
+    dout = _rows16(dout) if dout.dim() == 4 else _packed16(dout)
     at = _lse_bytes(shape)
     delta = torch.empty(at // 2 + 2 * b * hk, dtype=torch.float32, device=out.device)
     with base.device_of(out):
@@ -172,7 +180,7 @@ def _attention_bwd(dout, shape, q, k, v, out, stats, lengths, scale, causal, dq,
             dout.data_ptr(), q[0], k[0], v[0], out.data_ptr(), stats.data_ptr(), stats.data_ptr() + at if _rest_bytes(shape, lengths, causal) else None,
             delta.data_ptr(), dq[0], dk[0], dv[0],
             base.ptr(lengths), int(lengths is not None and lengths.dtype == torch.int64), b, s, h, hk, d, base.code(out),
-            _strides(q, k, v, _view(out), _view(dout), dq, dk, dv), scale, int(causal), base.stream()), "attention_bwd")
+            _strides(q, k, v, _heads_view(out, shape), _heads_view(dout, shape), dq, dk, dv), scale, int(causal), base.stream()), "attention_bwd")
     base.count_launches(1)
 
 
@@ -187,7 +195,7 @@ class _AttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @base.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, stats, lengths = ctx.saved_tensors
         shape, scale, causal = ctx.meta
@@ -209,20 +217,20 @@ class _PackedOwnAttentionFn(torch.autograd.Function):
         qkv = _packed16(qkv)
         b, s, width = qkv.shape
         shape = (b, s, h, hk, width // (h + 2 * hk))
-        out, stats = _attention_fwd(qkv, shape, *_packed_views(qkv, h, hk, shape[4]), lengths, scale, causal, grad)
+        out, stats = _attention_fwd(qkv, shape, *_packed_views(qkv, h, hk, shape[4]), lengths, scale, causal, grad, flat=True)
         ctx.save_for_backward(qkv, out, stats, lengths)
         ctx.meta = (shape, scale, causal)
-        return out.view(b, s, h * shape[4])
+        return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @base.once_differentiable
     def backward(ctx, dy):
         qkv, out, stats, lengths = ctx.saved_tensors
         shape, scale, causal = ctx.meta
         _, _, h, hk, d = shape
-        qkv, out, stats = _packed16(qkv), _rows16(out), _packed16(stats)
+        qkv, out, stats = _packed16(qkv), _packed16(out), _packed16(stats)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _attention_bwd(dy.reshape(out.shape), shape, *_packed_views(qkv, h, hk, d), out, stats, lengths, scale, causal,
+        _attention_bwd(dy, shape, *_packed_views(qkv, h, hk, d), out, stats, lengths, scale, causal,
                        *_packed_views(dqkv, h, hk, d))
         return dqkv, None, None, None, None, None, None
 

@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -51,6 +52,18 @@ def stream() -> int:
     """Handle of the current stream of the current device (without building a torch.cuda.Stream object, which took a
     quarter of the host time of an encoder layer: one per launch)."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def once_differentiable(backward):
+    """torch's decorator for a backward pass whose gradients are refused, which switches the grad mode around every call, only for
+    the calls that want to go on differentiating (a twelfth of the host time of a small layer's backward pass otherwise)."""
+    refusing = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 class _Here:

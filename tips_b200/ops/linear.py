@@ -174,7 +174,7 @@ class _Linear8Fn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, act):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         if not x2.is_contiguous():
             x2 = x2.contiguous()
         need = ctx.needs_input_grad
@@ -182,10 +182,10 @@ class _Linear8Fn(torch.autograd.Function):
         ctx.save_for_backward(weight, x8, pre8)
         ctx.x_dtype, ctx.bias_dtype = x.dtype, None if bias is None else bias.dtype
         ctx.in_shape = x.shape
-        return y.view(*x.shape[:-1], weight.shape[0])
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @base.once_differentiable
     def backward(ctx, dy):
         return _linear8_backward(ctx, dy, None)
 
@@ -193,7 +193,7 @@ class _Linear8Fn(torch.autograd.Function):
 def _linear8_backward(ctx, dy, d_alias):
     weight, x8, pre8 = ctx.saved_tensors  # pre8: None without an activation
     n, k = weight.shape
-    dz = dy.reshape(-1, n)
+    dz = dy if dy.dim() == 2 else dy.reshape(-1, n)
     if not dz.is_contiguous():
         dz = dz.contiguous()
     want_dx, want_dw = ctx.needs_input_grad[:2]
@@ -218,7 +218,7 @@ def _linear8_backward(ctx, dy, d_alias):
                                          base.ptr(db), 0 if db is None else base.code(db), base.ptr(ws), m, n, k, weight.stride(0),
                                          int(into is not None), base.stream()), "linear8_bwd")
     base.count_launches(int(pre8 is not None or want_db is not None) + int(want_db is not None) + int(want_dx) + 2 * int(want_dw) - 1)
-    return None if dx is None else dx.view(ctx.in_shape), dw, db, None
+    return dx if dx is None or len(ctx.in_shape) == 2 else dx.view(ctx.in_shape), dw, db, None
 
 
 class _Linear8PassFn(torch.autograd.Function):
@@ -230,7 +230,7 @@ class _Linear8PassFn(torch.autograd.Function):
         return y, x.detach()
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @base.once_differentiable
     def backward(ctx, dy, d_alias):
         return _linear8_backward(ctx, dy, d_alias)
 
