@@ -924,9 +924,10 @@ __device__ __forceinline__ int GradExponent(const AttnParams& p, int b, int hk) 
 // unit's scores are ready in a second place when they are needed.  With 128 there is no second place; units have 64 positions and
 // alternate between two sets of eight warps, each with its own S and dP: while one waits for the tensor cores, the other
 // computes.  (Products of 64 columns take three quarters of the time of 128.)  Two blocks per SM with units of 64, which serve the forward
-// pass, gain nothing here (32 x 512, 16 heads of 64: 183 us where this takes 186; 4 x 2048: 273 and 269), and one warp for all
-// products makes the sets of 128 columns wait for one another (8192, 16 heads that share 4, causal: 1143 us where two take 790).
-// D included: 32 x 512, 16 heads of 64: 186 us = 463 TFLOP/s counting five products; 4 x 2048: 269 us = 640; 8192 positions, 16 heads
+// pass, take as long with full sequences (32 x 512, 16 heads of 64: 183 us both; 4 x 2048: 270 and 264), 114 us instead of 126 with
+// lengths spread over 1..512, and cost heads of 128 two per cent where both share their code; one warp for all products makes the
+// sets of 128 columns wait for one another (8192, 16 heads that share 4, causal: 1143 us where two take 790).
+// D included: 32 x 512, 16 heads of 64: 183 us = 470 TFLOP/s counting five products; 4 x 2048: 264 us = 650; 8192 positions, 16 heads
 // of 128 that share 4, causal: 790 us = 870.  Bound by the way from one unit to the next: S, exponentials, dP, dS and the
 // products' latencies follow one another, with the tensor cores busy a third of the time, the exponentials' unit half.
 template <int HD>
