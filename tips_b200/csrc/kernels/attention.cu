@@ -41,12 +41,6 @@ namespace {
 
 constexpr int kTile        = 128;  // rows of a tile of queries or keys
 constexpr int kBoxBytes    = kTile * 128;  // 128 rows of 64 16-bit values
-// Backward: softmax warps, and behind them one that issues TMA loads, two that issue MMAs (a wait costs such a warp as much time as an
-// MMA or two, so each gets half of the products) and one that clears rows beyond a sequence's length.
-constexpr int kSoftWarps = 16;
-constexpr int kTmaWarp = kSoftWarps, kMmaWarp = kSoftWarps + 1, kClearWarp = kSoftWarps + 3;
-constexpr int kWarps   = kSoftWarps + 4;
-constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kFwdPoly = 8;  // forward, one pair of exponentials in so many by a polynomial (one in 4: 57 us where 8 takes 54, none: 56)
 // fp16 has few exponents: forward, probabilities are held times 2^7 (so up to 2^15, see the lag of the maximum), which keeps those
@@ -919,41 +913,47 @@ __device__ __forceinline__ int GradExponent(const AttnParams& p, int b, int hk) 
 //   !kKeys    Q, dO            K, V               rows are queries                dQ += dS K
 // Both passes compute S and dP, seven products instead of five, and in exchange every sum has one owner: no atomics, no
 // fp32 copy of dQ in memory, and results that do not depend on the order of the blocks.
-// A unit goes through S, P, dP, dS in turn, and every step hands over between the tensor cores and the softmax warps, each of
-// which has 32 rows x 32 columns.  With 64 accumulator columns a unit has 128 positions and all sixteen warps, and the next
-// unit's scores are ready in a second place when they are needed.  With 128 there is no second place; units have 64 positions and
-// alternate between two sets of eight warps, each with its own S and dP: while one waits for the tensor cores, the other
-// computes.  (Products of 64 columns take three quarters of the time of 128.)  Two blocks per SM with units of 64, which serve the forward
-// pass, take as long with full sequences (32 x 512, 16 heads of 64: 183 us both; 4 x 2048: 270 and 264), 114 us instead of 126 with
-// lengths spread over 1..512, and cost heads of 128 two per cent where both share their code; one warp for all products makes the
-// sets of 128 columns wait for one another (8192, 16 heads that share 4, causal: 1143 us where two take 790).
-// D included: 32 x 512, 16 heads of 64: 183 us = 470 TFLOP/s counting five products; 4 x 2048: 264 us = 650; 8192 positions, 16 heads
-// of 128 that share 4, causal: 790 us = 870.  Bound by the way from one unit to the next: S, exponentials, dP, dS and the
-// products' latencies follow one another, with the tensor cores busy a third of the time, the exponentials' unit half.
+// A unit of 64 positions goes through S, P, dP, dS in turn, and every step hands over between the tensor cores and eight softmax
+// warps, each of which has 32 rows x 32 columns.  While one unit waits for the tensor cores, another computes:
+// with 64 accumulator columns that of the other block on the SM; with 128, where one block fills TMEM, that of a second set of
+// warps with its own S and dP.  There two warps issue the products (a wait costs such a warp as much time as an MMA or two, so each
+// gets half of them; one for all: 8192, 16 heads that share 4, causal, 1143 us where two take 810), and one clears rows beyond a
+// sequence's length; two blocks have no registers for more warps, so the one that issues clears as well.
+// D included: 32 x 512, 16 heads of 64: 182 us = 473 TFLOP/s counting five products, with lengths spread over 1..512: 114; 4 x 2048: 269 us =
+// 640; 8192 positions, 16 heads of 128 that share 4, causal: 810 us = 847.  (One block per SM with units of 128 for 64 columns, and the
+// next scores beside them: 183, 126 and 264.)  Bound by the way from one unit to the next: S, exponentials, dP, dS and the
+// products' latencies follow one another, with the tensor cores busy a third to a half of the time, the exponentials' unit half.
 template <int HD>
 struct BwdCfg {
   static constexpr int kTileBytes  = (HD / 64) * kBoxBytes;    // what stays: X1 or X2
+  static constexpr int kBlocks     = HD == 64 ? 2 : 1;         // per SM
   static constexpr int kSets       = HD == 64 ? 1 : 2;
-  static constexpr int kUnit       = kTile / kSets;            // positions of a streamed unit
-  static constexpr int kUnitBytes  = kTileBytes / kSets;
+  static constexpr int kSetWarps   = 8;
+  static constexpr int kSoftWarps  = kSets * kSetWarps;
+  static constexpr int kMmaWarps   = HD == 64 ? 1 : 2;
+  static constexpr int kTmaWarp    = kSoftWarps, kMmaWarp = kSoftWarps + 1;
+  static constexpr bool kClears    = kMmaWarps == 2;            // a warp of its own clears rows beyond a sequence's length
+  static constexpr int kClearWarp  = kClears ? kMmaWarp + 2 : -1;
+  static constexpr int kThreads    = (kSoftWarps + 1 + kMmaWarps + kClears) * 32;
+  static constexpr int kColumns    = kSets * 128 + 2 * HD;     // of TMEM
+  static constexpr int kUnit       = 64;                       // positions of a streamed unit
+  static constexpr int kUnitBytes  = kUnit * HD * 2;
   static constexpr int kStageBytes = 2 * kUnitBytes;           // Y1, Y2
   static constexpr int kStages     = 4;
-  static constexpr int kXBufs      = HD == 64 ? 2 : 1;         // what stays, of this piece of work and the next
-  static constexpr int kSBufs      = 2;                        // places for scores in TMEM: two of the one set, one of either
   static constexpr int kRowBytes   = 2 * kUnit * 4;            // -L and -D of a unit of queries
-  // shared memory: [kXBufs][X1, X2], the ring [kStages][Y1, Y2], [kStages][-L, -D], barriers
-  static constexpr int kRing       = kXBufs * 2 * kTileBytes;
+  // shared memory: X1, X2, the ring [kStages][Y1, Y2], [kStages][-L, -D], barriers
+  static constexpr int kRing       = 2 * kTileBytes;
   static constexpr int kRows       = kRing + kStages * kStageBytes;
-  static constexpr int kXRows      = kRows + kStages * kRowBytes;  // [kXBufs] -L and -D of the tile of queries that stays
-  static constexpr int kNext       = kXRows + kXBufs * 2 * kTile * 4;
+  static constexpr int kXRows      = kRows + kStages * kRowBytes;  // -L and -D of the tile of queries that stays
+  static constexpr int kNext       = kXRows + 2 * kTile * 4;
   static constexpr int kFull       = kNext + Pieces::kBytes;
   static constexpr int kEmpty      = kFull + 8 * kStages;
   static constexpr int kRaw        = kEmpty + 8 * kStages;       // a unit has arrived and has rows to clear before it counts as full
   static constexpr int kXFull      = kRaw + 8 * kStages;
-  static constexpr int kXEmpty     = kXFull + 8 * kXBufs;
-  static constexpr int kSFull      = kXEmpty + 8 * kXBufs;       // [SB] S of a unit is in TMEM
-  static constexpr int kSDone      = kSFull + 8 * kSBufs;        // [SB] keys: P has taken its place, queries: S has been read
-  static constexpr int kDpFull     = kSDone + 8 * kSBufs;        // [sets] dP is in TMEM
+  static constexpr int kXEmpty     = kXFull + 8;
+  static constexpr int kSFull      = kXEmpty + 8;                // [sets] S of a unit is in TMEM
+  static constexpr int kSDone      = kSFull + 8 * kSets;         // [sets] keys: P has taken its place, queries: S has been read
+  static constexpr int kDpFull     = kSDone + 8 * kSets;         // [sets] dP is in TMEM
   static constexpr int kDsFull     = kDpFull + 8 * kSets;        // [sets] dS has taken its place
   static constexpr int kTurn       = kDsFull + 8 * kSets;        // [sets] a unit's exponentials are done
   static constexpr int kAccFull    = kTurn + 8 * kSets;          // a piece's sums are complete
@@ -1004,24 +1004,24 @@ template <int HD>
 struct BwdSmem {
   using C = BwdCfg<HD>;
   uint32_t base, tmem;
-  __device__ __forceinline__ uint32_t X(uint32_t n) const { return base + n % C::kXBufs * (2 * C::kTileBytes); }
+  __device__ __forceinline__ uint32_t X() const { return base; }
   __device__ __forceinline__ uint32_t Y(uint32_t u) const { return base + C::kRing + u % C::kStages * C::kStageBytes; }
   __device__ __forceinline__ uint32_t Rows(uint32_t u) const { return base + C::kRows + u % C::kStages * C::kRowBytes; }
-  __device__ __forceinline__ uint32_t XRows(uint32_t n) const { return base + C::kXRows + n % C::kXBufs * (2 * kTile * 4); }
+  __device__ __forceinline__ uint32_t XRows() const { return base + C::kXRows; }
   __device__ __forceinline__ uint32_t Full(uint32_t u) const { return base + C::kFull + u % C::kStages * 8; }
   __device__ __forceinline__ uint32_t Empty(uint32_t u) const { return base + C::kEmpty + u % C::kStages * 8; }
   __device__ __forceinline__ uint32_t Raw(uint32_t u) const { return base + C::kRaw + u % C::kStages * 8; }
-  __device__ __forceinline__ uint32_t XFull(uint32_t n) const { return base + C::kXFull + n % C::kXBufs * 8; }
-  __device__ __forceinline__ uint32_t XEmpty(uint32_t n) const { return base + C::kXEmpty + n % C::kXBufs * 8; }
-  __device__ __forceinline__ uint32_t SFull(uint32_t u) const { return base + C::kSFull + u % C::kSBufs * 8; }
-  __device__ __forceinline__ uint32_t SDone(uint32_t u) const { return base + C::kSDone + u % C::kSBufs * 8; }
+  __device__ __forceinline__ uint32_t XFull() const { return base + C::kXFull; }
+  __device__ __forceinline__ uint32_t XEmpty() const { return base + C::kXEmpty; }
+  __device__ __forceinline__ uint32_t SFull(uint32_t u) const { return base + C::kSFull + u % C::kSets * 8; }
+  __device__ __forceinline__ uint32_t SDone(uint32_t u) const { return base + C::kSDone + u % C::kSets * 8; }
   __device__ __forceinline__ uint32_t DpFull(uint32_t u) const { return base + C::kDpFull + u % C::kSets * 8; }
   __device__ __forceinline__ uint32_t DsFull(uint32_t u) const { return base + C::kDsFull + u % C::kSets * 8; }
   __device__ __forceinline__ uint32_t Turn(uint32_t u) const { return base + C::kTurn + u % C::kSets * 8; }
-  // columns: S and dP, of one set or of either, then the accumulators and the one set's second S
-  __device__ __forceinline__ uint32_t S(uint32_t u) const { return tmem + (u & 1) * (C::kSets == 1 ? 384 : 128); }
-  __device__ __forceinline__ uint32_t Dp(uint32_t u) const { return C::kSets == 1 ? tmem + 128 : tmem + 64 + (u & 1) * 128; }
-  __device__ __forceinline__ uint32_t Acc(int i) const { return tmem + 256 + i * HD; }
+  // columns: S and dP of either set, then the accumulators
+  __device__ __forceinline__ uint32_t S(uint32_t u) const { return tmem + u % C::kSets * 128; }
+  __device__ __forceinline__ uint32_t Dp(uint32_t u) const { return S(u) + 64; }
+  __device__ __forceinline__ uint32_t Acc(int i) const { return tmem + C::kSets * 128 + i * HD; }
 };
 
 // What each kind of warp does for one piece.  u0: units so far, n: pieces with any so far.
@@ -1029,16 +1029,16 @@ template <int HD, bool kKeys>
 __device__ __forceinline__ bool BwdLoad(const AttnMaps& maps, const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w,
                                         uint32_t u0, uint32_t n) {  // one thread
   using Cfg = BwdCfg<HD>;
-  constexpr int XB = Cfg::kXBufs, ST = Cfg::kStages, kUnit = Cfg::kUnit;
-  if (!BarWaitOne(m.XEmpty(n), (n / XB) ^ 1)) return false;
-  BarExpect(m.XFull(n), 2 * Cfg::kTileBytes + (kKeys ? 0 : 2 * kTile * 4));
-  TmaLoadTile<HD, kTile, kUnit>(m.X(n), kKeys ? &maps.k : &maps.q, w.x0, w.head, w.b, m.XFull(n));
-  TmaLoadTile<HD, kTile, kUnit>(m.X(n) + Cfg::kTileBytes, kKeys ? &maps.v : &maps.dout, w.x0, w.head, w.b, m.XFull(n));
+  constexpr int ST = Cfg::kStages, kUnit = Cfg::kUnit;
+  if (!BarWaitOne(m.XEmpty(), n ^ 1)) return false;
+  BarExpect(m.XFull(), 2 * Cfg::kTileBytes + (kKeys ? 0 : 2 * kTile * 4));
+  TmaLoadTile<HD, kTile, kUnit>(m.X(), kKeys ? &maps.k : &maps.q, w.x0, w.head, w.b, m.XFull());
+  TmaLoadTile<HD, kTile, kUnit>(m.X() + Cfg::kTileBytes, kKeys ? &maps.v : &maps.dout, w.x0, w.head, w.b, m.XFull());
   const int64_t plane = static_cast<int64_t>(p.b) * p.h * p.sp;  // of -L, -D
   if (!kKeys) {
     const float* src = p.delta + (static_cast<int64_t>(w.b) * p.h + w.head) * p.sp + w.x0;
-    BulkLoad(m.XRows(n), src, kTile * 4, m.XFull(n));
-    BulkLoad(m.XRows(n) + kTile * 4, src + plane, kTile * 4, m.XFull(n));
+    BulkLoad(m.XRows(), src, kTile * 4, m.XFull());
+    BulkLoad(m.XRows() + kTile * 4, src + plane, kTile * 4, m.XFull());
   }
   const int group = p.h / p.hk;
   int at = 0, yh = kKeys ? w.head * group : w.head / group;  // unit within a head
@@ -1046,7 +1046,7 @@ __device__ __forceinline__ bool BwdLoad(const AttnMaps& maps, const AttnParams& 
     const uint32_t u = u0 + k;
     if (!BarWaitOne(m.Empty(u), (u / ST) ^ 1)) return false;
     const int y0 = (w.first + at) * kUnit;
-    const uint32_t bar = w.ragged && at == w.per - 1 ? m.Raw(u) : m.Full(u);
+    const uint32_t bar = Cfg::kClears && w.ragged && at == w.per - 1 ? m.Raw(u) : m.Full(u);
     BarExpect(bar, Cfg::kStageBytes + (kKeys ? Cfg::kRowBytes : 0));
     TmaLoadTile<HD, kUnit, kUnit>(m.Y(u), kKeys ? &maps.q : &maps.k, y0, yh, w.b, bar);
     TmaLoadTile<HD, kUnit, kUnit>(m.Y(u) + Cfg::kUnitBytes, kKeys ? &maps.dout : &maps.v, y0, yh, w.b, bar);
@@ -1075,8 +1075,7 @@ __device__ __forceinline__ void BwdClear(const BwdSmem<HD>& m, const BwdPiece<kK
   }
 }
 
-// Stores of a piece whose sums are, or will be, staged: the warp that issues S makes them when the next piece's first scores are
-// on their way, while the softmax warps work on these.
+// Stores of a piece whose sums are, or will be, staged in the place of its X.
 struct Owed {
   int b = -1, head, x0;
   bool keys;
@@ -1087,64 +1086,72 @@ __device__ __forceinline__ void BwdSettle(const AttnMaps& maps, const BwdSmem<HD
   using Cfg = BwdCfg<HD>;
   if (o.b < 0 || !wait(m.base + Cfg::kAccFree, o.n)) return;
   if (ElectOne()) {
-    TmaStoreTile<HD>(m.X(o.n), o.keys ? &maps.dk : &maps.dq, o.x0, o.head, o.b);
-    if (o.keys) TmaStoreTile<HD>(m.X(o.n) + Cfg::kTileBytes, &maps.dv, o.x0, o.head, o.b);
+    TmaStoreTile<HD>(m.X(), o.keys ? &maps.dk : &maps.dq, o.x0, o.head, o.b);
+    if (o.keys) TmaStoreTile<HD>(m.X() + Cfg::kTileBytes, &maps.dv, o.x0, o.head, o.b);
     StoresRead();
-    BarArrive(m.XEmpty(o.n));
+    BarArrive(m.XEmpty());
   }
   __syncwarp();
   o.b = -1;
 }
 
-// Which: 0 issues S and P^T dO, 1 issues dP and dS^T Q or dS K.
+// Which: 0 issues S and P^T dO, 1 issues dP and dS^T Q or dS K, 2 issues all.
 template <bool kBf16, bool kFine, int kWhich, int HD, bool kKeys>
 __device__ __forceinline__ void BwdMma(const AttnMaps& maps, const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w,
                                        uint32_t u0, uint32_t n, Owed& owed, Waiter& wait) {
   using Cfg = BwdCfg<HD>;
-  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs, XB = Cfg::kXBufs, NS = Cfg::kSets, kUnit = Cfg::kUnit;
+  constexpr int ST = Cfg::kStages, NS = Cfg::kSets, kUnit = Cfg::kUnit;
   const int ksteps = (p.d + 15) >> 4, n_out = ksteps * 16;
-  const uint32_t x1 = m.X(n), x2 = x1 + Cfg::kTileBytes;
+  const uint32_t x1 = m.X(), x2 = x1 + Cfg::kTileBytes;
   u0 = Uniform(u0);
   n  = Uniform(n);
   const uint32_t end = u0 + w.total;
-  auto arrived = [&](uint32_t u) { return wait(m.Full(u), u / ST); };
-  if (kWhich == 0 && XB == 1) BwdSettle(maps, m, owed, wait);  // this piece's X comes to the same place
-  wait(m.XFull(n), n / XB);
-  if (kWhich == 0) {
-    auto scores = [&](uint32_t u) {
-      IssueScores<kBf16, HD, kUnit>(m.S(u), x1, m.Y(u), ksteps);
-      BarCommit(m.SFull(u));
-      if (u + 1 == end) BarCommit(m.XEmpty(n));
-    };
-    for (uint32_t u = u0; u < min(u0 + SB, end) && arrived(u); ++u)
-      if (ElectOne()) scores(u);
-    BwdSettle(maps, m, owed, wait);
-    owed = Owed{w.b, w.head, w.x0, kKeys, n};
-    for (uint32_t u = u0; u < end && wait.ok; ++u) {
-      const uint32_t next = u + SB;
-      if ((next < end && !arrived(next)) || !wait(m.SDone(u), u / SB)) break;
+  int at = 0;  // the next unit's place within its head
+  auto arrived = [&](uint32_t u) {
+    if (!wait(m.Full(u), u / ST)) return false;
+    if (!Cfg::kClears && ++at == w.per) {
+      at = 0;
+      if (w.ragged) ClearRows<kUnit>(m.Y(u), 2 * (HD / 64), w.len % kUnit);
+    }
+    return true;
+  };
+  auto scores = [&](uint32_t u) {
+    IssueScores<kBf16, HD, kUnit>(m.S(u), x1, m.Y(u), ksteps);
+    BarCommit(m.SFull(u));
+    if (kWhich == 0 && u + 1 == end) BarCommit(m.XEmpty());
+  };
+  auto grads = [&](uint32_t u) {
+    IssueScores<kBf16, HD, kUnit>(m.Dp(u), x2, m.Y(u) + Cfg::kUnitBytes, ksteps);
+    BarCommit(m.DpFull(u));
+    if (u + 1 == end) BarCommit(m.XEmpty());
+  };
+  if (kWhich != 1) BwdSettle(maps, m, owed, wait);  // this piece's X comes to the same place
+  wait(m.XFull(), n);
+  for (uint32_t u = u0; u < min(u0 + NS, end) && arrived(u); ++u)
+    if (ElectOne()) {
+      if (kWhich != 1) scores(u);
+      if (kWhich != 0) grads(u);
+    }
+  if (kWhich != 1) owed = Owed{w.b, w.head, w.x0, kKeys, n};
+  for (uint32_t u = u0; u < end && wait.ok; ++u) {
+    const uint32_t next = u + NS;
+    if (next < end && !arrived(next)) break;
+    if (kWhich != 1) {
+      if (!wait(m.SDone(u), u / NS)) break;
       if (ElectOne()) {
         if (kKeys) IssueFromTmem<kBf16, kUnit, 32>(m.Acc(1), m.S(u), m.Y(u) + Cfg::kUnitBytes, n_out, u > u0);
-        BarCommit(m.Empty(u));
+        if (kWhich == 0) BarCommit(m.Empty(u));
         if (next < end) scores(next);  // in the place of P, which the product before it reads
       }
     }
-  } else {
-    auto grads = [&](uint32_t u) {
-      IssueScores<kBf16, HD, kUnit>(m.Dp(u), x2, m.Y(u) + Cfg::kUnitBytes, ksteps);
-      BarCommit(m.DpFull(u));
-      if (u + 1 == end) BarCommit(m.XEmpty(n));
-    };
-    for (uint32_t u = u0; u < min(u0 + NS, end) && arrived(u); ++u)
-      if (ElectOne()) grads(u);
-    for (uint32_t u = u0; u < end && wait.ok; ++u) {
-      if ((u + NS < end && !arrived(u + NS)) || !wait(m.DsFull(u), u / NS)) break;
-      if (u == u0 && n > 0 && !wait(m.base + Cfg::kAccFree, n - 1)) break;
+    if (kWhich != 0) {
+      if (!wait(m.DsFull(u), u / NS)) break;
+      if (kWhich == 1 && u == u0 && n > 0 && !wait(m.base + Cfg::kAccFree, n - 1)) break;
       if (ElectOne()) {
         IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(u), m.Y(u), n_out, u > u0);
         if (kFine) IssueFromTmem<kBf16, kUnit, 32>(m.Acc(0), m.Dp(u) + 16, m.Y(u), n_out, true);
         BarCommit(m.Empty(u));
-        if (u + NS < end) grads(u + NS);
+        if (next < end) grads(next);
       }
     }
   }
@@ -1155,19 +1162,19 @@ template <bool kBf16, bool kFine, int HD, bool kKeys>
 __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD>& m, const BwdPiece<kKeys>& w, uint32_t u0, uint32_t n,
                                            Waiter& wait) {
   using Cfg = BwdCfg<HD>;
-  constexpr int ST = Cfg::kStages, SB = Cfg::kSBufs, NS = Cfg::kSets, kUnit = Cfg::kUnit;
+  constexpr int ST = Cfg::kStages, NS = Cfg::kSets, kUnit = Cfg::kUnit;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3;      // TMEM lanes
-  const int set = NS == 1 ? 0 : warp >> 3;
-  const int col = ((warp >> 2) & (4 / NS - 1)) * 32;  // first column of this warp in a unit
+  const int set = warp / Cfg::kSetWarps;
+  const int col = warp / 4 % 2 * 32;  // first column of this warp in a unit
   const int row = w.x0 + quarter * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
   F2 row_l{}, row_d{};  // -L, -D
   if (w.total > 0) {
     if (!kKeys) {
-      wait(m.XFull(n), n / Cfg::kXBufs);
-      row_l = Both(LoadShared(m.XRows(n) + (quarter * 32 + lane) * 4));
-      row_d = Both(LoadShared(m.XRows(n) + (kTile + quarter * 32 + lane) * 4));
+      wait(m.XFull(), n);
+      row_l = Both(LoadShared(m.XRows() + (quarter * 32 + lane) * 4));
+      row_d = Both(LoadShared(m.XRows() + (kTile + quarter * 32 + lane) * 4));
     }
   }
   const F2 c2 = Both(p.c), grad2 = Both(kBf16 ? 1.f : TwoTo(w.exponent - kHalfP));
@@ -1175,7 +1182,7 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
   for (uint32_t u = u0 + at; u < u0 + w.total; u += NS, at += NS) {
     if (at >= w.per) at %= w.per;  // the group's next head
     const int y0 = (w.first + at) * kUnit;
-    if (!wait(m.SFull(u), u / SB)) break;
+    if (!wait(m.SFull(u), u / NS)) break;
     uint32_t s[32];
     TmemLoad32Async(m.S(u) + lanes + col, s);
     const bool here = !kKeys || wait(m.Full(u), u / ST);  // -L and -D
@@ -1255,15 +1262,14 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
   if (w.total > 0) wait(m.base + Cfg::kAccFull, n);
   if (!wait.ok) return;
   const bool live = row < w.len;
-  constexpr int kCols = HD / 4;
-  const int c0 = (warp >> 2) * kCols, r = quarter * 32 + lane;
+  constexpr int kCols = 32;  // of the accumulators, for every warp
+  const int c0 = warp / 4 * kCols, r = quarter * 32 + lane;
   if (w.total > 0) {  // dK (dQ) into the place of X1, dV of X2
 #pragma unroll
     for (int out = 0; out < (kKeys ? 2 : 1); ++out) {
       uint32_t o[kCols];
-      if constexpr (kCols == 32) TmemLoad32(m.Acc(out) + lanes + c0, o);
-      else TmemLoad16(m.Acc(out) + lanes + c0, o);
-      StageCols<kBf16, kCols>(m.X(n) + out * Cfg::kTileBytes, r, c0, o,
+      TmemLoad32(m.Acc(out) + lanes + c0, o);
+      StageCols<kBf16, kCols>(m.X() + out * Cfg::kTileBytes, r, c0, o,
                               out ? (kBf16 ? 1.f : TwoTo(-kHalfP)) : kBf16 ? p.scale : p.scale * TwoTo(-w.exponent), live);
     }
     TcFenceBefore();
@@ -1271,18 +1277,18 @@ __device__ __forceinline__ void BwdSoftmax(const AttnParams& p, const BwdSmem<HD
     __syncwarp();
     if (lane == 0) BarArrive(m.base + Cfg::kAccFree);
   } else {
-    const int first = w.x0 + warp * (kTile / kSoftWarps);
+    const int first = w.x0 + warp * (kTile / Cfg::kSoftWarps);
 #pragma unroll
     for (int out = 0; out < (kKeys ? 2 : 1); ++out)
       StoreZeroRows(out ? p.dv : kKeys ? p.dk : p.dq, out ? p.sdv : kKeys ? p.sdk : p.sdq, w.b, w.head, first,
-                    min(first + kTile / kSoftWarps, p.s), p.d);
+                    min(first + kTile / Cfg::kSoftWarps, p.s), p.d);
   }
 }
 
 // Both passes in one launch, so that neither leaves a tail of idle SMs.  kFine: dS as a sum of two values (a branch in the loop
 // instead costs long sequences 4 %).
 template <int HD, bool kBf16, bool kFine>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(BwdCfg<HD>::kThreads, BwdCfg<HD>::kBlocks)
 AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ AttnParams p) {
   using Cfg = BwdCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
@@ -1290,30 +1296,26 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   const Pieces pieces{m.base + Cfg::kNext};
   const int warp = Uniform(threadIdx.x >> 5);
   if (threadIdx.x == 0) {
-    pieces.Init(kWarps - 1);
+    pieces.Init(Cfg::kThreads / 32 - 1);
     for (int i = 0; i < Cfg::kStages; ++i) {
       BarInit(m.Full(i), 1);
-      BarInit(m.Empty(i), 2);  // both MMA warps
+      BarInit(m.Empty(i), Cfg::kMmaWarps);
       BarInit(m.Raw(i), 1);
     }
-    for (int i = 0; i < Cfg::kXBufs; ++i) {
-      BarInit(m.XFull(i), 1);
-      BarInit(m.XEmpty(i), 3);  // both MMA warps are done with it, and the sums that took its place are stored
-    }
-    for (int i = 0; i < Cfg::kSBufs; ++i) {
-      BarInit(m.SFull(i), 1);
-      BarInit(m.SDone(i), kSoftWarps / Cfg::kSets);
-    }
+    BarInit(m.XFull(), 1);
+    BarInit(m.XEmpty(), Cfg::kMmaWarps + 1);  // the products are done with it, and the sums that took its place are stored
     for (int i = 0; i < Cfg::kSets; ++i) {
+      BarInit(m.SFull(i), 1);
+      BarInit(m.SDone(i), Cfg::kSetWarps);
       BarInit(m.DpFull(i), 1);
-      BarInit(m.DsFull(i), kSoftWarps / Cfg::kSets);
-      BarInit(m.Turn(i), kSoftWarps / Cfg::kSets);
+      BarInit(m.DsFull(i), Cfg::kSetWarps);
+      BarInit(m.Turn(i), Cfg::kSetWarps);
     }
-    BarInit(m.base + Cfg::kAccFull, 2);
-    BarInit(m.base + Cfg::kAccFree, kSoftWarps);
+    BarInit(m.base + Cfg::kAccFull, Cfg::kMmaWarps);
+    BarInit(m.base + Cfg::kAccFree, Cfg::kSoftWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == kMmaWarp) AllocTmem(m.base + Cfg::kTmemSlot, 512);
+  if (warp == Cfg::kMmaWarp) AllocTmem(m.base + Cfg::kTmemSlot, Cfg::kColumns);
   TcFenceBefore();
   __syncthreads();
   TcFenceAfter();
@@ -1334,30 +1336,31 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
     int v[8];
     for (uint32_t turn = 0; pieces.Take<decltype(idle)::value>(turn, v); ++turn) each(v, step);
   };
-  if (warp == kTmaWarp) {
+  if (warp == Cfg::kTmaWarp) {
     if (ElectOne()) {
       const bool ok = pieces.Lead([&](int index, int (&v)[8]) { BwdWords::Describe<Cfg::kUnit, kBf16>(p, index, v); }, [&](const int (&v)[8]) {
         return each(v, [&](const auto& w) { return w.total == 0 || BwdLoad(maps, p, m, w, u0, n); });
       });
       if (!ok) atomicExch(&g_attn_error, 5);
     }
-  } else if (warp == kClearWarp) {
+  } else if (warp == Cfg::kClearWarp) {
     uint32_t uses = 0;
     IdleWaiter wait(6);
     follow(std::true_type{}, [&](const auto& w) {
       BwdClear(m, w, u0, uses, wait);
       return true;
     });
-  } else if (warp == kMmaWarp) {
+  } else if (warp == Cfg::kMmaWarp) {
+    constexpr int kWhich = Cfg::kMmaWarps == 1 ? 2 : 0;
     Waiter wait(6);
     Owed owed;
     follow(std::false_type{}, [&](const auto& w) {
-      if (w.total > 0 && wait.ok) BwdMma<kBf16, kFine, 0>(maps, p, m, w, u0, n, owed, wait);
+      if (w.total > 0 && wait.ok) BwdMma<kBf16, kFine, kWhich>(maps, p, m, w, u0, n, owed, wait);
       return true;
     });
     if (wait.ok) BwdSettle(maps, m, owed, wait);
     if (ElectOne()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  } else if (warp == kMmaWarp + 1) {
+  } else if (Cfg::kMmaWarps == 2 && warp == Cfg::kMmaWarp + 1) {
     Waiter wait(6);
     Owed none;
     follow(std::false_type{}, [&](const auto& w) {
@@ -1373,7 +1376,8 @@ AttnBwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
   }
   TcFenceBefore();
   __syncthreads();
-  if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(m.tmem), "r"(512u) : "memory");
+  if (warp == Cfg::kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(m.tmem), "r"(static_cast<uint32_t>(Cfg::kColumns)) : "memory");
 }
 
 // ---------------------------------------------------------------- host side
@@ -1468,7 +1472,7 @@ int LaunchBwd(const AttnMaps& maps, const AttnParams& p, cudaStream_t s) {
   AttnDeltaKernel<kBf16><<<dim3(std::min(p.sp / 32, 4096), runs, p.b), 256, 0, s>>>(p);
   TIPSK_LAUNCH_CHECK();
   const int grid = (p.sp / kTile) * p.b * (p.h + p.hk);
-  AttnBwdKernel<HD, kBf16, kFine><<<grid, kThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
+  AttnBwdKernel<HD, kBf16, kFine><<<grid, BwdCfg<HD>::kThreads, BwdCfg<HD>::kSmemBytes, s>>>(maps, p);
   TIPSK_LAUNCH_CHECK();
   return 0;
 }
