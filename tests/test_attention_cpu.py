@@ -64,7 +64,7 @@ def test_the_library_refuses_before_it_reads():
                                        a["scale"], 0, None)
 
     for kw in (dict(d=0), dict(d=12), dict(d=136), dict(hk=3), dict(h=0), dict(hk=0), dict(b=0), dict(s=0), dict(dtype=0),
-               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=3e38), dict(s=1 << 30, b=1 << 10), dict(h=1 << 18, hk=1 << 18),
+               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=3e38), dict(s=1 << 30, b=1 << 10), dict(h=1 << 18, hk=1 << 18), dict(s=(1 << 24) + 1, h=4, hk=2),
                dict(at=4100)):
         assert call(**kw) == -2, kw
     for i, x in ((1, 132), (3, 0), (8, -64), (11, 4)):

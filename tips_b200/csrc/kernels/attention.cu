@@ -1428,7 +1428,7 @@ int CheckSizes(int b, int s, int h, int hk, int d, int dtype, float scale) {
   TIPSK_REQUIRE(d > 0 && d <= 128 && d % 8 == 0, "attention: the head size must be a multiple of 8 up to 128");
   TIPSK_REQUIRE(scale > 0.f && std::isfinite(scale * kLog2e), "attention: scale must be positive and finite");
   // a tile's stream past a group's heads has to end well within the kernels' bounded waits
-  TIPSK_REQUIRE(b <= 65535 && h <= (1 << 17) && static_cast<int64_t>(s) * (h / hk) <= (1 << 26) &&
+  TIPSK_REQUIRE(b <= 65535 && h <= (1 << 17) && static_cast<int64_t>(s) * (h / hk) <= (1 << 25) &&
                     static_cast<int64_t>(b) * (h + hk) * TilesOf(s, kTile) < (int64_t{1} << 31),
                 "attention: too many rows for one launch");
   return 0;
