@@ -261,3 +261,21 @@ def test_encoder_keeps_less_and_trains_alike():
         if p.grad is not None and float(p.grad.float().norm()) > 0 and "qkv.bias" not in name:
             # a stored value is off by 0.8 % of its block's root mean square; through two layers that stays within 10 %
             assert (p.grad.float() - q.grad.float()).norm() <= 0.1 * p.grad.float().norm(), name
+
+
+def test_the_largest_fp16_values():
+    x = torch.randn(9, 32, device=DEV).to(torch.float16)
+    x[0, :3], x[4, 1], x[8, 30:] = torch.tensor([65504.0, 65030.0, -65024.0]), -65504.0, torch.tensor([65504.0, math.nan])
+    for y in (x, x.view(-1)[:101], x.float() * 4):  # whole blocks, a last one of five values, values beyond fp16
+        same(y)
+    y = pack8(x).unpack()
+    assert bool((y.isfinite() == x.isfinite()).all())
+    w = torch.zeros(64, 32, device=DEV, dtype=torch.float16, requires_grad=True)
+    dy = torch.full((9, 64), 2.0 ** -10, device=DEV, dtype=torch.float16)
+    dy[:, 3] = 0.0
+    (dw,) = torch.autograd.grad(linear(x[:8], w, save8=True), w, dy[:8])
+    kept = y[:8].double()
+    want = dy[:8].double().t() @ kept
+    # a half step of the result; sums of eight addends in 32 bits
+    bound = 2.0 ** -11 * want.abs() + 8 * 2.0 ** -24 * (dy[:8].double().t() @ kept.abs()) + 2.0 ** -25
+    assert bool(((dw.double() - want).abs() <= bound).all())

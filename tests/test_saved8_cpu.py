@@ -122,3 +122,28 @@ def test_module():
     y, alias = a(x, passthrough=True)
     assert torch.equal(y, b(x)) and torch.equal(alias, x)
     assert isinstance(pack8(x), Packed8)
+
+
+def test_the_largest_fp16_values_stay_finite():
+    """From 65024 on a value is stored as 64 * 2^10 = 65536, which fp16 does not have."""
+    x = torch.tensor([65504.0, 65030.0, -65504.0, -65024.0, 64999.0, 1000.0, 3.0, math.inf], dtype=torch.float16)
+    p = pack8(x)
+    assert p.unpack(torch.float32).tolist()[:5] == [65536.0, 65536.0, -65536.0, -65536.0, 64512.0]
+    y = p.unpack()
+    assert y.tolist()[:7] == [65504.0, 65504.0, -65504.0, -65504.0, 64512.0, 1024.0, 0.0] and bool(y[7].isnan())
+    assert bool(((y.double() - x.double())[:7].abs() <= 512).all())  # half a step
+    # another type's values beyond fp16's range are as far beyond it as they were
+    assert pack8(x.float()).unpack(torch.float16).tolist()[:2] == [math.inf, math.inf]
+
+
+def test_fp16_weight_gradient_at_the_top_of_the_range():
+    x = torch.full((4, 32), 1.0, dtype=torch.float16)
+    x[0, :2], x[3, 1] = torch.tensor([65504.0, 65100.0]), -65504.0
+    w = torch.zeros(8, 32, dtype=torch.float16, requires_grad=True)
+    dy = torch.full((4, 8), 2.0 ** -10, dtype=torch.float16)
+    dy[:, 3] = 0.0
+    (dw,) = torch.autograd.grad(linear(x, w, save8=True), w, dy)
+    want = dy.double().t() @ pack8(x).unpack().double()
+    # a half step of the result; sums of four addends in 32 bits
+    bound = 2.0 ** -11 * want.abs() + 4 * 2.0 ** -24 * (dy.double().t() @ x.double().abs())
+    assert bool(((dw.double() - want).abs() <= bound).all()) and not dw[3].any()

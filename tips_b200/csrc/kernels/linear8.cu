@@ -119,7 +119,7 @@ int tipsk_linear8_bwd(const void* dy, const void* w, const void* x8, const void*
   }
   if (rc == 0 && dw) {
     const int64_t mk = static_cast<int64_t>(m) * k;
-    rc = tipsk_unpack8(x8, static_cast<const char*>(x8) + ExponentsAt(mk), f.x, mk, kBF16, stream);
+    rc = tipsk_unpack8(x8, static_cast<const char*>(x8) + ExponentsAt(mk), f.x, mk, kBF16, 0, stream);
     const int splits = tipsk_gemm_splits(n, k, m);
     if (rc == 0) {
       rc = splits > 1 ? tipsk_gemm_bf16_split(2, dz, f.x, dw, nullptr, nullptr, partial, splits, n, k, m, n, k, k, 0, 0, stream)

@@ -76,9 +76,20 @@ __global__ void __launch_bounds__(256) Pack8Kernel(const T* __restrict__ x, int8
   }
 }
 
+// A stored value in fp16, at most `most` in magnitude (infinity: as it is).  What was fp16 may have been stored as 64 * 2^10, the first
+// number beyond fp16's 65504, from which 65504 is no further off than half a step, like what it stands for.
+__device__ __forceinline__ __half FromStored(float x, float most, __half) {
+  return FromFloat<__half>(x > most ? most : x < -most ? -most : x);  // a NaN stays one
+}
+template <typename T>
+__device__ __forceinline__ T FromStored(float x, float, T) {
+  return FromFloat<T>(x);
+}
+
 // Eight values per thread and step, four steps in flight.  Bound by HBM: 16384 x 4096 into bf16, 203 MB in 33 us (6.2 TB/s).
 template <typename T>
-__global__ void __launch_bounds__(256) Unpack8Kernel(const int8_t* __restrict__ q, const int8_t* __restrict__ e, T* __restrict__ y, int64_t n) {
+__global__ void __launch_bounds__(256) Unpack8Kernel(const int8_t* __restrict__ q, const int8_t* __restrict__ e, T* __restrict__ y, int64_t n,
+                                                     float most) {
   constexpr int N = 16 / sizeof(T), U = 4;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g * 8 < n; g += U * stride) {
@@ -102,11 +113,11 @@ __global__ void __launch_bounds__(256) Unpack8Kernel(const int8_t* __restrict__ 
         for (int k = 0; k < 8; k += N) {
           Vec16<T> o;
 #pragma unroll
-          for (int j = 0; j < N; ++j) o.v[j] = FromFloat<T>(v[k + j]);
+          for (int j = 0; j < N; ++j) o.v[j] = FromStored(v[k + j], most, T{});
           StoreVec(y + at + k, o);
         }
       } else {
-        for (int j = 0; at + j < n; ++j) y[at + j] = FromFloat<T>(Dequantise(q[at + j], PowerOfTwo(ex[u])));
+        for (int j = 0; at + j < n; ++j) y[at + j] = FromStored(Dequantise(q[at + j], PowerOfTwo(ex[u])), most, T{});
       }
     }
   }
@@ -254,16 +265,18 @@ int tipsk_pack8(const void* x, void* q, void* e, int64_t n, int dtype, void* str
   return 0;
 }
 
-/* y[n] = the values that q, e stand for; exact in fp32 and bf16, rounded to fp16 where that has fewer bits (below 2^-14). */
-int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, void* stream) {
+/* y[n] = the values that q, e stand for; exact in fp32 and bf16, rounded to fp16 where that has fewer bits (below 2^-14).  Values
+ * beyond fp16's range become infinite, or with `from_half`, which says that fp16 was packed, the nearest that it has. */
+int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, int from_half, void* stream) {
   TIPSK_REQUIRE(n > 0 && (dtype == kF32 || dtype == kBF16 || dtype == kF16), "unpack8: fp32, bf16 or fp16 and at least one value");
   TIPSK_REQUIRE(Aligned16(y) && Aligned16(q), "unpack8: the values must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int grid = Blocks((n + 7) / 8, 8);
   const int8_t *qq = static_cast<const int8_t*>(q), *ee = static_cast<const int8_t*>(e);
-  if (dtype == kF32) Unpack8Kernel<float><<<grid, 256, 0, s>>>(qq, ee, static_cast<float*>(y), n);
-  else if (dtype == kBF16) Unpack8Kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(qq, ee, static_cast<__nv_bfloat16*>(y), n);
-  else Unpack8Kernel<__half><<<grid, 256, 0, s>>>(qq, ee, static_cast<__half*>(y), n);
+  const float most = from_half ? 65504.f : INFINITY;
+  if (dtype == kF32) Unpack8Kernel<float><<<grid, 256, 0, s>>>(qq, ee, static_cast<float*>(y), n, most);
+  else if (dtype == kBF16) Unpack8Kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(qq, ee, static_cast<__nv_bfloat16*>(y), n, most);
+  else Unpack8Kernel<__half><<<grid, 256, 0, s>>>(qq, ee, static_cast<__half*>(y), n, most);
   TIPSK_LAUNCH_CHECK();
   return 0;
 }

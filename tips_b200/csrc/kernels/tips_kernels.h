@@ -242,7 +242,7 @@ int tipsk_attention_status(void);
 
 /* ---- activations in 8 bits (saved8.cu): q int8 per value, e int8 per block of 32, the step of a block is 2^e ---- */
 int tipsk_pack8(const void* x, void* q, void* e, int64_t n, int dtype, void* stream);
-int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, void* stream);
+int tipsk_unpack8(const void* q, const void* e, void* y, int64_t n, int dtype, int from_half, void* stream);
 int tipsk_act_bwd8_parts(int64_t rows, int cols);
 int tipsk_act_bwd8(const void* dy, const void* q, const void* e, void* dz, void* dbias, int bias_dtype, float* partial,
                    int64_t rows, int cols, int dtype, void* stream);

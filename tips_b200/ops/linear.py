@@ -204,7 +204,7 @@ def _linear8_backward(ctx, dy, d_alias):
         dx = _input_grad(dz, weight, d_alias).view(ctx.in_shape) if want_dx else None
         dw = None
         if want_dw:
-            dw = _weight_grad8(dz, saved8._unpack(x8, (m, k), ctx.x_dtype), weight.dtype).to(weight.dtype)
+            dw = _weight_grad8(dz, saved8._unpack(x8, (m, k), ctx.x_dtype, ctx.x_dtype), weight.dtype).to(weight.dtype)
         return dx, dw, db, None
     lib = base.K()
     with base.device_of(dz):

@@ -2,8 +2,9 @@
 
 ``pack8(x)`` stores a tensor in 33 bytes per 32 values and ``Packed8.unpack()`` reads it back.  The values of a block of 32
 (of the flattened tensor) share a power-of-two step: the least one for which the block's largest magnitude rounds to at
-most 127 of them.  A stored value is off by at most half a step, 1/127 of that magnitude; it is exact in fp32 and bf16.  A
-value that is not finite comes back as NaN.
+most 127 of them.  A stored value is off by at most half a step (a whole one where fp32's range ends), 1/127 of that
+magnitude; it is exact in fp32 and bf16, and read back into the packed tensor's own type it is finite.  A value that is not
+finite comes back as NaN.
 
 ``linear(..., save8=True)`` (and ``Linear``, ``BertMLM``) keeps its input and, with GELU, its pre-activation that way instead of
 in 16 bits: outputs and the input's gradient path are computed as before, the weight gradient from the stored input and the
@@ -21,6 +22,7 @@ from . import base
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 BLOCK = 32  # values that share a step
+_HALF_MAX = torch.finfo(torch.float16).max
 
 
 def _check(dtype, what):
@@ -61,10 +63,11 @@ def _pack_plain(x: torch.Tensor, buf: torch.Tensor) -> None:
     exponents.copy_(e.view(-1))
 
 
-def _unpack_plain(buf: torch.Tensor, n: int, dtype) -> torch.Tensor:
+def _unpack_plain(buf: torch.Tensor, n: int, dtype, from_half: bool) -> torch.Tensor:
     q, e = _parts(buf, n)
     step = ((e.to(torch.int32) + 127) << 23).view(torch.float32).repeat_interleave(BLOCK)[:n]
-    return torch.where(q == -128, float("nan"), q.float() * step).to(dtype)
+    x = torch.where(q == -128, float("nan"), q.float() * step)
+    return (x.clamp(-_HALF_MAX, _HALF_MAX) if from_half and dtype == torch.float16 else x).to(dtype)
 
 
 def _buffer(n: int, device) -> torch.Tensor:
@@ -87,15 +90,19 @@ def _pack(x: torch.Tensor) -> torch.Tensor:
     return buf
 
 
-def _unpack(buf: torch.Tensor, shape, dtype) -> torch.Tensor:
+def _unpack(buf: torch.Tensor, shape, dtype, packed) -> torch.Tensor:
+    """The values of a buffer in `dtype`; `packed`: the type of the tensor that was packed.  The largest fp16 values may be stored as
+    65536, which fp16 does not have: read back into it they are its largest number, which is within half a step of them as well."""
+    from_half = packed == torch.float16
     if not buf.is_cuda:
-        return _unpack_plain(buf, math.prod(shape), dtype).view(shape)
+        return _unpack_plain(buf, math.prod(shape), dtype, from_half).view(shape)
     y = torch.empty(shape, dtype=dtype, device=buf.device)
     n = y.numel()
     if n:
         with base.device_of(y):
             q = buf.data_ptr()
-            base.check(base.K().tipsk_unpack8(q, q + _exponents_at(n), y.data_ptr(), n, base.code(y), base.stream()), "unpack8")
+            base.check(base.K().tipsk_unpack8(q, q + _exponents_at(n), y.data_ptr(), n, base.code(y), int(from_half), base.stream()),
+                       "unpack8")
     return y
 
 
@@ -121,11 +128,11 @@ class Packed8:
         return self.buf.numel()
 
     def unpack(self, dtype: torch.dtype | None = None) -> torch.Tensor:
-        """The stored values, in `dtype` (default: that of the packed tensor).  fp16 rounds values below 2**-14 once more,
-        and values beyond its range become infinite."""
+        """The stored values, in `dtype` (default: that of the packed tensor).  fp16 rounds values below 2**-14 once more; values
+        beyond its range become infinite if another type was packed, and its largest number if it was fp16."""
         dtype = self.dtype if dtype is None else dtype
         _check(dtype, "unpack")
-        return _unpack(self.buf, self.shape, dtype)
+        return _unpack(self.buf, self.shape, dtype, self.dtype)
 
 
 def pack8(x: torch.Tensor) -> Packed8:
@@ -161,7 +168,7 @@ def act_bwd8(dy: torch.Tensor, z: torch.Tensor | None, bias_dtype=None):
         return (dy if dz is None else dz), db
     dz = dy.float()
     if z is not None:
-        v = _unpack(z, dy.shape, torch.float32)
+        v = _unpack(z, dy.shape, torch.float32, dy.dtype)
         dz = dz * (0.5 * (1 + torch.erf(v * 0.7071067811865476)) + v * torch.exp(-0.5 * v * v) * 0.3989422804014327)
         dy = dz.to(dy.dtype)
     return dy, None if bias_dtype is None else dz.sum(0).to(bias_dtype)
