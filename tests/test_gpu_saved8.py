@@ -279,3 +279,20 @@ def test_the_largest_fp16_values():
     # a half step of the result; sums of eight addends in 32 bits
     bound = 2.0 ** -11 * want.abs() + 8 * 2.0 ** -24 * (dy[:8].double().t() @ kept.abs()) + 2.0 ** -25
     assert bool(((dw.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_no_kernel_packs_without_a_backward_pass_to_come(act):
+    """One launch, that of the product, and the same output."""
+    from tips_b200.ops import base
+    g = torch.Generator(device=DEV)
+    g.manual_seed(7)
+    x = torch.randn(300, 128, generator=g, device=DEV).to(torch.bfloat16)
+    w = torch.randn(256, 128, generator=g, device=DEV).to(torch.bfloat16).requires_grad_()
+    want = linear(x, w, None, act, save8=True)
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            for fn in (lambda: linear(x, w, None, act, save8=True), lambda: linear_passthrough(x, w, None, act, save8=True)[0]):
+                before = base.launches()
+                y = fn()
+                assert base.launches() == before + 1 and torch.equal(y, want)

@@ -147,3 +147,19 @@ def test_fp16_weight_gradient_at_the_top_of_the_range():
     # a half step of the result; sums of four addends in 32 bits
     bound = 2.0 ** -11 * want.abs() + 4 * 2.0 ** -24 * (dy.double().t() @ x.double().abs())
     assert bool(((dw.double() - want).abs() <= bound).all()) and not dw[3].any()
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_nothing_is_packed_without_a_backward_pass_to_come(mode, monkeypatch):
+    from tips_b200.ops import saved8
+    packed = []
+    pack = saved8._pack
+    monkeypatch.setattr(saved8, "_pack", lambda t: packed.append(t.shape) or pack(t))
+    x = torch.randn(10, 24)
+    layer = Linear(24, 16, act="gelu", save8=True)
+    with mode():
+        y = layer(x)
+        for t in linear_passthrough(x, layer.weight, layer.bias, "gelu", save8=True):
+            assert not t.requires_grad
+    assert packed == []
+    assert torch.equal(layer(x), y) and len(packed) == 2

@@ -170,14 +170,15 @@ def _linear8_forward(x2, weight, bias, act, want_x8, want_pre8):
 
 
 class _Linear8Fn(torch.autograd.Function):
-    """linear(x) that keeps x and, with GELU, the value before the activation in 8 bits (ops/saved8.py)."""
+    """linear(x) that keeps x and, with GELU, the value before the activation in 8 bits (ops/saved8.py).  `grad`: whether a backward
+    pass can follow, which needs_input_grad does not tell (it is set for parameters without a grad mode as well)."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, act):
+    def forward(ctx, x, weight, bias, act, grad):
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         if not x2.is_contiguous():
             x2 = x2.contiguous()
-        need = ctx.needs_input_grad
+        need = [grad and n for n in ctx.needs_input_grad[:3]]
         y, x8, pre8 = _linear8_forward(x2, weight, bias, act, need[1], _ACT[act] == 2 and (need[0] or need[1] or need[2]))
         ctx.save_for_backward(weight, x8, pre8)
         ctx.x_dtype, ctx.bias_dtype = x.dtype, None if bias is None else bias.dtype
@@ -205,7 +206,7 @@ def _linear8_backward(ctx, dy, d_alias):
         dw = None
         if want_dw:
             dw = _weight_grad8(dz, saved8._unpack(x8, (m, k), ctx.x_dtype, ctx.x_dtype), weight.dtype).to(weight.dtype)
-        return dx, dw, db, None
+        return dx, dw, db, None, None
     lib = base.K()
     with base.device_of(dz):
         into = _accumulator(d_alias, k, dz) if want_dx else None
@@ -218,15 +219,15 @@ def _linear8_backward(ctx, dy, d_alias):
                                          base.ptr(db), 0 if db is None else base.code(db), base.ptr(ws), m, n, k, weight.stride(0),
                                          int(into is not None), base.stream()), "linear8_bwd")
     base.count_launches(int(pre8 is not None or want_db is not None) + int(want_db is not None) + int(want_dx) + 2 * int(want_dw) - 1)
-    return dx if dx is None or len(ctx.in_shape) == 2 else dx.view(ctx.in_shape), dw, db, None
+    return dx if dx is None or len(ctx.in_shape) == 2 else dx.view(ctx.in_shape), dw, db, None, None
 
 
 class _Linear8PassFn(torch.autograd.Function):
     """_LinearPassFn with the activations in 8 bits."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, act):
-        y = _Linear8Fn.forward(ctx, x, weight, bias, act)
+    def forward(ctx, x, weight, bias, act, grad):
+        y = _Linear8Fn.forward(ctx, x, weight, bias, act, grad)
         return y, x.detach()
 
     @staticmethod
@@ -332,7 +333,7 @@ def linear(x, weight, bias=None, act=None, save8=False):
     pre-activation, which is rounded to x's type before it is stored.  Gradients of gradients are refused."""
     if save8:
         _check_save8(x, act)
-        return _Linear8Fn.apply(x, weight, bias, act)
+        return _Linear8Fn.apply(x, weight, bias, act, torch.is_grad_enabled())
     return _LinearFn.apply(x, weight, bias, act)
 
 
@@ -341,7 +342,9 @@ def linear_passthrough(x, weight, bias=None, act=None, save8=False):
     if save8:
         _check_save8(x, act)
     if x.is_cuda and x.dtype == torch.bfloat16:
-        return (_Linear8PassFn if save8 else _LinearPassFn).apply(x, weight, bias, act)
+        if save8:
+            return _Linear8PassFn.apply(x, weight, bias, act, torch.is_grad_enabled())
+        return _LinearPassFn.apply(x, weight, bias, act)
     return linear(x, weight, bias, act, save8), x
 
 
