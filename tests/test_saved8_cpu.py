@@ -163,3 +163,14 @@ def test_nothing_is_packed_without_a_backward_pass_to_come(mode, monkeypatch):
             assert not t.requires_grad
     assert packed == []
     assert torch.equal(layer(x), y) and len(packed) == 2
+
+
+@pytest.mark.parametrize("fn", [linear, linear_passthrough])
+def test_sizes_and_devices_that_do_not_fit_are_refused(fn):
+    """A pass is one call with addresses and sizes, which would read beyond a weight with shorter rows or a shorter bias."""
+    x, w, b = torch.zeros(2, 5, 64), torch.zeros(128, 64), torch.zeros(128)
+    fn(x, w, b, save8=True)
+    for bad in ((x, w[:, :56], b), (x, w[0], b), (x[..., :8], w, b), (x, w, b[:127]), (x, w, b[:1]), (x, w, b[None]), (x[0, 0, 0], w, b),
+                (x, w.to("meta"), None), (x, w, b.to("meta"))):
+        with pytest.raises(ValueError):
+            fn(*bad, save8=True)

@@ -319,10 +319,17 @@ class _LinearPassFn(torch.autograd.Function):
         return _linear_backward(ctx, dy, d_alias)
 
 
-def _check_save8(x, act):
+def _check_save8(x, weight, bias, act):
     if _ACT[act] == 1:
         raise ValueError("save8 keeps the value before a GELU; a ReLU needs one bit per value, which it does not take")
     saved8._check(x.dtype, "save8")
+    # one call runs the whole pass from addresses and sizes: they have to fit each other
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"weight must be [out_features, in_features] and x [..., in_features], got {tuple(weight.shape)} and {tuple(x.shape)}")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != weight.shape[0]):
+        raise ValueError(f"bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    if weight.device != x.device or (bias is not None and bias.device != x.device):
+        raise ValueError(f"x is on {x.device}, weight on {weight.device}" + ("" if bias is None else f", bias on {bias.device}"))
 
 
 def linear(x, weight, bias=None, act=None, save8=False):
@@ -332,7 +339,7 @@ def linear(x, weight, bias=None, act=None, save8=False):
     output is the same; the weight's gradient is computed from the stored x, and with GELU all gradients from the stored
     pre-activation, which is rounded to x's type before it is stored.  Gradients of gradients are refused."""
     if save8:
-        _check_save8(x, act)
+        _check_save8(x, weight, bias, act)
         return _Linear8Fn.apply(x, weight, bias, act, torch.is_grad_enabled())
     return _LinearFn.apply(x, weight, bias, act)
 
@@ -340,7 +347,7 @@ def linear(x, weight, bias=None, act=None, save8=False):
 def linear_passthrough(x, weight, bias=None, act=None, save8=False):
     """(linear(x), alias of x): use the alias for the residual branch; see _LinearPassFn."""
     if save8:
-        _check_save8(x, act)
+        _check_save8(x, weight, bias, act)
     if x.is_cuda and x.dtype == torch.bfloat16:
         if save8:
             return _Linear8PassFn.apply(x, weight, bias, act, torch.is_grad_enabled())
