@@ -346,3 +346,18 @@ def test_encoder_on_a_padded_batch():
     full = torch.full((3,), 64, device=DEV)
     a, b = model.encode(ids), model.encode(ids, full)
     assert (a.float() - b.float()).norm() <= 2 ** -5 * a.float().norm()
+
+
+def test_the_status_waits_for_every_stream():
+    """A launch that is still running, or to come, on a stream of its own is not reported as sound."""
+    from tips_b200.ops.linear import gemm_status
+    q, k, v, do = make(1, 64, 1, 1, 64, torch.bfloat16)
+    run(q, k, v, do)
+    torch.cuda.synchronize()
+    for ask in (status, gemm_status):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(400_000_000)  # about a fifth of a second
+            run(q, k, v, do)
+        assert not side.query()
+        assert ask() == 0 and side.query()

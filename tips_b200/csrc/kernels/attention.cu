@@ -1562,10 +1562,12 @@ int tipsk_attention_bwd(const void* dout, const void* q, const void* k, const vo
   return d <= 64 ? LaunchBwd<64, false>(maps, p, st) : LaunchBwd<128, false>(maps, p, st);
 }
 
-/* Reads and clears the attention error word of the current device (0: ok). Synchronises. */
+/* Reads and clears the attention error word of the current device (0: ok), once all that was launched on any of its streams is
+ * done (a copy by itself waits for the streams that synchronise with the default one only, which PyTorch's do not). */
 int tipsk_attention_status(void) {
   int32_t v = 0;
   const int32_t zero = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -7;
   if (cudaMemcpyFromSymbol(&v, g_attn_error, sizeof(v)) != cudaSuccess) return -7;
   if (v && cudaMemcpyToSymbol(g_attn_error, &zero, sizeof(zero)) != cudaSuccess) return -7;
   return v;

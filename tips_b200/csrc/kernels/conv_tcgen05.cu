@@ -1707,11 +1707,12 @@ int tipsk_stem_conv_wgrad(const void* xp, const void* dy, float* dw, int n, int 
                   static_cast<cudaStream_t>(stream));
 }
 
-/* Reads and clears the convolution error word (0 ok; 1/2/3/4 = which wait ran out). Synchronises. */
+/* Reads and clears the convolution error word (0 ok; 1/2/3/4 = which wait ran out), once all streams of the device are done. */
 int tipsk_conv_status(void) {
   int32_t* w = ConvErrorWord();
   if (!w) return -7;
   int32_t v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -7;
   if (cudaMemcpy(&v, w, sizeof(v), cudaMemcpyDeviceToHost) != cudaSuccess) return -7;
   if (v) cudaMemset(w, 0, sizeof(v));
   return v;

@@ -1266,11 +1266,12 @@ int tipsk_gemm_bf16_tt(const void* a, const void* b, void* c, int m, int n, int 
   return LaunchPair<true, true, kOutPlain>(ta, tb, tc, tc, p, static_cast<cudaStream_t>(stream));
 }
 
-/* Reads and clears the GEMM error word (0 ok; 1/2/3 = producer / MMA / epilogue wait ran out). Synchronises. */
+/* Reads and clears the GEMM error word (0 ok; 1/2/3 = producer / MMA / epilogue wait ran out), once all streams of the device are done. */
 int tipsk_gemm_status(void) {
   int32_t* w = GemmErrorWord();
   if (!w) return -7;
   int32_t v = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return -7;
   if (cudaMemcpy(&v, w, sizeof(v), cudaMemcpyDeviceToHost) != cudaSuccess) return -7;
   if (v) cudaMemset(w, 0, sizeof(v));
   return v;

@@ -236,7 +236,8 @@ class _PackedOwnAttentionFn(torch.autograd.Function):
 
 
 def attention_status() -> int:
-    """0 when no attention launch on the current device since the last call reported a bounded-wait timeout (synchronises)."""
+    """0 when no attention launch on the current device since the last call reported a bounded-wait timeout
+    (waits for all of its streams)."""
     return int(base.K().tipsk_attention_status())
 
 

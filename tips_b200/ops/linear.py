@@ -115,7 +115,7 @@ def _weight_grad(dz: torch.Tensor, x2: torch.Tensor, dtype: torch.dtype | None =
 
 
 def gemm_status() -> int:
-    """0 when no GEMM launch since the last call reported a bounded-wait timeout (synchronises)."""
+    """0 when no GEMM launch since the last call reported a bounded-wait timeout (waits for all streams of the device)."""
     lib = base.K()
     return int(lib.tipsk_gemm_status()) or int(lib.tipsk_conv_status())  # the weight gradient runs on the conv kernels
 
