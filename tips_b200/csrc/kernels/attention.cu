@@ -725,7 +725,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
       const int row = w.q0 + i * kTile + r, count = i ? w.count1 : w.count0;
       float m = 0.f, l = 0.f;  // row maximum (of the raw scores) that the exponents refer to, and the sum
       for (int j = 0; j < count; ++j, ++done) {
-        wait(s_full, done);  // on a failure the values are void, and nothing is stored
+        wait(s_full, done);  // on a failure the values are void: they are neither handed on nor stored
         uint32_t s[kUnit / 32][32];
 #pragma unroll
         for (int g = 0; g < kUnit / 32; ++g) TmemLoad32Async(ts + g * 32, s[g]);
@@ -788,7 +788,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         TmemStoreWait();
         TcFenceBefore();
         __syncwarp();
-        if (lane == 0) BarArrive(p_full);
+        if (lane == 0 && wait.ok) BarArrive(p_full);
       }
       const bool live = row < w.len;
       uint16_t* dst = static_cast<uint16_t*>(p.o) + w.b * p.so.b + row * p.so.s + w.h * p.so.h;
@@ -808,7 +808,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         if (Cfg::kStaged) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) BarArrive(base + Cfg::kOStaged + i * 8);
+          if (lane == 0 && wait.ok) BarArrive(base + Cfg::kOStaged + i * 8);
         }
       }
       pieces_done += w.total > 0;
@@ -816,7 +816,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         const int first = w.q0 + i * kTile + quarter * 32;
         StoreZeroRows(p.o, p.so, w.b, w.h, max(first, w.len), min(first + 32, p.s), p.d);
       }
-      if (row < p.sp)
+      if (row < p.sp && wait.ok)
         p.lse[(static_cast<int64_t>(w.b) * p.h + w.h) * p.sp + row] = live ? fmaf(m, p.c, log2f(l) - (kBf16 ? 0.f : kHalfShift)) : INFINITY;
     }
   }
