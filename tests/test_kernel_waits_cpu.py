@@ -17,3 +17,12 @@ def test_attention_hands_nothing_on_after_a_failed_wait():
     assert softmax.count("BarArrive(") == len(arrivals)
     stores = re.findall(r"if \(([^;]*)\)\s*(?:StoreCols|StoreRest|p\.lse\[)", softmax)
     assert len(stores) == 3 and all("wait.ok" in condition for condition in stores)
+
+
+def test_epilogue_warps_decide_on_a_failed_wait_as_a_whole():
+    """What follows the wait for an accumulator are instructions of a whole warp (loads from TMEM, votes, barriers): lanes that went on
+    alone would wait for those that did not."""
+    for name in ("gemm_tcgen05.cu", "conv_tcgen05.cu"):
+        waits = re.findall(r"(\w+)\(&?tmem_full\b[^;{]*\)", (KERNELS / name).read_text())
+        waits = [w for w in waits if w.startswith("Mbar") and "Wait" in w]
+        assert len(waits) == 4 and set(waits) == {"MbarWaitWarp"}, name

@@ -256,7 +256,7 @@ ConvTapsKernel(const __grid_constant__ ConvMaps maps, const __grid_constant__ Co
       const int h0 = ((mt / p.tiles_w) % p.tiles_h) * p.th;
       const int n0 = (mt / (p.tiles_w * p.tiles_h)) * p.tn;
       const int buf = local & 1;
-      if (ok && !MbarWait(&tmem_full[buf], (local >> 1) & 1)) {
+      if (ok && !MbarWaitWarp(&tmem_full[buf], (local >> 1) & 1)) {
         if (lane == 0) atomicExch(p.error, 3);
         ok = false;
       }
@@ -534,7 +534,7 @@ ConvRowPairKernel(const __grid_constant__ RowPairMaps maps, const __grid_constan
     bool ok = true;
     for (int u = blockIdx.x; u < p.units; u += gridDim.x, ++it) {
       const int buf = it & 1;
-      if (ok && !MbarWait(&tmem_full[buf], (it >> 1) & 1)) {
+      if (ok && !MbarWaitWarp(&tmem_full[buf], (it >> 1) & 1)) {
         if (lane == 0) atomicExch(p.error, 3);
         ok = false;
       }
@@ -796,7 +796,7 @@ ConvWgradKernel(const __grid_constant__ WgradMaps maps, const __grid_constant__ 
     }
   } else {
     const int q = warp & 3;
-    const bool ok = MbarWait(tmem_full, 0);
+    const bool ok = MbarWaitWarp(tmem_full, 0);
     if (!ok && lane == 0) atomicExch(p.error, 3);
     TcFenceAfter();
     if (ok && num_k > 0) {
@@ -1033,7 +1033,7 @@ ConvWgradHaloKernel(const __grid_constant__ WgradHaloMaps maps, const __grid_con
     if (ElectOne()) UmmaCommit(tmem_full);
   } else if (warp > 1) {
     const int q = warp & 3;
-    const bool ok = MbarWait(tmem_full, 0);
+    const bool ok = MbarWaitWarp(tmem_full, 0);
     if (!ok && lane == 0) atomicExch(p.error, 3);
     TcFenceAfter();
     if (ok && blockIdx.x < p.units) {

@@ -195,7 +195,7 @@ GemmTnKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__
     }
   } else {
     const int q = warp & 3;  // TMEM lane quarter this warp may access
-    const bool ok = MbarWait(tmem_full, 0);
+    const bool ok = MbarWaitWarp(tmem_full, 0);
     if (!ok && lane == 0) atomicExch(p.error, 3);
     TcFenceAfter();
     const int row = m0 + q * 32 + lane;
@@ -430,7 +430,7 @@ GemmTnPersistentKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
       const int m0 = (tile / tiles_n) * kBM, n0 = (tile % tiles_n) * BN;
       const int buf = local & 1;
-      if (ok && !MbarWait(&tmem_full[buf], (local >> 1) & 1)) {
+      if (ok && !MbarWaitWarp(&tmem_full[buf], (local >> 1) & 1)) {
         if (lane == 0) atomicExch(p.error, 3);
         ok = false;
       }
@@ -697,7 +697,7 @@ GemmPairKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     for (int tile = pair; tile < num_tiles; tile += pairs, ++local) {
       const int m0 = (tile / tiles_n) * 2 * kBM + cta * kBM, n0 = (tile % tiles_n) * BN + g * 64;
       const int buf = local & 1;
-      if (ok && !MbarWait(&tmem_full[buf], (local >> 1) & 1)) {
+      if (ok && !MbarWaitWarp(&tmem_full[buf], (local >> 1) & 1)) {
         if (lane == 0) atomicExch(p.error, 3);
         ok = false;
       }
@@ -765,7 +765,7 @@ GemmPairKernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       const int mn = kSplit ? tile % plane : tile;
       const int m0 = (mn / tiles_n) * 2 * kBM + cta * kBM, n0 = (mn % tiles_n) * BN + g * (BN / 2);
       const int buf = local & 1;
-      if (ok && !MbarWait(&tmem_full[buf], (local >> 1) & 1)) {
+      if (ok && !MbarWaitWarp(&tmem_full[buf], (local >> 1) & 1)) {
         if (lane == 0) atomicExch(p.error, 3);
         ok = false;
       }
