@@ -7,6 +7,7 @@ attention skips the padding; with --save8 the linear layers keep their activatio
     python -m torch.distributed.run --nproc-per-node 8 examples/bert_pretrain.py --steps 50 --fused-update
 """
 import argparse
+import itertools
 import os
 import sys
 import time
@@ -18,6 +19,22 @@ import tips_b200 as tips  # noqa: E402
 from tips_b200.models.bert import bert_large, synthetic_mlm_batch  # noqa: E402
 from tips_b200.ops.optim import FusedAdamW  # noqa: E402
 from tips_b200.utils.checkpoint import save_checkpoint  # noqa: E402
+
+
+def device_batches(host, dev):
+    """The pinned host batches in turn, on the device: each is copied on a side stream while the one before is computed on."""
+    copy_stream = torch.cuda.Stream()
+    for i in itertools.count():
+        with torch.cuda.stream(copy_stream):
+            nxt = [t.to(dev, non_blocking=True) for t in host[i % len(host)]]
+            ready = copy_stream.record_event()
+        if i > 0:
+            yield batch
+        here = torch.cuda.current_stream()
+        here.wait_event(ready)
+        for t in nxt:
+            t.record_stream(here)  # its memory takes no other batch before the work that reads it is done
+        batch = nxt
 
 
 def main():
@@ -43,7 +60,7 @@ def main():
     opt = tips.DistributedOptimizer(FusedAdamW(model.parameters(), lr=a.lr, weight_decay=0.01),
                                     fused_update=a.fused_update if size > 1 else None)
     tips.broadcast_parameters(model.state_dict(), root_rank=0, optimizer=opt)
-    # three host batches in pinned memory, copied while the previous step computes
+    # three host batches in pinned memory
     host = []
     for i in range(3):
         ids, pos, labels = synthetic_mlm_batch(a.batch, a.seq, 30522, seed=31 * rank + i)
@@ -52,22 +69,16 @@ def main():
             lengths = torch.randint(a.seq // 4, a.seq + 1, (a.batch,), generator=torch.Generator().manual_seed(31 * rank + i))
             labels = labels.masked_fill(pos >= lengths[:, None], -100)  # masked positions in the padding do not count
         host.append(tuple(t.pin_memory() for t in (ids, pos, labels, lengths)))
-    copy_stream = torch.cuda.Stream()
-    nxt = [t.to(dev, non_blocking=True) for t in host[0]]
     t0 = None
-    for step in range(a.steps):
+    for step, (ids, pos, labels, lengths) in zip(range(a.steps), device_batches(host, dev)):
         if step == 5:
             torch.cuda.synchronize()
             t0 = time.time()
-        ids, pos, labels, lengths = nxt
-        with torch.cuda.stream(copy_stream):
-            nxt = [t.to(dev, non_blocking=True) for t in host[(step + 1) % 3]]
         for g in opt.param_groups:                      # linear warm-up; the fused kernels read lr every step
             g["lr"] = a.lr * min(1.0, (step + 1) / max(1, a.warmup_steps))
         loss = model.loss(ids, pos, labels, lengths=lengths if a.padded else None)
         loss.backward()
         opt.step()
-        torch.cuda.current_stream().wait_stream(copy_stream)
         if step % 10 == 0 or step == a.steps - 1:
             avg = tips.metric_average(loss.detach().float(), "loss")
             if rank == 0:
