@@ -84,6 +84,7 @@ def main():
             if rank == 0:
                 print(f"step {step}: loss {avg:.4f} lr {opt.param_groups[0]['lr']:.2e}", flush=True)
     torch.cuda.synchronize()
+    model.check()
     if t0 is not None and a.steps > 5 and rank == 0:
         dt = (time.time() - t0) / (a.steps - 5)
         print(f"{a.batch * a.seq * size / dt:,.0f} tokens/s on {size} GPU(s), {dt * 1e3:.1f} ms/step", flush=True)

@@ -94,3 +94,17 @@ def test_encoder_on_a_padded_batch():
     a, b = (model.loss(x, pos, labels, lengths=n) for x in (ids, other))
     assert torch.allclose(a, b, rtol=1e-5)
     assert not torch.allclose(a, model.loss(ids, pos, labels), rtol=1e-5)
+
+
+def test_the_encoder_reports_launches_whose_waits_ran_out(monkeypatch):
+    from tips_b200.models.bert import tiny_bert
+    from tips_b200.ops import attention as a, linear
+    model = tiny_bert(dtype=torch.float32, device="cpu")
+    for gemm, att, message in ((0, 0, None), (0, 4, "attention"), (3, 0, "GEMM")):
+        monkeypatch.setattr(linear, "gemm_status", lambda: gemm)
+        monkeypatch.setattr(a, "attention_status", lambda: att)
+        if message is None:
+            model.check()
+        else:
+            with pytest.raises(RuntimeError, match=message):
+                model.check()

@@ -1,9 +1,13 @@
 """The encoder's training example on a GPU."""
 import importlib.util
 import os
+import subprocess
+import sys
 
 import pytest
 import torch
+
+from mp_util import free_port
 
 pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -28,3 +32,14 @@ def test_a_batch_stays_until_it_has_been_read():
     for i, batch in enumerate(seen):
         for got, want in zip(batch, host[i % 3]):
             assert torch.equal(got.cpu(), want), i
+
+
+@pytest.mark.parametrize("options", [[], ["--padded", "--save8"]])
+def test_the_encoder_example_runs(options, tmp_path):
+    path = tmp_path / "model.pt"
+    cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=1", "--master-addr", "127.0.0.1", "--master-port",
+           str(free_port()), os.path.join(ROOT, "examples", "bert_pretrain.py"), "--steps", "7", "--batch", "3", "--seq", "100", "--layers", "1",
+           "--checkpoint", str(path), *options]
+    r = subprocess.run(cmd, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-3000:]
+    assert "step 6: loss" in r.stdout and "tokens/s" in r.stdout and path.exists()

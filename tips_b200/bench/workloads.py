@@ -430,8 +430,7 @@ def run_bert(batch: int, seq: int, steps: int, warmup: int, layers: int = 24, fu
         return loss
 
     ms, launches = timed(step_resident, steps, warmup)
-    from tips_b200.ops.linear import gemm_status
-    assert gemm_status() == 0
+    model.check()
     value = batch * seq * tips.size() * steps / (ms / 1e3)
     pre = _Prefetcher(host)
     last = {}
@@ -446,6 +445,7 @@ def run_bert(batch: int, seq: int, steps: int, warmup: int, layers: int = 24, fu
 
     ms2, _ = timed(step_e2e, steps, max(5, warmup))
     last["loss"] = reader.drain()
+    model.check()
     e2e = {"value": batch * seq * tips.size() * steps / (ms2 / 1e3), "unit": "tokens/s", "ms_per_step": ms2 / steps,
            "h2d_bytes_per_step": pre.bytes_per_step, "d2h_bytes_per_step": 4, "last_loss": last.get("loss")}
     return {"value": value, "ms_per_step": ms / steps, "gpu_launches": launches, "e2e": e2e,

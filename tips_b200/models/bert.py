@@ -90,6 +90,16 @@ class BertMLM(nn.Module):
         logits = linear(hcur, self.tok.weight, self.decoder_bias)
         return softmax_cross_entropy(logits, masked_labels.reshape(-1))
 
+    def check(self):
+        """Raises if a launch on the current device ran out of a bounded wait, after which results are void.  Waits for the device:
+        for the end of a run or now and then, not for every step."""
+        from ..ops.attention import attention_status
+        from ..ops.linear import gemm_status
+        if gemm_status() != 0:
+            raise RuntimeError("a GEMM launch reported a bounded-wait timeout")
+        if attention_status() != 0:
+            raise RuntimeError("an attention launch reported a bounded-wait timeout")
+
 
 def bert_large(dtype=torch.bfloat16, device="cuda", **kw):
     return BertMLM(**kw).to(device=device, dtype=dtype)
