@@ -108,3 +108,21 @@ def test_the_encoder_reports_launches_whose_waits_ran_out(monkeypatch):
         else:
             with pytest.raises(RuntimeError, match=message):
                 model.check()
+
+
+def test_what_is_too_large_for_a_gpu_is_a_value_error():
+    """Without a GPU: the checks look at a tensor's type, device and number of sequences only."""
+    from types import SimpleNamespace
+
+    from tips_b200.ops.attention import _check_attention
+
+    def check(b=1, s=16, h=2, hk=2, d=64, scale=None):
+        return _check_attention(SimpleNamespace(shape=(b, s), dtype=torch.bfloat16, device="cuda", is_cuda=True), s, h, hk, d, None, scale)
+
+    for ok in (dict(), dict(b=65535), dict(h=1 << 17, hk=1 << 17), dict(s=1 << 25), dict(s=1 << 24, h=4), dict(b=0, s=1 << 26), dict(b=1 << 20, s=0),
+               dict(scale=2.0 ** -149), dict(scale=2.3e38)):
+        check(**ok)
+    for bad in (dict(b=65536), dict(h=(1 << 17) + 1, hk=(1 << 17) + 1), dict(s=(1 << 25) + 1), dict(s=(1 << 24) + 1, h=4), dict(b=1 << 12, s=1 << 16, h=512, hk=512),
+                dict(scale=1e-50), dict(scale=2.4e38)):
+        with pytest.raises(ValueError):
+            check(**bad)

@@ -361,3 +361,15 @@ def test_the_status_waits_for_every_stream():
             run(q, k, v, do)
         assert not side.query()
         assert ask() == 0 and side.query()
+
+
+def test_the_most_sequences_of_a_launch():
+    from tips_b200.ops.attention import attention, packed_attention
+    q, k, v, do = make(65535, 3, 1, 1, 8, torch.bfloat16, seed=40)
+    check(run(q, k, v, do, causal=True), *reference(q, k, v, do, True))
+    assert status() == 0
+    x = torch.zeros(65536, 3, 1, 8, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        attention(x, x, x)
+    with pytest.raises(ValueError):
+        packed_attention(x.expand(65536, 3, 3, 8).reshape(65536, 3, 24), 1, scale=1.0)

@@ -80,7 +80,8 @@ class BertMLM(nn.Module):
 
     def loss(self, ids, masked_positions, masked_labels, lengths=None):
         """ids [B, S]; masked_positions [B, P] indices into S; masked_labels [B, P] (-100 = unused slot); lengths [B]: of a
-        padded batch, positions from a sequence's length on are not attended to (their ids must still be valid)."""
+        padded batch, positions from a sequence's length on are not attended to (their ids must still be valid; on a GPU
+        the model has to be in bfloat16 or float16 for it)."""
         x = self.encode(ids, lengths)
         b, p = masked_positions.shape
         picked = torch.gather(x, 1, masked_positions[..., None].expand(b, p, x.shape[-1])).reshape(b * p, -1)

@@ -104,6 +104,12 @@ def _check_attention(t, s, h, hk, d, lengths, scale) -> float:
             raise TypeError(f"attention on a GPU takes bfloat16 or float16, got {t.dtype}")
         if d % 8 != 0 or d > 128:
             raise ValueError(f"attention on a GPU takes head sizes that are multiples of 8 up to 128, got {d}")
+        b, group = t.shape[0], h // hk
+        if b * s > 0 and (b > 65535 or h > 1 << 17 or s * group > 1 << 25 or b * (h + hk) * -(-s // 128) >= 1 << 31):
+            raise ValueError("attention on a GPU takes up to 65535 sequences, 2**17 heads, 2**25 positions times query heads per key head "
+                             f"and 2**31 tiles of 128 positions of a head, got {b} sequences of {s} with {h} heads and {hk} key heads")
+        if not 2.0 ** -149 <= scale <= 2.3e38:
+            raise ValueError(f"scale must be within the range of 32 bits, got {scale}")
     return scale
 
 
@@ -275,10 +281,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     to ``1 / sqrt(d)``.
 
     On a GPU: bfloat16 or float16, d a multiple of 8 up to 128, any strides (inputs whose last axis is not contiguous, or
-    whose rows do not start on 16 bytes, are copied).  The softmax is held in fp32; the probabilities, and their
-    gradient in the backward pass, are rounded to the inputs' type as operands of the products (for float16 at a scale that keeps
-    them within its range; the gradient as a sum of two values where seq is at most 128).  Gradients do not depend on the order
-    of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
+    whose rows do not start on 16 bytes, are copied), up to 65535 sequences, 2**17 heads, and 2**25 for seq times the query
+    heads of a key head.  The softmax is held in fp32; the probabilities, and their gradient in the backward pass, are rounded
+    to the inputs' type as operands of the products (for float16 at a scale that keeps them within its range; the gradient as a
+    sum of two values where seq is at most 128).  Gradients do not depend on the order of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
     do not see it, as 0 * inf does in the formula.  `lengths` may not change between forward and backward."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
