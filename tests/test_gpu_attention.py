@@ -373,3 +373,45 @@ def test_the_most_sequences_of_a_launch():
         attention(x, x, x)
     with pytest.raises(ValueError):
         packed_attention(x.expand(65536, 3, 3, 8).reshape(65536, 3, 24), 1, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("h,hk,d", [(4, 4, 128), (6, 2, 80), (4, 1, 128), (3, 1, 96)])
+@pytest.mark.parametrize("lengths", [[0, 1, 333, 128], [65, 256, 257, 191]])
+def test_padded_batches_of_larger_heads(lengths, h, hk, d, causal, dtype):
+    """Heads above 64 have a warp that clears what lies beyond a length, two sets of softmax warps, and outputs that are stored
+    directly: lengths around units of 64 and tiles of 128, NaN and infinities in the padding."""
+    q, k, v, do = make(4, 333, h, hk, d, dtype, seed=sum(lengths) + d)
+    n = torch.tensor(lengths, device=DEV)
+    want, bound = reference(q, k, v, do, causal, n)
+    with torch.no_grad():
+        for i, m in enumerate(lengths):
+            for t, x in ((q, -math.inf), (k, math.nan), (v, math.inf), (do, math.nan)):
+                t[i, m:] = x
+    got = run(q, k, v, do, causal=causal, lengths=n)
+    check(got, want, bound)
+    for i, m in enumerate(lengths):
+        for x in got.values():
+            assert not x[i, m:].any()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_padded_pieces_follow_one_another(causal, d):
+    """Several pieces of work per block, of one unit to many and some of none, most of them with rows to clear: what a block carries
+    over from piece to piece (phases of its barriers, ring places, stores that are owed) does not depend on where a piece ends."""
+    b, s, h, hk = 40, 700, 8, 2
+    q, k, v, do = make(b, s, h, hk, d, torch.bfloat16, seed=50)
+    g = torch.Generator()
+    g.manual_seed(51)
+    n = torch.randint(0, s + 1, (b,), generator=g)
+    n[3], n[17], n[30] = 0, s, 1
+    n = n.to(DEV)
+    got = run(q, k, v, do, causal=causal, lengths=n)
+    assert status() == 0
+    for i in range(0, b, 8):  # in parts: the reference holds several [heads, s, s] matrices in 64 bits
+        part = slice(i, i + 8)
+        want, bound = reference(q[part], k[part], v[part], do[part], causal, n[part])
+        check({name: x[part] for name, x in got.items()}, want, bound)
