@@ -415,3 +415,22 @@ def test_padded_pieces_follow_one_another(causal, d):
         part = slice(i, i + 8)
         want, bound = reference(q[part], k[part], v[part], do[part], causal, n[part])
         check({name: x[part] for name, x in got.items()}, want, bound)
+
+
+def test_scores_of_minus_infinity_at_a_large_scale():
+    """What stands for the maximum of a row whose first keys' scores are -inf stays finite when it is scaled."""
+    from tips_b200.ops.attention import attention
+    q, k, v, _ = make(1, 300, 2, 2, 64, torch.bfloat16, seed=14)
+    with torch.no_grad():
+        q.mul_(2.0 ** -30)
+        q[..., 0] = -1.0
+        k[..., 0] = 0.0
+        k[:, :140, :, 0] = math.inf
+        got = attention(q, k, v, scale=2.0 ** 29)
+        seen = slice(140, 300)
+        x = (q.double().transpose(1, 2) @ k[:, seen].double().transpose(1, 2).mT) * 2.0 ** 29
+        p, vd = torch.softmax(x, -1), v[:, seen].double().transpose(1, 2)
+        want = (p @ vd).transpose(1, 2)
+        # the probabilities and the output are rounded once each; 2^-14 for what is held in 32 bits
+        bound = (2.0 ** -8 + 2.0 ** -14) * (p @ vd.abs()).transpose(1, 2) + 2.0 ** -8 * want.abs()
+    assert ((got.double() - want).abs() <= bound).all()

@@ -62,6 +62,7 @@ struct AttnParams {
   int h, hk, d;
   int causal;
   float scale, c;       // c = scale * log2(e)
+  float low;            // stands for the maximum of a row whose scores are -inf so far: low * c is finite
   float* lse;           // [b, h, sp]
   float* delta;         // [2][b, h, sp], and for fp16 [2][b, hk]
   uint8_t* rest;        // [b, min(s, 128), h, d]: what rounding dropped of O, times RestScale, as e5m2; null: not kept
@@ -750,7 +751,7 @@ AttnFwdKernel(const __grid_constant__ AttnMaps maps, const __grid_constant__ Att
         float top = MaxNan(MaxNan(part[0], part[1], part[2]), part[3]);
         // a row whose scores are -inf so far: any finite reference below the scores to come; and inf - inf: the row is NaN, as by the
         // formula
-        if (top == -INFINITY) top = -1e30f;
+        if (top == -INFINITY) top = p.low;
         else if (top == INFINITY) top = __uint_as_float(0x7fc00000u);
         // The exponents' reference may lag behind the maximum by up to 2^8: probabilities of up to 256 lose nothing in 16 bits,
         // and the output in TMEM is rescaled a few times per row instead of with every new maximum.
@@ -1445,6 +1446,7 @@ AttnParams MakeParams(const void* lengths, int len64, int b, int s, int h, int h
   p.causal  = causal ? 1 : 0;
   p.scale   = scale;
   p.c       = scale * kLog2e;
+  p.low     = std::max(-1e30f, -1e37f / p.c);
   return p;
 }
 
