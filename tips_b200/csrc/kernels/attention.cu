@@ -519,7 +519,8 @@ __device__ __forceinline__ uint32_t AlignedSmem(const uint8_t* raw) { return (Sm
 // with 64 output columns, units of 64 keys leave TMEM for two blocks per SM, four tiles that run apart from each other
 // (32 x 512, 16 heads of 64: 53 us; one block with units of 128, next scores beside the probabilities, and a row shared
 // by two threads: 61).  With 128 one block fills TMEM, units have 128 keys, and one warp issues the products of both tiles, which
-// makes them take turns (8192, 16 heads of 128 that share 4, causal: 225 us = 1220 TFLOP/s; with a warp for each tile 248).
+// makes them take turns (8192, 16 heads of 128 that share 4, causal: 225 us = 1220 TFLOP/s; with a warp for each tile 248; in a long loop
+// of forward and backward passes, at the 1665 MHz that the power limit leaves, 268).
 // Bound, within a long piece of 64 columns, by the unit for exponentials, which is busy four fifths of the time, and by issue slots
 // beside it; at 512 positions also by the start and the end of a piece.  With 128 columns by the way from a tile's scores through its
 // probabilities and products to its next scores (3300 clocks, of which the tensor cores work 2050 for both tiles).
@@ -921,8 +922,8 @@ __device__ __forceinline__ int GradExponent(const AttnParams& p, int b, int hk) 
 // gets half of them; one for all: 8192, 16 heads that share 4, causal, 1143 us where two take 810), and one clears rows beyond a
 // sequence's length; two blocks have no registers for more warps, so the one that issues clears as well.
 // D included: 32 x 512, 16 heads of 64: 182 us = 473 TFLOP/s counting five products, with lengths spread over 1..512: 114; 4 x 2048: 269 us =
-// 640; 8192 positions, 16 heads of 128 that share 4, causal: 810 us = 847.  (One block per SM with units of 128 for 64 columns, and the
-// next scores beside them: 183, 126 and 264.)  Bound by the way from one unit to the next: S, exponentials, dP, dS and the
+// 640; 8192 positions, 16 heads of 128 that share 4, causal: 810 us = 847 (906 at 1665 MHz, see above).  (One block per SM with units of 128
+// for 64 columns, and the next scores beside them: 183, 126 and 264.)  Bound by the way from one unit to the next: S, exponentials, dP, dS and the
 // products' latencies follow one another, with the tensor cores busy a third to a half of the time, the exponentials' unit half.
 template <int HD>
 struct BwdCfg {
