@@ -110,6 +110,26 @@ def tiny_bert(dtype=torch.bfloat16, device="cuda", **kw):
     return BertMLM(vocab=1024, hidden=128, layers=2, heads=4, ffn=512, max_seq=64, **kw).to(device=device, dtype=dtype)
 
 
+def smoke_step(device):
+    """Two steps of the small encoder on a padded batch, with its activations in 8 bits: used by the smoke test."""
+    model = tiny_bert(device=device, save8=True)
+    ids, pos, labels = (t.to(device) for t in synthetic_mlm_batch(4, 64, 1024, seed=1))
+    lengths = torch.tensor([64, 20, 1, 33], device=device)
+    losses = []
+    for _ in range(2):
+        loss = model.loss(ids, pos % lengths[:, None], labels, lengths=lengths)
+        loss.backward()
+        with torch.no_grad():
+            for p in model.parameters():
+                if p.grad is not None:
+                    p -= 0.05 * p.grad
+                    p.grad = None
+        losses.append(loss.item())
+    model.check()
+    assert all(x == x for x in losses), losses
+    return losses
+
+
 def synthetic_mlm_batch(batch, seq, vocab, seed, mask_frac=0.15):
     """Token ids uniform over the vocabulary, 15% of positions masked uniformly."""
     g = torch.Generator().manual_seed(seed)
