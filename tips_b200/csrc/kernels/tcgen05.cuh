@@ -49,9 +49,28 @@ __device__ __forceinline__ bool MbarWait(uint64_t* bar, uint32_t parity) {
   }
   return false;
 }
-// The same for a whole warp: every lane waits, and all of them get one answer, so that the warp stays converged.
+// The same for a whole warp: every lane polls, and all of them get one answer, so that the warp stays converged.  The vote is part of
+// the loop: behind a loop that each lane leaves by itself it cost the small products of a CTR step about 1 us in 280.
 __device__ __forceinline__ bool MbarWaitWarp(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, MbarWait(bar, parity));
+  const uint32_t addr = SmemAddr(bar);
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (__all_sync(0xffffffffu, done)) return true;
+    if ((i & 0xff) == 0) {
+      uint64_t now;
+      asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
+      if (t0 == 0) t0 = now;
+      else if (__any_sync(0xffffffffu, now - t0 > kWaitBudgetNs)) return false;
+    }
+  }
 }
 // True in one lane of a converged warp, always the same one.  The instructions that a single thread issues (tcgen05.mma,
 // commits, TMA) take their operands from uniform registers: behind this predicate, in a loop that the whole warp walks,
