@@ -284,8 +284,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     whose rows do not start on 16 bytes, are copied), up to 65535 sequences, 2**17 heads, and 2**25 for seq times the query
     heads of a key head.  The softmax is held in fp32; the probabilities, and their gradient in the backward pass, are rounded
     to the inputs' type as operands of the products (for float16 at a scale that keeps them within its range; the gradient as a
-    sum of two values where seq is at most 128).  Gradients do not depend on the order of the blocks.  An infinity or NaN in a valid position may reach every row of a causal batch, also those that
-    do not see it, as 0 * inf does in the formula.  `lengths` may not change between forward and backward."""
+    sum of two values where seq is at most 128).  Gradients do not depend on the order of the blocks.  An infinity or NaN in a
+    valid position may reach every row of a causal batch, also those that do not see it, as 0 * inf does in the formula.
+    `lengths` may not change between forward and backward."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
             raise ValueError(f"{name} must be [batch, seq, heads, head_size], got {tuple(t.shape)}")
