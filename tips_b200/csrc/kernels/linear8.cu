@@ -1,7 +1,7 @@
 // A linear layer that keeps its activations in 8 bits: its forward and its backward pass as one call each, on the kernels of
 // gemm_tcgen05.cu and saved8.cu.  A small layer waits for the host, not for the GPU, and most of what the
-// host does is done per call: 128 rows of 128 into 512, forward and backward, took 197 us with a call per kernel and takes 147.
-// A large one is bound by its three products.  16384 rows of 1024 into 4096 with GELU, pass after pass: 479 us at the 1620 MHz that
+// host does is done per call: 128 rows of 128 into 512, forward and backward, took 197 us with a call per kernel and takes 143.
+// A large one is bound by its three products.  16384 rows of 1024 into 4096 with GELU, pass after pass: 476 us at the 1620 MHz that
 // the power limit leaves; with events between the kernels 488: first product with GELU and the 8-bit form 155, dx 112, dw 112, GELU's
 // derivative and the bias gradient 77, packing and unpacking x 17 + 15.  A few passes at 1965 MHz: 427, 133 + 96 + 96 + 73 + 16 + 15.
 #include <algorithm>
